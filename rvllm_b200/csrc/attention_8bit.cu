@@ -1,0 +1,875 @@
+// Paged causal attention over keys and values held in 8 bits (cache_8bit.cu: int8 [pages][kv heads][page size]
+// [head size], one power-of-two scale per page and head), single tokens and portions of prompts.  Compiled for one head
+// size at a time (RV_HD: a multiple of 16, at most 256).
+//
+// A warp works alone.  It owns 8 (or 16) rows -- a row is a query token and one of the query heads that share the key/value head --
+// and walks tiles of keys, which it copies itself (cp.async) into a ring of its own in shared memory: nothing
+// but the warp's own copies is waited for.  Scores are computed transposed, S^T = K Q^T, by m16n8k16 products of float16
+// operands with float32 sums: 16 keys are the rows of the left operand, 8 query rows the columns of the right one.
+// With few query heads per key/value head the other order would leave most of a product's 16 rows empty.
+//
+//   int8 -> float16   the byte q + 128 behind the exponent byte 0x64 is the float16 1024 + 128 + q; minus
+//                     1152 leaves q exactly: a byte permutation and a subtraction for two values.
+//   keys              a lane's four k-steps of 64 dimensions are 16 bytes that lie side by side: the order of a sum's
+//                     terms is free, so the queries are put in that order and the keys need no transposition.
+//   queries           times 2^e per row so that the largest is in [256, 512): float16 holds the bfloat16 values then to 2^-33
+//                     of the largest; float32 ones as a sum of two float16 values, 22 bits.
+//   values            pairs of dimensions transposed by ldmatrix (two bytes travel as one 16-bit element), so even and odd
+//                     dimensions come out as the two halves of a product's 16 rows.
+//   scales            u_j = s_kj (k_j . q) scale log2(e) + log2(s_vj) in float32; p'_j = 2^(u_j - M) with M some 2^6 below
+//                     the largest u.  O = sum p'_j v8_j, l = sum p'_j / s_vj, and O / l is the result: the value's scale
+//                     rides in the exponent, so p' is as large as the term that it stands for.  p' is rounded to
+//                     float16 for the product (2^-12 of itself; 2^-23 in two parts for float32 rows); l adds the unrounded.
+//
+// M moves lazily: only when a u has passed it by more than 2^14 is O rescaled, so most tiles need no
+// reduction over lanes at all.
+//
+// Single tokens (attention_8bit_stream): as many warps as the GPU holds, the tiles of all requests and heads cut evenly
+// among them; a warp's part of one request's heads is a segment, left in scratch for the merge kernel.  Portions
+// (attention_8bit_rows): a warp, or `nsplit` warps that share its tiles, for every 8 or 16 rows.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+#ifndef RV_HD
+#define RV_HD 64
+#endif
+#define A8_HD RV_HD
+static_assert(A8_HD % 16 == 0 && A8_HD >= 16 && A8_HD <= 256, "head sizes");
+#define A8_KEYS (A8_HD <= 64 ? 64 : A8_HD <= 128 ? 32 : 16)       // a tile
+#define A8_CHUNKS (A8_HD / 16)                                    // 16-byte pieces of a row
+#define A8_STAGES 3
+#define A8_STREAM_WARPS 8                                         // one block a multiprocessor
+#define A8_ROWS_WARPS 4                                           // two blocks
+
+#define A8_STAGE_BYTES (2 * A8_KEYS * A8_HD + 2 * A8_KEYS * 4)
+#define A8_WARP_BYTES (A8_STAGES * A8_STAGE_BYTES)
+
+struct A8Args {
+    const void* q;
+    const signed char *k, *v;
+    const float *k_scale, *v_scale;
+    const int *block_table, *q_start, *ctx_lens;
+    const float* sinks;
+    void* out;
+    float* part_o;                     // [places][rows][HD]
+    float2* part_ml;                   // [places][rows]: M, l
+    long long q_stride, pages;
+    int max_blocks, first_req, n_reqs, num_heads, num_kv_heads, page_size, window, nsplit, row_tiles, vec;
+    float scale_log2;
+};
+
+__device__ __forceinline__ unsigned a8_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void a8_copy16(unsigned dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void a8_copy4(unsigned dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void a8_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                       unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned a8_transpose(unsigned x) {
+    unsigned y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float a8_exp2(float x) {              // -inf: 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Bytes `sel` of x, each behind 0x64, minus 1152 (x: bytes of q + 128).
+__device__ __forceinline__ unsigned a8_pair(unsigned x, unsigned sel) {
+    const unsigned h = __byte_perm(x, 0x64646464u, sel);
+    const __half2 v = __hsub2(*(const __half2*)&h, __half2half2(__ushort_as_half((unsigned short)0x6480)));
+    return *(const unsigned*)&v;
+}
+__device__ __forceinline__ unsigned a8_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const unsigned*)&h;
+}
+// What the rounding to float16 left.
+__device__ __forceinline__ unsigned a8_rest(float a, float b, unsigned packed) {
+    const float2 f = __half22float2(*(const __half2*)&packed);
+    return a8_pack(a - f.x, b - f.y);
+}
+// Where 16-byte piece c of a tile's row lies: moved so that what a warp reads at once is spread over the banks.
+// Values: eight rows' pieces c (ldmatrix); keys: two rows' four pieces.
+__device__ __forceinline__ int a8_vpiece(int row, int c) {
+    constexpr int n = A8_CHUNKS;
+    return n % 8 == 0 ? c ^ (row & 7) : n % 4 == 0 ? c ^ ((row >> 1) & 3) : n % 2 == 0 ? c ^ ((row >> 2) & 1) : c;
+}
+__device__ __forceinline__ int a8_kpiece(int row, int c) { return A8_CHUNKS % 8 == 0 ? c ^ ((row & 1) << 2) : c; }
+
+__device__ __forceinline__ float a8_load(const float* p) { return *p; }
+__device__ __forceinline__ float a8_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+// N values from p on; `vec`: p is 16-byte aligned.
+template <int N>
+__device__ __forceinline__ void a8_load_n(const float* p, bool vec, float (&v)[N]) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 f = *(const float4*)(p + i);
+            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = p[i];
+    }
+}
+template <int N>
+__device__ __forceinline__ void a8_load_n(const __nv_bfloat16* p, bool vec, float (&v)[N]) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint2 u = *(const uint2*)(p + i);
+            const float2 a = __bfloat1622float2(*(const __nv_bfloat162*)&u.x), b = __bfloat1622float2(*(const __nv_bfloat162*)&u.y);
+            v[i] = a.x; v[i + 1] = a.y; v[i + 2] = b.x; v[i + 3] = b.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __bfloat162float(p[i]);
+    }
+}
+
+// ---- how single tokens' tiles are shared out --------------------------------------------------------
+// The tiles of (request, unit), one after the other, cut evenly into as many runs as there are warps (`used` of them
+// where there are fewer tiles).  A unit: a key/value head and 8 * NT of its query heads.  From one segment to the next
+// the run or the unit grows, so run + request * units + unit is a place of its own.
+struct A8Shares {
+    const int* ctx_lens;
+    int n_reqs, units, window, most;
+    long long total;
+    int used;
+    __device__ __forceinline__ int first(int clen) const { return window > 0 ? max(0, clen - window) / A8_KEYS : 0; }
+    // A context that the block table cannot hold has no tiles: the merge marks its rows.
+    __device__ __forceinline__ int tiles(int clen) const {
+        return clen > 0 && clen <= most ? (clen - 1) / A8_KEYS - first(clen) + 1 : 0;
+    }
+    __device__ __forceinline__ int length(int r) const { return r < n_reqs ? ctx_lens[r] : 0; }
+    // Tiles of a unit over the requests before r (a whole warp asks).
+    __device__ __forceinline__ long long before(int r) const {
+        long long sum = 0;
+        const int lane = threadIdx.x & 31;
+        for (int at = 0; at < r; at += 32)
+            sum += __reduce_add_sync(0xffffffffu, (unsigned)(at + lane < r ? tiles(length(at + lane)) : 0));
+        return sum;
+    }
+    __device__ __forceinline__ A8Shares(const int* lens, int reqs, int u, int win, long long slots, int runs)
+        : ctx_lens(lens), n_reqs(reqs), units(u), window(win), most((int)min(slots, 0x7fffffffll)) {
+        total = before(reqs) * units;
+        used = (int)min((long long)runs, max(1ll, total));
+    }
+    __device__ __forceinline__ long long start(int run) const { return (long long)run * total / used; }
+    __device__ __forceinline__ int run_of(long long tile) const { return (int)(((tile + 1) * used - 1) / total); }
+};
+
+// ---- one warp's work ----------------------------------------------------------------------------------
+// A place in the walk over tiles: the tile `tile` of (request r, unit u).
+struct A8Cursor {
+    int r, u, tile, last, clen;
+};
+
+template <typename T, int NT, int PARTS>
+struct A8Warp {
+    const A8Args& a;
+    unsigned char* ring;
+    const int lane, g, t;
+    int rows_first, rows_count, kvh, G, qs;        // of the segment: its first row, rows, head, query heads a head, first token
+    float o[A8_CHUNKS][NT][4];
+    unsigned q[A8_CHUNKS][NT][PARTS][2];
+    float f[NT][2], M[NT][2], l[NT][2];
+    int hi[NT][2], lo[NT][2], p_min, lo_max;
+
+    __device__ __forceinline__ A8Warp(const A8Args& args, unsigned char* mem)
+        : a(args), ring(mem), lane(threadIdx.x & 31), g((threadIdx.x & 31) >> 2), t(threadIdx.x & 3) {
+        G = a.num_heads / a.num_kv_heads;
+    }
+
+    // The pages of a tile's keys: this lane's key (and the one 32 after it).
+    __device__ __forceinline__ void pages_of(const A8Cursor& c, int (&page)[2]) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            page[i] = -1;
+            const int in_tile = lane + 32 * i, key = c.tile * A8_KEYS + in_tile;
+            if (in_tile < A8_KEYS && key < c.clen) {
+                const int blk = key / a.page_size;
+                if (blk < a.max_blocks) page[i] = a.block_table[(size_t)c.r * a.max_blocks + blk];
+            }
+        }
+    }
+    __device__ __forceinline__ void request(const A8Cursor& c, int head, const int (&page)[2], int stage) const {
+        unsigned char* base = ring + stage * A8_STAGE_BYTES;
+        unsigned row[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int in_tile = lane + 32 * i, key = c.tile * A8_KEYS + in_tile;
+            const bool ok = page[i] >= 0 && page[i] < a.pages;
+            const long long block = ok ? (long long)page[i] * a.num_kv_heads + head : 0;
+            row[i] = ok ? (unsigned)(block * a.page_size + key % a.page_size) : 0xffffffffu;
+            if (in_tile < A8_KEYS) {
+                const unsigned s = a8_smem(base + 2 * A8_KEYS * A8_HD + in_tile * 4);
+                a8_copy4(s, a.k_scale + block, ok);
+                a8_copy4(s + A8_KEYS * 4, a.v_scale + block, ok);
+            }
+        }
+        const unsigned kd = a8_smem(base), vd = kd + A8_KEYS * A8_HD;
+#pragma unroll
+        for (int it = 0; it < (A8_KEYS * A8_CHUNKS + 31) / 32; ++it) {
+            const int id = it * 32 + lane, key = id / A8_CHUNKS, c16 = id - key * A8_CHUNKS;
+            unsigned from = __shfl_sync(0xffffffffu, row[0], key & 31);
+            if (A8_KEYS > 32) {
+                const unsigned second = __shfl_sync(0xffffffffu, row[1], key & 31);
+                from = key < 32 ? from : second;
+            }
+            if (id < A8_KEYS * A8_CHUNKS) {
+                const bool ok = from != 0xffffffffu;
+                const size_t at = ok ? (size_t)from * A8_HD + c16 * 16 : 0;
+                a8_copy16(kd + key * A8_HD + a8_kpiece(key, c16) * 16, a.k + at, ok);
+                a8_copy16(vd + key * A8_HD + a8_vpiece(key, c16) * 16, a.v + at, ok);
+            }
+        }
+    }
+
+    // Rows [first, first + 8 NT) of the `qlen` tokens times G heads of request r.
+    __device__ __forceinline__ void begin(int r, int head, int first, int qlen, int q_first, int clen) {
+        rows_first = first;
+        rows_count = min(8 * NT, qlen * G - first);
+        kvh = head;
+        qs = q_first;
+        p_min = clen;
+        lo_max = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            // the row whose values this lane holds: column g
+            const int i = first + 8 * n + g, tok = i / G;
+            const bool real = i < qlen * G;
+            const T* src = (const T*)a.q + (size_t)(qs + (real ? tok : 0)) * a.q_stride +
+                           (size_t)(kvh * G + (real ? i - tok * G : 0)) * A8_HD;
+            float most = 0.f;
+            float x[A8_CHUNKS][4];
+#pragma unroll
+            for (int c = 0; c < A8_HD / 64; ++c) {
+                float w[16];
+                a8_load_n<16>(src + 64 * c + 16 * t, a.vec, w);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[4 * c + (k >> 2)][k & 3] = w[k];
+            }
+#pragma unroll
+            for (int c = A8_HD / 64 * 4; c < A8_CHUNKS; ++c) a8_load_n<4>(src + 16 * c + 4 * t, a.vec, x[c]);
+#pragma unroll
+            for (int c = 0; c < A8_CHUNKS; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (!real) x[c][k] = 0.f;
+                    most = fmaxf(most, fabsf(x[c][k]));
+                }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            // 2^(8 - exponent): within what float32 holds
+            int e = 8 - ((int)(__float_as_uint(most) >> 23) - 127);
+            e = most > 0.f ? max(-100, min(100, e)) : 0;
+            const float up = __uint_as_float((unsigned)(e + 127) << 23), down = __uint_as_float((unsigned)(127 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < A8_CHUNKS; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float x0 = x[c][2 * h] * up, x1 = x[c][2 * h + 1] * up;
+                    q[c][n][0][h] = a8_pack(x0, x1);
+                    if (PARTS == 2) q[c][n][PARTS - 1][h] = a8_rest(x0, x1, q[c][n][0][h]);
+                }
+            const float mine = down * a.scale_log2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // the rows of this lane's scores: columns 2 t, 2 t + 1
+                f[n][h] = __shfl_sync(0xffffffffu, mine, (2 * t + h) * 4);
+                const int j = first + 8 * n + 2 * t + h;
+                hi[n][h] = j < qlen * G ? clen - qlen + j / G : -1;
+                lo[n][h] = a.window > 0 ? max(0, hi[n][h] - a.window + 1) : 0;
+                M[n][h] = -INFINITY;
+                l[n][h] = 0.f;
+            }
+        }
+        // rows come in the order of their tokens
+        p_min = clen - qlen + first / G;
+        const int p_max = clen - qlen + (first + rows_count - 1) / G;
+        lo_max = a.window > 0 ? max(0, p_max - a.window + 1) : 0;
+#pragma unroll
+        for (int c = 0; c < A8_CHUNKS; ++c)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[c][n][k] = 0.f;
+    }
+
+    __device__ __forceinline__ void tile(int tile_at, int stage) {
+        const unsigned char* base = ring + stage * A8_STAGE_BYTES;
+        const float* ks = (const float*)(base + 2 * A8_KEYS * A8_HD);
+        const float* vs = ks + A8_KEYS;
+        constexpr int MT = A8_KEYS / 16;
+        float s[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[m][n][k] = 0.f;
+        // ---- S^T = K Q^T -------------------------------------------------------------------------
+        auto step = [&](int m, int c, unsigned w0, unsigned w1) {     // 16 dimensions of 16 keys
+            w0 ^= 0x80808080u;
+            w1 ^= 0x80808080u;
+            const unsigned a0 = a8_pair(w0, 0x4140), a2 = a8_pair(w0, 0x4342);
+            const unsigned a1 = a8_pair(w1, 0x4140), a3 = a8_pair(w1, 0x4342);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) a8_mma(s[m][n], a0, a1, a2, a3, q[c][n][p][0], q[c][n][p][1]);
+        };
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const int r0 = 16 * m + g, r1 = r0 + 8;
+#pragma unroll
+            for (int c = 0; c < A8_HD / 64; ++c) {
+                const uint4 x = *(const uint4*)(base + r0 * A8_HD + a8_kpiece(r0, 4 * c + t) * 16);
+                const uint4 y = *(const uint4*)(base + r1 * A8_HD + a8_kpiece(r1, 4 * c + t) * 16);
+                step(m, 4 * c, x.x, y.x);
+                step(m, 4 * c + 1, x.y, y.y);
+                step(m, 4 * c + 2, x.z, y.z);
+                step(m, 4 * c + 3, x.w, y.w);
+            }
+#pragma unroll
+            for (int c = A8_HD / 64 * 4; c < A8_CHUNKS; ++c)
+                step(m, c, *(const unsigned*)(base + r0 * A8_HD + a8_kpiece(r0, c) * 16 + 4 * t),
+                     *(const unsigned*)(base + r1 * A8_HD + a8_kpiece(r1, c) * 16 + 4 * t));
+        }
+        // ---- u, its largest -------------------------------------------------------------------------
+        const int key0 = tile_at * A8_KEYS;
+        const bool edge = key0 + A8_KEYS - 1 > p_min || key0 < lo_max;
+        float inv[MT][2], mx[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = 16 * m + 8 * h + g;
+                const float sk = ks[key], sv = vs[key];
+                // log2 of the scale; a key without a page (its scales are zeros) weighs nothing
+                const int e = max(-60, min(60, (int)((__float_as_uint(sv) >> 23) & 0xff) - 127));
+                inv[m][h] = __uint_as_float((unsigned)(127 - e) << 23);
+                const float ev = sk == 0.f ? -INFINITY : (float)e;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float u = fmaf(s[m][n][2 * h + j] * f[n][j], sk, ev);
+                        if (edge && (key0 + key > hi[n][j] || key0 + key < lo[n][j])) u = -INFINITY;
+                        s[m][n][2 * h + j] = u;
+                        mx[n][j] = fmaxf(mx[n][j], u);
+                    }
+            }
+        bool moves = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) moves |= mx[n][j] > M[n][j] + 14.f;          // also from -inf
+        if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x = mx[n][j];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(x - 6.f, M[n][j]);
+                    const float corr = x == -INFINITY ? 1.f : a8_exp2(M[n][j] - x);   // M = -inf: 0
+                    M[n][j] = x;
+                    l[n][j] *= corr;
+#pragma unroll
+                    for (int c = 0; c < A8_CHUNKS; ++c) {
+                        o[c][n][j] *= corr;
+                        o[c][n][2 + j] *= corr;
+                    }
+                }
+        }
+        // ---- p', l, and O^T += V^T P^T ----------------------------------------------------------------
+        float off[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) off[n][j] = M[n][j] == -INFINITY ? 0.f : M[n][j];
+        const unsigned vbase = a8_smem(base + A8_KEYS * A8_HD);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            unsigned p[NT][PARTS][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p0 = a8_exp2(s[m][n][2 * h] - off[n][0]), p1 = a8_exp2(s[m][n][2 * h + 1] - off[n][1]);
+                    l[n][0] = fmaf(p0, inv[m][h], l[n][0]);
+                    l[n][1] = fmaf(p1, inv[m][h], l[n][1]);
+                    const unsigned w = a8_pack(p0, p1);
+                    p[n][0][h] = a8_transpose(w);
+                    if (PARTS == 2) p[n][PARTS - 1][h] = a8_transpose(a8_rest(p0, p1, w));
+                }
+            // pieces c and c + 1 of the 16 keys' rows: lanes 0-7, 8-15 name keys 0-7, 8-15 of piece c, the others of c + 1
+            const int key = 16 * m + (lane & 15);
+#pragma unroll
+            for (int c = 0; c < A8_CHUNKS; c += 2) {
+                unsigned w[4];
+                if (c + 1 < A8_CHUNKS) {
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                 : "r"(vbase + key * A8_HD + a8_vpiece(key, c + (lane >> 4)) * 16) : "memory");
+                } else {
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                                 : "=r"(w[0]), "=r"(w[1])
+                                 : "r"(vbase + key * A8_HD + a8_vpiece(key, c) * 16) : "memory");
+                    w[2] = w[3] = 0u;
+                }
+#pragma unroll
+                for (int k = 0; k < 2 && c + k < A8_CHUNKS; ++k) {
+                    const unsigned x = w[2 * k] ^ 0x80808080u, y = w[2 * k + 1] ^ 0x80808080u;
+                    const unsigned a0 = a8_pair(x, 0x4240), a1 = a8_pair(x, 0x4341);
+                    const unsigned a2 = a8_pair(y, 0x4240), a3 = a8_pair(y, 0x4341);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < PARTS; ++i) a8_mma(o[c + k][n], a0, a1, a2, a3, p[n][i][0], p[n][i][1]);
+                }
+            }
+        }
+    }
+
+    // Sums over the lanes that share a row.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+                l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+            }
+    }
+    __device__ __forceinline__ void leave(size_t place) {
+        finish();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = 8 * n + 2 * t + j;
+                if (row >= rows_count) continue;
+                const size_t at = place * (8 * NT) + row;
+                if (g == 0) a.part_ml[at] = make_float2(M[n][j], l[n][j]);
+#pragma unroll
+                for (int c = 0; c < A8_CHUNKS; ++c)
+                    *(float2*)(a.part_o + at * A8_HD + 16 * c + 2 * g) = make_float2(o[c][n][j], o[c][n][2 + j]);
+            }
+    }
+    __device__ __forceinline__ void write() {
+        finish();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = 8 * n + 2 * t + j;
+                if (row >= rows_count) continue;
+                const int i = rows_first + row, tok = i / G, head = kvh * G + i - tok * G;
+                float L = l[n][j];
+                if (a.sinks && L != 0.f) L += a8_exp2(a.sinks[head] * 1.4426950408889634f - M[n][j]);
+                const float by = L == 0.f ? 0.f : 1.f / L;
+                T* dst = (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD + 2 * g;
+#pragma unroll
+                for (int c = 0; c < A8_CHUNKS; ++c) {
+                    rv_store(dst + 16 * c, o[c][n][j] * by);
+                    rv_store(dst + 16 * c + 1, o[c][n][2 + j] * by);
+                }
+            }
+    }
+};
+
+#define A8_WAIT_STAGE() asm volatile("cp.async.wait_group %0;" ::"n"(A8_STAGES - 2) : "memory")
+#define A8_COMMIT() asm volatile("cp.async.commit_group;" ::: "memory")
+
+// Requests [0, n_reqs) with one token each.
+template <typename T, int NT, int PARTS>
+__global__ void __launch_bounds__(A8_STREAM_WARPS * 32, 1) attention_8bit_stream_kernel(const __grid_constant__ A8Args a) {
+    rv_pdl_prologue();
+    extern __shared__ __align__(128) unsigned char smem[];
+    A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
+    const int per_head = (w.G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
+    // neighbours in the order of tiles on different multiprocessors
+    const int run = (int)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
+    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size,
+                      gridDim.x * A8_STREAM_WARPS);
+    if (run >= sh.used || sh.total == 0) return;
+    const long long from = sh.start(run);
+    int n = (int)(sh.start(run + 1) - from);
+    // where the run begins
+    A8Cursor c = {0, 0, 0, 0, 0};
+    {
+        const int lane = threadIdx.x & 31;
+        long long sum = 0;
+        for (int at = 0; at < a.n_reqs; at += 32) {
+            const int mine = sh.tiles(sh.length(at + lane));
+            int upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += v;
+            }
+            const bool has = (sum + upto) * units > from;
+            const unsigned who = __ballot_sync(0xffffffffu, has);
+            if (who) {
+                const int l = __ffs(who) - 1;
+                const int tiles = __shfl_sync(0xffffffffu, mine, l);
+                const long long in = from - (sum + __shfl_sync(0xffffffffu, upto, l) - tiles) * units;
+                c.r = at + l;
+                c.clen = sh.length(c.r);
+                c.u = (int)(in / tiles);
+                c.tile = sh.first(c.clen) + (int)(in - (long long)c.u * tiles);
+                c.last = (c.clen - 1) / A8_KEYS;
+                break;
+            }
+            sum += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    auto advance = [&](A8Cursor& x) {
+        if (++x.tile <= x.last) return;
+        if (++x.u == units) {
+            x.u = 0;
+            do ++x.r;
+            while (x.r < a.n_reqs && sh.tiles(sh.length(x.r)) == 0);
+            x.clen = sh.length(x.r);
+            x.last = (x.clen - 1) / A8_KEYS;
+        }
+        x.tile = sh.first(x.clen);
+    };
+    A8Cursor ahead = c;
+    int page[2], requested = 0;
+    w.pages_of(ahead, page);
+    auto request_next = [&](int stage) {
+        if (requested < n) {
+            w.request(ahead, ahead.u / per_head, page, stage);
+            if (++requested < n) {
+                advance(ahead);
+                w.pages_of(ahead, page);
+            }
+        }
+        A8_COMMIT();
+    };
+    for (int i = 0; i < A8_STAGES - 1; ++i) request_next(i);
+    bool fresh = true;
+    int stage = 0;
+    for (int i = 0; i < n; ++i) {
+        if (fresh) {
+            const int head = c.u / per_head;
+            w.begin(c.r, head, (c.u - head * per_head) * 8 * NT, 1, c.r, c.clen);
+            fresh = false;
+        }
+        A8_WAIT_STAGE();
+        __syncwarp();
+        request_next(stage == 0 ? A8_STAGES - 1 : stage - 1);
+        w.tile(c.tile, stage);
+        __syncwarp();
+        stage = stage + 1 == A8_STAGES ? 0 : stage + 1;
+        if (c.tile == c.last || i + 1 == n) {
+            w.leave((size_t)run + (size_t)c.r * units + c.u);
+            fresh = true;
+        }
+        if (i + 1 < n) advance(c);
+    }
+}
+
+// Requests [first_req, first_req + n_reqs) with any number of tokens.  A warp: (request, key/value head, 8 NT rows,
+// part of their tiles).  blockIdx.z: request, y: head, x and warp: rows and part.
+template <typename T, int NT, int PARTS>
+__global__ void __launch_bounds__(A8_ROWS_WARPS * 32, 2) attention_8bit_rows_kernel(const __grid_constant__ A8Args a) {
+    rv_pdl_prologue();
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int id = blockIdx.x * A8_ROWS_WARPS + (threadIdx.x >> 5);
+    const int rt = id / a.nsplit, part = id - rt * a.nsplit;
+    const int r = a.first_req + blockIdx.z, head = blockIdx.y;
+    const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs, clen = a.ctx_lens[r];
+    A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
+    // the rows with the longest contexts first
+    const int tiles = (qlen * w.G + 8 * NT - 1) / (8 * NT);
+    if (rt >= tiles) return;
+    const int first = (tiles - 1 - rt) * 8 * NT;
+    const int end = min(qlen * w.G, first + 8 * NT);
+    const int p_first = clen - qlen + first / w.G, p_last = clen - qlen + (end - 1) / w.G;
+    const bool fits = clen <= (long long)a.max_blocks * a.page_size;
+    const int t_all = (a.window > 0 ? max(0, p_first - a.window + 1) : 0) / A8_KEYS;
+    const int count = p_last >= 0 && fits ? p_last / A8_KEYS - t_all + 1 : 0;
+    const int t_lo = t_all + (int)((long long)count * part / a.nsplit), n = t_all + (int)((long long)count * (part + 1) / a.nsplit) - t_lo;
+    w.begin(r, head, first, qlen, qs, clen);
+    A8Cursor ahead = {r, 0, t_lo, t_lo + n - 1, clen};
+    int page[2], requested = 0;
+    w.pages_of(ahead, page);
+    auto request_next = [&](int stage) {
+        if (requested < n) {
+            w.request(ahead, head, page, stage);
+            ++ahead.tile;
+            if (++requested < n) w.pages_of(ahead, page);
+        }
+        A8_COMMIT();
+    };
+    for (int i = 0; i < A8_STAGES - 1; ++i) request_next(i);
+    int stage = 0;
+    for (int i = 0; i < n; ++i) {
+        A8_WAIT_STAGE();
+        __syncwarp();
+        request_next(stage == 0 ? A8_STAGES - 1 : stage - 1);
+        w.tile(t_lo + i, stage);
+        __syncwarp();
+        stage = stage + 1 == A8_STAGES ? 0 : stage + 1;
+    }
+    if (!fits) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k) w.l[k][0] = w.l[k][1] = NAN;      // more keys than the table holds
+    }
+    if (a.nsplit > 1)
+        w.leave((((size_t)blockIdx.z * a.num_kv_heads + head) * a.row_tiles + rt) * a.nsplit + part);
+    else
+        w.write();
+}
+
+// ---- segments put together, in order --------------------------------------------------------------------
+// A warp a row; a lane has two of every 64 dimensions.
+template <typename T>
+__device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, int stride_rows, int row, int head, T* dst, bool bad) {
+    const int lane = threadIdx.x & 31;
+    constexpr int PER = (A8_HD + 63) / 64;
+    float2 o[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) o[k] = make_float2(0.f, 0.f);
+    float M = -INFINITY, L = 0.f;
+    for (int at = 0; at < n; at += 32) {
+        const int cnt = min(32, n - at);
+        const float2 ml = lane < cnt ? a.part_ml[(place + at + lane) * stride_rows + row] : make_float2(-INFINITY, 0.f);
+        const float most = fmaxf(M, rv_warp_max(ml.x));
+        if (most == -INFINITY) {
+            L += rv_warp_sum(ml.y);                                   // zeros, or what is not a number
+            continue;
+        }
+        const float keep = a8_exp2(M - most), w = a8_exp2(ml.x - most);
+        L = L * keep + rv_warp_sum(ml.y * w);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            o[k].x *= keep;
+            o[k].y *= keep;
+        }
+        for (int i = 0; i < cnt; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* src = a.part_o + ((place + at + i) * stride_rows + row) * A8_HD;
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (64 * k + 2 * lane < A8_HD) {
+                    const float2 v = *(const float2*)(src + 64 * k + 2 * lane);
+                    o[k].x = fmaf(v.x, wi, o[k].x);
+                    o[k].y = fmaf(v.y, wi, o[k].y);
+                }
+        }
+        M = most;
+    }
+    if (a.sinks && L != 0.f) L += a8_exp2(a.sinks[head] * 1.4426950408889634f - M);
+    const float by = bad ? NAN : L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (64 * k + 2 * lane < A8_HD) {
+            rv_store(dst + 64 * k + 2 * lane, bad ? NAN : o[k].x * by);
+            rv_store(dst + 64 * k + 2 * lane + 1, bad ? NAN : o[k].y * by);
+        }
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(128) attention_8bit_stream_merge_kernel(const __grid_constant__ A8Args a, int runs) {
+    rv_pdl_prologue();
+    const int G = a.num_heads / a.num_kv_heads, per_head = (G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
+    const int r = blockIdx.y, head = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (head >= a.num_heads) return;
+    const int kvh = head / G, in = head - kvh * G, u = kvh * per_head + in / (8 * NT);
+    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size, runs);
+    const int clen = sh.length(r), tiles = sh.tiles(clen);
+    int run0 = 0, n = 0;
+    if (tiles) {
+        const long long start = sh.before(r) * units + (long long)u * tiles;
+        run0 = sh.run_of(start);
+        n = sh.run_of(start + tiles - 1) - run0 + 1;
+    }
+    a8_merge<T>(a, (size_t)run0 + (size_t)r * units + u, n, 8 * NT, in % (8 * NT), head,
+                (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(128) attention_8bit_rows_merge_kernel(const __grid_constant__ A8Args a) {
+    rv_pdl_prologue();
+    const int G = a.num_heads / a.num_kv_heads, r = a.first_req + blockIdx.z, kvh = blockIdx.y;
+    const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs;
+    const int tiles = (qlen * G + 8 * NT - 1) / (8 * NT);
+    const int i = blockIdx.x * 4 + (threadIdx.x >> 5);                 // the row
+    if (i >= qlen * G) return;
+    const int rt = tiles - 1 - i / (8 * NT), tok = i / G, head = kvh * G + i - tok * G;
+    if (rt >= a.row_tiles) return;                                     // a longer portion than the launch was told of
+    a8_merge<T>(a, (((size_t)blockIdx.z * a.num_kv_heads + kvh) * a.row_tiles + rt) * a.nsplit, a.nsplit, 8 * NT,
+                i % (8 * NT), head, (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD, false);
+}
+
+// ---- host side ----------------------------------------------------------------------------------------
+static thread_local char g_a8_error[512] = "";
+#define A8_FAIL(...) do { snprintf(g_a8_error, sizeof(g_a8_error), __VA_ARGS__); return 1; } while (0)
+#define A8_CAT2(x, y) x##y
+#define A8_CAT(x, y) A8_CAT2(x, y)
+#define A8_SYM(name) A8_CAT(A8_CAT(name, _hd), RV_HD)
+
+extern "C" const char* A8_SYM(rv_attention_8bit_last_error)() { return g_a8_error; }
+
+// Rows of a warp: 16 where a key/value head has more than 8 of them and the accumulators fit the registers.
+static int a8_nt(int rows) { return rows > 8 && A8_HD <= 128 ? 2 : 1; }
+static long long a8_place_bytes(int nt) { return 8ll * nt * (A8_HD * 4 + 8); }
+
+// How many warps share the tiles of 8 NT rows of a portion: until there are warps for every place of the GPU, four
+// tiles each at least.
+static int a8_nsplit(long long warps, int max_ctx_len, int window, int max_q_len, int n_sms) {
+    const long long places = 8ll * n_sms;
+    long long keys = max_ctx_len;
+    if (window > 0 && (long long)window + max_q_len < keys) keys = (long long)window + max_q_len;
+    const long long most = (keys + A8_KEYS - 1) / A8_KEYS / 4;
+    long long n = warps > 0 ? places / warps : 1;
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+static long long a8_rows_places(int n_reqs, int max_q_len, int max_ctx_len, int num_heads, int num_kv_heads, int window, int n_sms,
+                                int* nsplit, int* row_tiles) {
+    const int G = num_heads / num_kv_heads;
+    const long long rows = (long long)max_q_len * G;
+    const int nt = a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows);
+    *row_tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+    const long long warps = (long long)*row_tiles * num_kv_heads * n_reqs;
+    *nsplit = a8_nsplit(warps, max_ctx_len, window, max_q_len, n_sms);
+    return *nsplit > 1 ? warps * *nsplit : 0;
+}
+
+// Scratch for a call: requests [0, n_decode) with one token, [n_decode, n_reqs) with up to max_q_len.
+extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode, int n_reqs, int max_q_len, int max_ctx_len,
+                                                                   int num_heads, int num_kv_heads, int window, int n_sms) {
+    const int G = num_heads / num_kv_heads;
+    long long need = 0;
+    if (n_decode > 0) {
+        const int nt = a8_nt(G);
+        const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
+        need = ((long long)n_sms * A8_STREAM_WARPS + n_decode * units) * a8_place_bytes(nt);
+    }
+    if (n_reqs > n_decode) {
+        int nsplit, row_tiles;
+        const long long rows = (long long)max_q_len * G;
+        const long long b = a8_rows_places(n_reqs - n_decode, max_q_len, max_ctx_len, num_heads, num_kv_heads, window, n_sms,
+                                           &nsplit, &row_tiles) * a8_place_bytes(a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows));
+        if (b > need) need = b;
+    }
+    return need;
+}
+
+// The limit of shared memory is a kernel's on a device: raised once on each.
+#define A8_CONFIGURE(kernel, smem)                                                                              \
+    do {                                                                                                        \
+        static bool done[64];                                                                                   \
+        int dev = 0;                                                                                            \
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) A8_FAIL("paged_attention_8bit: no device"); \
+        if (!done[dev]) {                                                                                       \
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem)); \
+            if (e != cudaSuccess) A8_FAIL("paged_attention_8bit: %s", cudaGetErrorString(e));                   \
+            done[dev] = true;                                                                                   \
+        }                                                                                                       \
+    } while (0)
+
+template <typename T, int NT, int PARTS>
+static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
+    const size_t smem = (size_t)A8_STREAM_WARPS * A8_WARP_BYTES;
+    auto kernel = attention_8bit_stream_kernel<T, NT, PARTS>;
+    A8_CONFIGURE(kernel, smem);
+    const int G = a.num_heads / a.num_kv_heads;
+    const long long places = (long long)n_sms * A8_STREAM_WARPS +
+                             (long long)a.n_reqs * a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT));
+    a.part_ml = (float2*)(a.part_o + places * 8 * NT * A8_HD);
+    rv_launch(kernel, dim3(n_sms), dim3(A8_STREAM_WARPS * 32), smem, stream, a);
+    rv_launch(attention_8bit_stream_merge_kernel<T, NT>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a,
+              n_sms * A8_STREAM_WARPS);
+    return 0;
+}
+template <typename T, int NT, int PARTS>
+static int a8_rows(A8Args a, int max_q_len, cudaStream_t stream) {
+    const size_t smem = (size_t)A8_ROWS_WARPS * A8_WARP_BYTES;
+    auto kernel = attention_8bit_rows_kernel<T, NT, PARTS>;
+    A8_CONFIGURE(kernel, smem);
+    a.part_ml = (float2*)(a.part_o + (long long)a.row_tiles * a.num_kv_heads * a.n_reqs * a.nsplit * 8 * NT * A8_HD);
+    const long long warps = (long long)a.row_tiles * a.nsplit;
+    rv_launch(kernel,
+              dim3((unsigned)((warps + A8_ROWS_WARPS - 1) / A8_ROWS_WARPS), a.num_kv_heads, a.n_reqs), dim3(A8_ROWS_WARPS * 32), smem,
+              stream, a);
+    if (a.nsplit > 1) {
+        const long long rows = (long long)max_q_len * (a.num_heads / a.num_kv_heads);
+        rv_launch(attention_8bit_rows_merge_kernel<T, NT>, dim3((unsigned)((rows + 3) / 4), a.num_kv_heads, a.n_reqs), dim3(128), 0,
+                  stream, a);
+    }
+    return 0;
+}
+
+// Requests [0, n_decode) bring one token each, [n_decode, n_reqs) up to max_q_len; `portions` 0: the former only.
+extern "C" int A8_SYM(rv_paged_attention_8bit)(
+    const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
+    const float* v_scale, long long pages, const int* block_table, int max_blocks, const int* q_start, const int* ctx_lens,
+    void* out, void* scratch, long long scratch_bytes, int n_decode, int n_reqs, int portions, int max_q_len, int max_ctx_len,
+    int num_heads, int num_kv_heads, int page_size, float scale, int window, const float* sinks, int n_sms, void* stream) {
+    if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
+        A8_FAIL("paged_attention_8bit: invalid head counts: %d query, %d KV", num_heads, num_kv_heads);
+    if (n_decode < 0 || n_reqs < n_decode || max_q_len < 0 || max_ctx_len < 0 || max_blocks < 0 || page_size <= 0 || window < 0 ||
+        n_sms <= 0 || pages < 0)
+        A8_FAIL("paged_attention_8bit: bad sizes");
+    if (n_reqs > 65535 || num_kv_heads > 65535) A8_FAIL("paged_attention_8bit: too many requests or heads");
+    if (pages * num_kv_heads * page_size >= 0xffffffffll) A8_FAIL("paged_attention_8bit: more rows than 32 bits count");
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) A8_FAIL("paged_attention_8bit: pages must be 16-byte aligned");
+    const long long need = A8_SYM(rv_paged_attention_8bit_scratch_bytes)(n_decode, portions ? n_reqs : n_decode, max_q_len,
+                                                                       max_ctx_len, num_heads, num_kv_heads, window, n_sms);
+    if (need > scratch_bytes) A8_FAIL("paged_attention_8bit: scratch too small");
+    const int G = num_heads / num_kv_heads;
+    A8Args a = {q, (const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens, sinks,
+                out, (float*)scratch, nullptr, q_stride, pages, max_blocks, 0, n_decode, num_heads, num_kv_heads, page_size,
+                window, 1, 0, 0, scale * 1.4426950408889634f};
+    a.vec = (uintptr_t)q % 16 == 0 && q_stride * (dtype == RV_DTYPE_F32 ? 4 : 2) % 16 == 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) A8_FAIL("paged_attention_8bit: unknown dtype code %d", dtype);
+    if (n_decode > 0) {
+        const int nt = a8_nt(G);
+        int rc;
+        if (dtype == RV_DTYPE_BF16)
+            rc = nt == 1 ? a8_stream<__nv_bfloat16, 1, 1>(a, n_sms, s) : a8_stream<__nv_bfloat16, A8_HD <= 128 ? 2 : 1, 1>(a, n_sms, s);
+        else
+            rc = nt == 1 ? a8_stream<float, 1, 2>(a, n_sms, s) : a8_stream<float, A8_HD <= 128 ? 2 : 1, 2>(a, n_sms, s);
+        if (rc) return rc;
+    }
+    if (portions && n_reqs > n_decode && max_q_len > 0) {
+        a.first_req = n_decode;
+        a.n_reqs = n_reqs - n_decode;
+        const long long rows = (long long)max_q_len * G;
+        if (rows > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
+        const int nt = a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows);
+        a8_rows_places(a.n_reqs, max_q_len, max_ctx_len, num_heads, num_kv_heads, window, n_sms, &a.nsplit, &a.row_tiles);
+        int rc;
+        if (dtype == RV_DTYPE_BF16)
+            rc = nt == 1 ? a8_rows<__nv_bfloat16, 1, 1>(a, max_q_len, s)
+                         : a8_rows<__nv_bfloat16, A8_HD <= 128 ? 2 : 1, 1>(a, max_q_len, s);
+        else
+            rc = nt == 1 ? a8_rows<float, 1, 2>(a, max_q_len, s) : a8_rows<float, A8_HD <= 128 ? 2 : 1, 2>(a, max_q_len, s);
+        if (rc) return rc;
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) A8_FAIL("paged_attention_8bit: %s", cudaGetErrorString(e));
+    return 0;
+}

@@ -1,0 +1,361 @@
+// Keys and values in 8 bits: the write of a step's rows into the paged cache, and pages read back.
+//
+// A page holds int8 [kv heads][page size][head size], and each (page, head) one float32 scale s, a power of two:
+// the value that q stands for is q * s.  s = 2^e for the smallest e in [-60, 60] with max |x| <= 127 * 2^e over the
+// block's finite values; q = rint(x / s), clamped to [-127, 127]; NaN becomes 0, an infinity +-127.  Powers of
+// two: then q * s is a bfloat16 exactly (what the tensor cores are fed carries no second rounding), x / s is exact, and a block
+// whose scale has to grow loses at most the bits that the larger scale drops.  A finer scale, max |x| / 127, would halve
+// a block's rounding error at best (a quarter on average) and lose the three.
+//
+// A page is filled from its first slot on.  A call that writes slot 0 begins the page anew: its scale comes from
+// the call's rows alone, whatever an earlier holder of the page left.  Otherwise the scale is the larger
+// of the old one and what the rows need, and where it grew the other slots become rint(q * old / new).
+// A page's tokens stand together in the call (nothing but tokens without a slot between them).
+//
+// One kernel: warps for the query heads (a warp has 32 / (head size / 16) heads of a token) and warps
+// for the key/value heads.  The latter take a range of tokens and one key or value head, find where pages begin in
+// the range and take such a run of tokens whole: the rows' largest value, then the scale, then the rows.  A
+// lane has 8 dimensions of a head's first half and the 8 that they turn with.
+#include "common.cuh"
+
+#define C8_MAX_HEAD 256
+#define C8_WARPS 4
+
+struct C8Write {
+    const void* rows;                  // [tokens][heads q | kv heads k | kv heads v], `row_stride` elements apart
+    void* q_out;                       // [tokens][heads * head size]
+    const float *q_weight, *k_weight, *cos_table, *sin_table;
+    const int *positions, *slots;
+    signed char *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    long long row_stride, total_slots, table_rows;
+    float eps;
+    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, range, aligned;
+    long long q_warps;
+};
+
+__device__ __forceinline__ void c8_load8(const float* p, bool vec, float (&v)[8]) {
+    if (vec) {
+        const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[i];
+    }
+}
+__device__ __forceinline__ void c8_load8(const __nv_bfloat16* p, bool vec, float (&v)[8]) {
+    if (vec) {
+        const uint4 raw = *(const uint4*)p;
+        const __nv_bfloat162* h = (const __nv_bfloat162*)&raw;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __bfloat1622float2(h[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __bfloat162float(p[i]);
+    }
+}
+__device__ __forceinline__ void c8_store8(float* p, bool vec, const float (&v)[8]) {
+    if (vec) {
+        *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = v[i];
+    }
+}
+__device__ __forceinline__ void c8_store8(__nv_bfloat16* p, bool vec, const float (&v)[8]) {
+    if (vec) {
+        uint4 raw;
+        __nv_bfloat162* h = (__nv_bfloat162*)&raw;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        *(uint4*)p = raw;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+
+// The smallest e in [-60, 60] with most <= 127 * 2^e (127 = 1.984375 * 2^6), most >= 0 and finite.
+__device__ __forceinline__ int c8_exponent(float most) {
+    const unsigned b = __float_as_uint(most);
+    const int e = (int)((b + (0x7fffffu - 0x7e0000u)) >> 23) - 127 - 6;
+    return max(-60, min(60, e));
+}
+__device__ __forceinline__ float c8_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// One head of one token: norm and rotation in float32.  `lane0`: the first of the `lph` lanes that have the head.
+template <typename T>
+__device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const float* w, bool turn, int t, bool live, int d0,
+                                        int lane0, int lph, float (&x)[8], float (&y)[8]) {
+    const int half = a.head_dim >> 1;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+    if (live) {
+        c8_load8(src + d0, a.aligned, x);
+        c8_load8(src + half + d0, a.aligned, y);
+    }
+    if (w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+        if ((lph & (lph - 1)) == 0) {
+            for (int o = lph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        } else {
+            float sum = 0.f;
+            for (int k = 0; k < lph; ++k) sum += __shfl_sync(0xffffffffu, ss, (lane0 + k) & 31);
+            ss = sum;
+        }
+        const float rms = sqrtf(ss / (float)a.head_dim + a.eps);
+        if (live) {
+            float wx[8], wy[8];
+            c8_load8(w + d0, a.aligned, wx);
+            c8_load8(w + half + d0, a.aligned, wy);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = x[i] / rms * wx[i];
+                y[i] = y[i] / rms * wy[i];
+            }
+        }
+    }
+    if (turn && live) {
+        const long long p = a.positions[t];
+        float c[8], s[8];
+        if (p >= 0 && p < a.table_rows) {
+            c8_load8(a.cos_table + p * half + d0, a.aligned, c);
+            c8_load8(a.sin_table + p * half + d0, a.aligned, s);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float xr = x[i] * c[i] - y[i] * s[i];
+                y[i] = x[i] * s[i] + y[i] * c[i];
+                x[i] = xr;
+            }
+        } else {                                               // no angle: shows in what is read later
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = y[i] = NAN;
+        }
+    }
+}
+
+__device__ __forceinline__ float c8_most(const float (&x)[8], float most) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = fabsf(x[i]);
+        if (v <= 3.402823466e38f) most = fmaxf(most, v);       // finite ones
+    }
+    return most;
+}
+__device__ __forceinline__ uint2 c8_pack(const float (&x)[8], float inv) {
+    unsigned u[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int q = max(-127, min(127, __float2int_rn(x[i] * inv)));     // NaN: 0
+        u[i >> 2] |= (unsigned)(q & 0xff) << (8 * (i & 3));
+    }
+    return make_uint2(u[0], u[1]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
+    rv_pdl_prologue();
+    const long long id = (long long)blockIdx.x * C8_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int lph = a.head_dim >> 4, per = 32 / lph;           // lanes a head, heads a warp
+    const int sub = lane / lph, d0 = (lane - sub * lph) * 8, lane0 = sub * lph;
+    const int half = a.head_dim >> 1;
+    float x[8], y[8];
+    if (id < a.q_warps) {
+        // ---- query heads --------------------------------------------------------------------
+        const int groups = (a.num_heads + per - 1) / per;
+        const int t = (int)(id / groups), h = (int)(id - (long long)t * groups) * per + sub;
+        const bool live = sub < per && h < a.num_heads;
+        c8_head(a, (const T*)a.rows + (size_t)t * a.row_stride + (size_t)(live ? h : 0) * a.head_dim, a.q_weight,
+                a.cos_table != nullptr, t, live, d0, lane0, lph, x, y);
+        if (!live) return;
+        T* dst = (T*)a.q_out + ((size_t)t * a.num_heads + h) * a.head_dim;
+        c8_store8(dst + d0, a.aligned, x);
+        c8_store8(dst + half + d0, a.aligned, y);
+        return;
+    }
+    // ---- one key or value head of the pages that begin within a range of tokens ---------------
+    const int pairs = 2 * a.num_kv_heads;
+    const long long kv = id - a.q_warps;
+    const int first = (int)(kv / pairs) * a.range, pair = (int)(kv % pairs);
+    if (first >= a.n_tokens) return;
+    const bool is_k = pair < a.num_kv_heads;
+    const int g = is_k ? pair : pair - a.num_kv_heads;
+    const T* src = (const T*)a.rows + (size_t)(a.num_heads + pair) * a.head_dim;
+    const float* w = is_k ? a.k_weight : nullptr;
+    const bool turn = is_k && a.cos_table != nullptr;
+    signed char* cache = is_k ? a.k_cache : a.v_cache;
+    float* scales = is_k ? a.k_scale : a.v_scale;
+    auto slot_of = [&](int t) {
+        const int s = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
+        return s >= 0 && s < a.total_slots ? s : -1;
+    };
+    const int mine = lane < a.range ? slot_of(first + lane) : -1;
+    const int my_page = mine >= 0 ? mine / a.page_size : -1;
+    // the page of the last token with a slot before the range
+    int before = -1;
+    for (int at = first - 1; at >= 0; at -= 32) {
+        const int s = slot_of(at - lane);
+        const unsigned have = __ballot_sync(0xffffffffu, s >= 0);
+        if (have) {
+            before = __shfl_sync(0xffffffffu, s, __ffs(have) - 1) / a.page_size;
+            break;
+        }
+    }
+    unsigned real = __ballot_sync(0xffffffffu, mine >= 0);
+    while (real) {
+        const int l = __ffs(real) - 1;
+        real &= real - 1;
+        const int page = __shfl_sync(0xffffffffu, my_page, l);
+        const bool begins = page != before;
+        before = page;
+        if (!begins) continue;
+        // the run: tokens [t0, t1), all with a slot of this page or with none
+        const int t0 = first + l;
+        int t1 = t0, lowest = a.page_size;
+        for (bool more = true; more;) {
+            const int s = slot_of(t1 + lane);
+            const bool here = s >= 0 && s / a.page_size == page;
+            const bool ends = (s >= 0 && !here) || t1 + lane >= a.n_tokens;
+            const unsigned stop = __ballot_sync(0xffffffffu, ends);
+            const int n = stop ? __ffs(stop) - 1 : 32;
+            lowest = min(lowest, (int)__reduce_min_sync(0xffffffffu, here && lane < n ? s - page * a.page_size : a.page_size));
+            t1 += n;
+            more = n == 32;
+        }
+        float most = 0.f;
+        for (int t = t0; t < t1; t += per) {
+            const int tt = t + sub;
+            const bool live = sub < per && tt < t1 && slot_of(tt) >= 0;
+            c8_head(a, src + (size_t)(live ? tt : t0) * a.row_stride, w, turn, tt, live, d0, lane0, lph, x, y);
+            most = c8_most(y, c8_most(x, most));
+        }
+        most = rv_warp_max(most);
+        const size_t block = (size_t)page * a.num_kv_heads + g;
+        signed char* held = cache + block * a.page_size * a.head_dim;
+        float s = c8_pow2(c8_exponent(most));
+        if (lowest > 0) {
+            const float old = scales[block];
+            s = fmaxf(old, s);
+            if (s != old) {                                     // the other slots follow the larger scale
+                const float ratio = old / s;
+                for (int i = lane * 16; i < a.page_size * a.head_dim; i += 512) {
+                    int4 v = *(const int4*)(held + i);
+                    signed char* b = (signed char*)&v;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) b[k] = (signed char)__float2int_rn((float)b[k] * ratio);
+                    *(int4*)(held + i) = v;
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) scales[block] = s;
+        const float inv = 1.f / s;
+        for (int t = t0; t < t1; t += per) {
+            const int tt = t + sub;
+            const int slot = sub < per && tt < t1 ? slot_of(tt) : -1;
+            const bool live = slot >= 0;
+            c8_head(a, src + (size_t)(live ? tt : t0) * a.row_stride, w, turn, tt, live, d0, lane0, lph, x, y);
+            // (of two tokens with one slot the later one is written)
+            bool later = false;
+            for (int k = 1; k < per; ++k) {
+                const int other = __shfl_sync(0xffffffffu, slot, ((sub + k) * lph) & 31);
+                later |= sub + k < per && other == slot;
+            }
+            if (live && !later) {
+                signed char* dst = held + (size_t)(slot - page * a.page_size) * a.head_dim;
+                *(uint2*)(dst + d0) = c8_pack(x, inv);
+                *(uint2*)(dst + half + d0) = c8_pack(y, inv);
+            }
+            __syncwarp();
+        }
+    }
+}
+
+extern "C" int rv_qk_norm_rope_write_8bit(const void* rows, int dtype, long long row_stride, int n_tokens, int num_heads,
+                                          int num_kv_heads, int head_dim, const float* q_weight, const float* k_weight,
+                                          float eps, const float* cos_table, const float* sin_table, long long table_rows,
+                                          const int* positions, const int* slots, void* q_out, void* k_cache, void* v_cache,
+                                          float* k_scale, float* v_scale, long long pages, int page_size, void* stream) {
+    if (n_tokens == 0) return 0;
+    if (n_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || pages < 0)
+        RV_FAIL("qk_norm_rope_write_8bit: bad sizes");
+    if (head_dim <= 0 || head_dim % 16 || head_dim > C8_MAX_HEAD)
+        RV_FAIL("qk_norm_rope_write_8bit: head size %d is not supported (a multiple of 16, at most %d)", head_dim, C8_MAX_HEAD);
+    if (pages * page_size > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: more slots than int32 counts");
+    if ((cos_table == nullptr) != (sin_table == nullptr) || (cos_table && !positions))
+        RV_FAIL("qk_norm_rope_write_8bit: incomplete rotation table arguments");
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) RV_FAIL("qk_norm_rope_write_8bit: pages must be 16-byte aligned");
+    C8Write a = {rows, q_out, q_weight, k_weight, cos_table, sin_table, positions, slots, (signed char*)k_cache,
+                 (signed char*)v_cache, k_scale, v_scale, row_stride, pages * page_size, table_rows, eps, n_tokens,
+                 num_heads, num_kv_heads, head_dim, page_size, 1, 0, 0};
+    const int size = dtype == RV_DTYPE_F32 ? 4 : 2, per = 32 / (head_dim >> 4);
+    a.aligned = ((uintptr_t)rows | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
+                 (uintptr_t)sin_table) % 16 == 0 && row_stride * size % 16 == 0;
+    a.q_warps = (long long)n_tokens * ((num_heads + per - 1) / per);
+    // tokens whose pages a warp looks after
+    const int sms = rv_sm_count();
+    a.range = n_tokens <= 2 * sms ? 1 : (n_tokens <= 8 * sms ? 4 : 16);
+    const long long kv_warps = (long long)((n_tokens + a.range - 1) / a.range) * 2 * num_kv_heads;
+    const long long blocks = (a.q_warps + kv_warps + C8_WARPS - 1) / C8_WARPS;
+    if (blocks > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: too many rows");
+    RV_DISPATCH_DTYPE(dtype, "qk_norm_rope_write_8bit",
+                      (rv_launch(qk_norm_rope_write_8bit_kernel<T>, dim3((int)blocks), dim3(C8_WARPS * 32), 0,
+                                 (cudaStream_t)stream, a)));
+    RV_CHECK_LAUNCH("qk_norm_rope_write_8bit");
+    return 0;
+}
+
+// ---- pages read back ----------------------------------------------------------------------------
+// Page `ids[i]` as values.  A thread has 16 of them.  An id that is no page gives zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) read_8bit_kernel(const signed char* __restrict__ cache, const float* __restrict__ scales,
+                                                        const int* __restrict__ ids, T* __restrict__ out, long long total,
+                                                        int heads, int head_bytes, long long pages) {
+    rv_pdl_prologue();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 16;
+    if (i >= total) return;
+    const long long block = i / head_bytes, n = block / heads;
+    const int page = ids[n];
+    T* dst = out + i;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = 0.f;
+    if (page >= 0 && page < pages) {
+        const long long from = (long long)page * heads + (block - n * heads);
+        const float s = scales[from];
+        const int4 raw = *(const int4*)(cache + from * head_bytes + (i - block * head_bytes));
+        const signed char* b = (const signed char*)&raw;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = (float)b[k] * s;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; k += 8) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = v[k + j];
+        c8_store8(dst + k, true, w);
+    }
+}
+
+extern "C" int rv_read_8bit(const void* cache, const float* scales, const int* ids, void* out, int dtype, int n, int heads,
+                            int page_size, int head_dim, long long pages, void* stream) {
+    if (n == 0) return 0;
+    if (n < 0 || heads <= 0 || page_size <= 0 || head_dim <= 0 || head_dim % 16) RV_FAIL("read_8bit: bad sizes");
+    if (((uintptr_t)cache | (uintptr_t)out) % 16) RV_FAIL("read_8bit: pages must be 16-byte aligned");
+    const long long head_bytes = (long long)page_size * head_dim, total = (long long)n * heads * head_bytes;
+    const long long blocks = (total / 16 + 255) / 256;
+    if (blocks > 0x7fffffffLL || head_bytes > 0x7fffffffLL) RV_FAIL("read_8bit: too many pages");
+    RV_DISPATCH_DTYPE(dtype, "read_8bit",
+                      (rv_launch(read_8bit_kernel<T>, dim3((int)blocks), dim3(256), 0, (cudaStream_t)stream,
+                                 (const signed char*)cache, scales, ids, (T*)out, total, heads, (int)head_bytes, pages)));
+    RV_CHECK_LAUNCH("read_8bit");
+    return 0;
+}

@@ -827,6 +827,168 @@ class CudaOps:
             c_int(num_heads), c_int(num_kv_heads), c_int(head_dim), c_int(group.page_size),
             c_float(scale), c_int(window if window else 0), self._stream()), "paged_attention")
 
+    # ---- keys and values in 8 bits ------------------------------------------------------
+
+    @staticmethod
+    def _need_here(what, *tensors):
+        """Every tensor on the device whose stream the kernels are launched on."""
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
+                raise KernelError(f"{what}: a tensor is on {t.device}, not on the current CUDA device")
+
+    def _need_pages_8bit(self, what, cache, scale, num_kv_heads=None, head_dim=None):
+        self._need(cache, "8-bit pages", torch.int8)
+        self._need(scale, "scales", torch.float32)
+        if cache.dim() != 4 or scale.shape != cache.shape[:2]:
+            raise KernelError(f"{what}: pages are [pages, kv heads, page size, head size], scales [pages, kv heads]")
+        if head_dim is not None and (cache.shape[1] != num_kv_heads or cache.shape[3] != head_dim):
+            raise KernelError(f"{what}: pages of {cache.shape[1]} heads of {cache.shape[3]}, "
+                              f"asked for {num_kv_heads} of {head_dim}")
+        if cache.shape[3] % 16 or not 16 <= cache.shape[3] <= 256:
+            raise KernelError(f"{what}: head size {cache.shape[3]} is not supported (a multiple of 16, at most 256)")
+
+    @staticmethod
+    def _need_rows(what, rows, width=None):
+        """[tokens, width or more] whose values of a token lie side by side."""
+        if rows.dim() != 2 or (width is not None and rows.shape[1] < width):
+            raise KernelError(f"{what}: rows and head counts disagree")
+        if rows.shape[1] > 1 and rows.stride(1) != 1 or rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
+            raise KernelError(f"{what}: the values of a row must lie side by side")
+
+    def _need_index(self, what, t, n):
+        self._need(t, what, torch.int32)
+        if t.dim() != 1 or t.shape[0] < n:
+            raise KernelError(f"{what}: {n} int32 wanted, got {tuple(t.shape)}")
+
+    def qk_norm_rope_write_8bit(self, qkv, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps,
+                                table, positions, slot_mapping, q_out, k_cache, v_cache, k_scale, v_scale):
+        """`qk_norm_rope_write` into pages of 8 bits: the query heads of `qkv` [tokens, (heads + 2 kv heads) *
+        head_dim or more] (any stride between rows) are normed, rotated and written to `q_out` [tokens, heads *
+        head_dim]; keys (normed and rotated) and values go to `k_cache` and `v_cache`, int8 [pages, kv heads,
+        page size, head_dim], at `slot_mapping` int32 [tokens] (page * page size + slot; negative: nowhere), with
+        `k_scale` and `v_scale` float32 [pages, kv heads].
+
+        A page's values are q * scale, scale a power of two between 2^-60 and 2^60, the smallest with which the block's
+        largest value is 127 or less.  NaN is held as 0, infinities and what 127 * 2^60 does not reach as
+        the largest value.  Writing slot 0 begins a page anew; otherwise the scale only grows, and the page's other
+        slots follow it.  The tokens of one page stand together in the call (tokens without a slot may
+        stand between them), and each slot comes once (of several tokens for one slot the last is kept)."""
+        what = "qk_norm_rope_write_8bit"
+        _code(qkv.dtype)
+        self._need_here(what, qkv, q_weight, k_weight, positions, slot_mapping, q_out, k_cache, v_cache,
+                        k_scale, v_scale, *(table or ()))
+        if num_heads <= 0 or num_kv_heads <= 0:
+            raise KernelError(f"{what}: invalid head counts: {num_heads} query, {num_kv_heads} KV")
+        self._need_rows(what, qkv, (num_heads + 2 * num_kv_heads) * head_dim)
+        n = qkv.shape[0]
+        self._need(q_out, "query rows", qkv.dtype)
+        if q_out.shape != (n, num_heads * head_dim):
+            raise KernelError(f"{what}: the query rows have another shape")
+        self._need_pages_8bit(what, k_cache, k_scale, num_kv_heads, head_dim)
+        self._need_pages_8bit(what, v_cache, v_scale, num_kv_heads, head_dim)
+        if k_cache.shape != v_cache.shape:
+            raise KernelError(f"{what}: key and value pages differ in shape")
+        for w in (q_weight, k_weight):
+            if w is not None:
+                self._need(w, "norm weight", torch.float32)
+                if w.shape != (head_dim,):
+                    raise KernelError(f"{what}: a norm weight has another width")
+        self._need_index("slots", slot_mapping, n)
+        cos, sin = table if table is not None else (None, None)
+        if table is not None:
+            self._need_index("positions", positions, n)
+            for t in (cos, sin):
+                self._need(t, "rotation table", torch.float32)
+                if t.shape != (cos.shape[0], head_dim // 2):
+                    raise KernelError(f"{what}: a rotation table has another width")
+        self._check(self.lib.rv_qk_norm_rope_write_8bit(
+            _ptr(qkv), c_int(_code(qkv.dtype)), c_longlong(qkv.stride(0)), c_int(n), c_int(num_heads), c_int(num_kv_heads),
+            c_int(head_dim), _ptr(q_weight), _ptr(k_weight), c_float(eps), _ptr(cos), _ptr(sin),
+            c_longlong(cos.shape[0] if cos is not None else 0), _ptr(positions), _ptr(slot_mapping), _ptr(q_out),
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), c_longlong(k_cache.shape[0]),
+            c_int(k_cache.shape[2]), self._stream()), what)
+
+    def read_8bit(self, cache, scale, pages, dtype):
+        """The pages `pages` (int32 [n]) of an 8-bit cache as values, `dtype` [n, kv heads, page size,
+        head_dim] (exact in bfloat16 too, but for scales near the ends of their range).  A number that is no page
+        gives zeros."""
+        self._need_here("read_8bit", cache, scale, pages)
+        self._need_pages_8bit("read_8bit", cache, scale)
+        self._need_index("pages", pages, 0)
+        out = torch.empty((pages.shape[0],) + cache.shape[1:], dtype=dtype, device=cache.device)
+        self._check(self.lib.rv_read_8bit(
+            _ptr(cache), _ptr(scale), _ptr(pages), _ptr(out), c_int(_code(dtype)), c_int(pages.shape[0]),
+            c_int(cache.shape[1]), c_int(cache.shape[2]), c_int(cache.shape[3]), c_longlong(cache.shape[0]),
+            self._stream()), "read_8bit")
+        return out
+
+    def _attn8_lib(self, head_dim: int):
+        """The library for attention over 8-bit pages with heads of this size, built at first use."""
+        key = ("8bit", head_dim)
+        lib = self._attn_libs.get(key)
+        if lib is None:
+            path = build_variant("attention_8bit.cu", {"RV_HD": head_dim}, f"attn8_hd{head_dim}",
+                                 verbose=self._verbose_build)
+            try:
+                lib = ctypes.CDLL(path)
+            except OSError as e:
+                raise KernelError(f"cannot load the kernel library {path}: {e}") from None
+            getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}").restype = ctypes.c_char_p
+            getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}").restype = c_longlong
+            self._attn_libs[key] = lib
+        return lib
+
+    def paged_attention_8bit(self, q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale,
+                             ctx, group, scale, window, out, sinks=None):
+        """`paged_attention` over pages of 8 bits (`qk_norm_rope_write_8bit`).  `q` [tokens, heads * head_dim or
+        more], float32 or bfloat16, any stride between rows; `out` [tokens, heads * head_dim] of its type.
+        Requests [0, ctx.n_decode) bring one token each, the others any number; the key at position j is seen from
+        position p iff j <= p and, with a window, j > p - window.  A row that sees nothing is zeros; keys whose
+        block-table entry is no page are not seen; a context longer than the table gives NaN.  Scratch is
+        allocated per call (in a captured graph: from the graph's pool)."""
+        what = "paged_attention_8bit"
+        _code(q.dtype)
+        self._need_here(what, q, k_cache, v_cache, k_scale, v_scale, out, sinks, group.block_table,
+                        ctx.q_start, ctx.ctx_lens)
+        if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+            raise KernelError(f"{what}: invalid head counts: {num_heads} query, {num_kv_heads} KV")
+        self._need_pages_8bit(what, k_cache, k_scale, num_kv_heads, head_dim)
+        self._need_pages_8bit(what, v_cache, v_scale, num_kv_heads, head_dim)
+        if k_cache.shape != v_cache.shape or k_cache.shape[2] != group.page_size:
+            raise KernelError(f"{what}: key pages, value pages and the page size disagree")
+        self._need_rows(what, q, num_heads * head_dim)
+        self._need(out, "attention output", q.dtype)
+        if out.shape != (q.shape[0], num_heads * head_dim) or q.shape[0] < ctx.n_tokens:
+            raise KernelError(f"{what}: output, rows and head counts disagree")
+        if not 0 <= ctx.n_decode <= ctx.n_reqs or ctx.n_tokens < ctx.n_decode:
+            raise KernelError(f"{what}: {ctx.n_decode} single tokens among {ctx.n_reqs} requests, {ctx.n_tokens} tokens")
+        self._need_index("context lengths", ctx.ctx_lens, ctx.n_reqs)
+        self._need_index("first tokens", ctx.q_start, ctx.n_reqs + 1)
+        self._need(group.block_table, "block table", torch.int32)
+        if group.block_table.dim() != 2 or group.block_table.shape[0] < ctx.n_reqs:
+            raise KernelError(f"{what}: a row of the block table for every request")
+        if window is not None and window < 0:
+            raise KernelError(f"{what}: a window of {window}")
+        if sinks is not None:
+            self._need(sinks, "sinks", torch.float32)
+            if sinks.shape != (num_heads,):
+                raise KernelError(f"{what}: one sink per query head")
+        lib, win = self._attn8_lib(head_dim), c_int(window if window else 0)
+        portions = ctx.n_tokens > ctx.n_decode
+        sizes = (c_int(ctx.max_q_len), c_int(ctx.max_ctx_len), c_int(num_heads), c_int(num_kv_heads))
+        need = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")(
+            c_int(ctx.n_decode), c_int(ctx.n_reqs if portions else ctx.n_decode), *sizes, win, c_int(self._sm_count))
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        rc = getattr(lib, f"rv_paged_attention_8bit_hd{head_dim}")(
+            _ptr(q), c_int(_code(q.dtype)), c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+            _ptr(v_scale), c_longlong(k_cache.shape[0]), _ptr(group.block_table), c_int(group.block_table.shape[1]),
+            _ptr(ctx.q_start), _ptr(ctx.ctx_lens), _ptr(out), _ptr(scratch), c_longlong(need), c_int(ctx.n_decode),
+            c_int(ctx.n_reqs), c_int(portions), *sizes, c_int(group.page_size), c_float(scale), win, _ptr(sinks),
+            c_int(self._sm_count), self._stream())
+        self.launches += (2 if ctx.n_decode else 0) + (1 if portions else 0)
+        if rc != 0:
+            raise KernelError(getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}")().decode())
+
     # ---- gated short convolution -----------------------------------------------------
 
     def short_conv(self, proj, filt, in_bias, conv_bias, state, ctx, out):
@@ -1729,3 +1891,28 @@ class CudaOps:
                                        c_int(logits.shape[0]), c_int(logits.shape[1]),
                                        self._stream()), "sample")
         return out
+
+    def token_logprobs(self, logits, tokens, top=0):
+        """Of every row of `logits` (float32 or bfloat16 [rows, vocabulary], any stride between rows) and its
+        token (int32 [rows]): (log probability, rank, entropy in nats, log probabilities of the `top` largest logits, their
+        ids), float32 [rows], int32 [rows], float32 [rows], float32 [rows, top], int32 [rows, top].  The rank is 1
+        plus the number of larger logits; equal logits come in the order of their ids; `top` is at most 32.
+        A token outside the vocabulary has log probability NaN and rank 0.  A NaN or an infinity among a row's logits
+        makes its probabilities NaN, as do logits that are all -inf; NaN is never among the largest (id -1 where
+        there are not enough others)."""
+        what = "token_logprobs"
+        code = _code(logits.dtype)
+        self._need_here(what, logits, tokens)
+        self._need_rows(what, logits)
+        rows, vocab = logits.shape
+        self._need_index("tokens", tokens, rows)
+        if vocab < 1 or not 0 <= top <= min(32, vocab):
+            raise KernelError(f"{what}: {top} alternatives of {vocab} (0 to 32)")
+        floats = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
+        rank = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        self._check(self.lib.rv_token_logprobs(
+            _ptr(logits), c_int(code), c_longlong(logits.stride(0)), c_int(rows), c_int(vocab), _ptr(tokens), c_int(top),
+            _ptr(floats[0]), _ptr(rank), _ptr(floats[1]), _ptr(best), _ptr(ids), self._stream()), what)
+        return floats[0], rank, floats[1], best, ids
