@@ -36,12 +36,18 @@
 #endif
 #define A8_HD RV_HD
 static_assert(A8_HD % 16 == 0 && A8_HD >= 16 && A8_HD <= 256, "head sizes");
-#define A8_KEYS (A8_HD <= 64 ? 64 : A8_HD <= 128 ? 32 : 16)       // a tile
+#define A8_KEYS 32                                                // a tile, a lane's key each
 #define A8_CHUNKS (A8_HD / 16)                                    // 16-byte pieces of a row
-#define A8_STAGES 3
-#define A8_STREAM_WARPS 8                                         // one block a multiprocessor
-#define A8_ROWS_WARPS 4                                           // two blocks
+// Warps of a multiprocessor: what the registers (16: 128 a thread, 12: 168, 8: 255) and the rings leave room for.
+template <int NT, int PARTS> constexpr int a8_warps() {
+    return A8_HD <= 64 ? (NT * PARTS == 1 ? 16 : NT * PARTS == 2 ? 12 : 8) : A8_HD <= 192 ? 8 : 6;
+}
+#define A8_MOST_WARPS 16
+#define A8_BLOCK_WARPS (A8_HD <= 192 ? 4 : 3)
 
+#ifndef A8_STAGES
+#define A8_STAGES (A8_HD <= 128 ? 3 : 2)
+#endif
 #define A8_STAGE_BYTES (2 * A8_KEYS * A8_HD + 2 * A8_KEYS * 4)
 #define A8_WARP_BYTES (A8_STAGES * A8_STAGE_BYTES)
 
@@ -55,25 +61,61 @@ struct A8Args {
     float* part_o;                     // [places][rows][HD]
     float2* part_ml;                   // [places][rows]: M, l
     long long q_stride, pages;
-    int max_blocks, first_req, n_reqs, num_heads, num_kv_heads, page_size, window, nsplit, row_tiles, vec;
+    int max_blocks, first_req, n_reqs, num_heads, num_kv_heads, page_size, page_shift, window, nsplit, row_tiles, vec;
     float scale_log2;
 };
 
 __device__ __forceinline__ unsigned a8_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void a8_copy16(unsigned dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void a8_copy16(unsigned dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void a8_copy4(unsigned dst, const void* src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void a8_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                        unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void a8_mma_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                             unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// int8 times int8 (U: times uint8), sums in int32; 32 terms, or the 16 of a0, a1, b0; `first`: of these alone.
+#define A8_IMMA(shape, kind, a_regs, b_regs, ...)                                                                          \
+    do {                                                                                                                   \
+        if (first)                                                                                                         \
+            asm("mma.sync.aligned." shape ".row.col.s32.s8." kind ".s32 {%0,%1,%2,%3}, " a_regs ", " b_regs ", {0,0,0,0};" \
+                : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : __VA_ARGS__);                                           \
+        else                                                                                                               \
+            asm("mma.sync.aligned." shape ".row.col.s32.s8." kind ".s32 {%0,%1,%2,%3}, " a_regs ", " b_regs ", {%0,%1,%2,%3};" \
+                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : __VA_ARGS__);                                           \
+    } while (0)
+template <bool U>
+__device__ __forceinline__ void a8_imma(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1,
+                                        bool first) {
+    if (U) A8_IMMA("m16n8k32", "u8", "{%4,%5,%6,%7}", "{%8,%9}", "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else A8_IMMA("m16n8k32", "s8", "{%4,%5,%6,%7}", "{%8,%9}", "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool U>
+__device__ __forceinline__ void a8_imma(int (&c)[4], unsigned a0, unsigned a1, unsigned b0, bool first) {
+    if (U) A8_IMMA("m16n8k16", "u8", "{%4,%5}", "{%6}", "r"(a0), "r"(a1), "r"(b0));
+    else A8_IMMA("m16n8k16", "s8", "{%4,%5}", "{%6}", "r"(a0), "r"(a1), "r"(b0));
 }
 __device__ __forceinline__ unsigned a8_transpose(unsigned x) {
     unsigned y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned a8_lds(unsigned at) {
+    unsigned v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float a8_max_nan(float a, float b) {       // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
 __device__ __forceinline__ float a8_exp2(float x) {              // -inf: 0
@@ -96,13 +138,11 @@ __device__ __forceinline__ unsigned a8_rest(float a, float b, unsigned packed) {
     const float2 f = __half22float2(*(const __half2*)&packed);
     return a8_pack(a - f.x, b - f.y);
 }
-// Where 16-byte piece c of a tile's row lies: moved so that what a warp reads at once is spread over the banks.
-// Values: eight rows' pieces c (ldmatrix); keys: two rows' four pieces.
-__device__ __forceinline__ int a8_vpiece(int row, int c) {
+// Where 16-byte piece c of a tile's row lies: moved so that eight rows' pieces c (ldmatrix) are spread over the banks.
+__device__ __forceinline__ int a8_piece(int row, int c) {
     constexpr int n = A8_CHUNKS;
     return n % 8 == 0 ? c ^ (row & 7) : n % 4 == 0 ? c ^ ((row >> 1) & 3) : n % 2 == 0 ? c ^ ((row >> 2) & 1) : c;
 }
-__device__ __forceinline__ int a8_kpiece(int row, int c) { return A8_CHUNKS % 8 == 0 ? c ^ ((row & 1) << 2) : c; }
 
 __device__ __forceinline__ float a8_load(const float* p) { return *p; }
 __device__ __forceinline__ float a8_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -142,29 +182,47 @@ __device__ __forceinline__ void a8_load_n(const __nv_bfloat16* p, bool vec, floa
 struct A8Shares {
     const int* ctx_lens;
     int n_reqs, units, window, most;
-    long long total;
+    long long total, before;           // tiles of all units; of a unit over the requests before the one asked for
     int used;
+    bool narrow;
+    static constexpr int KEPT = 4;
+    int kept[KEPT];                    // this lane's request's tiles of the first groups of 32 requests
     __device__ __forceinline__ int first(int clen) const { return window > 0 ? max(0, clen - window) / A8_KEYS : 0; }
     // A context that the block table cannot hold has no tiles: the merge marks its rows.
     __device__ __forceinline__ int tiles(int clen) const {
         return clen > 0 && clen <= most ? (clen - 1) / A8_KEYS - first(clen) + 1 : 0;
     }
     __device__ __forceinline__ int length(int r) const { return r < n_reqs ? ctx_lens[r] : 0; }
-    // Tiles of a unit over the requests before r (a whole warp asks).
-    __device__ __forceinline__ long long before(int r) const {
-        long long sum = 0;
+    // (a whole warp at once)
+    __device__ __forceinline__ A8Shares(const int* lens, int reqs, int u, int win, long long slots, int runs, int r)
+        : ctx_lens(lens), n_reqs(reqs), units(u), window(win), most((int)min(slots, 0x7fffffffll)), total(0), before(0) {
         const int lane = threadIdx.x & 31;
-        for (int at = 0; at < r; at += 32)
-            sum += __reduce_add_sync(0xffffffffu, (unsigned)(at + lane < r ? tiles(length(at + lane)) : 0));
-        return sum;
-    }
-    __device__ __forceinline__ A8Shares(const int* lens, int reqs, int u, int win, long long slots, int runs)
-        : ctx_lens(lens), n_reqs(reqs), units(u), window(win), most((int)min(slots, 0x7fffffffll)) {
-        total = before(reqs) * units;
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) kept[k] = 32 * k < n_reqs ? length(32 * k + lane) : 0;
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+            kept[k] = tiles(kept[k]);
+            if (32 * k < n_reqs) {
+                total += __reduce_add_sync(0xffffffffu, (unsigned)kept[k]);
+                if (32 * k < r) before += __reduce_add_sync(0xffffffffu, (unsigned)(32 * k + lane < r ? kept[k] : 0));
+            }
+        }
+        for (int at = 32 * KEPT; at < n_reqs; at += 32) {
+            const int mine = tiles(length(at + lane));
+            total += __reduce_add_sync(0xffffffffu, (unsigned)mine);
+            before += __reduce_add_sync(0xffffffffu, (unsigned)(at + lane < r ? mine : 0));
+        }
+        total *= units;
         used = (int)min((long long)runs, max(1ll, total));
+        narrow = total * (used + 1) < 0xffffffffll;
     }
-    __device__ __forceinline__ long long start(int run) const { return (long long)run * total / used; }
-    __device__ __forceinline__ int run_of(long long tile) const { return (int)(((tile + 1) * used - 1) / total); }
+    // (A division of 64 bits takes long enough to be seen.)
+    __device__ __forceinline__ long long start(int run) const {
+        return narrow ? (long long)((unsigned)run * (unsigned)total / (unsigned)used) : (long long)run * total / used;
+    }
+    __device__ __forceinline__ int run_of(long long tile) const {
+        return narrow ? (int)(((unsigned)(tile + 1) * (unsigned)used - 1u) / (unsigned)total) : (int)(((tile + 1) * used - 1) / total);
+    }
 };
 
 // ---- one warp's work ----------------------------------------------------------------------------------
@@ -176,61 +234,48 @@ struct A8Cursor {
 template <typename T, int NT, int PARTS>
 struct A8Warp {
     const A8Args& a;
-    unsigned char* ring;
+    const unsigned ring;               // in shared memory
     const int lane, g, t;
     int rows_first, rows_count, kvh, G, qs;        // of the segment: its first row, rows, head, query heads a head, first token
+    static constexpr bool WHOLE = PARTS == 1;      // queries as whole numbers of 16 bits
+    // O^T of 16 dimensions and 8 rows: dimension 2 g (even ones) of rows 2 t, 2 t + 1, then 2 g + 1 of the same
     float o[A8_CHUNKS][NT][4];
-    unsigned q[A8_CHUNKS][NT][PARTS][2];
+    unsigned q[A8_CHUNKS][NT][2];                  // WHOLE: upper and lower bytes of 4 values; else of 2 and 2, float16
+    unsigned q2[WHOLE ? 1 : A8_CHUNKS][NT][2];     // what float16 left of them
     float f[NT][2], M[NT][2], l[NT][2];
     int hi[NT][2], lo[NT][2], p_min, lo_max;
 
     __device__ __forceinline__ A8Warp(const A8Args& args, unsigned char* mem)
-        : a(args), ring(mem), lane(threadIdx.x & 31), g((threadIdx.x & 31) >> 2), t(threadIdx.x & 3) {
+        : a(args), ring(a8_smem(mem)), lane(threadIdx.x & 31), g((threadIdx.x & 31) >> 2), t(threadIdx.x & 3) {
         G = a.num_heads / a.num_kv_heads;
     }
 
-    // The pages of a tile's keys: this lane's key (and the one 32 after it).
-    __device__ __forceinline__ void pages_of(const A8Cursor& c, int (&page)[2]) const {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            page[i] = -1;
-            const int in_tile = lane + 32 * i, key = c.tile * A8_KEYS + in_tile;
-            if (in_tile < A8_KEYS && key < c.clen) {
-                const int blk = key / a.page_size;
-                if (blk < a.max_blocks) page[i] = a.block_table[(size_t)c.r * a.max_blocks + blk];
-            }
-        }
+    // The page of this lane's key of a tile (-1: none).  (page_shift: pages of 2^page_shift tokens, or -1.)
+    __device__ __forceinline__ int page_of(const A8Cursor& c) const {
+        const int key = c.tile * A8_KEYS + lane;
+        if (key >= c.clen) return -1;
+        const int blk = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+        return blk < a.max_blocks ? a.block_table[(size_t)c.r * a.max_blocks + blk] : -1;
     }
-    __device__ __forceinline__ void request(const A8Cursor& c, int head, const int (&page)[2], int stage) const {
-        unsigned char* base = ring + stage * A8_STAGE_BYTES;
-        unsigned row[2];
+    // A tile's keys and values, piece by piece, and their scales.  In the place of a key without a page comes some row,
+    // with scales of 0.
+    __device__ __forceinline__ void request(const A8Cursor& c, int head, int page, int stage) const {
+        const unsigned base = ring + stage * A8_STAGE_BYTES;
+        const int key = c.tile * A8_KEYS + lane;
+        const bool ok = page >= 0 && page < a.pages;
+        const unsigned block = ok ? (unsigned)page * (unsigned)a.num_kv_heads + (unsigned)head : 0u;
+        const int slot = a.page_shift >= 0 ? key & (a.page_size - 1) : key % a.page_size;
+        const unsigned row = ok ? block * (unsigned)a.page_size + (unsigned)slot : 0u;
+        const unsigned s = base + 2 * A8_KEYS * A8_HD + lane * 4;
+        a8_copy4(s, a.k_scale + block, ok);
+        a8_copy4(s + A8_KEYS * 4, a.v_scale + block, ok);
+        if (a.pages == 0) return;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int in_tile = lane + 32 * i, key = c.tile * A8_KEYS + in_tile;
-            const bool ok = page[i] >= 0 && page[i] < a.pages;
-            const long long block = ok ? (long long)page[i] * a.num_kv_heads + head : 0;
-            row[i] = ok ? (unsigned)(block * a.page_size + key % a.page_size) : 0xffffffffu;
-            if (in_tile < A8_KEYS) {
-                const unsigned s = a8_smem(base + 2 * A8_KEYS * A8_HD + in_tile * 4);
-                a8_copy4(s, a.k_scale + block, ok);
-                a8_copy4(s + A8_KEYS * 4, a.v_scale + block, ok);
-            }
-        }
-        const unsigned kd = a8_smem(base), vd = kd + A8_KEYS * A8_HD;
-#pragma unroll
-        for (int it = 0; it < (A8_KEYS * A8_CHUNKS + 31) / 32; ++it) {
-            const int id = it * 32 + lane, key = id / A8_CHUNKS, c16 = id - key * A8_CHUNKS;
-            unsigned from = __shfl_sync(0xffffffffu, row[0], key & 31);
-            if (A8_KEYS > 32) {
-                const unsigned second = __shfl_sync(0xffffffffu, row[1], key & 31);
-                from = key < 32 ? from : second;
-            }
-            if (id < A8_KEYS * A8_CHUNKS) {
-                const bool ok = from != 0xffffffffu;
-                const size_t at = ok ? (size_t)from * A8_HD + c16 * 16 : 0;
-                a8_copy16(kd + key * A8_HD + a8_kpiece(key, c16) * 16, a.k + at, ok);
-                a8_copy16(vd + key * A8_HD + a8_vpiece(key, c16) * 16, a.v + at, ok);
-            }
+        for (int it = 0; it < A8_CHUNKS; ++it) {                       // 32 keys: a piece a lane each
+            const int id = it * 32 + lane, k = id / A8_CHUNKS, c16 = id - k * A8_CHUNKS;
+            const size_t at = (size_t)__shfl_sync(0xffffffffu, row, k) * A8_HD + c16 * 16;
+            a8_copy16(base + k * A8_HD + a8_piece(k, c16) * 16, a.k + at);
+            a8_copy16(base + A8_KEYS * A8_HD + k * A8_HD + a8_piece(k, c16) * 16, a.v + at);
         }
     }
 
@@ -252,35 +297,43 @@ struct A8Warp {
             float most = 0.f;
             float x[A8_CHUNKS][4];
 #pragma unroll
-            for (int c = 0; c < A8_HD / 64; ++c) {
-                float w[16];
-                a8_load_n<16>(src + 64 * c + 16 * t, a.vec, w);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) x[4 * c + (k >> 2)][k & 3] = w[k];
-            }
-#pragma unroll
-            for (int c = A8_HD / 64 * 4; c < A8_CHUNKS; ++c) a8_load_n<4>(src + 16 * c + 4 * t, a.vec, x[c]);
+            for (int c = 0; c < A8_CHUNKS; ++c) a8_load_n<4>(src + 16 * c + 4 * t, a.vec, x[c]);
 #pragma unroll
             for (int c = 0; c < A8_CHUNKS; ++c)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (!real) x[c][k] = 0.f;
-                    most = fmaxf(most, fabsf(x[c][k]));
+                    most = a8_max_nan(most, fabsf(x[c][k]));
                 }
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            // 2^(8 - exponent): within what float32 holds
-            int e = 8 - ((int)(__float_as_uint(most) >> 23) - 127);
-            e = most > 0.f ? max(-100, min(100, e)) : 0;
-            const float up = __uint_as_float((unsigned)(e + 127) << 23), down = __uint_as_float((unsigned)(127 - e) << 23);
+            most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            // the largest in [2^14, 2^15), or in [2^8, 2^9)
+            int e = (WHOLE ? 14 : 8) - ((int)(__float_as_uint(most) >> 23) - 127);
+            e = most > 0.f ? max(-100, min(100, e)) : 0;                // (NaN: 0)
+            const float up = __uint_as_float((unsigned)(e + 127) << 23);
+            float down = __uint_as_float((unsigned)(127 - e) << 23);
+            if (WHOLE && !(most <= 3.402823466e38f)) down = NAN;       // whole numbers hold no infinity
 #pragma unroll
-            for (int c = 0; c < A8_CHUNKS; ++c)
+            for (int c = 0; c < A8_CHUNKS; ++c) {
+                if constexpr (WHOLE) {
+                    unsigned upper = 0u, lower = 0u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float x0 = x[c][2 * h] * up, x1 = x[c][2 * h + 1] * up;
-                    q[c][n][0][h] = a8_pack(x0, x1);
-                    if (PARTS == 2) q[c][n][PARTS - 1][h] = a8_rest(x0, x1, q[c][n][0][h]);
+                    for (int k = 0; k < 4; ++k) {
+                        const int v = min(32767, __float2int_rn(x[c][k] * up));
+                        upper |= ((unsigned)(v >> 8) & 0xffu) << (8 * k);
+                        lower |= ((unsigned)v & 0xffu) << (8 * k);
+                    }
+                    q[c][n][0] = upper;
+                    q[c][n][1] = lower;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float x0 = x[c][2 * h] * up, x1 = x[c][2 * h + 1] * up;
+                        q[c][n][h] = a8_pack(x0, x1);
+                        q2[c][n][h] = a8_rest(x0, x1, q[c][n][h]);
+                    }
                 }
+            }
             const float mine = down * a.scale_log2;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -305,49 +358,85 @@ struct A8Warp {
                 for (int k = 0; k < 4; ++k) o[c][n][k] = 0.f;
     }
 
-    __device__ __forceinline__ void tile(int tile_at, int stage) {
-        const unsigned char* base = ring + stage * A8_STAGE_BYTES;
-        const float* ks = (const float*)(base + 2 * A8_KEYS * A8_HD);
-        const float* vs = ks + A8_KEYS;
-        constexpr int MT = A8_KEYS / 16;
-        float s[MT][NT][4];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[m][n][k] = 0.f;
-        // ---- S^T = K Q^T -------------------------------------------------------------------------
-        auto step = [&](int m, int c, unsigned w0, unsigned w1) {     // 16 dimensions of 16 keys
+    // S^T of 16 keys as float32.
+    __device__ __forceinline__ void scores(unsigned base, int m, float (&s)[NT][4]) {
+        // pieces c and c + 1 of the 16 keys' rows: lanes 0-7, 8-15 name keys 0-7, 8-15 of piece c, the others of c + 1
+        const int key = 16 * m + (lane & 15);
+        int up[NT][4], low[NT][4];
+        auto half = [&](int c, unsigned w0, unsigned w1) {            // 16 dimensions, float16
             w0 ^= 0x80808080u;
             w1 ^= 0x80808080u;
             const unsigned a0 = a8_pair(w0, 0x4140), a2 = a8_pair(w0, 0x4342);
             const unsigned a1 = a8_pair(w1, 0x4140), a3 = a8_pair(w1, 0x4342);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) a8_mma(s[m][n], a0, a1, a2, a3, q[c][n][p][0], q[c][n][p][1]);
+            for (int n = 0; n < NT; ++n) {
+                if (c == 0) a8_mma_first(s[n], a0, a1, a2, a3, q[c][n][0], q[c][n][1]);
+                else a8_mma(s[n], a0, a1, a2, a3, q[c][n][0], q[c][n][1]);
+                a8_mma(s[n], a0, a1, a2, a3, q2[WHOLE ? 0 : c][n][0], q2[WHOLE ? 0 : c][n][1]);
+            }
         };
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int r0 = 16 * m + g, r1 = r0 + 8;
+        for (int c = 0; c < A8_CHUNKS; c += 2) {
+            unsigned w[4];
+            if (c + 1 < A8_CHUNKS) {
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(base + key * A8_HD + a8_piece(key, c + (lane >> 4)) * 16));
+                if constexpr (WHOLE) {
 #pragma unroll
-            for (int c = 0; c < A8_HD / 64; ++c) {
-                const uint4 x = *(const uint4*)(base + r0 * A8_HD + a8_kpiece(r0, 4 * c + t) * 16);
-                const uint4 y = *(const uint4*)(base + r1 * A8_HD + a8_kpiece(r1, 4 * c + t) * 16);
-                step(m, 4 * c, x.x, y.x);
-                step(m, 4 * c + 1, x.y, y.y);
-                step(m, 4 * c + 2, x.z, y.z);
-                step(m, 4 * c + 3, x.w, y.w);
+                    for (int n = 0; n < NT; ++n) {
+                        a8_imma<false>(up[n], w[0], w[1], w[2], w[3], q[c][n][0], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][0], c == 0);
+                        a8_imma<true>(low[n], w[0], w[1], w[2], w[3], q[c][n][1], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][1], c == 0);
+                    }
+                } else {
+                    half(c, w[0], w[1]);
+                    half(c + 1, w[2], w[3]);
+                }
+            } else {
+                asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+                             : "=r"(w[0]), "=r"(w[1]) : "r"(base + key * A8_HD + a8_piece(key, c) * 16));
+                if constexpr (WHOLE) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        a8_imma<false>(up[n], w[0], w[1], q[c][n][0], c == 0);
+                        a8_imma<true>(low[n], w[0], w[1], q[c][n][1], c == 0);
+                    }
+                } else {
+                    half(c, w[0], w[1]);
+                }
             }
-#pragma unroll
-            for (int c = A8_HD / 64 * 4; c < A8_CHUNKS; ++c)
-                step(m, c, *(const unsigned*)(base + r0 * A8_HD + a8_kpiece(r0, c) * 16 + 4 * t),
-                     *(const unsigned*)(base + r1 * A8_HD + a8_kpiece(r1, c) * 16 + 4 * t));
         }
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[n][k] = (float)(up[n][k] * 256 + low[n][k]);
+        }
+    }
+
+    // The rows' references to x, which are larger: O and l follow.
+    __device__ __forceinline__ void move(int n, int j, float x) {
+        const float corr = x == -INFINITY ? 1.f : a8_exp2(M[n][j] - x);                 // M = -inf: 0
+        M[n][j] = x;
+        l[n][j] *= corr;
+#pragma unroll
+        for (int c = 0; c < A8_CHUNKS; ++c)
+#pragma unroll
+            for (int k = j; k < 4; k += 2) o[c][n][k] *= corr;
+    }
+    __device__ __forceinline__ void tile(int tile_at, int stage) {
+        const unsigned base = ring + stage * A8_STAGE_BYTES, scales = base + 2 * A8_KEYS * A8_HD + 4 * lane;
+        constexpr int MT = A8_KEYS / 16;
+        float s[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) scores(base, m, s[m]);
         // ---- u, its largest -------------------------------------------------------------------------
         const int key0 = tile_at * A8_KEYS;
-        const bool edge = key0 + A8_KEYS - 1 > p_min || key0 < lo_max;
+        // this lane's key: its scale, log2 of its value's scale and one over that; a key without a page (its scales
+        // are zeros) weighs nothing
+        const float sk1 = __uint_as_float(a8_lds(scales));
+        const int e1 = max(-60, min(60, (int)((a8_lds(scales + 4 * A8_KEYS) >> 23) & 0xff) - 127));
+        const float inv1 = __uint_as_float((unsigned)(127 - e1) << 23), ev1 = sk1 == 0.f ? -INFINITY : (float)e1;
         float inv[MT][2], mx[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
@@ -356,26 +445,38 @@ struct A8Warp {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int key = 16 * m + 8 * h + g;
-                const float sk = ks[key], sv = vs[key];
-                // log2 of the scale; a key without a page (its scales are zeros) weighs nothing
-                const int e = max(-60, min(60, (int)((__float_as_uint(sv) >> 23) & 0xff) - 127));
-                inv[m][h] = __uint_as_float((unsigned)(127 - e) << 23);
-                const float ev = sk == 0.f ? -INFINITY : (float)e;
+                const float sk = __shfl_sync(0xffffffffu, sk1, key), ev = __shfl_sync(0xffffffffu, ev1, key);
+                inv[m][h] = __shfl_sync(0xffffffffu, inv1, key);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float u = fmaf(s[m][n][2 * h + j] * f[n][j], sk, ev);
-                        if (edge && (key0 + key > hi[n][j] || key0 + key < lo[n][j])) u = -INFINITY;
-                        s[m][n][2 * h + j] = u;
-                        mx[n][j] = fmaxf(mx[n][j], u);
-                    }
+                    for (int j = 0; j < 2; ++j) s[m][n][2 * h + j] = fmaf(s[m][n][2 * h + j] * f[n][j], sk, ev);
             }
+        if (key0 + A8_KEYS - 1 > p_min || key0 < lo_max) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int key = key0 + 16 * m + 8 * h + g;
+                            if (key > hi[n][j] || key < lo[n][j]) s[m][n][2 * h + j] = -INFINITY;
+                        }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) mx[n][j] = fmaxf(mx[n][j], fmaxf(s[m][n][j], s[m][n][2 + j]));
+        // p' is at most 2^6 when its reference is set and may grow to 2^14
         bool moves = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) moves |= mx[n][j] > M[n][j] + 14.f;          // also from -inf
+            for (int j = 0; j < 2; ++j) moves |= mx[n][j] > M[n][j] + 14.f;           // also from -inf
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -385,15 +486,7 @@ struct A8Warp {
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(x - 6.f, M[n][j]);
-                    const float corr = x == -INFINITY ? 1.f : a8_exp2(M[n][j] - x);   // M = -inf: 0
-                    M[n][j] = x;
-                    l[n][j] *= corr;
-#pragma unroll
-                    for (int c = 0; c < A8_CHUNKS; ++c) {
-                        o[c][n][j] *= corr;
-                        o[c][n][2 + j] *= corr;
-                    }
+                    move(n, j, fmaxf(x - 6.f, M[n][j]));
                 }
         }
         // ---- p', l, and O^T += V^T P^T ----------------------------------------------------------------
@@ -402,10 +495,10 @@ struct A8Warp {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) off[n][j] = M[n][j] == -INFINITY ? 0.f : M[n][j];
-        const unsigned vbase = a8_smem(base + A8_KEYS * A8_HD);
+        const unsigned vbase = base + A8_KEYS * A8_HD;
+        unsigned p[NT][MT][2], p2[NT][MT][2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            unsigned p[NT][PARTS][2];
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -414,9 +507,11 @@ struct A8Warp {
                     l[n][0] = fmaf(p0, inv[m][h], l[n][0]);
                     l[n][1] = fmaf(p1, inv[m][h], l[n][1]);
                     const unsigned w = a8_pack(p0, p1);
-                    p[n][0][h] = a8_transpose(w);
-                    if (PARTS == 2) p[n][PARTS - 1][h] = a8_transpose(a8_rest(p0, p1, w));
+                    p[n][m][h] = a8_transpose(w);
+                    if (!WHOLE) p2[n][m][h] = a8_transpose(a8_rest(p0, p1, w));
                 }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
             // pieces c and c + 1 of the 16 keys' rows: lanes 0-7, 8-15 name keys 0-7, 8-15 of piece c, the others of c + 1
             const int key = 16 * m + (lane & 15);
 #pragma unroll
@@ -425,11 +520,11 @@ struct A8Warp {
                 if (c + 1 < A8_CHUNKS) {
                     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                 : "r"(vbase + key * A8_HD + a8_vpiece(key, c + (lane >> 4)) * 16) : "memory");
+                                 : "r"(vbase + key * A8_HD + a8_piece(key, c + (lane >> 4)) * 16));
                 } else {
                     asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
                                  : "=r"(w[0]), "=r"(w[1])
-                                 : "r"(vbase + key * A8_HD + a8_vpiece(key, c) * 16) : "memory");
+                                 : "r"(vbase + key * A8_HD + a8_piece(key, c) * 16));
                     w[2] = w[3] = 0u;
                 }
 #pragma unroll
@@ -438,14 +533,14 @@ struct A8Warp {
                     const unsigned a0 = a8_pair(x, 0x4240), a1 = a8_pair(x, 0x4341);
                     const unsigned a2 = a8_pair(y, 0x4240), a3 = a8_pair(y, 0x4341);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < PARTS; ++i) a8_mma(o[c + k][n], a0, a1, a2, a3, p[n][i][0], p[n][i][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        a8_mma(o[c + k][n], a0, a1, a2, a3, p[n][m][0], p[n][m][1]);
+                        if (!WHOLE) a8_mma(o[c + k][n], a0, a1, a2, a3, p2[n][m][0], p2[n][m][1]);
+                    }
                 }
             }
         }
     }
-
     // Sums over the lanes that share a row.
     __device__ __forceinline__ void finish() {
 #pragma unroll
@@ -499,15 +594,16 @@ struct A8Warp {
 
 // Requests [0, n_reqs) with one token each.
 template <typename T, int NT, int PARTS>
-__global__ void __launch_bounds__(A8_STREAM_WARPS * 32, 1) attention_8bit_stream_kernel(const __grid_constant__ A8Args a) {
-    rv_pdl_prologue();
+__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_stream_kernel(const __grid_constant__ A8Args a) {
+    rv_pdl_wait();
+    rv_pdl_launch_dependents();        // the merge may read what was there before this launch as soon as it begins
     extern __shared__ __align__(128) unsigned char smem[];
     A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
     const int per_head = (w.G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
     // neighbours in the order of tiles on different multiprocessors
     const int run = (int)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
     const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size,
-                      gridDim.x * A8_STREAM_WARPS);
+                      gridDim.x * A8_BLOCK_WARPS, 0);
     if (run >= sh.used || sh.total == 0) return;
     const long long from = sh.start(run);
     int n = (int)(sh.start(run + 1) - from);
@@ -516,29 +612,32 @@ __global__ void __launch_bounds__(A8_STREAM_WARPS * 32, 1) attention_8bit_stream
     {
         const int lane = threadIdx.x & 31;
         long long sum = 0;
-        for (int at = 0; at < a.n_reqs; at += 32) {
-            const int mine = sh.tiles(sh.length(at + lane));
+        bool found = false;
+        auto look = [&](int at, int mine) {
             int upto = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, upto, d);
                 if (lane >= d) upto += v;
             }
-            const bool has = (sum + upto) * units > from;
-            const unsigned who = __ballot_sync(0xffffffffu, has);
+            const unsigned who = __ballot_sync(0xffffffffu, (sum + upto) * units > from);
             if (who) {
                 const int l = __ffs(who) - 1;
                 const int tiles = __shfl_sync(0xffffffffu, mine, l);
-                const long long in = from - (sum + __shfl_sync(0xffffffffu, upto, l) - tiles) * units;
+                const unsigned in = (unsigned)(from - (sum + __shfl_sync(0xffffffffu, upto, l) - tiles) * units);
                 c.r = at + l;
                 c.clen = sh.length(c.r);
-                c.u = (int)(in / tiles);
-                c.tile = sh.first(c.clen) + (int)(in - (long long)c.u * tiles);
+                c.u = (int)(in / (unsigned)tiles);
+                c.tile = sh.first(c.clen) + (int)(in - (unsigned)c.u * (unsigned)tiles);
                 c.last = (c.clen - 1) / A8_KEYS;
-                break;
+                found = true;
             }
             sum += __shfl_sync(0xffffffffu, upto, 31);
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < A8Shares::KEPT; ++k)
+            if (!found && 32 * k < a.n_reqs) look(32 * k, sh.kept[k]);
+        for (int at = 32 * A8Shares::KEPT; !found && at < a.n_reqs; at += 32) look(at, sh.tiles(sh.length(at + lane)));
     }
     auto advance = [&](A8Cursor& x) {
         if (++x.tile <= x.last) return;
@@ -552,14 +651,13 @@ __global__ void __launch_bounds__(A8_STREAM_WARPS * 32, 1) attention_8bit_stream
         x.tile = sh.first(x.clen);
     };
     A8Cursor ahead = c;
-    int page[2], requested = 0;
-    w.pages_of(ahead, page);
+    int page = w.page_of(ahead), requested = 0;
     auto request_next = [&](int stage) {
         if (requested < n) {
             w.request(ahead, ahead.u / per_head, page, stage);
             if (++requested < n) {
                 advance(ahead);
-                w.pages_of(ahead, page);
+                page = w.page_of(ahead);
             }
         }
         A8_COMMIT();
@@ -590,10 +688,10 @@ __global__ void __launch_bounds__(A8_STREAM_WARPS * 32, 1) attention_8bit_stream
 // Requests [first_req, first_req + n_reqs) with any number of tokens.  A warp: (request, key/value head, 8 NT rows,
 // part of their tiles).  blockIdx.z: request, y: head, x and warp: rows and part.
 template <typename T, int NT, int PARTS>
-__global__ void __launch_bounds__(A8_ROWS_WARPS * 32, 2) attention_8bit_rows_kernel(const __grid_constant__ A8Args a) {
+__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_rows_kernel(const __grid_constant__ A8Args a) {
     rv_pdl_prologue();
     extern __shared__ __align__(128) unsigned char smem[];
-    const int id = blockIdx.x * A8_ROWS_WARPS + (threadIdx.x >> 5);
+    const int id = blockIdx.x * A8_BLOCK_WARPS + (threadIdx.x >> 5);
     const int rt = id / a.nsplit, part = id - rt * a.nsplit;
     const int r = a.first_req + blockIdx.z, head = blockIdx.y;
     const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs, clen = a.ctx_lens[r];
@@ -610,13 +708,12 @@ __global__ void __launch_bounds__(A8_ROWS_WARPS * 32, 2) attention_8bit_rows_ker
     const int t_lo = t_all + (int)((long long)count * part / a.nsplit), n = t_all + (int)((long long)count * (part + 1) / a.nsplit) - t_lo;
     w.begin(r, head, first, qlen, qs, clen);
     A8Cursor ahead = {r, 0, t_lo, t_lo + n - 1, clen};
-    int page[2], requested = 0;
-    w.pages_of(ahead, page);
+    int page = w.page_of(ahead), requested = 0;
     auto request_next = [&](int stage) {
         if (requested < n) {
             w.request(ahead, head, page, stage);
             ++ahead.tile;
-            if (++requested < n) w.pages_of(ahead, page);
+            if (++requested < n) page = w.page_of(ahead);
         }
         A8_COMMIT();
     };
@@ -641,42 +738,69 @@ __global__ void __launch_bounds__(A8_ROWS_WARPS * 32, 2) attention_8bit_rows_ker
 }
 
 // ---- segments put together, in order --------------------------------------------------------------------
-// A warp a row; a lane has two of every 64 dimensions.
-template <typename T>
+// `W` warps a row, which share its segments (eight where there may be many; a lane has two of every 64 dimensions and
+// requests eight segments' before it uses any: one memory latency for eight).
+template <typename T, int W>
 __device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, int stride_rows, int row, int head, T* dst, bool bad) {
-    const int lane = threadIdx.x & 31;
-    constexpr int PER = (A8_HD + 63) / 64;
+    const int lane = threadIdx.x & 31, part = W == 1 ? 0 : threadIdx.x >> 5;
+    constexpr int PER = (A8_HD + 63) / 64, AHEAD = 8;
     float2 o[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) o[k] = make_float2(0.f, 0.f);
     float M = -INFINITY, L = 0.f;
-    for (int at = 0; at < n; at += 32) {
-        const int cnt = min(32, n - at);
-        const float2 ml = lane < cnt ? a.part_ml[(place + at + lane) * stride_rows + row] : make_float2(-INFINITY, 0.f);
+    for (int at = part * AHEAD; at < n; at += W * AHEAD) {
+        const float2 ml = lane < AHEAD && at + lane < n ? a.part_ml[(place + at + lane) * stride_rows + row] : make_float2(-INFINITY, 0.f);
+        float2 v[AHEAD][PER];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                v[i][k] = at + i < n && (A8_HD % 64 == 0 || 64 * k + 2 * lane < A8_HD)
+                              ? *(const float2*)(a.part_o + ((place + at + i) * stride_rows + row) * A8_HD + 64 * k + 2 * lane)
+                              : make_float2(0.f, 0.f);
         const float most = fmaxf(M, rv_warp_max(ml.x));
-        if (most == -INFINITY) {
-            L += rv_warp_sum(ml.y);                                   // zeros, or what is not a number
-            continue;
-        }
-        const float keep = a8_exp2(M - most), w = a8_exp2(ml.x - most);
-        L = L * keep + rv_warp_sum(ml.y * w);
+        const float off = most == -INFINITY ? 0.f : most;
+        const float keep = a8_exp2(M - off), w = a8_exp2(ml.x - off);
+        L = L * keep + rv_warp_sum(ml.x == -INFINITY ? ml.y : ml.y * w);      // (without a reference: 0, or not a number)
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             o[k].x *= keep;
             o[k].y *= keep;
         }
-        for (int i = 0; i < cnt; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* src = a.part_o + ((place + at + i) * stride_rows + row) * A8_HD;
 #pragma unroll
-            for (int k = 0; k < PER; ++k)
-                if (64 * k + 2 * lane < A8_HD) {
-                    const float2 v = *(const float2*)(src + 64 * k + 2 * lane);
-                    o[k].x = fmaf(v.x, wi, o[k].x);
-                    o[k].y = fmaf(v.y, wi, o[k].y);
-                }
+        for (int i = 0; i < AHEAD; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                o[k].x = fmaf(v[i][k].x, wi, o[k].x);
+                o[k].y = fmaf(v[i][k].y, wi, o[k].y);
+            }
         }
         M = most;
+    }
+    if (W > 1) {
+        __shared__ float2 rows[W][PER * 32], ml[W];
+        if (lane == 0) ml[part] = make_float2(M, L);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) rows[part][32 * k + lane] = o[k];
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int i = 0; i < W; ++i) M = fmaxf(M, ml[i].x);
+        const float off = M == -INFINITY ? 0.f : M;
+        L = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) o[k] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float w = a8_exp2(ml[i].x - off);
+            L += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * w;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) {
+                o[k].x = fmaf(rows[i][32 * k + lane].x, w, o[k].x);
+                o[k].y = fmaf(rows[i][32 * k + lane].y, w, o[k].y);
+            }
+        }
     }
     if (a.sinks && L != 0.f) L += a8_exp2(a.sinks[head] * 1.4426950408889634f - M);
     const float by = bad ? NAN : L == 0.f ? 0.f : 1.f / L;
@@ -688,37 +812,43 @@ __device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, i
         }
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(128) attention_8bit_stream_merge_kernel(const __grid_constant__ A8Args a, int runs) {
-    rv_pdl_prologue();
+// A warp (W = 1: four rows a block) or a block a row; blockIdx.y: request, x: head.
+template <typename T, int NT, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_merge_kernel(const __grid_constant__ A8Args a, int runs) {
+    rv_pdl_launch_dependents();
     const int G = a.num_heads / a.num_kv_heads, per_head = (G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
-    const int r = blockIdx.y, head = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (head >= a.num_heads) return;
+    const int r = blockIdx.y, head = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (head >= a.num_heads) {
+        rv_pdl_wait();
+        return;
+    }
     const int kvh = head / G, in = head - kvh * G, u = kvh * per_head + in / (8 * NT);
-    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size, runs);
+    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size, runs, r);
     const int clen = sh.length(r), tiles = sh.tiles(clen);
     int run0 = 0, n = 0;
     if (tiles) {
-        const long long start = sh.before(r) * units + (long long)u * tiles;
+        const long long start = sh.before * units + (long long)u * tiles;
         run0 = sh.run_of(start);
         n = sh.run_of(start + tiles - 1) - run0 + 1;
     }
-    a8_merge<T>(a, (size_t)run0 + (size_t)r * units + u, n, 8 * NT, in % (8 * NT), head,
-                (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
+    rv_pdl_wait();
+    a8_merge<T, W>(a, (size_t)run0 + (size_t)r * units + u, n, 8 * NT, in % (8 * NT), head,
+                   (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(128) attention_8bit_rows_merge_kernel(const __grid_constant__ A8Args a) {
+// blockIdx.z: request, y: key/value head, x: rows.
+template <typename T, int NT, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_rows_merge_kernel(const __grid_constant__ A8Args a) {
     rv_pdl_prologue();
     const int G = a.num_heads / a.num_kv_heads, r = a.first_req + blockIdx.z, kvh = blockIdx.y;
     const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs;
     const int tiles = (qlen * G + 8 * NT - 1) / (8 * NT);
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 5);                 // the row
+    const int i = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;         // the row
     if (i >= qlen * G) return;
     const int rt = tiles - 1 - i / (8 * NT), tok = i / G, head = kvh * G + i - tok * G;
     if (rt >= a.row_tiles) return;                                     // a longer portion than the launch was told of
-    a8_merge<T>(a, (((size_t)blockIdx.z * a.num_kv_heads + kvh) * a.row_tiles + rt) * a.nsplit, a.nsplit, 8 * NT,
-                i % (8 * NT), head, (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD, false);
+    a8_merge<T, W>(a, (((size_t)blockIdx.z * a.num_kv_heads + kvh) * a.row_tiles + rt) * a.nsplit, a.nsplit, 8 * NT,
+                   i % (8 * NT), head, (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD, false);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------
@@ -730,6 +860,7 @@ static thread_local char g_a8_error[512] = "";
 
 extern "C" const char* A8_SYM(rv_attention_8bit_last_error)() { return g_a8_error; }
 
+static int a8_waves(){ static int w=[]{const char*e=getenv("A8W");return e?atoi(e):1;}(); return w; }
 // Rows of a warp: 16 where a key/value head has more than 8 of them and the accumulators fit the registers.
 static int a8_nt(int rows) { return rows > 8 && A8_HD <= 128 ? 2 : 1; }
 static long long a8_place_bytes(int nt) { return 8ll * nt * (A8_HD * 4 + 8); }
@@ -764,7 +895,7 @@ extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode,
     if (n_decode > 0) {
         const int nt = a8_nt(G);
         const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
-        need = ((long long)n_sms * A8_STREAM_WARPS + n_decode * units) * a8_place_bytes(nt);
+        need = ((long long)n_sms * A8_MOST_WARPS * a8_waves() + n_decode * units) * a8_place_bytes(nt);
     }
     if (n_reqs > n_decode) {
         int nsplit, row_tiles;
@@ -791,32 +922,42 @@ extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode,
 
 template <typename T, int NT, int PARTS>
 static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
-    const size_t smem = (size_t)A8_STREAM_WARPS * A8_WARP_BYTES;
+    const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
+    const int blocks = n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) * a8_waves();
     auto kernel = attention_8bit_stream_kernel<T, NT, PARTS>;
     A8_CONFIGURE(kernel, smem);
     const int G = a.num_heads / a.num_kv_heads;
-    const long long places = (long long)n_sms * A8_STREAM_WARPS +
+    const long long places = (long long)blocks * A8_BLOCK_WARPS +
                              (long long)a.n_reqs * a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT));
     a.part_ml = (float2*)(a.part_o + places * 8 * NT * A8_HD);
-    rv_launch(kernel, dim3(n_sms), dim3(A8_STREAM_WARPS * 32), smem, stream, a);
-    rv_launch(attention_8bit_stream_merge_kernel<T, NT>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a,
-              n_sms * A8_STREAM_WARPS);
+    rv_launch(kernel, dim3(blocks), dim3(A8_BLOCK_WARPS * 32), smem, stream, a);
+    // segments of a request's heads, about
+    const int units = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT));
+    if (blocks * A8_BLOCK_WARPS > 8ll * a.n_reqs * units)
+        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 8>, dim3(a.num_heads, a.n_reqs), dim3(256), 0, stream, a,
+                  blocks * A8_BLOCK_WARPS);
+    else
+        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 1>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a,
+                  blocks * A8_BLOCK_WARPS);
     return 0;
 }
 template <typename T, int NT, int PARTS>
 static int a8_rows(A8Args a, int max_q_len, cudaStream_t stream) {
-    const size_t smem = (size_t)A8_ROWS_WARPS * A8_WARP_BYTES;
+    const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
     auto kernel = attention_8bit_rows_kernel<T, NT, PARTS>;
     A8_CONFIGURE(kernel, smem);
     a.part_ml = (float2*)(a.part_o + (long long)a.row_tiles * a.num_kv_heads * a.n_reqs * a.nsplit * 8 * NT * A8_HD);
     const long long warps = (long long)a.row_tiles * a.nsplit;
     rv_launch(kernel,
-              dim3((unsigned)((warps + A8_ROWS_WARPS - 1) / A8_ROWS_WARPS), a.num_kv_heads, a.n_reqs), dim3(A8_ROWS_WARPS * 32), smem,
+              dim3((unsigned)((warps + A8_BLOCK_WARPS - 1) / A8_BLOCK_WARPS), a.num_kv_heads, a.n_reqs), dim3(A8_BLOCK_WARPS * 32), smem,
               stream, a);
     if (a.nsplit > 1) {
         const long long rows = (long long)max_q_len * (a.num_heads / a.num_kv_heads);
-        rv_launch(attention_8bit_rows_merge_kernel<T, NT>, dim3((unsigned)((rows + 3) / 4), a.num_kv_heads, a.n_reqs), dim3(128), 0,
-                  stream, a);
+        if (a.nsplit > 8)
+            rv_launch(attention_8bit_rows_merge_kernel<T, NT, 8>, dim3((unsigned)rows, a.num_kv_heads, a.n_reqs), dim3(256), 0, stream, a);
+        else
+            rv_launch(attention_8bit_rows_merge_kernel<T, NT, 1>, dim3((unsigned)((rows + 3) / 4), a.num_kv_heads, a.n_reqs), dim3(128),
+                      0, stream, a);
     }
     return 0;
 }
@@ -841,7 +982,7 @@ extern "C" int A8_SYM(rv_paged_attention_8bit)(
     const int G = num_heads / num_kv_heads;
     A8Args a = {q, (const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens, sinks,
                 out, (float*)scratch, nullptr, q_stride, pages, max_blocks, 0, n_decode, num_heads, num_kv_heads, page_size,
-                window, 1, 0, 0, scale * 1.4426950408889634f};
+                (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, window, 1, 0, 0, scale * 1.4426950408889634f};
     a.vec = (uintptr_t)q % 16 == 0 && q_stride * (dtype == RV_DTYPE_F32 ? 4 : 2) % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) A8_FAIL("paged_attention_8bit: unknown dtype code %d", dtype);

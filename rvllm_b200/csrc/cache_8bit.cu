@@ -12,10 +12,12 @@
 // of the old one and what the rows need, and where it grew the other slots become rint(q * old / new).
 // A page's tokens stand together in the call (nothing but tokens without a slot between them).
 //
-// One kernel: warps for the query heads (a warp has 32 / (head size / 16) heads of a token) and warps
-// for the key/value heads.  The latter take a range of tokens and one key or value head, find where pages begin in
-// the range and take such a run of tokens whole: the rows' largest value, then the scale, then the rows.  A
-// lane has 8 dimensions of a head's first half and the 8 that they turn with.
+// One kernel.  A lane has 8 dimensions of a head's first half and the 8 that they turn with, so a warp has
+// 32 / (head size / 16) heads at a time: of one token for the queries; for keys and values of as many tokens, one
+// head.  A warp of the latter takes a range of so many tokens and of it the pages that begin there, to their last token in the
+// call.  The rows are read once (three rounds of them stay in registers: the largest of a page has to be known before any is
+// written), the pages' scales settled a lane each, then the rows written.  Bound by a chain of four reads that
+// wait for one another (slots, positions, angles and rows, scales) where tokens are few.
 #include "common.cuh"
 
 #define C8_MAX_HEAD 256
@@ -30,8 +32,8 @@ struct C8Write {
     float *k_scale, *v_scale;
     long long row_stride, total_slots, table_rows;
     float eps;
-    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, range, aligned;
-    long long q_warps;
+    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, aligned;
+    long long kv_warps;
 };
 
 __device__ __forceinline__ void c8_load8(const float* p, bool vec, float (&v)[8]) {
@@ -159,22 +161,33 @@ __device__ __forceinline__ uint2 c8_pack(const float (&x)[8], float inv) {
     return make_uint2(u[0], u[1]);
 }
 
+// What a warp knows of the pages that begin in its range.
+struct C8Runs {
+    unsigned most[32];                 // bits of the largest finite |x| of each
+    float inv[32];                     // 1 / scale
+    int lowest[32];                    // first slot written
+    int page[32];
+};
+
 template <typename T>
 __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
     rv_pdl_prologue();
+    __shared__ C8Runs runs_of[C8_WARPS];
     const long long id = (long long)blockIdx.x * C8_WARPS + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int lph = a.head_dim >> 4, per = 32 / lph;           // lanes a head, heads a warp
     const int sub = lane / lph, d0 = (lane - sub * lph) * 8, lane0 = sub * lph;
     const int half = a.head_dim >> 1;
     float x[8], y[8];
-    if (id < a.q_warps) {
+    if (id >= a.kv_warps) {
         // ---- query heads --------------------------------------------------------------------
         const int groups = (a.num_heads + per - 1) / per;
-        const int t = (int)(id / groups), h = (int)(id - (long long)t * groups) * per + sub;
+        const long long t = (id - a.kv_warps) / groups;
+        const int h = (int)(id - a.kv_warps - t * groups) * per + sub;
+        if (t >= a.n_tokens) return;
         const bool live = sub < per && h < a.num_heads;
         c8_head(a, (const T*)a.rows + (size_t)t * a.row_stride + (size_t)(live ? h : 0) * a.head_dim, a.q_weight,
-                a.cos_table != nullptr, t, live, d0, lane0, lph, x, y);
+                a.cos_table != nullptr, (int)t, live, d0, lane0, lph, x, y);
         if (!live) return;
         T* dst = (T*)a.q_out + ((size_t)t * a.num_heads + h) * a.head_dim;
         c8_store8(dst + d0, a.aligned, x);
@@ -183,9 +196,7 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     }
     // ---- one key or value head of the pages that begin within a range of tokens ---------------
     const int pairs = 2 * a.num_kv_heads;
-    const long long kv = id - a.q_warps;
-    const int first = (int)(kv / pairs) * a.range, pair = (int)(kv % pairs);
-    if (first >= a.n_tokens) return;
+    const int first = (int)(id / pairs) * per, pair = (int)(id % pairs);
     const bool is_k = pair < a.num_kv_heads;
     const int g = is_k ? pair : pair - a.num_kv_heads;
     const T* src = (const T*)a.rows + (size_t)(a.num_heads + pair) * a.head_dim;
@@ -193,89 +204,147 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     const bool turn = is_k && a.cos_table != nullptr;
     signed char* cache = is_k ? a.k_cache : a.v_cache;
     float* scales = is_k ? a.k_scale : a.v_scale;
+    C8Runs& run = runs_of[threadIdx.x >> 5];
     auto slot_of = [&](int t) {
         const int s = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
         return s >= 0 && s < a.total_slots ? s : -1;
     };
-    const int mine = lane < a.range ? slot_of(first + lane) : -1;
+    const unsigned full = 0xffffffffu, below = (1u << lane) - 1u;
+    // this window's tokens, and the page of the last token with a slot before it
+    const int mine = slot_of(first + lane);
+    int back = slot_of(first - 1 - lane);
     const int my_page = mine >= 0 ? mine / a.page_size : -1;
-    // the page of the last token with a slot before the range
+    const unsigned real = __ballot_sync(full, mine >= 0);
     int before = -1;
-    for (int at = first - 1; at >= 0; at -= 32) {
-        const int s = slot_of(at - lane);
-        const unsigned have = __ballot_sync(0xffffffffu, s >= 0);
+    for (int at = first - 1;;) {
+        const unsigned have = __ballot_sync(full, back >= 0);
         if (have) {
-            before = __shfl_sync(0xffffffffu, s, __ffs(have) - 1) / a.page_size;
+            before = __shfl_sync(full, back, __ffs(have) - 1) / a.page_size;
             break;
         }
+        at -= 32;
+        if (at < 0) break;
+        back = slot_of(at - lane);
     }
-    unsigned real = __ballot_sync(0xffffffffu, mine >= 0);
-    while (real) {
-        const int l = __ffs(real) - 1;
-        real &= real - 1;
-        const int page = __shfl_sync(0xffffffffu, my_page, l);
-        const bool begins = page != before;
-        before = page;
-        if (!begins) continue;
-        // the run: tokens [t0, t1), all with a slot of this page or with none
-        const int t0 = first + l;
-        int t1 = t0, lowest = a.page_size;
-        for (bool more = true; more;) {
-            const int s = slot_of(t1 + lane);
-            const bool here = s >= 0 && s / a.page_size == page;
-            const bool ends = (s >= 0 && !here) || t1 + lane >= a.n_tokens;
-            const unsigned stop = __ballot_sync(0xffffffffu, ends);
-            const int n = stop ? __ffs(stop) - 1 : 32;
-            lowest = min(lowest, (int)__reduce_min_sync(0xffffffffu, here && lane < n ? s - page * a.page_size : a.page_size));
-            t1 += n;
-            more = n == 32;
-        }
-        float most = 0.f;
-        for (int t = t0; t < t1; t += per) {
-            const int tt = t + sub;
-            const bool live = sub < per && tt < t1 && slot_of(tt) >= 0;
-            c8_head(a, src + (size_t)(live ? tt : t0) * a.row_stride, w, turn, tt, live, d0, lane0, lph, x, y);
-            most = c8_most(y, c8_most(x, most));
-        }
-        most = rv_warp_max(most);
-        const size_t block = (size_t)page * a.num_kv_heads + g;
-        signed char* held = cache + block * a.page_size * a.head_dim;
-        float s = c8_pow2(c8_exponent(most));
-        if (lowest > 0) {
-            const float old = scales[block];
-            s = fmaxf(old, s);
-            if (s != old) {                                     // the other slots follow the larger scale
-                const float ratio = old / s;
-                for (int i = lane * 16; i < a.page_size * a.head_dim; i += 512) {
-                    int4 v = *(const int4*)(held + i);
-                    signed char* b = (signed char*)&v;
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) b[k] = (signed char)__float2int_rn((float)b[k] * ratio);
-                    *(int4*)(held + i) = v;
-                }
+    const unsigned earlier = real & below;
+    int prev = __shfl_sync(full, my_page, earlier ? 31 - __clz(earlier) : 0);
+    if (!earlier) prev = before;
+    const bool changes = mine >= 0 && my_page != prev;
+    const unsigned begins = __ballot_sync(full, changes);
+    const unsigned owned = begins & (per < 32 ? (1u << per) - 1u : full);
+    if (!owned) return;
+    const int n_runs = __popc(owned), l0 = __ffs(owned) - 1, last = 31 - __clz(owned);
+    // tokens [t0, t1): up to the first token behind the range that has a slot of another page
+    const int t0 = first + l0;
+    int t1 = first + 32;
+    {
+        const unsigned after = begins & ~((2u << last) - 1u);
+        const int last_page = __shfl_sync(full, my_page, last);
+        if (after) {
+            t1 = first + __ffs(after) - 1;
+        } else {
+            for (bool more = t1 < a.n_tokens; more;) {
+                const int s = slot_of(t1 + lane);
+                const unsigned stop = __ballot_sync(full, (s >= 0 && s / a.page_size != last_page) || t1 + lane >= a.n_tokens);
+                t1 += stop ? __ffs(stop) - 1 : 32;
+                more = !stop;
             }
+            t1 = min(t1, a.n_tokens);
+        }
+    }
+    run.most[lane] = 0u;
+    run.lowest[lane] = a.page_size;
+    if ((owned >> lane) & 1u) run.page[__popc(owned & below)] = my_page;
+    __syncwarp();
+    // lane i looks after run i: its page and what its scale was
+    const int page_i = lane < n_runs ? run.page[lane] : 0;
+    const size_t block_i = (size_t)page_i * a.num_kv_heads + g;
+    const float old = lane < n_runs ? scales[block_i] : 0.f;
+    __syncwarp();
+    // A group of lanes a token: `slot` (-1: none) and the number of its run.
+    auto whose = [&](int t, int& slot, int& number) {
+        const int in = t - first;
+        const int s = __shfl_sync(full, mine, in & 31);
+        slot = in < 32 ? s : slot_of(t);
+        if (sub >= per || t >= t1) slot = -1;
+        number = in < 32 ? __popc(owned & ((2u << in) - 1u)) - 1 : n_runs - 1;
+    };
+    constexpr int HOLD = 3;             // rounds whose rows stay in registers: a range and the page that it ends in
+    float hx[HOLD][8], hy[HOLD][8];
+    auto measure = [&](int t, int slot, int number, float (&u)[8], float (&v)[8]) {
+        c8_head(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
+        if (slot >= 0) {
+            atomicMax(&run.most[number], __float_as_uint(c8_most(v, c8_most(u, 0.f))));
+            atomicMin(&run.lowest[number], slot % a.page_size);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+        if (t0 + i * per < t1) {
+            int slot, number;
+            whose(t0 + i * per + sub, slot, number);
+            measure(t0 + i * per + sub, slot, number, hx[i], hy[i]);
+        }
+    for (int t = t0 + HOLD * per; t < t1; t += per) {
+        int slot, number;
+        whose(t + sub, slot, number);
+        measure(t + sub, slot, number, x, y);
+    }
+    __syncwarp();
+    bool grows = false;
+    float ratio = 0.f;
+    if (lane < n_runs) {
+        float s = c8_pow2(c8_exponent(__uint_as_float(run.most[lane])));
+        if (run.lowest[lane] > 0) {
+            s = fmaxf(old, s);
+            grows = s != old;
+            ratio = old / s;
+        }
+        scales[block_i] = s;
+        run.inv[lane] = 1.f / s;
+    }
+    // pages whose scale grew: what they hold follows (the slots written below too, which does no harm)
+    for (unsigned todo = __ballot_sync(full, grows); todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1;
+        const float by = __shfl_sync(full, ratio, i);
+        signed char* held = cache + ((size_t)__shfl_sync(full, page_i, i) * a.num_kv_heads + g) * a.page_size * a.head_dim;
+        for (int at = lane * 16; at < a.page_size * a.head_dim; at += 512) {
+            int4 v = *(const int4*)(held + at);
+            signed char* b = (signed char*)&v;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) b[k] = (signed char)__float2int_rn((float)b[k] * by);
+            *(int4*)(held + at) = v;
+        }
+    }
+    __syncwarp();
+    auto store = [&](int slot, int number, const float (&u)[8], const float (&v)[8]) {
+        // (of two tokens with one slot the later one is written)
+        bool later = false;
+        for (int k = 1; k < per; ++k) {
+            const int other = __shfl_sync(full, slot, ((sub + k) * lph) & 31);
+            later |= sub + k < per && other == slot;
+        }
+        if (slot >= 0 && !later) {
+            const float inv = run.inv[number];
+            const int page = slot / a.page_size;
+            signed char* dst = cache + (((size_t)page * a.num_kv_heads + g) * a.page_size + (slot - page * a.page_size)) * a.head_dim;
+            *(uint2*)(dst + d0) = c8_pack(u, inv);
+            *(uint2*)(dst + half + d0) = c8_pack(v, inv);
         }
         __syncwarp();
-        if (lane == 0) scales[block] = s;
-        const float inv = 1.f / s;
-        for (int t = t0; t < t1; t += per) {
-            const int tt = t + sub;
-            const int slot = sub < per && tt < t1 ? slot_of(tt) : -1;
-            const bool live = slot >= 0;
-            c8_head(a, src + (size_t)(live ? tt : t0) * a.row_stride, w, turn, tt, live, d0, lane0, lph, x, y);
-            // (of two tokens with one slot the later one is written)
-            bool later = false;
-            for (int k = 1; k < per; ++k) {
-                const int other = __shfl_sync(0xffffffffu, slot, ((sub + k) * lph) & 31);
-                later |= sub + k < per && other == slot;
-            }
-            if (live && !later) {
-                signed char* dst = held + (size_t)(slot - page * a.page_size) * a.head_dim;
-                *(uint2*)(dst + d0) = c8_pack(x, inv);
-                *(uint2*)(dst + half + d0) = c8_pack(y, inv);
-            }
-            __syncwarp();
+    };
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i)
+        if (t0 + i * per < t1) {
+            int slot, number;
+            whose(t0 + i * per + sub, slot, number);
+            store(slot, number, hx[i], hy[i]);
         }
+    for (int t = t0 + HOLD * per; t < t1; t += per) {
+        int slot, number;
+        whose(t + sub, slot, number);
+        c8_head(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
+        store(slot, number, x, y);
     }
 }
 
@@ -295,16 +364,13 @@ extern "C" int rv_qk_norm_rope_write_8bit(const void* rows, int dtype, long long
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) RV_FAIL("qk_norm_rope_write_8bit: pages must be 16-byte aligned");
     C8Write a = {rows, q_out, q_weight, k_weight, cos_table, sin_table, positions, slots, (signed char*)k_cache,
                  (signed char*)v_cache, k_scale, v_scale, row_stride, pages * page_size, table_rows, eps, n_tokens,
-                 num_heads, num_kv_heads, head_dim, page_size, 1, 0, 0};
+                 num_heads, num_kv_heads, head_dim, page_size, 0, 0};
     const int size = dtype == RV_DTYPE_F32 ? 4 : 2, per = 32 / (head_dim >> 4);
     a.aligned = ((uintptr_t)rows | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
                  (uintptr_t)sin_table) % 16 == 0 && row_stride * size % 16 == 0;
-    a.q_warps = (long long)n_tokens * ((num_heads + per - 1) / per);
-    // tokens whose pages a warp looks after
-    const int sms = rv_sm_count();
-    a.range = n_tokens <= 2 * sms ? 1 : (n_tokens <= 8 * sms ? 4 : 16);
-    const long long kv_warps = (long long)((n_tokens + a.range - 1) / a.range) * 2 * num_kv_heads;
-    const long long blocks = (a.q_warps + kv_warps + C8_WARPS - 1) / C8_WARPS;
+    const long long q_warps = (long long)n_tokens * ((num_heads + per - 1) / per);
+    a.kv_warps = (long long)((n_tokens + per - 1) / per) * 2 * num_kv_heads;
+    const long long blocks = (a.kv_warps + q_warps + C8_WARPS - 1) / C8_WARPS;
     if (blocks > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: too many rows");
     RV_DISPATCH_DTYPE(dtype, "qk_norm_rope_write_8bit",
                       (rv_launch(qk_norm_rope_write_8bit_kernel<T>, dim3((int)blocks), dim3(C8_WARPS * 32), 0,

@@ -7,13 +7,15 @@
 // log p = (x - m) - log s and H = log s - ln 2 w / s.  x - m comes first, so logits of a type's lowest value are
 // ordinary numbers.
 //
-// The largest: a warp keeps the best 32 so far, sorted over its lanes, as 64-bit keys (the value's bits in the order of
-// values, then the index reversed), so one comparison has both.  Values above the last one wanted collect in a
-// buffer of shared memory and are sorted and merged 32 at a time (bitonic); while the list is not full yet the
-// 32 lanes' largest give a first bound, and the block's warps share their bounds, so few values get that far.
+// The largest: values that may still be among them collect in the block's shared memory, as 64-bit keys (the value's
+// bits in the order of values, then the index reversed: one comparison has both).  What may be is bounded from
+// below, round by round of loads: if r lanes of each of the 8 warps have met a value of at least b, then 8 r values are
+// that large, and with 8 r >= `top` nothing below b is wanted -- r lanes by r maxima over a warp, the smallest of the
+// warps' bounds.  Some tens of values are left at the end; each counts the larger ones, which is its place.  A
+// round that would overflow the memory is taken again with the bound that the values in it give.
 //
 // A row is a cluster's of 1 to 8 blocks (as many as the GPU has room for when rows are few); parts meet in the
-// first block's shared memory in a fixed order, so a row's results do not depend on what else is in the launch.
+// first block in a fixed order, so a row's results do not depend on what else is in the launch.
 // Bound by reading the logits.
 #include "common.cuh"
 
@@ -22,6 +24,8 @@
 #define LP_MAX_CLUSTER 8
 #define LP_LOG2E 1.4426950408889634f
 #define LP_LN2 0.6931471805599453f
+
+#define LP_ROOM 640                    // values that a block can collect
 
 typedef unsigned long long u64;
 
@@ -42,26 +46,6 @@ __device__ __forceinline__ unsigned lp_key(float x) {
 }
 __device__ __forceinline__ float lp_value(unsigned k) {
     return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
-}
-__device__ __forceinline__ u64 lp_exchange(u64 x, int mask, bool larger) {
-    const u64 y = __shfl_xor_sync(0xffffffffu, x, mask);
-    return (x > y) == larger ? x : y;
-}
-// Descending over the lanes.
-__device__ __forceinline__ u64 lp_sort(u64 x, int lane) {
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) x = lp_exchange(x, j, ((lane & j) == 0) == ((lane & k) == 0));
-    return x;
-}
-// The 32 largest of two descending lists, descending.
-__device__ __forceinline__ u64 lp_merge(u64 a, u64 b, int lane) {
-    const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
-    u64 x = a > r ? a : r;
-#pragma unroll
-    for (int j = 16; j > 0; j >>= 1) x = lp_exchange(x, j, (lane & j) == 0);
-    return x;
 }
 
 template <typename T> struct LpVec;
@@ -85,32 +69,53 @@ template <> struct LpVec<__nv_bfloat16> {
     }
 };
 
-struct LpPart { float m, s, w; int above; };
-
-// What a part leaves for the row's first block.
-struct LpShared {
-    LpPart part[LP_WARPS];
-    LpPart whole;
-    u64 list[LP_WARPS][32];
-    u64 buffer[LP_WARPS][64];
-    unsigned bound;
-};
+struct __align__(16) LpPart { float m, s, w; int above; };
 
 __device__ __forceinline__ float lp_ref(float m) { return m == -INFINITY ? 0.f : m; }
-__device__ __forceinline__ void lp_add(LpPart& a, float m, float s, float w) {
+// From one reference to a larger one, in units of log2; far ones stay finite (2^-300 is 0).
+__device__ __forceinline__ float lp_move(float from, float to) { return fmaxf((from - to) * LP_LOG2E, -300.f); }
+__device__ __forceinline__ void lp_add(LpPart& a, const LpPart& b) {
     // both to the larger reference
-    const float top = fmaxf(a.m, m), c = lp_ref(top);
+    const float top = fmaxf(a.m, b.m), c = lp_ref(top);
     if (a.s != 0.f) {
-        const float d = (lp_ref(a.m) - c) * LP_LOG2E, f = lp_exp2(d);
+        const float d = lp_move(lp_ref(a.m), c), f = lp_exp2(d);
         a.w = (a.w + a.s * d) * f;
         a.s *= f;
     }
-    if (s != 0.f) {
-        const float d = (lp_ref(m) - c) * LP_LOG2E, f = lp_exp2(d);
-        a.w += (w + s * d) * f;
-        a.s += s * f;
+    if (b.s != 0.f) {
+        const float d = lp_move(lp_ref(b.m), c), f = lp_exp2(d);
+        a.w += (b.w + b.s * d) * f;
+        a.s += b.s * f;
     }
     a.m = top;
+    a.above += b.above;
+}
+
+template <bool TOP> struct LpShared {
+    LpPart part[LP_WARPS];
+    LpPart whole;
+};
+template <> struct LpShared<true> {
+    LpPart part[LP_WARPS];
+    LpPart whole;
+    u64 room[LP_ROOM];
+    u64 best[LP_MAX_CLUSTER][32];      // the parts' largest, descending; [0] is what this block leaves
+    unsigned bound[2][LP_WARPS];
+    int count;
+};
+
+// Places `n` keys of `from` by how many are larger; the first `top` of them go to `to`, the rest of `to` is 0.
+__device__ __forceinline__ void lp_place(const u64* from, int n, int top, u64* to) {
+    __syncthreads();
+    if (threadIdx.x >= n && threadIdx.x < 32) to[threadIdx.x] = 0ull;
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+        const u64 x = from[i];
+        int larger = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) larger += from[j] > x;
+        if (larger < 32) to[larger] = larger < top ? x : 0ull;
+    }
+    __syncthreads();
 }
 
 template <typename T, bool TOP>
@@ -119,36 +124,21 @@ struct LpThread {
     float m = -INFINITY, s = 0.f, w = 0.f;
     int above = 0;
     float given;
-    u64 best = 0;                      // this lane's place of the warp's list
-    u64 last = 0;                      // the list's last wanted key
-    int waiting = 0;                   // values in the buffer
-    int top, lane;
-    LpShared& sh;
-    u64* buffer;
+    int top;
+    // of the block, the same in every thread: only larger keys are wanted; how many are there
+    u64 least = 0ull;
+    int count = 0, round = 0;
+    LpShared<TOP>& sh;
 
-    __device__ __forceinline__ LpThread(LpShared& shared, int k, float x)
-        : given(x), top(k), lane(threadIdx.x & 31), sh(shared), buffer(shared.buffer[threadIdx.x >> 5]) {}
+    __device__ __forceinline__ LpThread(LpShared<TOP>& shared, int k, float x) : given(x), top(k), sh(shared) {}
 
-    __device__ __forceinline__ void flush() {            // the first 32 of the buffer into the list
-        __syncwarp();
-        const u64 x = lane < waiting ? buffer[lane] : 0ull;
-        best = lp_merge(best, lp_sort(x, lane), lane);
-        last = __shfl_sync(0xffffffffu, best, top - 1);
-        if (lane == 0) atomicMax(&sh.bound, (unsigned)(last >> 32));
-        __syncwarp();
-        if (lane + 32 < waiting) buffer[lane] = buffer[lane + 32];
-        waiting = max(0, waiting - 32);
-        __syncwarp();
-    }
-    // E values of this thread (every lane of the warp comes here): x[i] is column col(i); `real(i)`: it exists.
-    template <typename Col, typename Real>
-    __device__ __forceinline__ void take(const float (&x)[E], Col col, Real real) {
+    __device__ __forceinline__ float sums(const float (&x)[E]) {          // the largest x
         float bm = x[0];
 #pragma unroll
         for (int i = 1; i < E; ++i) bm = fmaxf(bm, x[i]);
         if (bm > m) {
             if (s != 0.f) {
-                const float d = (m - bm) * LP_LOG2E, f = lp_exp2(d);
+                const float d = lp_move(m, bm), f = lp_exp2(d);
                 w = (w + s * d) * f;
                 s *= f;
             }
@@ -158,35 +148,66 @@ struct LpThread {
         float s2[2] = {0.f, 0.f}, w2[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            // (far below: 2^t is 0, and so is its product with t)
-            const float t = lp_max_nan((x[i] - c) * LP_LOG2E, -200.f), e = lp_exp2(t);
+            // (far below: 2^u is 0, and so is its product with u)
+            const float u = lp_max_nan((x[i] - c) * LP_LOG2E, -200.f), e = lp_exp2(u);
             s2[i & 1] += e;
-            w2[i & 1] = fmaf(e, t, w2[i & 1]);
+            w2[i & 1] = fmaf(e, u, w2[i & 1]);
             above += x[i] > given;
         }
         s += s2[0] + s2[1];
         w += w2[0] + w2[1];
-        if (TOP) {
-            const unsigned own = (unsigned)(last >> 32);
-            unsigned shared = *(volatile unsigned*)&sh.bound;
-            const unsigned mine = bm == bm ? lp_key(bm) : 0u;
-            if (!__any_sync(0xffffffffu, mine >= own && mine >= shared)) return;
-            if (last == 0ull) {
-                // no full list yet: as many values as are wanted reach the lanes' largest down to this one
-                const u64 sorted = lp_sort((u64)mine << 32, lane);
-                shared = max(shared, (unsigned)(__shfl_sync(0xffffffffu, sorted, top - 1) >> 32));
+        return bm;
+    }
+    // E values of every thread of the block: x[i] is column col(i), if real(i).
+    template <typename Col, typename Real>
+    __device__ __forceinline__ void take(const float (&x)[E], Col col, Real real) {
+        const float bm = sums(x);
+        if constexpr (TOP) {
+            const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+            // r lanes' largest so far
+            const int r = (top + LP_WARPS - 1) / LP_WARPS;
+            unsigned mine = m == -INFINITY ? 0u : lp_key(m), b = 0u;
+            for (int k = 0; k < r; ++k) {
+                b = __reduce_max_sync(0xffffffffu, mine);
+                const unsigned who = __ballot_sync(0xffffffffu, mine == b);
+                if (lane == __ffs(who) - 1) mine = 0u;
             }
+            unsigned* bounds = sh.bound[round & 1];
+            ++round;
+            if (lane == 0) bounds[warp] = b;
+            __syncthreads();
+            b = bounds[0];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const unsigned k = real(i) ? lp_key(x[i]) : 0u;
-                const u64 whole = ((u64)k << 32) | (0xffffffffu - (unsigned)col(i));
-                const bool in = k != 0u && whole > last && k >= shared;
-                const unsigned who = __ballot_sync(0xffffffffu, in);
-                if (who) {
-                    if (in) buffer[waiting + __popc(who & ((1u << lane) - 1u))] = whole;
-                    waiting += __popc(who);
-                    if (waiting >= 32) flush();
+            for (int k = 1; k < LP_WARPS; ++k) b = min(b, bounds[k]);
+            if (b > (unsigned)(least >> 32)) least = ((u64)b << 32) - 1ull;
+            for (;;) {
+                if (lp_key(bm) >= (unsigned)(least >> 32))           // few threads have one
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const u64 key = ((u64)lp_key(x[i]) << 32) | (0xffffffffu - (unsigned)col(i));
+                    if (key > least && (key >> 32) != 0ull && real(i)) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < LP_ROOM) sh.room[at] = key;
+                    }
                 }
+                __syncthreads();
+                const int n = sh.count;
+                if (n <= LP_ROOM / 2) {
+                    count = n;
+                    break;
+                }
+                // too many: the largest of those that are here bound the others
+                lp_place(sh.room, min(n, LP_ROOM), top, sh.best[0]);
+                least = sh.best[0][top - 1];
+                if (n <= LP_ROOM) {                                  // all are here: keep the best
+                    if (tid < top) sh.room[tid] = sh.best[0][tid];
+                    count = top;
+                } else {
+                    --least;                                         // again, with the last of them let in
+                }
+                if (tid == 0) sh.count = count;
+                __syncthreads();
+                if (n <= LP_ROOM) break;
             }
         }
     }
@@ -199,7 +220,7 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
     int* __restrict__ top_id, int parts) {
     rv_pdl_prologue();
     constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U;
-    __shared__ LpShared sh;
+    __shared__ LpShared<TOP> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - row * parts);
@@ -207,8 +228,10 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
     const int token = tokens[row];
     const bool known = token >= 0 && token < vocab;
     const float given = known ? rv_load(x + token) : INFINITY;
-    if (tid == 0) sh.bound = 0u;
-    __syncthreads();
+    if constexpr (TOP) {
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+    }
     LpThread<T, TOP> th(sh, top, given);
     // whole 16-byte vectors from the first aligned one on, shared out over the parts; what lies
     // before and behind them is the last part's
@@ -238,24 +261,20 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
         th.take(v, [&](int i) { return base + (i / N) * LP_THREADS * N + i % N; },
                 [&](int i) { return at + (i / N) * LP_THREADS + tid < v1; });
     }
-    if (part == parts - 1 && warp == 0 && head + vocab - tail > 0) {
-        const int col = lane < head ? lane : tail + lane - head;
+    if (part == parts - 1 && head + vocab - tail > 0) {
+        const int col = tid < head ? tid : tail + tid - head;
         const bool have = col < vocab;
         v[0] = have ? rv_load(x + col) : -INFINITY;
 #pragma unroll
         for (int i = 1; i < E; ++i) v[i] = -INFINITY;
         th.take(v, [&](int) { return col; }, [&](int i) { return i == 0 && have; });
     }
-    if (TOP) {
-        while (th.waiting > 0) th.flush();
-        sh.list[warp][lane] = th.best;
-    }
     // ---- the warp's, the block's, the cluster's ------------------------------------------------
     {
         const float most = rv_warp_max(th.m), c = lp_ref(most);
         float s = 0.f, w = 0.f;
         if (th.s != 0.f) {
-            const float d = (lp_ref(th.m) - c) * LP_LOG2E, f = lp_exp2(d);
+            const float d = lp_move(lp_ref(th.m), c), f = lp_exp2(d);
             s = th.s * f;
             w = (th.w + th.s * d) * f;
         }
@@ -264,70 +283,98 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
         const int above = __reduce_add_sync(0xffffffffu, th.above);
         if (lane == 0) sh.part[warp] = {most, s, w, above};
     }
-    __syncthreads();
+    if constexpr (TOP) lp_place(sh.room, th.count, top, sh.best[0]);
+    else __syncthreads();
     if (tid == 0) {
         LpPart p = sh.part[0];
-        for (int i = 1; i < LP_WARPS; ++i) {
-            lp_add(p, sh.part[i].m, sh.part[i].s, sh.part[i].w);
-            p.above += sh.part[i].above;
-        }
+        for (int i = 1; i < LP_WARPS; ++i) lp_add(p, sh.part[i]);
         sh.whole = p;
-    }
-    if (TOP) {
-#pragma unroll
-        for (int step = LP_WARPS / 2; step > 0; step >>= 1) {
-            if (warp < step) {
-                th.best = lp_merge(th.best, sh.list[warp + step][lane], lane);
-                sh.list[warp][lane] = th.best;
-            }
-            __syncthreads();
-        }
     }
     if (parts > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        if (part == 0 && warp == 0) {
+        if (part == 0) {
             auto remote = [](const void* p, int rank_) {
                 unsigned a;
                 asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank_));
                 return a;
             };
-            LpPart p = sh.whole, q[LP_MAX_CLUSTER];
-            u64 lists[LP_MAX_CLUSTER];
-#pragma unroll
-            for (int k = 1; k < LP_MAX_CLUSTER; ++k)
-                if (k < parts) {
+            if constexpr (TOP) {                                     // warp k brings part k's list
+                if (warp > 0 && warp < parts) {
+                    u64 key;
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(remote(&sh.best[0][lane], warp)) : "memory");
+                    sh.best[warp][lane] = key;
+                }
+            }
+            if (warp == 0) {
+                // lane k brings part k's sums
+                LpPart q = sh.whole;
+                if (lane > 0 && lane < parts)
                     asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(q[k].m), "=f"(q[k].s), "=f"(q[k].w), "=r"(q[k].above) : "r"(remote(&sh.whole, k)) : "memory");
-                    if (TOP) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(lists[k]) : "r"(remote(&sh.list[0][lane], k)) : "memory");
+                                 : "=f"(q.m), "=f"(q.s), "=f"(q.w), "=r"(q.above) : "r"(remote(&sh.whole, lane)) : "memory");
+                LpPart p = sh.whole;
+                for (int k = 1; k < parts; ++k) {
+                    LpPart o;
+                    o.m = __shfl_sync(0xffffffffu, q.m, k);
+                    o.s = __shfl_sync(0xffffffffu, q.s, k);
+                    o.w = __shfl_sync(0xffffffffu, q.w, k);
+                    o.above = __shfl_sync(0xffffffffu, q.above, k);
+                    lp_add(p, o);
                 }
-#pragma unroll
-            for (int k = 1; k < LP_MAX_CLUSTER; ++k)
-                if (k < parts) {
-                    lp_add(p, q[k].m, q[k].s, q[k].w);
-                    p.above += q[k].above;
-                    if (TOP) th.best = lp_merge(th.best, lists[k], lane);
-                }
-            if (lane == 0) sh.whole = p;
+                __syncwarp();
+                if (lane == 0) sh.whole = p;
+            }
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // nobody leaves while it is read
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (part != 0) return;
+    } else {
+        __syncthreads();
     }
-    if (part != 0 || warp != 0) return;
-    __syncwarp();
     const LpPart p = sh.whole;
     const float c = lp_ref(p.m), logs = logf(p.s);
-    if (lane == 0) {
+    if (tid == 0) {
         const float h = logs - LP_LN2 * (p.w / p.s);
         logprob[row] = known ? (given - c) - logs : NAN;
         rank[row] = known ? p.above + 1 : 0;
         entropy[row] = h < 0.f ? 0.f : h;
     }
-    if (TOP && lane < top) {
-        const bool have = th.best != 0ull;
-        const float y = lp_value((unsigned)(th.best >> 32));
-        top_logprob[row * top + lane] = have ? (y - c) - logs : NAN;
-        top_id[row * top + lane] = have ? (int)(0xffffffffu - (unsigned)th.best) : -1;
+    if constexpr (TOP) {
+        // a key of part `warp`: its place there, and in each other part by bisection
+        if (warp < parts && lane < top) {
+            const u64 key = sh.best[warp][lane];
+            int place = lane;
+            for (int k = 0; k < parts; ++k) {
+                if (k == warp) continue;
+                int lo = 0, hi = 32;                                 // how many of part k are larger
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (sh.best[k][mid] > key) lo = mid + 1;
+                    else hi = mid;
+                }
+                place += lo;
+            }
+            if (key != 0ull && place < top) {
+                top_logprob[row * top + place] = (lp_value((unsigned)(key >> 32)) - c) - logs;
+                top_id[row * top + place] = (int)(0xffffffffu - (unsigned)key);
+            }
+        }
+        if (warp == 0 && lane < top) {                               // places that nothing takes
+            int have = 0;
+            for (int k = 0; k < parts; ++k) {
+                int lo = 0, hi = 32;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (sh.best[k][mid] != 0ull) lo = mid + 1;
+                    else hi = mid;
+                }
+                have += lo;
+            }
+            if (lane >= have) {
+                top_logprob[row * top + lane] = NAN;
+                top_id[row * top + lane] = -1;
+            }
+        }
     }
 }
 

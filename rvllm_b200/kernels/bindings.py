@@ -117,6 +117,13 @@ class CudaOps:
         # memory and of the delta rule with a decay per channel (the reasons are where they are asked)
         self.mlstm_above = 384
         self.gated_delta_above = 288
+        P, I, L = c_void_p, c_int, c_longlong
+        self._write_8bit = self.lib.rv_qk_norm_rope_write_8bit
+        self._write_8bit.argtypes = [P, I, L, I, I, I, I, P, P, c_float, P, P, L, P, P, P, P, P, P, P, L, I, P]
+        self._read_8bit = self.lib.rv_read_8bit
+        self._read_8bit.argtypes = [P, P, P, P, I, I, I, I, I, L, P]
+        self._token_logprobs = self.lib.rv_token_logprobs
+        self._token_logprobs.argtypes = [P, I, L, I, I, P, I, P, P, P, P, P, P]
         # the library's float32 products must be float32: no TF32, no reduced-precision accumulation
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
@@ -828,37 +835,50 @@ class CudaOps:
             c_float(scale), c_int(window if window else 0), self._stream()), "paged_attention")
 
     # ---- keys and values in 8 bits ------------------------------------------------------
+    #
+    # These calls are short on the GPU (some 4 us a step of single tokens), so the host's part counts: one
+    # pass over the tensors, plain numbers handed to functions whose argument types are declared.
 
     @staticmethod
-    def _need_here(what, *tensors):
-        """Every tensor on the device whose stream the kernels are launched on."""
-        for t in tensors:
-            if t is not None and (not t.is_cuda or t.get_device() != torch.cuda.current_device()):
-                raise KernelError(f"{what}: a tensor is on {t.device}, not on the current CUDA device")
-
-    def _need_pages_8bit(self, what, cache, scale, num_kv_heads=None, head_dim=None):
-        self._need(cache, "8-bit pages", torch.int8)
-        self._need(scale, "scales", torch.float32)
-        if cache.dim() != 4 or scale.shape != cache.shape[:2]:
-            raise KernelError(f"{what}: pages are [pages, kv heads, page size, head size], scales [pages, kv heads]")
-        if head_dim is not None and (cache.shape[1] != num_kv_heads or cache.shape[3] != head_dim):
-            raise KernelError(f"{what}: pages of {cache.shape[1]} heads of {cache.shape[3]}, "
-                              f"asked for {num_kv_heads} of {head_dim}")
-        if cache.shape[3] % 16 or not 16 <= cache.shape[3] <= 256:
-            raise KernelError(f"{what}: head size {cache.shape[3]} is not supported (a multiple of 16, at most 256)")
+    def _here() -> int:
+        return torch._C._cuda_getDevice()          # (what torch.cuda.current_device comes to, without its checks)
 
     @staticmethod
-    def _need_rows(what, rows, width=None):
-        """[tokens, width or more] whose values of a token lie side by side."""
-        if rows.dim() != 2 or (width is not None and rows.shape[1] < width):
-            raise KernelError(f"{what}: rows and head counts disagree")
-        if rows.shape[1] > 1 and rows.stride(1) != 1 or rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
-            raise KernelError(f"{what}: the values of a row must lie side by side")
+    def _fault(what: str, message: str):
+        raise KernelError(f"{what}: {message}")
 
-    def _need_index(self, what, t, n):
-        self._need(t, what, torch.int32)
-        if t.dim() != 1 or t.shape[0] < n:
-            raise KernelError(f"{what}: {n} int32 wanted, got {tuple(t.shape)}")
+    def _held(self, what, *tensors):
+        """(tensor, name, type) each: contiguous, of that type, on the device whose stream is launched on."""
+        here = self._here()
+        for t, name, dtype in tensors:
+            if t.get_device() != here:
+                self._fault(what, f"{name} on {t.device}, not on the current CUDA device {here}")
+            if t.dtype is not dtype:
+                self._fault(what, f"{name} must be {dtype}, got {t.dtype}")
+            if not t.is_contiguous():
+                self._fault(what, f"{name} must be contiguous")
+
+    def _row_shape(self, what, rows, width):
+        """Tokens of `rows` [tokens, width or more], whose values of a token lie side by side."""
+        if rows.get_device() != self._here():
+            self._fault(what, f"rows on {rows.device}, not on the current CUDA device")
+        if rows.dim() != 2 or rows.size(1) < width:
+            self._fault(what, "row width and head counts disagree")
+        n, have = rows.shape
+        stride, step = rows.stride()
+        if (have > 1 and step != 1) or (n > 1 and stride < have):
+            self._fault(what, "the values of a row must lie side by side")
+        return n, stride
+
+    def _page_shape(self, what, cache, scale, other=None, other_scale=None):
+        shape = cache.shape
+        if len(shape) != 4 or tuple(scale.shape) != tuple(shape[:2]):
+            self._fault(what, "pages are [pages, kv heads, page size, head size], scales [pages, kv heads]")
+        if other is not None and (other.shape != shape or other_scale.shape != scale.shape):
+            self._fault(what, "key and value pages differ in shape")
+        if shape[3] % 16 or not 16 <= shape[3] <= 256:
+            self._fault(what, f"head size {shape[3]} is not supported (a multiple of 16, at most 256)")
+        return shape
 
     def qk_norm_rope_write_8bit(self, qkv, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps,
                                 table, positions, slot_mapping, q_out, k_cache, v_cache, k_scale, v_scale):
@@ -874,69 +894,81 @@ class CudaOps:
         slots follow it.  The tokens of one page stand together in the call (tokens without a slot may
         stand between them), and each slot comes once (of several tokens for one slot the last is kept)."""
         what = "qk_norm_rope_write_8bit"
-        _code(qkv.dtype)
-        self._need_here(what, qkv, q_weight, k_weight, positions, slot_mapping, q_out, k_cache, v_cache,
-                        k_scale, v_scale, *(table or ()))
+        dtype = qkv.dtype
+        code = _code(dtype)
+        f32, i32 = torch.float32, torch.int32
         if num_heads <= 0 or num_kv_heads <= 0:
-            raise KernelError(f"{what}: invalid head counts: {num_heads} query, {num_kv_heads} KV")
-        self._need_rows(what, qkv, (num_heads + 2 * num_kv_heads) * head_dim)
-        n = qkv.shape[0]
-        self._need(q_out, "query rows", qkv.dtype)
+            self._fault(what, f"invalid head counts: {num_heads} query, {num_kv_heads} KV")
+        n, stride = self._row_shape(what, qkv, (num_heads + 2 * num_kv_heads) * head_dim)
+        self._held(what, (q_out, "query rows", dtype), (k_cache, "key pages", torch.int8),
+                   (v_cache, "value pages", torch.int8), (k_scale, "key scales", f32), (v_scale, "value scales", f32),
+                   (slot_mapping, "slots", i32))
+        pages, heads, page_size, dim = self._page_shape(what, k_cache, k_scale, v_cache, v_scale)
+        if heads != num_kv_heads or dim != head_dim:
+            self._fault(what, f"pages of {heads} heads of {dim}, asked for {num_kv_heads} of {head_dim}")
         if q_out.shape != (n, num_heads * head_dim):
-            raise KernelError(f"{what}: the query rows have another shape")
-        self._need_pages_8bit(what, k_cache, k_scale, num_kv_heads, head_dim)
-        self._need_pages_8bit(what, v_cache, v_scale, num_kv_heads, head_dim)
-        if k_cache.shape != v_cache.shape:
-            raise KernelError(f"{what}: key and value pages differ in shape")
+            self._fault(what, "the query rows have another shape")
+        if slot_mapping.dim() != 1 or slot_mapping.size(0) < n:
+            self._fault(what, "a slot for every token")
         for w in (q_weight, k_weight):
             if w is not None:
-                self._need(w, "norm weight", torch.float32)
+                self._held(what, (w, "norm weight", f32))
                 if w.shape != (head_dim,):
-                    raise KernelError(f"{what}: a norm weight has another width")
-        self._need_index("slots", slot_mapping, n)
-        cos, sin = table if table is not None else (None, None)
+                    self._fault(what, "a norm weight has another width")
+        cos = sin = at = None
+        angles = 0
         if table is not None:
-            self._need_index("positions", positions, n)
-            for t in (cos, sin):
-                self._need(t, "rotation table", torch.float32)
-                if t.shape != (cos.shape[0], head_dim // 2):
-                    raise KernelError(f"{what}: a rotation table has another width")
-        self._check(self.lib.rv_qk_norm_rope_write_8bit(
-            _ptr(qkv), c_int(_code(qkv.dtype)), c_longlong(qkv.stride(0)), c_int(n), c_int(num_heads), c_int(num_kv_heads),
-            c_int(head_dim), _ptr(q_weight), _ptr(k_weight), c_float(eps), _ptr(cos), _ptr(sin),
-            c_longlong(cos.shape[0] if cos is not None else 0), _ptr(positions), _ptr(slot_mapping), _ptr(q_out),
-            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), c_longlong(k_cache.shape[0]),
-            c_int(k_cache.shape[2]), self._stream()), what)
+            cos, sin = table
+            self._held(what, (cos, "rotation table", f32), (sin, "rotation table", f32), (positions, "positions", i32))
+            if cos.dim() != 2 or cos.size(1) != head_dim // 2 or sin.shape != cos.shape:
+                self._fault(what, "a rotation table has another width")
+            if positions.dim() != 1 or positions.size(0) < n:
+                self._fault(what, "a position for every token")
+            angles, at = cos.size(0), positions.data_ptr()
+        self._check(self._write_8bit(
+            qkv.data_ptr(), code, stride, n, num_heads, num_kv_heads, head_dim,
+            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), angles, at, slot_mapping.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), pages, page_size, self._stream()), what)
 
     def read_8bit(self, cache, scale, pages, dtype):
         """The pages `pages` (int32 [n]) of an 8-bit cache as values, `dtype` [n, kv heads, page size,
-        head_dim] (exact in bfloat16 too, but for scales near the ends of their range).  A number that is no page
-        gives zeros."""
-        self._need_here("read_8bit", cache, scale, pages)
-        self._need_pages_8bit("read_8bit", cache, scale)
-        self._need_index("pages", pages, 0)
-        out = torch.empty((pages.shape[0],) + cache.shape[1:], dtype=dtype, device=cache.device)
-        self._check(self.lib.rv_read_8bit(
-            _ptr(cache), _ptr(scale), _ptr(pages), _ptr(out), c_int(_code(dtype)), c_int(pages.shape[0]),
-            c_int(cache.shape[1]), c_int(cache.shape[2]), c_int(cache.shape[3]), c_longlong(cache.shape[0]),
-            self._stream()), "read_8bit")
+        head_dim] (exact in bfloat16 too).  A number that is no page gives zeros."""
+        what = "read_8bit"
+        code = _code(dtype)
+        self._held(what, (cache, "8-bit pages", torch.int8), (scale, "scales", torch.float32),
+                   (pages, "page numbers", torch.int32))
+        have, heads, page_size, dim = self._page_shape(what, cache, scale)
+        if pages.dim() != 1:
+            self._fault(what, "page numbers are one row")
+        n = pages.size(0)
+        out = torch.empty((n, heads, page_size, dim), dtype=dtype, device=cache.device)
+        self._check(self._read_8bit(cache.data_ptr(), scale.data_ptr(), pages.data_ptr(), out.data_ptr(), code, n, heads,
+                                    page_size, dim, have, self._stream()), what)
         return out
 
     def _attn8_lib(self, head_dim: int):
-        """The library for attention over 8-bit pages with heads of this size, built at first use."""
+        """The functions for attention over 8-bit pages with heads of this size (call, scratch, last error), built
+        at first use."""
         key = ("8bit", head_dim)
-        lib = self._attn_libs.get(key)
-        if lib is None:
+        hit = self._attn_libs.get(key)
+        if hit is None:
             path = build_variant("attention_8bit.cu", {"RV_HD": head_dim}, f"attn8_hd{head_dim}",
                                  verbose=self._verbose_build)
             try:
                 lib = ctypes.CDLL(path)
             except OSError as e:
                 raise KernelError(f"cannot load the kernel library {path}: {e}") from None
-            getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}").restype = ctypes.c_char_p
-            getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}").restype = c_longlong
-            self._attn_libs[key] = lib
-        return lib
+            error = getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}")
+            error.restype = ctypes.c_char_p
+            call = getattr(lib, f"rv_paged_attention_8bit_hd{head_dim}")
+            P, I, L = c_void_p, c_int, c_longlong
+            call.argtypes = [P, I, L, P, P, P, P, L, P, I, P, P, P, P, L, I, I, I, I, I, I, I, I, c_float, I, P, I, P]
+            scratch = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")
+            scratch.restype = c_longlong
+            scratch.argtypes = [I] * 8
+            hit = self._attn_libs[key] = (call, scratch, error)
+        return hit
 
     def paged_attention_8bit(self, q, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale,
                              ctx, group, scale, window, out, sinks=None):
@@ -947,47 +979,48 @@ class CudaOps:
         block-table entry is no page are not seen; a context longer than the table gives NaN.  Scratch is
         allocated per call (in a captured graph: from the graph's pool)."""
         what = "paged_attention_8bit"
-        _code(q.dtype)
-        self._need_here(what, q, k_cache, v_cache, k_scale, v_scale, out, sinks, group.block_table,
-                        ctx.q_start, ctx.ctx_lens)
+        dtype = q.dtype
+        code = _code(dtype)
+        f32, i32 = torch.float32, torch.int32
         if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
-            raise KernelError(f"{what}: invalid head counts: {num_heads} query, {num_kv_heads} KV")
-        self._need_pages_8bit(what, k_cache, k_scale, num_kv_heads, head_dim)
-        self._need_pages_8bit(what, v_cache, v_scale, num_kv_heads, head_dim)
-        if k_cache.shape != v_cache.shape or k_cache.shape[2] != group.page_size:
-            raise KernelError(f"{what}: key pages, value pages and the page size disagree")
-        self._need_rows(what, q, num_heads * head_dim)
-        self._need(out, "attention output", q.dtype)
-        if out.shape != (q.shape[0], num_heads * head_dim) or q.shape[0] < ctx.n_tokens:
-            raise KernelError(f"{what}: output, rows and head counts disagree")
-        if not 0 <= ctx.n_decode <= ctx.n_reqs or ctx.n_tokens < ctx.n_decode:
-            raise KernelError(f"{what}: {ctx.n_decode} single tokens among {ctx.n_reqs} requests, {ctx.n_tokens} tokens")
-        self._need_index("context lengths", ctx.ctx_lens, ctx.n_reqs)
-        self._need_index("first tokens", ctx.q_start, ctx.n_reqs + 1)
-        self._need(group.block_table, "block table", torch.int32)
-        if group.block_table.dim() != 2 or group.block_table.shape[0] < ctx.n_reqs:
-            raise KernelError(f"{what}: a row of the block table for every request")
-        if window is not None and window < 0:
-            raise KernelError(f"{what}: a window of {window}")
+            self._fault(what, f"invalid head counts: {num_heads} query, {num_kv_heads} KV")
+        table, q_start, ctx_lens = group.block_table, ctx.q_start, ctx.ctx_lens
+        n_decode, n_reqs, n_tokens = ctx.n_decode, ctx.n_reqs, ctx.n_tokens
+        n, stride = self._row_shape(what, q, num_heads * head_dim)
+        self._held(what, (k_cache, "key pages", torch.int8), (v_cache, "value pages", torch.int8),
+                   (k_scale, "key scales", f32), (v_scale, "value scales", f32), (out, "attention output", dtype),
+                   (table, "block table", i32), (q_start, "first tokens", i32), (ctx_lens, "context lengths", i32))
+        pages, heads, page_size, dim = self._page_shape(what, k_cache, k_scale, v_cache, v_scale)
+        if heads != num_kv_heads or dim != head_dim or page_size != group.page_size:
+            self._fault(what, f"pages of {heads} heads of {dim}, {page_size} tokens each, asked for {num_kv_heads} of "
+                              f"{head_dim}, {group.page_size} tokens")
+        if n < n_tokens or out.shape != (n, num_heads * head_dim):
+            self._fault(what, "output, rows and head counts disagree")
+        if not 0 <= n_decode <= n_reqs or n_tokens < n_decode:
+            self._fault(what, f"{n_decode} single tokens among {n_reqs} requests, {n_tokens} tokens")
+        if ctx_lens.numel() < n_reqs or q_start.numel() <= n_reqs or table.dim() != 2 or table.size(0) < n_reqs:
+            self._fault(what, "a length, a first token and a row of the block table for every request")
+        window = window or 0
+        if window < 0:
+            self._fault(what, f"a window of {window}")
         if sinks is not None:
-            self._need(sinks, "sinks", torch.float32)
+            self._held(what, (sinks, "sinks", f32))
             if sinks.shape != (num_heads,):
-                raise KernelError(f"{what}: one sink per query head")
-        lib, win = self._attn8_lib(head_dim), c_int(window if window else 0)
-        portions = ctx.n_tokens > ctx.n_decode
-        sizes = (c_int(ctx.max_q_len), c_int(ctx.max_ctx_len), c_int(num_heads), c_int(num_kv_heads))
-        need = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")(
-            c_int(ctx.n_decode), c_int(ctx.n_reqs if portions else ctx.n_decode), *sizes, win, c_int(self._sm_count))
+                self._fault(what, "one sink per query head")
+        call, scratch_bytes, error = self._attn8_lib(head_dim)
+        portions = n_tokens > n_decode
+        longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
+        need = scratch_bytes(n_decode, n_reqs if portions else n_decode, longest, deepest, num_heads, num_kv_heads, window,
+                             sms)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        rc = getattr(lib, f"rv_paged_attention_8bit_hd{head_dim}")(
-            _ptr(q), c_int(_code(q.dtype)), c_longlong(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-            _ptr(v_scale), c_longlong(k_cache.shape[0]), _ptr(group.block_table), c_int(group.block_table.shape[1]),
-            _ptr(ctx.q_start), _ptr(ctx.ctx_lens), _ptr(out), _ptr(scratch), c_longlong(need), c_int(ctx.n_decode),
-            c_int(ctx.n_reqs), c_int(portions), *sizes, c_int(group.page_size), c_float(scale), win, _ptr(sinks),
-            c_int(self._sm_count), self._stream())
-        self.launches += (2 if ctx.n_decode else 0) + (1 if portions else 0)
+        rc = call(q.data_ptr(), code, stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                  v_scale.data_ptr(), pages, table.data_ptr(), table.size(1), q_start.data_ptr(), ctx_lens.data_ptr(),
+                  out.data_ptr(), None if scratch is None else scratch.data_ptr(), need, n_decode, n_reqs, portions,
+                  longest, deepest, num_heads, num_kv_heads, page_size, scale, window,
+                  None if sinks is None else sinks.data_ptr(), sms, self._stream())
+        self.launches += (2 if n_decode else 0) + portions
         if rc != 0:
-            raise KernelError(getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}")().decode())
+            raise KernelError(error().decode())
 
     # ---- gated short convolution -----------------------------------------------------
 
@@ -1902,17 +1935,20 @@ class CudaOps:
         there are not enough others)."""
         what = "token_logprobs"
         code = _code(logits.dtype)
-        self._need_here(what, logits, tokens)
-        self._need_rows(what, logits)
-        rows, vocab = logits.shape
-        self._need_index("tokens", tokens, rows)
-        if vocab < 1 or not 0 <= top <= min(32, vocab):
-            raise KernelError(f"{what}: {top} alternatives of {vocab} (0 to 32)")
-        floats = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
-        rank = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        best = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        self._check(self.lib.rv_token_logprobs(
-            _ptr(logits), c_int(code), c_longlong(logits.stride(0)), c_int(rows), c_int(vocab), _ptr(tokens), c_int(top),
-            _ptr(floats[0]), _ptr(rank), _ptr(floats[1]), _ptr(best), _ptr(ids), self._stream()), what)
-        return floats[0], rank, floats[1], best, ids
+        rows, stride = self._row_shape(what, logits, 1)
+        vocab = logits.size(1)
+        self._held(what, (tokens, "tokens", torch.int32))
+        if tokens.dim() != 1 or tokens.size(0) != rows:
+            self._fault(what, "a token for every row")
+        if not 0 <= top <= min(32, vocab):
+            self._fault(what, f"{top} alternatives of {vocab} (0 to 32)")
+        f32, i32, device = torch.float32, torch.int32, logits.device
+        logprob = torch.empty(rows, dtype=f32, device=device)
+        entropy = torch.empty(rows, dtype=f32, device=device)
+        rank = torch.empty(rows, dtype=i32, device=device)
+        best = torch.empty((rows, top), dtype=f32, device=device)
+        ids = torch.empty((rows, top), dtype=i32, device=device)
+        self._check(self._token_logprobs(
+            logits.data_ptr(), code, stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(),
+            entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), self._stream()), what)
+        return logprob, rank, entropy, best, ids
