@@ -43,6 +43,7 @@ template <int NT, int PARTS> constexpr int a8_warps() {
     return A8_HD <= 64 ? (NT * PARTS == 1 ? 16 : NT * PARTS == 2 ? 12 : 8) : A8_HD <= 192 ? 8 : 6;
 }
 #define A8_MOST_WARPS 16
+#define A8_CLUSTER 8                                              // blocks of a cluster at most
 #define A8_BLOCK_WARPS (A8_HD <= 192 ? 4 : 3)
 
 #ifndef A8_STAGES
@@ -61,7 +62,7 @@ struct A8Args {
     float* part_o;                     // [places][rows][HD]
     float2* part_ml;                   // [places][rows]: M, l
     long long q_stride, pages;
-    int max_blocks, first_req, n_reqs, num_heads, num_kv_heads, page_size, page_shift, window, nsplit, row_tiles, vec;
+    int max_blocks, first_req, n_reqs, num_heads, num_kv_heads, page_size, page_shift, window, nsplit, vec;
     float scale_log2;
 };
 
@@ -567,26 +568,6 @@ struct A8Warp {
                     *(float2*)(a.part_o + at * A8_HD + 16 * c + 2 * g) = make_float2(o[c][n][j], o[c][n][2 + j]);
             }
     }
-    __device__ __forceinline__ void write() {
-        finish();
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = 8 * n + 2 * t + j;
-                if (row >= rows_count) continue;
-                const int i = rows_first + row, tok = i / G, head = kvh * G + i - tok * G;
-                float L = l[n][j];
-                if (a.sinks && L != 0.f) L += a8_exp2(a.sinks[head] * 1.4426950408889634f - M[n][j]);
-                const float by = L == 0.f ? 0.f : 1.f / L;
-                T* dst = (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD + 2 * g;
-#pragma unroll
-                for (int c = 0; c < A8_CHUNKS; ++c) {
-                    rv_store(dst + 16 * c, o[c][n][j] * by);
-                    rv_store(dst + 16 * c + 1, o[c][n][2 + j] * by);
-                }
-            }
-    }
 };
 
 #define A8_WAIT_STAGE() asm volatile("cp.async.wait_group %0;" ::"n"(A8_STAGES - 2) : "memory")
@@ -685,30 +666,76 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
     }
 }
 
-// Requests [first_req, first_req + n_reqs) with any number of tokens.  A warp: (request, key/value head, 8 NT rows,
-// part of their tiles).  blockIdx.z: request, y: head, x and warp: rows and part.
-template <typename T, int NT, int PARTS>
-__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_rows_kernel(const __grid_constant__ A8Args a) {
+// ---- rows whose tiles a warp, a block or a cluster of blocks has ---------------------------------------------
+__device__ __forceinline__ unsigned a8_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void a8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 a8_remote(const void* p, int rank) {
+    unsigned at;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(a8_smem(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+// What N parts of a row come to: their M and l (ml) and two of their dimensions.  A part with l = 0 weighs nothing.
+template <int N>
+__device__ __forceinline__ void a8_join(const float2 (&ml)[N], const float2 (&v)[N], float2& all, float2& o) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) M = fmaxf(M, ml[i].x);
+    const float off = M == -INFINITY ? 0.f : M;
+    all = make_float2(M, 0.f);
+    o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float w = a8_exp2(ml[i].x - off);
+        all.y += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * w;        // (without a reference: 0, or not a number)
+        o.x = fmaf(v[i].x, w, o.x);
+        o.y = fmaf(v[i].y, w, o.y);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void a8_put(const A8Args& a, int row_token, int head, int dim, float2 all, float2 o) {
+    float L = all.y;
+    if (a.sinks && L != 0.f) L += a8_exp2(a.sinks[head] * 1.4426950408889634f - all.x);       // a sink counts once
+    const float by = L == 0.f ? 0.f : 1.f / L;
+    T* dst = (T*)a.out + ((size_t)row_token * a.num_heads + head) * A8_HD + dim;
+    rv_store(dst, o.x * by);
+    rv_store(dst + 1, o.y * by);
+}
+
+// Requests [first_req, first_req + n_reqs) with any number of tokens.  blockIdx.z: request, y: key/value head, x: 8 NT rows
+// a warp (nsplit 0), or a cluster of nsplit blocks: their warps share the rows' tiles and meet in the blocks'
+// shared memory, then in the cluster's.
+template <typename T, int NT, int PARTS, bool SHARED>
+__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_rows_kernel(
+    const __grid_constant__ A8Args a) {
     rv_pdl_prologue();
     extern __shared__ __align__(128) unsigned char smem[];
-    const int id = blockIdx.x * A8_BLOCK_WARPS + (threadIdx.x >> 5);
-    const int rt = id / a.nsplit, part = id - rt * a.nsplit;
+    const int warp = threadIdx.x >> 5, rank = SHARED && a.nsplit > 1 ? (int)a8_rank() : 0;
+    const int rt = SHARED ? blockIdx.x / a.nsplit : blockIdx.x * A8_BLOCK_WARPS + warp;
+    const int parts = SHARED ? a.nsplit * A8_BLOCK_WARPS : 1, part = SHARED ? rank * A8_BLOCK_WARPS + warp : 0;
     const int r = a.first_req + blockIdx.z, head = blockIdx.y;
     const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs, clen = a.ctx_lens[r];
-    A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
+    A8Warp<T, NT, PARTS> w(a, smem + warp * A8_WARP_BYTES);
     // the rows with the longest contexts first
     const int tiles = (qlen * w.G + 8 * NT - 1) / (8 * NT);
-    if (rt >= tiles) return;
+    if (rt >= tiles) return;                                           // (a whole cluster)
     const int first = (tiles - 1 - rt) * 8 * NT;
     const int end = min(qlen * w.G, first + 8 * NT);
     const int p_first = clen - qlen + first / w.G, p_last = clen - qlen + (end - 1) / w.G;
     const bool fits = clen <= (long long)a.max_blocks * a.page_size;
     const int t_all = (a.window > 0 ? max(0, p_first - a.window + 1) : 0) / A8_KEYS;
     const int count = p_last >= 0 && fits ? p_last / A8_KEYS - t_all + 1 : 0;
-    const int t_lo = t_all + (int)((long long)count * part / a.nsplit), n = t_all + (int)((long long)count * (part + 1) / a.nsplit) - t_lo;
-    w.begin(r, head, first, qlen, qs, clen);
+    const int t_lo = t_all + (int)((long long)count * part / parts), n = t_all + (int)((long long)count * (part + 1) / parts) - t_lo;
     A8Cursor ahead = {r, 0, t_lo, t_lo + n - 1, clen};
-    int page = w.page_of(ahead), requested = 0;
+    int page = n > 0 ? w.page_of(ahead) : -1, requested = 0;
     auto request_next = [&](int stage) {
         if (requested < n) {
             w.request(ahead, head, page, stage);
@@ -718,6 +745,7 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
         A8_COMMIT();
     };
     for (int i = 0; i < A8_STAGES - 1; ++i) request_next(i);
+    w.begin(r, head, first, qlen, qs, clen);
     int stage = 0;
     for (int i = 0; i < n; ++i) {
         A8_WAIT_STAGE();
@@ -731,10 +759,74 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
 #pragma unroll
         for (int k = 0; k < NT; ++k) w.l[k][0] = w.l[k][1] = NAN;      // more keys than the table holds
     }
-    if (a.nsplit > 1)
-        w.leave((((size_t)blockIdx.z * a.num_kv_heads + head) * a.row_tiles + rt) * a.nsplit + part);
-    else
-        w.write();
+    w.finish();
+    if constexpr (!SHARED) {
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = first + 8 * k + 2 * w.t + j, tok = i / w.G;
+                if (i < end)
+#pragma unroll
+                    for (int c = 0; c < A8_CHUNKS; ++c)
+                        a8_put<T>(a, qs + tok, head * w.G + i - tok * w.G, 16 * c + 2 * w.g, make_float2(w.M[k][j], w.l[k][j]),
+                                  make_float2(w.o[c][k][j], w.o[c][k][2 + j]));
+            }
+    } else {
+        // [row][HD + 8] of a warp, in the place of its ring (every copy into it has been waited for)
+        constexpr int STRIDE = A8_HD + 8;
+        static_assert(8 * NT * STRIDE * 4 <= A8_WARP_BYTES, "a warp's rows fit its ring");
+        __shared__ float2 ml[A8_BLOCK_WARPS][8 * NT], ml_block[8 * NT];
+        float* rows_of = (float*)(smem + warp * A8_WARP_BYTES);
+#pragma unroll
+        for (int k = 0; k < NT; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = 8 * k + 2 * w.t + j;
+                if (w.g == 0) ml[warp][row] = make_float2(w.M[k][j], w.l[k][j]);
+#pragma unroll
+                for (int c = 0; c < A8_CHUNKS; ++c)
+                    *(float2*)(rows_of + row * STRIDE + 16 * c + 2 * w.g) = make_float2(w.o[c][k][j], w.o[c][k][2 + j]);
+            }
+        __syncthreads();
+        const int rows = end - first;
+        for (int i = threadIdx.x; i < rows * (A8_HD / 2); i += A8_BLOCK_WARPS * 32) {
+            const int row = i / (A8_HD / 2), dim = (i - row * (A8_HD / 2)) * 2, at = row * STRIDE + dim;
+            float2 m[A8_BLOCK_WARPS], v[A8_BLOCK_WARPS], all, o;
+#pragma unroll
+            for (int k = 0; k < A8_BLOCK_WARPS; ++k) {
+                m[k] = ml[k][row];
+                v[k] = *(const float2*)((const float*)(smem + k * A8_WARP_BYTES) + at);
+            }
+            a8_join(m, v, all, o);
+            if (a.nsplit == 1) {
+                const int x = first + row, tok = x / w.G;
+                a8_put<T>(a, qs + tok, head * w.G + x - tok * w.G, dim, all, o);
+            } else {
+                *(float2*)((float*)smem + at) = o;                     // nobody else's
+                if (dim == 0) ml_block[row] = all;
+            }
+        }
+        if (a.nsplit == 1) return;
+        a8_cluster_sync();
+        for (int i = rank * A8_BLOCK_WARPS * 32 + threadIdx.x; i < rows * (A8_HD / 2); i += a.nsplit * A8_BLOCK_WARPS * 32) {
+            const int row = i / (A8_HD / 2), dim = (i - row * (A8_HD / 2)) * 2, at = row * STRIDE + dim;
+            float2 m[A8_CLUSTER], v[A8_CLUSTER], all, o;
+#pragma unroll
+            for (int k = 0; k < A8_CLUSTER; ++k) {
+                m[k] = make_float2(-INFINITY, 0.f);
+                v[k] = make_float2(0.f, 0.f);
+                if (k < a.nsplit) {
+                    m[k] = a8_remote(&ml_block[row], k);
+                    v[k] = a8_remote((const float*)smem + at, k);
+                }
+            }
+            a8_join(m, v, all, o);
+            const int x = first + row, tok = x / w.G;
+            a8_put<T>(a, qs + tok, head * w.G + x - tok * w.G, dim, all, o);
+        }
+        a8_cluster_sync();                                             // nobody leaves while its rows are read
+    }
 }
 
 // ---- segments put together, in order --------------------------------------------------------------------
@@ -836,21 +928,6 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_m
                    (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
 }
 
-// blockIdx.z: request, y: key/value head, x: rows.
-template <typename T, int NT, int W>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_rows_merge_kernel(const __grid_constant__ A8Args a) {
-    rv_pdl_prologue();
-    const int G = a.num_heads / a.num_kv_heads, r = a.first_req + blockIdx.z, kvh = blockIdx.y;
-    const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs;
-    const int tiles = (qlen * G + 8 * NT - 1) / (8 * NT);
-    const int i = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;         // the row
-    if (i >= qlen * G) return;
-    const int rt = tiles - 1 - i / (8 * NT), tok = i / G, head = kvh * G + i - tok * G;
-    if (rt >= a.row_tiles) return;                                     // a longer portion than the launch was told of
-    a8_merge<T, W>(a, (((size_t)blockIdx.z * a.num_kv_heads + kvh) * a.row_tiles + rt) * a.nsplit, a.nsplit, 8 * NT,
-                   i % (8 * NT), head, (T*)a.out + ((size_t)(qs + tok) * a.num_heads + head) * A8_HD, false);
-}
-
 // ---- host side ----------------------------------------------------------------------------------------
 static thread_local char g_a8_error[512] = "";
 #define A8_FAIL(...) do { snprintf(g_a8_error, sizeof(g_a8_error), __VA_ARGS__); return 1; } while (0)
@@ -860,51 +937,42 @@ static thread_local char g_a8_error[512] = "";
 
 extern "C" const char* A8_SYM(rv_attention_8bit_last_error)() { return g_a8_error; }
 
-static int a8_waves(){ static int w=[]{const char*e=getenv("A8W");return e?atoi(e):1;}(); return w; }
 // Rows of a warp: 16 where a key/value head has more than 8 of them and the accumulators fit the registers.
-static int a8_nt(int rows) { return rows > 8 && A8_HD <= 128 ? 2 : 1; }
+static int a8_nt(long long rows) { return rows > 8 && A8_HD <= 128 ? 2 : 1; }
 static long long a8_place_bytes(int nt) { return 8ll * nt * (A8_HD * 4 + 8); }
 
-// How many warps share the tiles of 8 NT rows of a portion: until there are warps for every place of the GPU, four
-// tiles each at least.
-static int a8_nsplit(long long warps, int max_ctx_len, int window, int max_q_len, int n_sms) {
-    const long long places = 8ll * n_sms;
+static long long a8_tiles(int max_ctx_len, int window, int max_q_len) {
     long long keys = max_ctx_len;
     if (window > 0 && (long long)window + max_q_len < keys) keys = (long long)window + max_q_len;
-    const long long most = (keys + A8_KEYS - 1) / A8_KEYS / 4;
-    long long n = warps > 0 ? places / warps : 1;
-    if (n > most) n = most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    return (keys + A8_KEYS - 1) / A8_KEYS;
 }
-static long long a8_rows_places(int n_reqs, int max_q_len, int max_ctx_len, int num_heads, int num_kv_heads, int window, int n_sms,
-                                int* nsplit, int* row_tiles) {
-    const int G = num_heads / num_kv_heads;
-    const long long rows = (long long)max_q_len * G;
-    const int nt = a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows);
-    *row_tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
-    const long long warps = (long long)*row_tiles * num_kv_heads * n_reqs;
-    *nsplit = a8_nsplit(warps, max_ctx_len, window, max_q_len, n_sms);
-    return *nsplit > 1 ? warps * *nsplit : 0;
+// Blocks whose warps share the tiles of 8 NT rows: 0 (a warp has them alone) where there are warps enough, else as many as the
+// GPU holds at once, up to a cluster, while every warp has a tile.  (us by warps alone / a block / two / four / eight: 32 / 8
+// heads of 64, 128 requests of 700 keys 35 / 25 / 35 / 54 / 85, 32 of 1,000 23 / 12.4 / 12.5 / 18 / 26, 16 of 4,000 72 / 27 / 22 / 18.5 / 23.)
+static int a8_nsplit(long long units, long long tiles, int block_places) {
+    if (units > 4ll * block_places || tiles < 2) return 0;
+    int n = 1;
+    while (2 * n <= A8_CLUSTER && units * 2 * n <= block_places && tiles >= 2ll * n * A8_BLOCK_WARPS) n *= 2;
+    return n;
+}
+// Single tokens by blocks or clusters, which need no scratch and no second launch, but take as long as the longest context: while
+// a warp has no more than eight tiles of that, in two rounds at most.  (us so / by the stream: 32 / 8 heads of 64, 1 request of
+// 700 keys 6.3 / 8.3, 64 of 100 8.3 / 12.4, 64 of 700 14 / 18.5, 128 of 700 25 / 27, 16 of 4,000 18.5 / 20.7; 8 / 8 heads of 128,
+// 32 of 1,000 14 / 19, 128 of 300 (1,024 blocks for 296 places) 27 / 23.  64 of 2,000 alike would take 29 / 33 too, but of
+// 2,340 to 3,900 52 / 44.)
+static bool a8_few(long long units, long long tiles, int n_sms) {
+    const int places = (A8_HD <= 64 ? 4 : 2) * n_sms;
+    const int n = a8_nsplit(units, tiles, places);
+    return units <= 2ll * places && tiles <= 8ll * A8_BLOCK_WARPS * (n ? n : 1);
 }
 
-// Scratch for a call: requests [0, n_decode) with one token, [n_decode, n_reqs) with up to max_q_len.
-extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode, int n_reqs, int max_q_len, int max_ctx_len,
-                                                                   int num_heads, int num_kv_heads, int window, int n_sms) {
-    const int G = num_heads / num_kv_heads;
-    long long need = 0;
-    if (n_decode > 0) {
-        const int nt = a8_nt(G);
-        const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
-        need = ((long long)n_sms * A8_MOST_WARPS * a8_waves() + n_decode * units) * a8_place_bytes(nt);
-    }
-    if (n_reqs > n_decode) {
-        int nsplit, row_tiles;
-        const long long rows = (long long)max_q_len * G;
-        const long long b = a8_rows_places(n_reqs - n_decode, max_q_len, max_ctx_len, num_heads, num_kv_heads, window, n_sms,
-                                           &nsplit, &row_tiles) * a8_place_bytes(a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows));
-        if (b > need) need = b;
-    }
-    return need;
+// Scratch for single tokens: requests [0, n_decode).
+extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode, int max_ctx_len, int num_heads, int num_kv_heads,
+                                                                   int window, int n_sms) {
+    const int G = num_heads / num_kv_heads, nt = a8_nt(G);
+    const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
+    if (n_decode <= 0 || a8_few(units * n_decode, a8_tiles(max_ctx_len, window, 1), n_sms)) return 0;
+    return ((long long)n_sms * A8_MOST_WARPS + n_decode * units) * a8_place_bytes(nt);
 }
 
 // The limit of shared memory is a kernel's on a device: raised once on each.
@@ -923,7 +991,7 @@ extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode,
 template <typename T, int NT, int PARTS>
 static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
     const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
-    const int blocks = n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) * a8_waves();
+    const int blocks = n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS);
     auto kernel = attention_8bit_stream_kernel<T, NT, PARTS>;
     A8_CONFIGURE(kernel, smem);
     const int G = a.num_heads / a.num_kv_heads;
@@ -942,24 +1010,52 @@ static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
     return 0;
 }
 template <typename T, int NT, int PARTS>
-static int a8_rows(A8Args a, int max_q_len, cudaStream_t stream) {
+static int a8_rows(A8Args a, int max_q_len, int max_ctx_len, int n_sms, cudaStream_t stream) {
     const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
-    auto kernel = attention_8bit_rows_kernel<T, NT, PARTS>;
-    A8_CONFIGURE(kernel, smem);
-    a.part_ml = (float2*)(a.part_o + (long long)a.row_tiles * a.num_kv_heads * a.n_reqs * a.nsplit * 8 * NT * A8_HD);
-    const long long warps = (long long)a.row_tiles * a.nsplit;
-    rv_launch(kernel,
-              dim3((unsigned)((warps + A8_BLOCK_WARPS - 1) / A8_BLOCK_WARPS), a.num_kv_heads, a.n_reqs), dim3(A8_BLOCK_WARPS * 32), smem,
-              stream, a);
-    if (a.nsplit > 1) {
-        const long long rows = (long long)max_q_len * (a.num_heads / a.num_kv_heads);
-        if (a.nsplit > 8)
-            rv_launch(attention_8bit_rows_merge_kernel<T, NT, 8>, dim3((unsigned)rows, a.num_kv_heads, a.n_reqs), dim3(256), 0, stream, a);
-        else
-            rv_launch(attention_8bit_rows_merge_kernel<T, NT, 1>, dim3((unsigned)((rows + 3) / 4), a.num_kv_heads, a.n_reqs), dim3(128),
-                      0, stream, a);
+    const long long rows = (long long)max_q_len * (a.num_heads / a.num_kv_heads);
+    if (rows > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
+    const int row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
+    a.nsplit = a8_nsplit((long long)row_tiles * a.num_kv_heads * a.n_reqs, a8_tiles(max_ctx_len, a.window, max_q_len),
+                         n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS));
+    if (a.nsplit == 0) {
+        auto kernel = attention_8bit_rows_kernel<T, NT, PARTS, false>;
+        A8_CONFIGURE(kernel, smem);
+        rv_launch(kernel, dim3((unsigned)((row_tiles + A8_BLOCK_WARPS - 1) / A8_BLOCK_WARPS), a.num_kv_heads, a.n_reqs),
+                  dim3(A8_BLOCK_WARPS * 32), smem, stream, a);
+        return 0;
     }
+    auto kernel = attention_8bit_rows_kernel<T, NT, PARTS, true>;
+    A8_CONFIGURE(kernel, smem);
+    if ((long long)row_tiles * a.nsplit > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(row_tiles * a.nsplit), a.num_kv_heads, a.n_reqs);
+    cfg.blockDim = dim3(A8_BLOCK_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = rv_pdl_enabled();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.nsplit;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.nsplit > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) A8_FAIL("paged_attention_8bit: %s", cudaGetErrorString(e));
     return 0;
+}
+template <typename T, int PARTS>
+static int a8_portions(const A8Args& a, int max_q_len, int max_ctx_len, int n_sms, cudaStream_t stream) {
+    return a8_nt(max_q_len * (long long)(a.num_heads / a.num_kv_heads)) == 1
+               ? a8_rows<T, 1, PARTS>(a, max_q_len, max_ctx_len, n_sms, stream)
+               : a8_rows<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, max_q_len, max_ctx_len, n_sms, stream);
+}
+template <typename T, int PARTS>
+static int a8_singles(const A8Args& a, int max_ctx_len, int n_sms, cudaStream_t stream) {
+    const int G = a.num_heads / a.num_kv_heads, nt = a8_nt(G);
+    if (a8_few((long long)a.n_reqs * a.num_kv_heads * ((G + 8 * nt - 1) / (8 * nt)), a8_tiles(max_ctx_len, a.window, 1), n_sms))
+        return a8_portions<T, PARTS>(a, 1, max_ctx_len, n_sms, stream);
+    return nt == 1 ? a8_stream<T, 1, PARTS>(a, n_sms, stream) : a8_stream<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, n_sms, stream);
 }
 
 // Requests [0, n_decode) bring one token each, [n_decode, n_reqs) up to max_q_len; `portions` 0: the former only.
@@ -976,38 +1072,24 @@ extern "C" int A8_SYM(rv_paged_attention_8bit)(
     if (n_reqs > 65535 || num_kv_heads > 65535) A8_FAIL("paged_attention_8bit: too many requests or heads");
     if (pages * num_kv_heads * page_size >= 0xffffffffll) A8_FAIL("paged_attention_8bit: more rows than 32 bits count");
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) A8_FAIL("paged_attention_8bit: pages must be 16-byte aligned");
-    const long long need = A8_SYM(rv_paged_attention_8bit_scratch_bytes)(n_decode, portions ? n_reqs : n_decode, max_q_len,
-                                                                       max_ctx_len, num_heads, num_kv_heads, window, n_sms);
-    if (need > scratch_bytes) A8_FAIL("paged_attention_8bit: scratch too small");
-    const int G = num_heads / num_kv_heads;
+    if (A8_SYM(rv_paged_attention_8bit_scratch_bytes)(n_decode, max_ctx_len, num_heads, num_kv_heads, window, n_sms) > scratch_bytes)
+        A8_FAIL("paged_attention_8bit: scratch too small");
     A8Args a = {q, (const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens, sinks,
                 out, (float*)scratch, nullptr, q_stride, pages, max_blocks, 0, n_decode, num_heads, num_kv_heads, page_size,
-                (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, window, 1, 0, 0, scale * 1.4426950408889634f};
+                (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, window, 0, 0, scale * 1.4426950408889634f};
     a.vec = (uintptr_t)q % 16 == 0 && q_stride * (dtype == RV_DTYPE_F32 ? 4 : 2) % 16 == 0;
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) A8_FAIL("paged_attention_8bit: unknown dtype code %d", dtype);
     if (n_decode > 0) {
-        const int nt = a8_nt(G);
-        int rc;
-        if (dtype == RV_DTYPE_BF16)
-            rc = nt == 1 ? a8_stream<__nv_bfloat16, 1, 1>(a, n_sms, s) : a8_stream<__nv_bfloat16, A8_HD <= 128 ? 2 : 1, 1>(a, n_sms, s);
-        else
-            rc = nt == 1 ? a8_stream<float, 1, 2>(a, n_sms, s) : a8_stream<float, A8_HD <= 128 ? 2 : 1, 2>(a, n_sms, s);
+        const int rc = dtype == RV_DTYPE_BF16 ? a8_singles<__nv_bfloat16, 1>(a, max_ctx_len, n_sms, s)
+                                              : a8_singles<float, 2>(a, max_ctx_len, n_sms, s);
         if (rc) return rc;
     }
     if (portions && n_reqs > n_decode && max_q_len > 0) {
         a.first_req = n_decode;
         a.n_reqs = n_reqs - n_decode;
-        const long long rows = (long long)max_q_len * G;
-        if (rows > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
-        const int nt = a8_nt(rows > 1 << 20 ? 1 << 20 : (int)rows);
-        a8_rows_places(a.n_reqs, max_q_len, max_ctx_len, num_heads, num_kv_heads, window, n_sms, &a.nsplit, &a.row_tiles);
-        int rc;
-        if (dtype == RV_DTYPE_BF16)
-            rc = nt == 1 ? a8_rows<__nv_bfloat16, 1, 1>(a, max_q_len, s)
-                         : a8_rows<__nv_bfloat16, A8_HD <= 128 ? 2 : 1, 1>(a, max_q_len, s);
-        else
-            rc = nt == 1 ? a8_rows<float, 1, 2>(a, max_q_len, s) : a8_rows<float, A8_HD <= 128 ? 2 : 1, 2>(a, max_q_len, s);
+        const int rc = dtype == RV_DTYPE_BF16 ? a8_portions<__nv_bfloat16, 1>(a, max_q_len, max_ctx_len, n_sms, s)
+                                              : a8_portions<float, 2>(a, max_q_len, max_ctx_len, n_sms, s);
         if (rc) return rc;
     }
     const cudaError_t e = cudaGetLastError();

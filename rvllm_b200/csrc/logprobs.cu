@@ -9,10 +9,11 @@
 //
 // The largest: values that may still be among them collect in the block's shared memory, as 64-bit keys (the value's
 // bits in the order of values, then the index reversed: one comparison has both).  What may be is bounded from
-// below, round by round of loads: if r lanes of each of the 8 warps have met a value of at least b, then 8 r values are
-// that large, and with 8 r >= `top` nothing below b is wanted -- r lanes by r maxima over a warp, the smallest of the
-// warps' bounds.  Some tens of values are left at the end; each counts the larger ones, which is its place.  A
-// round that would overflow the memory is taken again with the bound that the values in it give.
+// below: if r lanes of each of the 8 warps have met a value of at least b, then 8 r values are that large, and
+// with 8 r >= `top` nothing below b is wanted -- r lanes by r maxima over a warp when one of its lanes has met a larger value,
+// the smallest of the warps' bounds; warps read one another's without waiting, as bounds only grow.  Some tens of values are
+// left at the end; each counts the larger ones, which is its place.  Where so many qualify that the memory
+// would not hold them (rising rows, values all alike) the row is walked a second time, the block together.
 //
 // A row is a cluster's of 1 to 8 blocks (as many as the GPU has room for when rows are few); parts meet in the
 // first block in a fixed order, so a row's results do not depend on what else is in the launch.
@@ -22,6 +23,7 @@
 #define LP_THREADS 256
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_MAX_CLUSTER 8
+#define LP_RESIDENT 4                  // blocks of a multiprocessor
 #define LP_LOG2E 1.4426950408889634f
 #define LP_LN2 0.6931471805599453f
 
@@ -98,10 +100,10 @@ template <bool TOP> struct LpShared {
 template <> struct LpShared<true> {
     LpPart part[LP_WARPS];
     LpPart whole;
-    u64 room[LP_ROOM];
+    u64 room[LP_ROOM], left[LP_ROOM];
     u64 best[LP_MAX_CLUSTER][32];      // the parts' largest, descending; [0] is what this block leaves
-    unsigned bound[2][LP_WARPS];
-    int count;
+    unsigned bound[LP_WARPS];
+    int count, kept;
 };
 
 // Places `n` keys of `from` by how many are larger; the first `top` of them go to `to`, the rest of `to` is 0.
@@ -123,16 +125,16 @@ struct LpThread {
     static constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U;
     float m = -INFINITY, s = 0.f, w = 0.f;
     int above = 0;
+    bool first = true;
     float given;
     int top;
-    // of the block, the same in every thread: only larger keys are wanted; how many are there
-    u64 least = 0ull;
-    int count = 0, round = 0;
+    u64 least = 0ull;                  // only larger keys are wanted
     LpShared<TOP>& sh;
 
     __device__ __forceinline__ LpThread(LpShared<TOP>& shared, int k, float x) : given(x), top(k), sh(shared) {}
 
-    __device__ __forceinline__ float sums(const float (&x)[E]) {          // the largest x
+    // Of E values: the sums; the largest.
+    __device__ __forceinline__ float sums(const float (&x)[E]) {
         float bm = x[0];
 #pragma unroll
         for (int i = 1; i < E; ++i) bm = fmaxf(bm, x[i]);
@@ -158,68 +160,124 @@ struct LpThread {
         w += w2[0] + w2[1];
         return bm;
     }
-    // E values of every thread of the block: x[i] is column col(i), if real(i).
+    // The r-th largest of a warp's lanes.
+    __device__ __forceinline__ unsigned rth(unsigned mine, int r) const {
+        unsigned b = 0u;
+        for (int k = 0; k < r; ++k) {
+            b = __reduce_max_sync(0xffffffffu, mine);
+            const unsigned who = __ballot_sync(0xffffffffu, mine == b);
+            if ((int)(threadIdx.x & 31) == __ffs(who) - 1) mine = 0u;
+        }
+        return b;
+    }
+    template <typename Col, typename Real>
+    __device__ __forceinline__ void collect(const float (&x)[E], float limit, Col col, Real real) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (x[i] >= limit) {                                     // few
+                const u64 key = ((u64)lp_key(x[i]) << 32) | (0xffffffffu - (unsigned)col(i));
+                if (key > least && real(i)) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < LP_ROOM) sh.room[at] = key;
+                }
+            }
+    }
+    // Adds E values of this thread (the whole block comes here): x[i] is column col(i), if real(i).
     template <typename Col, typename Real>
     __device__ __forceinline__ void take(const float (&x)[E], Col col, Real real) {
-        const float bm = sums(x);
+        const float was = m, bm = sums(x);
         if constexpr (TOP) {
-            const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-            // r lanes' largest so far
-            const int r = (top + LP_WARPS - 1) / LP_WARPS;
-            unsigned mine = m == -INFINITY ? 0u : lp_key(m), b = 0u;
-            for (int k = 0; k < r; ++k) {
-                b = __reduce_max_sync(0xffffffffu, mine);
-                const unsigned who = __ballot_sync(0xffffffffu, mine == b);
-                if (lane == __ffs(who) - 1) mine = 0u;
+            const int lane = threadIdx.x & 31;
+            if (__any_sync(0xffffffffu, m > was)) {
+                const unsigned b = rth(m == -INFINITY ? 0u : lp_key(m), (top + LP_WARPS - 1) / LP_WARPS);
+                if (lane == 0) sh.bound[threadIdx.x >> 5] = b;
+                __syncwarp();
             }
-            unsigned* bounds = sh.bound[round & 1];
-            ++round;
-            if (lane == 0) bounds[warp] = b;
-            __syncthreads();
-            b = bounds[0];
-#pragma unroll
-            for (int k = 1; k < LP_WARPS; ++k) b = min(b, bounds[k]);
-            if (b > (unsigned)(least >> 32)) least = ((u64)b << 32) - 1ull;
-            for (;;) {
-                if (lp_key(bm) >= (unsigned)(least >> 32))           // few threads have one
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const u64 key = ((u64)lp_key(x[i]) << 32) | (0xffffffffu - (unsigned)col(i));
-                    if (key > least && (key >> 32) != 0ull && real(i)) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < LP_ROOM) sh.room[at] = key;
-                    }
-                }
-                __syncthreads();
-                const int n = sh.count;
-                if (n <= LP_ROOM / 2) {
-                    count = n;
-                    break;
-                }
-                // too many: the largest of those that are here bound the others
-                lp_place(sh.room, min(n, LP_ROOM), top, sh.best[0]);
-                least = sh.best[0][top - 1];
-                if (n <= LP_ROOM) {                                  // all are here: keep the best
-                    if (tid < top) sh.room[tid] = sh.best[0][tid];
-                    count = top;
-                } else {
-                    --least;                                         // again, with the last of them let in
-                }
-                if (tid == 0) sh.count = count;
-                __syncthreads();
-                if (n <= LP_ROOM) break;
-            }
+            if (first) __syncthreads();                              // every warp has a bound
+            first = false;
+            // the warps' bounds as they are: they only grow, so older ones hold too
+            const unsigned b = __reduce_min_sync(0xffffffffu, *(volatile unsigned*)&sh.bound[lane & (LP_WARPS - 1)]);
+            const float limit = b ? lp_value(b) : -INFINITY;
+            if (bm >= limit) collect(x, limit, col, real);
+            __syncwarp();
         }
+    }
+    // The same for the largest alone, a block together and never too many: what would overflow the memory is
+    // taken again with the bound that the values in it give.
+    template <typename Col, typename Real>
+    __device__ __forceinline__ void take_again(const float (&x)[E], Col col, Real real) {
+        const int before = sh.count;
+        for (;;) {
+            __syncthreads();
+            collect(x, -INFINITY, col, real);
+            __syncthreads();
+            const int n = sh.count;
+            if (n <= LP_ROOM / 2) break;
+            lp_place(sh.room, min(n, LP_ROOM), top, sh.best[0]);
+            least = sh.best[0][top - 1];
+            if (n <= LP_ROOM) {                                      // all are here: keep the best
+                if (threadIdx.x < top) sh.room[threadIdx.x] = sh.best[0][threadIdx.x];
+            } else {
+                --least;                                             // again, with the last of them let in
+            }
+            if (threadIdx.x == 0) sh.count = n <= LP_ROOM ? top : before;
+            __syncthreads();
+            if (n <= LP_ROOM) break;
+        }
+        __syncthreads();
     }
 };
 
+// Walks a row's part: `body(values, column of value i, whether there is one)` of every thread, round by round; the next round's
+// values are requested before a round is taken.
+template <typename T, typename Body>
+__device__ __forceinline__ void lp_walk(const T* x, int vocab, int part, int parts, Body body) {
+    constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U, ROUND = U * LP_THREADS;
+    const int tid = threadIdx.x;
+    // whole 16-byte vectors from the first aligned one on, shared out over the parts; what lies
+    // before and behind them is the last part's
+    const int head = min(vocab, (int)((((16 - ((uintptr_t)x & 15)) & 15)) / sizeof(T)));
+    const int vectors = (vocab - head) / N, tail = head + vectors * N;
+    const int v0 = (int)((long long)vectors * part / parts), v1 = (int)((long long)vectors * (part + 1) / parts);
+    const T* from = x + head;
+    float next[E], v[E];
+    auto load = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = at + u * LP_THREADS + tid;
+            if (i < v1) {
+                LpVec<T>::load(from + (size_t)i * N, next + u * N);
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) next[u * N + k] = -INFINITY;
+            }
+        }
+    };
+    if (v0 < v1) load(v0);
+    for (int at = v0; at < v1; at += ROUND) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = next[i];
+        if (at + ROUND < v1) load(at + ROUND);
+        const int base = head + (at + tid) * N, mine = at + tid;
+        body(v, [&](int i) { return base + (i / N) * LP_THREADS * N + i % N; },
+             [&](int i) { return mine + (i / N) * LP_THREADS < v1; });
+    }
+    if (part == parts - 1 && head + vocab - tail > 0) {
+        const int col = tid < head ? tid : tail + tid - head;
+        const bool have = col < vocab;
+        v[0] = have ? rv_load(x + col) : -INFINITY;
+#pragma unroll
+        for (int i = 1; i < E; ++i) v[i] = -INFINITY;
+        body(v, [&](int) { return col; }, [&](int i) { return i == 0 && have; });
+    }
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
+__global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel(
     const T* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ tokens, int top,
     float* __restrict__ logprob, int* __restrict__ rank, float* __restrict__ entropy, float* __restrict__ top_logprob,
     int* __restrict__ top_id, int parts) {
     rv_pdl_prologue();
-    constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U;
     __shared__ LpShared<TOP> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row = blockIdx.x / parts;
@@ -229,46 +287,12 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
     const bool known = token >= 0 && token < vocab;
     const float given = known ? rv_load(x + token) : INFINITY;
     if constexpr (TOP) {
-        if (tid == 0) sh.count = 0;
+        if (tid == 0) sh.count = sh.kept = 0;
+        if (tid < LP_WARPS) sh.bound[tid] = 0u;
         __syncthreads();
     }
     LpThread<T, TOP> th(sh, top, given);
-    // whole 16-byte vectors from the first aligned one on, shared out over the parts; what lies
-    // before and behind them is the last part's
-    const int head = min(vocab, (int)((((16 - ((uintptr_t)x & 15)) & 15)) / sizeof(T)));
-    const int vectors = (vocab - head) / N, tail = head + vectors * N;
-    const int v0 = (int)((long long)vectors * part / parts), v1 = (int)((long long)vectors * (part + 1) / parts);
-    const T* body = x + head;
-    float v[E];
-    int at = v0;
-    for (; at + U * LP_THREADS <= v1; at += U * LP_THREADS) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) LpVec<T>::load(body + (size_t)(at + u * LP_THREADS + tid) * N, v + u * N);
-        const int base = head + (at + tid) * N;
-        th.take(v, [&](int i) { return base + (i / N) * LP_THREADS * N + i % N; }, [](int) { return true; });
-    }
-    if (at < v1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (at + u * LP_THREADS + tid < v1) {
-                LpVec<T>::load(body + (size_t)(at + u * LP_THREADS + tid) * N, v + u * N);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i) v[u * N + i] = -INFINITY;
-            }
-        }
-        const int base = head + (at + tid) * N;
-        th.take(v, [&](int i) { return base + (i / N) * LP_THREADS * N + i % N; },
-                [&](int i) { return at + (i / N) * LP_THREADS + tid < v1; });
-    }
-    if (part == parts - 1 && head + vocab - tail > 0) {
-        const int col = tid < head ? tid : tail + tid - head;
-        const bool have = col < vocab;
-        v[0] = have ? rv_load(x + col) : -INFINITY;
-#pragma unroll
-        for (int i = 1; i < E; ++i) v[i] = -INFINITY;
-        th.take(v, [&](int) { return col; }, [&](int i) { return i == 0 && have; });
-    }
+    lp_walk(x, vocab, part, parts, [&](auto& v, auto col, auto real) { th.take(v, col, real); });
     // ---- the warp's, the block's, the cluster's ------------------------------------------------
     {
         const float most = rv_warp_max(th.m), c = lp_ref(most);
@@ -283,12 +307,34 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
         const int above = __reduce_add_sync(0xffffffffu, th.above);
         if (lane == 0) sh.part[warp] = {most, s, w, above};
     }
-    if constexpr (TOP) lp_place(sh.room, th.count, top, sh.best[0]);
-    else __syncthreads();
+    __syncthreads();
     if (tid == 0) {
         LpPart p = sh.part[0];
         for (int i = 1; i < LP_WARPS; ++i) lp_add(p, sh.part[i]);
         sh.whole = p;
+    }
+    if constexpr (TOP) {
+        const int n = sh.count;
+        unsigned b = sh.bound[0];
+#pragma unroll
+        for (int k = 1; k < LP_WARPS; ++k) b = min(b, sh.bound[k]);
+        if (n > LP_ROOM) {
+            // rising values, or too many alike: the part once more
+            __syncthreads();
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            th.least = b ? ((u64)b << 32) - 1ull : 0ull;
+            lp_walk(x, vocab, part, parts, [&](auto& v, auto col, auto real) { th.take_again(v, col, real); });
+            lp_place(sh.room, sh.count, top, sh.best[0]);
+        } else {
+            // those that the last bound leaves
+            for (int i = tid; i < n; i += LP_THREADS)
+                if ((unsigned)(sh.room[i] >> 32) >= b) sh.left[atomicAdd(&sh.kept, 1)] = sh.room[i];
+            __syncthreads();
+            lp_place(sh.left, sh.kept, top, sh.best[0]);
+        }
+    } else {
+        __syncthreads();
     }
     if (parts > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -328,8 +374,6 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // nobody leaves while it is read
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (part != 0) return;
-    } else {
-        __syncthreads();
     }
     const LpPart p = sh.whole;
     const float c = lp_ref(p.m), logs = logf(p.s);
@@ -340,37 +384,29 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(
         entropy[row] = h < 0.f ? 0.f : h;
     }
     if constexpr (TOP) {
-        // a key of part `warp`: its place there, and in each other part by bisection
+        // a key of part `warp`: how many are larger in each part, by bisection
         if (warp < parts && lane < top) {
             const u64 key = sh.best[warp][lane];
-            int place = lane;
-            for (int k = 0; k < parts; ++k) {
-                if (k == warp) continue;
-                int lo = 0, hi = 32;                                 // how many of part k are larger
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (sh.best[k][mid] > key) lo = mid + 1;
-                    else hi = mid;
-                }
-                place += lo;
-            }
+            int larger[LP_MAX_CLUSTER];                              // how many of part k are
+#pragma unroll
+            for (int k = 0; k < LP_MAX_CLUSTER; ++k) larger[k] = 0;
+#pragma unroll
+            for (int step = 32; step > 0; step >>= 1)
+#pragma unroll
+                for (int k = 0; k < LP_MAX_CLUSTER; ++k)
+                    if (k < parts && larger[k] + step <= 32 && sh.best[k][larger[k] + step - 1] > key) larger[k] += step;
+            int place = 0;
+#pragma unroll
+            for (int k = 0; k < LP_MAX_CLUSTER; ++k) place += larger[k];
             if (key != 0ull && place < top) {
                 top_logprob[row * top + place] = (lp_value((unsigned)(key >> 32)) - c) - logs;
                 top_id[row * top + place] = (int)(0xffffffffu - (unsigned)key);
             }
         }
-        if (warp == 0 && lane < top) {                               // places that nothing takes
+        if (warp == 0) {                                             // places that nothing takes
             int have = 0;
-            for (int k = 0; k < parts; ++k) {
-                int lo = 0, hi = 32;
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (sh.best[k][mid] != 0ull) lo = mid + 1;
-                    else hi = mid;
-                }
-                have += lo;
-            }
-            if (lane >= have) {
+            for (int k = 0; k < parts; ++k) have += __popc(__ballot_sync(0xffffffffu, sh.best[k][lane] != 0ull));
+            if (lane < top && lane >= have) {
                 top_logprob[row * top + lane] = NAN;
                 top_id[row * top + lane] = -1;
             }
@@ -384,11 +420,11 @@ extern "C" int rv_token_logprobs(const void* logits, int dtype, long long row_st
     if (rows == 0) return 0;
     if (rows < 0 || vocab <= 0) RV_FAIL("token_logprobs: bad sizes");
     if (top < 0 || top > 32 || top > vocab) RV_FAIL("token_logprobs: %d alternatives (0 to 32, at most the vocabulary)", top);
-    // blocks a row: until there are some two a multiprocessor, parts of four rounds of loads at least
+    // blocks a row: as many as the GPU holds at once, a round of loads each at least
     const int size = dtype == RV_DTYPE_F32 ? 4 : 2, sms = rv_sm_count();
     int parts = 1;
-    while (2 * parts <= LP_MAX_CLUSTER && (long long)rows * 2 * parts <= 4ll * sms &&
-           (long long)vocab * size >= (long long)2 * parts * LP_THREADS * 16)
+    while (2 * parts <= LP_MAX_CLUSTER && (long long)rows * 2 * parts <= (long long)LP_RESIDENT * sms &&
+           (long long)vocab * size >= (long long)2 * parts * LP_THREADS * 64)
         parts *= 2;
     if ((long long)rows * parts > 0x7fffffffLL) RV_FAIL("token_logprobs: too many rows");
     cudaLaunchConfig_t cfg = {};

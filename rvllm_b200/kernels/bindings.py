@@ -836,46 +836,51 @@ class CudaOps:
 
     # ---- keys and values in 8 bits ------------------------------------------------------
     #
-    # These calls are short on the GPU (some 4 us a step of single tokens), so the host's part counts: one
-    # pass over the tensors, plain numbers handed to functions whose argument types are declared.
+    # These calls are short on the GPU (some 4 us a step of single tokens), so the host's part counts: each tensor is
+    # looked at once, in line, and plain numbers go to functions whose argument types are declared.
 
     @staticmethod
     def _here() -> int:
         return torch._C._cuda_getDevice()          # (what torch.cuda.current_device comes to, without its checks)
 
+    def _raw_stream(self, device: int):
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
+
     @staticmethod
     def _fault(what: str, message: str):
         raise KernelError(f"{what}: {message}")
 
-    def _held(self, what, *tensors):
-        """(tensor, name, type) each: contiguous, of that type, on the device whose stream is launched on."""
-        here = self._here()
-        for t, name, dtype in tensors:
-            if t.get_device() != here:
-                self._fault(what, f"{name} on {t.device}, not on the current CUDA device {here}")
-            if t.dtype is not dtype:
-                self._fault(what, f"{name} must be {dtype}, got {t.dtype}")
-            if not t.is_contiguous():
-                self._fault(what, f"{name} must be contiguous")
+    def _not_held(self, what, t, name, dtype, here):
+        """What is wrong with a tensor that should be contiguous, of that type, on the current device."""
+        if t.get_device() != here:
+            self._fault(what, f"{name} on {t.device}, not on the current CUDA device {here}")
+        if t.dtype is not dtype:
+            self._fault(what, f"{name} must be {dtype}, got {t.dtype}")
+        self._fault(what, f"{name} must be contiguous")
 
-    def _row_shape(self, what, rows, width):
-        """Tokens of `rows` [tokens, width or more], whose values of a token lie side by side."""
-        if rows.get_device() != self._here():
-            self._fault(what, f"rows on {rows.device}, not on the current CUDA device")
-        if rows.dim() != 2 or rows.size(1) < width:
+    def _row_shape(self, what, rows, width, here):
+        """Tokens of `rows` [tokens, width or more], whose values of a token lie side by side, and their stride."""
+        if rows.get_device() != here:
+            self._fault(what, f"rows on {rows.device}, not on the current CUDA device {here}")
+        shape = rows.shape
+        if len(shape) != 2 or shape[1] < width:
             self._fault(what, "row width and head counts disagree")
-        n, have = rows.shape
+        n, have = shape
         stride, step = rows.stride()
         if (have > 1 and step != 1) or (n > 1 and stride < have):
             self._fault(what, "the values of a row must lie side by side")
         return n, stride
 
-    def _page_shape(self, what, cache, scale, other=None, other_scale=None):
+    def _page_shape(self, what, cache, scale, here, name="key"):
+        """Shape of `cache` int8 [pages, kv heads, page size, head size] with `scale` float32 [pages, kv heads]."""
+        if cache.dtype is not torch.int8 or not cache.is_contiguous() or cache.get_device() != here:
+            self._not_held(what, cache, f"{name} pages", torch.int8, here)
+        if scale.dtype is not torch.float32 or not scale.is_contiguous() or scale.get_device() != here:
+            self._not_held(what, scale, f"{name} scales", torch.float32, here)
         shape = cache.shape
-        if len(shape) != 4 or tuple(scale.shape) != tuple(shape[:2]):
+        if len(shape) != 4 or scale.shape != shape[:2]:
             self._fault(what, "pages are [pages, kv heads, page size, head size], scales [pages, kv heads]")
-        if other is not None and (other.shape != shape or other_scale.shape != scale.shape):
-            self._fault(what, "key and value pages differ in shape")
         if shape[3] % 16 or not 16 <= shape[3] <= 256:
             self._fault(what, f"head size {shape[3]} is not supported (a multiple of 16, at most 256)")
         return shape
@@ -894,57 +899,72 @@ class CudaOps:
         slots follow it.  The tokens of one page stand together in the call (tokens without a slot may
         stand between them), and each slot comes once (of several tokens for one slot the last is kept)."""
         what = "qk_norm_rope_write_8bit"
-        dtype = qkv.dtype
+        dtype, here = qkv.dtype, self._here()
         code = _code(dtype)
         f32, i32 = torch.float32, torch.int32
         if num_heads <= 0 or num_kv_heads <= 0:
             self._fault(what, f"invalid head counts: {num_heads} query, {num_kv_heads} KV")
-        n, stride = self._row_shape(what, qkv, (num_heads + 2 * num_kv_heads) * head_dim)
-        self._held(what, (q_out, "query rows", dtype), (k_cache, "key pages", torch.int8),
-                   (v_cache, "value pages", torch.int8), (k_scale, "key scales", f32), (v_scale, "value scales", f32),
-                   (slot_mapping, "slots", i32))
-        pages, heads, page_size, dim = self._page_shape(what, k_cache, k_scale, v_cache, v_scale)
+        n, stride = self._row_shape(what, qkv, (num_heads + 2 * num_kv_heads) * head_dim, here)
+        shape = self._page_shape(what, k_cache, k_scale, here)
+        if self._page_shape(what, v_cache, v_scale, here, "value") != shape:
+            self._fault(what, "key and value pages differ in shape")
+        pages, heads, page_size, dim = shape
         if heads != num_kv_heads or dim != head_dim:
             self._fault(what, f"pages of {heads} heads of {dim}, asked for {num_kv_heads} of {head_dim}")
+        if q_out.dtype is not dtype or not q_out.is_contiguous() or q_out.get_device() != here:
+            self._not_held(what, q_out, "query rows", dtype, here)
         if q_out.shape != (n, num_heads * head_dim):
             self._fault(what, "the query rows have another shape")
-        if slot_mapping.dim() != 1 or slot_mapping.size(0) < n:
+        if slot_mapping.dtype is not i32 or not slot_mapping.is_contiguous() or slot_mapping.get_device() != here:
+            self._not_held(what, slot_mapping, "slots", i32, here)
+        if slot_mapping.dim() != 1 or slot_mapping.numel() < n:
             self._fault(what, "a slot for every token")
-        for w in (q_weight, k_weight):
-            if w is not None:
-                self._held(what, (w, "norm weight", f32))
-                if w.shape != (head_dim,):
-                    self._fault(what, "a norm weight has another width")
-        cos = sin = at = None
+        qw = kw = cos_at = sin_at = at = None
+        if q_weight is not None:
+            if q_weight.dtype is not f32 or not q_weight.is_contiguous() or q_weight.get_device() != here:
+                self._not_held(what, q_weight, "norm weight", f32, here)
+            if q_weight.shape != (head_dim,):
+                self._fault(what, "a norm weight has another width")
+            qw = q_weight.data_ptr()
+        if k_weight is not None:
+            if k_weight.dtype is not f32 or not k_weight.is_contiguous() or k_weight.get_device() != here:
+                self._not_held(what, k_weight, "norm weight", f32, here)
+            if k_weight.shape != (head_dim,):
+                self._fault(what, "a norm weight has another width")
+            kw = k_weight.data_ptr()
         angles = 0
         if table is not None:
             cos, sin = table
-            self._held(what, (cos, "rotation table", f32), (sin, "rotation table", f32), (positions, "positions", i32))
+            if cos.dtype is not f32 or not cos.is_contiguous() or cos.get_device() != here:
+                self._not_held(what, cos, "rotation table", f32, here)
+            if sin.dtype is not f32 or not sin.is_contiguous() or sin.get_device() != here:
+                self._not_held(what, sin, "rotation table", f32, here)
+            if positions.dtype is not i32 or not positions.is_contiguous() or positions.get_device() != here:
+                self._not_held(what, positions, "positions", i32, here)
             if cos.dim() != 2 or cos.size(1) != head_dim // 2 or sin.shape != cos.shape:
                 self._fault(what, "a rotation table has another width")
-            if positions.dim() != 1 or positions.size(0) < n:
+            if positions.dim() != 1 or positions.numel() < n:
                 self._fault(what, "a position for every token")
-            angles, at = cos.size(0), positions.data_ptr()
+            angles, cos_at, sin_at, at = cos.size(0), cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
         self._check(self._write_8bit(
-            qkv.data_ptr(), code, stride, n, num_heads, num_kv_heads, head_dim,
-            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
-            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), angles, at, slot_mapping.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), pages, page_size, self._stream()), what)
+            qkv.data_ptr(), code, stride, n, num_heads, num_kv_heads, head_dim, qw, kw, eps, cos_at, sin_at, angles, at,
+            slot_mapping.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), pages, page_size, self._raw_stream(here)), what)
 
     def read_8bit(self, cache, scale, pages, dtype):
         """The pages `pages` (int32 [n]) of an 8-bit cache as values, `dtype` [n, kv heads, page size,
         head_dim] (exact in bfloat16 too).  A number that is no page gives zeros."""
-        what = "read_8bit"
+        what, here = "read_8bit", self._here()
         code = _code(dtype)
-        self._held(what, (cache, "8-bit pages", torch.int8), (scale, "scales", torch.float32),
-                   (pages, "page numbers", torch.int32))
-        have, heads, page_size, dim = self._page_shape(what, cache, scale)
+        have, heads, page_size, dim = self._page_shape(what, cache, scale, here, "8-bit")
+        if pages.dtype is not torch.int32 or not pages.is_contiguous() or pages.get_device() != here:
+            self._not_held(what, pages, "page numbers", torch.int32, here)
         if pages.dim() != 1:
             self._fault(what, "page numbers are one row")
-        n = pages.size(0)
+        n = pages.numel()
         out = torch.empty((n, heads, page_size, dim), dtype=dtype, device=cache.device)
         self._check(self._read_8bit(cache.data_ptr(), scale.data_ptr(), pages.data_ptr(), out.data_ptr(), code, n, heads,
-                                    page_size, dim, have, self._stream()), what)
+                                    page_size, dim, have, self._raw_stream(here)), what)
         return out
 
     def _attn8_lib(self, head_dim: int):
@@ -966,7 +986,7 @@ class CudaOps:
             call.argtypes = [P, I, L, P, P, P, P, L, P, I, P, P, P, P, L, I, I, I, I, I, I, I, I, c_float, I, P, I, P]
             scratch = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")
             scratch.restype = c_longlong
-            scratch.argtypes = [I] * 8
+            scratch.argtypes = [I] * 6
             hit = self._attn_libs[key] = (call, scratch, error)
         return hit
 
@@ -979,21 +999,29 @@ class CudaOps:
         block-table entry is no page are not seen; a context longer than the table gives NaN.  Scratch is
         allocated per call (in a captured graph: from the graph's pool)."""
         what = "paged_attention_8bit"
-        dtype = q.dtype
+        dtype, here = q.dtype, self._here()
         code = _code(dtype)
-        f32, i32 = torch.float32, torch.int32
+        i32 = torch.int32
         if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
             self._fault(what, f"invalid head counts: {num_heads} query, {num_kv_heads} KV")
         table, q_start, ctx_lens = group.block_table, ctx.q_start, ctx.ctx_lens
         n_decode, n_reqs, n_tokens = ctx.n_decode, ctx.n_reqs, ctx.n_tokens
-        n, stride = self._row_shape(what, q, num_heads * head_dim)
-        self._held(what, (k_cache, "key pages", torch.int8), (v_cache, "value pages", torch.int8),
-                   (k_scale, "key scales", f32), (v_scale, "value scales", f32), (out, "attention output", dtype),
-                   (table, "block table", i32), (q_start, "first tokens", i32), (ctx_lens, "context lengths", i32))
-        pages, heads, page_size, dim = self._page_shape(what, k_cache, k_scale, v_cache, v_scale)
+        n, stride = self._row_shape(what, q, num_heads * head_dim, here)
+        shape = self._page_shape(what, k_cache, k_scale, here)
+        if self._page_shape(what, v_cache, v_scale, here, "value") != shape:
+            self._fault(what, "key and value pages differ in shape")
+        pages, heads, page_size, dim = shape
         if heads != num_kv_heads or dim != head_dim or page_size != group.page_size:
             self._fault(what, f"pages of {heads} heads of {dim}, {page_size} tokens each, asked for {num_kv_heads} of "
                               f"{head_dim}, {group.page_size} tokens")
+        if out.dtype is not dtype or not out.is_contiguous() or out.get_device() != here:
+            self._not_held(what, out, "attention output", dtype, here)
+        if table.dtype is not i32 or not table.is_contiguous() or table.get_device() != here:
+            self._not_held(what, table, "block table", i32, here)
+        if q_start.dtype is not i32 or not q_start.is_contiguous() or q_start.get_device() != here:
+            self._not_held(what, q_start, "first tokens", i32, here)
+        if ctx_lens.dtype is not i32 or not ctx_lens.is_contiguous() or ctx_lens.get_device() != here:
+            self._not_held(what, ctx_lens, "context lengths", i32, here)
         if n < n_tokens or out.shape != (n, num_heads * head_dim):
             self._fault(what, "output, rows and head counts disagree")
         if not 0 <= n_decode <= n_reqs or n_tokens < n_decode:
@@ -1003,22 +1031,24 @@ class CudaOps:
         window = window or 0
         if window < 0:
             self._fault(what, f"a window of {window}")
+        sinks_at = None
         if sinks is not None:
-            self._held(what, (sinks, "sinks", f32))
+            if sinks.dtype is not torch.float32 or not sinks.is_contiguous() or sinks.get_device() != here:
+                self._not_held(what, sinks, "sinks", torch.float32, here)
             if sinks.shape != (num_heads,):
                 self._fault(what, "one sink per query head")
+            sinks_at = sinks.data_ptr()
         call, scratch_bytes, error = self._attn8_lib(head_dim)
         portions = n_tokens > n_decode
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
-        need = scratch_bytes(n_decode, n_reqs if portions else n_decode, longest, deepest, num_heads, num_kv_heads, window,
-                             sms)
+        need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
         rc = call(q.data_ptr(), code, stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
                   v_scale.data_ptr(), pages, table.data_ptr(), table.size(1), q_start.data_ptr(), ctx_lens.data_ptr(),
                   out.data_ptr(), None if scratch is None else scratch.data_ptr(), need, n_decode, n_reqs, portions,
-                  longest, deepest, num_heads, num_kv_heads, page_size, scale, window,
-                  None if sinks is None else sinks.data_ptr(), sms, self._stream())
-        self.launches += (2 if n_decode else 0) + portions
+                  longest, deepest, num_heads, num_kv_heads, page_size, scale, window, sinks_at, sms,
+                  self._raw_stream(here))
+        self.launches += (n_decode > 0) + (need > 0) + portions
         if rc != 0:
             raise KernelError(error().decode())
 
@@ -1933,12 +1963,13 @@ class CudaOps:
         A token outside the vocabulary has log probability NaN and rank 0.  A NaN or an infinity among a row's logits
         makes its probabilities NaN, as do logits that are all -inf; NaN is never among the largest (id -1 where
         there are not enough others)."""
-        what = "token_logprobs"
+        what, here = "token_logprobs", self._here()
         code = _code(logits.dtype)
-        rows, stride = self._row_shape(what, logits, 1)
+        rows, stride = self._row_shape(what, logits, 1, here)
         vocab = logits.size(1)
-        self._held(what, (tokens, "tokens", torch.int32))
-        if tokens.dim() != 1 or tokens.size(0) != rows:
+        if tokens.dtype is not torch.int32 or not tokens.is_contiguous() or tokens.get_device() != here:
+            self._not_held(what, tokens, "tokens", torch.int32, here)
+        if tokens.dim() != 1 or tokens.numel() != rows:
             self._fault(what, "a token for every row")
         if not 0 <= top <= min(32, vocab):
             self._fault(what, f"{top} alternatives of {vocab} (0 to 32)")
@@ -1950,5 +1981,5 @@ class CudaOps:
         ids = torch.empty((rows, top), dtype=i32, device=device)
         self._check(self._token_logprobs(
             logits.data_ptr(), code, stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(),
-            entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), self._stream()), what)
+            entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), self._raw_stream(here)), what)
         return logprob, rank, entropy, best, ids
