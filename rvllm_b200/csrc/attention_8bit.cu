@@ -434,10 +434,10 @@ struct A8Warp {
         // ---- u, its largest -------------------------------------------------------------------------
         const int key0 = tile_at * A8_KEYS;
         // this lane's key: its scale, log2 of its value's scale and one over that; a key without a page (its scales
-        // are zeros) weighs nothing
+        // are zeros) shows in every row that may see it
         const float sk1 = __uint_as_float(a8_lds(scales));
         const int e1 = max(-60, min(60, (int)((a8_lds(scales + 4 * A8_KEYS) >> 23) & 0xff) - 127));
-        const float inv1 = __uint_as_float((unsigned)(127 - e1) << 23), ev1 = sk1 == 0.f ? -INFINITY : (float)e1;
+        const float inv1 = __uint_as_float((unsigned)(127 - e1) << 23), ev1 = sk1 == 0.f ? NAN : (float)e1;
         float inv[MT][2], mx[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;

@@ -425,3 +425,82 @@ extern "C" int rv_read_8bit(const void* cache, const float* scales, const int* i
     RV_CHECK_LAUNCH("read_8bit");
     return 0;
 }
+
+// ---- contexts widened for long portions ------------------------------------------------------------
+// The keys and values that requests' portions may see, as bfloat16 pages of 64 tokens [page][64][kv heads][head size]
+// and a block table for them, as the tcgen05 attention reads them.  Its blocks of 128 rows each read a request's whole context, so that
+// one pass here costs less than widening the tiles in each of them (a prompt of 2,048 tokens, 32 / 8 heads of 64: 64
+// blocks a head; 68 us with the tiles widened in place by three warps a block, which they keep waiting).  Exact,
+// as scales are powers of two.
+// blockIdx.x: a page of 64, y: request, z: key/value head.  Slots behind the context are zeros, keys without a page NaN.
+// Rows of a portion before position 0 are not the attention's: they are set to zero here.
+struct C8Widen {
+    const signed char *k, *v;
+    const float *k_scale, *v_scale;
+    const int *block_table, *q_start, *ctx_lens;
+    __nv_bfloat16 *wide_k, *wide_v, *out;
+    int* wide_table;
+    long long pages;
+    int max_blocks, first_req, num_heads, num_kv_heads, head_dim, page_size, window, width, room;
+};
+__global__ void __launch_bounds__(256) widen_8bit_kernel(const __grid_constant__ C8Widen a) {
+    rv_pdl_prologue();
+    const int i = blockIdx.y, r = a.first_req + i, g = blockIdx.z;
+    const int clen = a.ctx_lens[r], qs = a.q_start[r], qlen = a.q_start[r + 1] - qs;
+    const int lo = a.window > 0 ? max(0, clen - qlen - a.window + 1) : 0, b0 = lo / 64, b = b0 + blockIdx.x;
+    if (blockIdx.x == 0 && g == 0)
+        for (int k = threadIdx.x; k < a.width; k += 256)
+            a.wide_table[(size_t)i * a.width + k] =
+                k >= b0 && k < b0 + a.room && (long long)k * 64 < clen && qlen > 0 ? i * a.room + k - b0 : -1;
+    if (blockIdx.x == 0 && clen < qlen) {
+        const int per = a.num_heads / a.num_kv_heads * a.head_dim, pairs = per / 2;
+        for (long long k = threadIdx.x; k < (long long)(qlen - clen) * pairs; k += 256) {
+            const long long tok = k / pairs;
+            ((unsigned*)(a.out + ((size_t)(qs + tok) * a.num_kv_heads + g) * per))[k - tok * pairs] = 0u;
+        }
+    }
+    if ((long long)b * 64 >= clen || qlen <= 0) return;
+    const int pieces = a.head_dim / 16;
+    for (int k = threadIdx.x; k < 64 * pieces; k += 256) {
+        const int in = k / pieces, c = k - in * pieces, key = b * 64 + in, blk = key / a.page_size;
+        const int page = key < clen && blk < a.max_blocks ? a.block_table[(size_t)r * a.max_blocks + blk] : -1;
+        const bool ok = page >= 0 && page < a.pages;
+        const size_t block = ok ? (size_t)page * a.num_kv_heads + g : 0;
+        const size_t from = (block * a.page_size + (ok ? key - blk * a.page_size : 0)) * a.head_dim + 16 * c;
+        const size_t to = (((size_t)i * a.room + blockIdx.x) * 64 + in) * a.num_kv_heads * a.head_dim + (size_t)g * a.head_dim + 16 * c;
+        const int4 zero = make_int4(0, 0, 0, 0);
+        const int4 kr = ok ? *(const int4*)(a.k + from) : zero, vr = ok ? *(const int4*)(a.v + from) : zero;
+        const float sk = ok ? a.k_scale[block] : key < clen ? NAN : 0.f, sv = ok ? a.v_scale[block] : 0.f;
+        const signed char *kb = (const signed char*)&kr, *vb = (const signed char*)&vr;
+#pragma unroll
+        for (int h = 0; h < 16; h += 8) {
+            float x[8], y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = (float)kb[h + j] * sk;
+                y[j] = (float)vb[h + j] * sv;
+            }
+            c8_store8(a.wide_k + to + h, true, x);
+            c8_store8(a.wide_v + to + h, true, y);
+        }
+    }
+}
+
+// Requests [first_req, first_req + n_reqs): `room` pages of 64 for each in `wide_k` and `wide_v`, `width` entries in `wide_table`.
+extern "C" int rv_widen_8bit(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, long long pages,
+                             const int* block_table, int max_blocks, const int* q_start, const int* ctx_lens, void* wide_k,
+                             void* wide_v, int* wide_table, int width, int room, void* out, int first_req, int n_reqs, int num_heads,
+                             int num_kv_heads, int head_dim, int page_size, int window, void* stream) {
+    if (n_reqs == 0) return 0;
+    if (n_reqs < 0 || n_reqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_heads % num_kv_heads ||
+        head_dim <= 0 || head_dim % 16 || page_size <= 0 || window < 0 || width < 0 || room <= 0)
+        RV_FAIL("widen_8bit: bad sizes");
+    if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)wide_k | (uintptr_t)wide_v) % 16)
+        RV_FAIL("widen_8bit: pages must be 16-byte aligned");
+    const C8Widen a = {(const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens,
+                       (__nv_bfloat16*)wide_k, (__nv_bfloat16*)wide_v, (__nv_bfloat16*)out, wide_table, pages, max_blocks, first_req,
+                       num_heads, num_kv_heads, head_dim, page_size, window, width, room};
+    rv_launch(widen_8bit_kernel, dim3(room, n_reqs, num_kv_heads), dim3(256), 0, (cudaStream_t)stream, a);
+    RV_CHECK_LAUNCH("widen_8bit");
+    return 0;
+}

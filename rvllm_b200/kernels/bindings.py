@@ -72,6 +72,11 @@ class CudaOps:
         # tcgen05 where it applies, else mma
         self.prefill_attention = os.environ.get("RVLLM_PREFILL_ATTENTION", "auto")
         self.decode_attention = os.environ.get("RVLLM_DECODE_ATTENTION", "mma")
+        # portions over 8-bit pages: "rows" = mma.sync from the pages, any head size and type; "tcgen05" = bfloat16
+        # pages for the step, then the tcgen05 kernel (bfloat16, head sizes 64 and 128); "auto" = the faster one,
+        # while those pages take no more than `widen_8bit_bytes`
+        self.widen_8bit_bytes = 1 << 30
+        self.prefill_8bit = os.environ.get("RVLLM_PREFILL_8BIT", "auto")
         # keys per block of the tensor-core decode kernel: 256 (four warps) or 128 (two)
         self.decode_split = int(os.environ.get("RVLLM_ATTN_DECODE_SPLIT", "256"))
         # "stream": one persistent block per SM whose warps each stream their work items'
@@ -122,6 +127,8 @@ class CudaOps:
         self._write_8bit.argtypes = [P, I, L, I, I, I, I, P, P, c_float, P, P, L, P, P, P, P, P, P, P, L, I, P]
         self._read_8bit = self.lib.rv_read_8bit
         self._read_8bit.argtypes = [P, P, P, P, I, I, I, I, I, L, P]
+        self._widen_8bit = self.lib.rv_widen_8bit
+        self._widen_8bit.argtypes = [P, P, P, P, L, P, I, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P]
         self._token_logprobs = self.lib.rv_token_logprobs
         self._token_logprobs.argtypes = [P, I, L, I, I, P, I, P, P, P, P, P, P]
         # the library's float32 products must be float32: no TF32, no reduced-precision accumulation
@@ -995,9 +1002,10 @@ class CudaOps:
         """`paged_attention` over pages of 8 bits (`qk_norm_rope_write_8bit`).  `q` [tokens, heads * head_dim or
         more], float32 or bfloat16, any stride between rows; `out` [tokens, heads * head_dim] of its type.
         Requests [0, ctx.n_decode) bring one token each, the others any number; the key at position j is seen from
-        position p iff j <= p and, with a window, j > p - window.  A row that sees nothing is zeros; keys whose
-        block-table entry is no page are not seen; a context longer than the table gives NaN.  Scratch is
-        allocated per call (in a captured graph: from the graph's pool)."""
+        position p iff j <= p and, with a window, j > p - window.  A row that sees nothing is zeros; one that may see a key
+        whose block-table entry is no page, or a request whose context is longer than its row of the table, has no valid
+        result (nothing outside the pages is read).  Scratch is allocated per call (in a captured graph: from the graph's
+        pool); long bfloat16 portions (heads of 64 or 128) take bfloat16 copies of what they may see for the call's duration."""
         what = "paged_attention_8bit"
         dtype, here = q.dtype, self._here()
         code = _code(dtype)
@@ -1041,16 +1049,78 @@ class CudaOps:
         call, scratch_bytes, error = self._attn8_lib(head_dim)
         portions = n_tokens > n_decode
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
-        need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        rc = call(q.data_ptr(), code, stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                  v_scale.data_ptr(), pages, table.data_ptr(), table.size(1), q_start.data_ptr(), ctx_lens.data_ptr(),
-                  out.data_ptr(), None if scratch is None else scratch.data_ptr(), need, n_decode, n_reqs, portions,
-                  longest, deepest, num_heads, num_kv_heads, page_size, scale, window, sinks_at, sms,
-                  self._raw_stream(here))
-        self.launches += (n_decode > 0) + (need > 0) + portions
+        stream = self._raw_stream(here)
+        tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window)
+        if n_decode or not tcgen05:
+            need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms)
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+            rc = call(q.data_ptr(), code, stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                      v_scale.data_ptr(), pages, table.data_ptr(), table.size(1), q_start.data_ptr(), ctx_lens.data_ptr(),
+                      out.data_ptr(), None if scratch is None else scratch.data_ptr(), need, n_decode, n_reqs,
+                      portions and not tcgen05, longest, deepest, num_heads, num_kv_heads, page_size, scale, window, sinks_at,
+                      sms, stream)
+            self.launches += (n_decode > 0) + (need > 0) + (portions and not tcgen05)
+            if rc != 0:
+                raise KernelError(error().decode())
+        if tcgen05:
+            self._attend_widened(q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
+                                 page_size, scale, window, out, sinks_at, stream)
+
+    def _tcgen05_8bit(self, q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window) -> bool:
+        """Whether portions are widened to bfloat16 and go to the tcgen05 kernel."""
+        group, reqs, longest = num_heads // num_kv_heads, ctx.n_reqs - ctx.n_decode, ctx.max_q_len
+        if (self.prefill_8bit == "rows" or code != _BF16 or head_dim not in (64, 128) or group > 128 or stride % head_dim
+                or (q.data_ptr() | out.data_ptr()) % 16 or reqs > 4095 or longest > 65535 * (128 // group)):
+            return False
+        keys = min(ctx.max_ctx_len, window + longest) if window else ctx.max_ctx_len
+        if 4 * reqs * keys * num_kv_heads * head_dim > self.widen_8bit_bytes:
+            return False
+        # tiles of 16 rows and 32 keys, of 64 dimensions.  us by mma.sync from the pages / widened: 32 / 8 heads of 64, 64 tokens
+        # after 1,000 (4,352 tiles) 12 / 18, 16 x 20 after 500 (10,880) 22.5 / 23, 512 (16,384) 23 / 16.5, 2,048 135 / 45; 16 / 8
+        # heads 16 x 20 after 500 (6,528) 14.5 / 23, 64 after 16,000 (32,128) 39 / 37; 16 / 2 heads of 128 16 x 20 after 500
+        # (10,880) 26 / 23, 2,048 91 / 50; 8 / 8 heads of 128 512 (8,192) 14.5 / 16.5
+        tiles = -(-longest * group // 16) * -(-keys // 32) * reqs * num_kv_heads * (head_dim // 64)
+        return self.prefill_8bit == "tcgen05" or tiles > 10000
+
+    def _attend_widened(self, q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
+                        page_size, scale, window, out, sinks_at, stream):
+        """Portions: what they may see of their contexts as bfloat16 pages, then the tcgen05 attention over those."""
+        nd, device = ctx.n_decode, q.device
+        reqs, longest, deepest = ctx.n_reqs - nd, ctx.max_q_len, ctx.max_ctx_len
+        width = -(-deepest // 64)
+        room = min(width, (window + longest) // 64 + 2) if window else width
+        wide = torch.empty((2, reqs * room * 64, num_kv_heads, head_dim), dtype=torch.bfloat16, device=device)
+        wide_table = torch.empty((reqs, width), dtype=torch.int32, device=device)
+        wide_at = wide.data_ptr()
+        wide_v = wide_at + wide.numel()                               # half of its bytes
+        self._check(self._widen_8bit(
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0), table.data_ptr(),
+            table.size(1), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), wide_at, wide_v, wide_table.data_ptr(), width, room,
+            out.data_ptr(), nd, reqs, num_heads, num_kv_heads, head_dim, page_size, window, stream), "widen_8bit")
+        fn, error = self._attn5_wide(head_dim)
+        # room for the parts of a short portion's blocks at the end of a long context
+        need = self._prefill_scratch_bytes(head_dim) if deepest - longest >= 512 else 0
+        scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        # (the attention's requests are counted from the first portion: its arrays begin there)
+        rc = fn(q.data_ptr(), stride, q.size(0), wide_at, wide_v, reqs * room * 64, wide_table.data_ptr(), width,
+                ctx.q_start.data_ptr() + 4 * nd, ctx.ctx_lens.data_ptr() + 4 * nd, out.data_ptr(), 0, reqs, longest, deepest,
+                num_heads, num_kv_heads, 64, scale, window, self._gemm_status(device).data_ptr(),
+                None if scratch is None else scratch.data_ptr(), need, self._sm_count, sinks_at, stream)
+        self.launches += 1
         if rc != 0:
-            raise KernelError(error().decode())
+            raise KernelError(f"paged_attention_8bit: {error().decode()}")
+
+    def _attn5_wide(self, head_dim: int):
+        """The tcgen05 attention (call, last error) with its argument types declared."""
+        key = ("tcgen05 declared", head_dim)
+        hit = self._attn_libs.get(key)
+        if hit is None:
+            lib = self._attn5_lib(head_dim)
+            fn = lib[f"rv_paged_attention_prefill_tcgen05_hd{head_dim}"]
+            P, I, L = c_void_p, c_int, c_longlong
+            fn.argtypes = [P, I, I, P, P, L, P, I, P, P, P, I, I, I, I, I, I, I, c_float, I, P, P, L, I, P, P]
+            hit = self._attn_libs[key] = (fn, getattr(lib, f"rv_attention_tcgen05_last_error_hd{head_dim}"))
+        return hit
 
     # ---- gated short convolution -----------------------------------------------------
 

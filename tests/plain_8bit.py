@@ -116,10 +116,13 @@ def attention(q, heads, kv, dim, k8, v8, ks, vs, ctx, group, scale, window, sink
         v = v8[p0, :, j % ps].double() * vs[p0].double()[..., None]
         for t in range(a, b):
             p = clen - (b - a) + (t - a)
-            seen = there & (j <= p)
+            seen = j <= p
             if window:
                 seen &= j > p - window
             if not bool(seen.any()):
+                continue
+            if bool((seen & ~there).any()):                       # a visible key without a page
+                out[t] = math.nan
                 continue
             for h in range(heads):
                 x = q[t, h * dim:(h + 1) * dim].double()
@@ -154,7 +157,7 @@ def logprobs(x, tokens, top):
     return out
 
 
-def attention_room(dtype, want, most):
+def attention_room(dtype, want, most, first_portion=None):
     """How far attention may be off, per element.
 
     float32: the result's rounding (2^-24); weights and scores from float32 sums, operands of 22 bits and exponentials of 2^-22: 2^-20
@@ -162,10 +165,14 @@ def attention_room(dtype, want, most):
     rounding (2^-8), the same, weights rounded to float16 (half a step is 2^-11 of itself: as much of the largest value;
     below 2^-14 of at most 2^6 steps are 2^-24: 2^-31 sqrt(keys) of the largest term), and queries as whole numbers of 16
     bits, in steps of 2^-14 of a row's largest at most: over a key's dimensions a score off by 6 * 2^-14 / sqrt(12) max
-    |q| |k| scale (six standard deviations), a weight by as much of itself, the result by twice that of the largest value."""
+    |q| |k| scale (six standard deviations), a weight by as much of itself, the result by twice that of the largest value.
+    Tokens from `first_portion` on: weights rounded to bfloat16 (half a step is 2^-8 of itself), queries as they are."""
     dim = want.shape[1] // most.shape[1]
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
     room = most[..., 0] * 2.0 ** -20 * (most[..., 1] + 8)
     if dtype == torch.bfloat16:
-        room += most[..., 0] * (2.0 ** -11 + 2 * 6 / math.sqrt(12) * 2.0 ** -14 * most[..., 2]) + 2.0 ** -31 * most[..., 4] * most[..., 3]
+        n = want.shape[0] if first_portion is None else first_portion
+        whole = most[..., 0] * (2.0 ** -11 + 2 * 6 / math.sqrt(12) * 2.0 ** -14 * most[..., 2]) + 2.0 ** -31 * most[..., 4] * most[..., 3]
+        room[:n] += whole[:n]
+        room[n:] += most[n:, :, 0] * 2.0 ** -8
     return half * want.abs() + room.repeat_interleave(dim, 1) + 1e-30
