@@ -1059,11 +1059,30 @@ static int a8_singles(const A8Args& a, int max_ctx_len, int n_sms, cudaStream_t 
 }
 
 // Requests [0, n_decode) bring one token each, [n_decode, n_reqs) up to max_q_len; `portions` 0: the former only.
-extern "C" int A8_SYM(rv_paged_attention_8bit)(
-    const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
-    const float* v_scale, long long pages, const int* block_table, int max_blocks, const int* q_start, const int* ctx_lens,
-    void* out, void* scratch, long long scratch_bytes, int n_decode, int n_reqs, int portions, int max_q_len, int max_ctx_len,
-    int num_heads, int num_kv_heads, int page_size, float scale, int window, const float* sinks, int n_sms, void* stream) {
+// Arguments packed, 8 bytes each, as the calls of cache_8bit.cu.
+struct A8Call {
+    const void *q, *k_cache, *v_cache;
+    const float *k_scale, *v_scale;
+    const int *block_table, *q_start, *ctx_lens;
+    void *out, *scratch;
+    const float* sinks;
+    void* stream;
+    long long dtype, q_stride, pages, max_blocks, scratch_bytes, n_decode, n_reqs, portions, max_q_len, max_ctx_len, num_heads,
+        num_kv_heads, page_size, window, n_sms;
+    double scale;
+};
+extern "C" int A8_SYM(rv_paged_attention_8bit)(const A8Call* c) {
+    const void *q = c->q, *k_cache = c->k_cache, *v_cache = c->v_cache;
+    void *out = c->out, *scratch = c->scratch, *stream = c->stream;
+    const float *k_scale = c->k_scale, *v_scale = c->v_scale, *sinks = c->sinks, scale = (float)c->scale;
+    const int *block_table = c->block_table, *q_start = c->q_start, *ctx_lens = c->ctx_lens;
+    const long long q_stride = c->q_stride, pages = c->pages, scratch_bytes = c->scratch_bytes;
+    for (const long long v : {c->max_blocks, c->n_reqs, c->max_q_len, c->max_ctx_len, c->num_heads, c->page_size, c->window})
+        if (v > 0x7fffffff) A8_FAIL("paged_attention_8bit: bad sizes");
+    const int dtype = (int)c->dtype, max_blocks = (int)c->max_blocks, n_decode = (int)c->n_decode, n_reqs = (int)c->n_reqs;
+    const int portions = (int)c->portions, max_q_len = (int)c->max_q_len, max_ctx_len = (int)c->max_ctx_len;
+    const int num_heads = (int)c->num_heads, num_kv_heads = (int)c->num_kv_heads, page_size = (int)c->page_size;
+    const int window = (int)c->window, n_sms = (int)c->n_sms;
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
         A8_FAIL("paged_attention_8bit: invalid head counts: %d query, %d KV", num_heads, num_kv_heads);
     if (n_decode < 0 || n_reqs < n_decode || max_q_len < 0 || max_ctx_len < 0 || max_blocks < 0 || page_size <= 0 || window < 0 ||

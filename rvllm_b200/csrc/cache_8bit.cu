@@ -348,11 +348,29 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     }
 }
 
-extern "C" int rv_qk_norm_rope_write_8bit(const void* rows, int dtype, long long row_stride, int n_tokens, int num_heads,
-                                          int num_kv_heads, int head_dim, const float* q_weight, const float* k_weight,
-                                          float eps, const float* cos_table, const float* sin_table, long long table_rows,
-                                          const int* positions, const int* slots, void* q_out, void* k_cache, void* v_cache,
-                                          float* k_scale, float* v_scale, long long pages, int page_size, void* stream) {
+// The entry points take their arguments packed, 8 bytes each (addresses, then sizes, then numbers), in the order of these
+// records: a host call that hands over twenty arguments one by one takes 2 us, a record 0.4.
+struct C8WriteCall {
+    const void* rows;
+    const float *q_weight, *k_weight, *cos_table, *sin_table;
+    const int *positions, *slots;
+    void *q_out, *k_cache, *v_cache;
+    float *k_scale, *v_scale;
+    void* stream;
+    long long dtype, row_stride, n_tokens, num_heads, num_kv_heads, head_dim, table_rows, pages, page_size;
+    double eps;
+};
+extern "C" int rv_qk_norm_rope_write_8bit(const C8WriteCall* c) {
+    const void* rows = c->rows;
+    const float *q_weight = c->q_weight, *k_weight = c->k_weight, *cos_table = c->cos_table, *sin_table = c->sin_table;
+    const int *positions = c->positions, *slots = c->slots;
+    void *q_out = c->q_out, *k_cache = c->k_cache, *v_cache = c->v_cache, *stream = c->stream;
+    float *k_scale = c->k_scale, *v_scale = c->v_scale, eps = (float)c->eps;
+    const long long row_stride = c->row_stride, table_rows = c->table_rows, pages = c->pages;
+    const int dtype = (int)c->dtype, num_heads = (int)c->num_heads, num_kv_heads = (int)c->num_kv_heads;
+    const int head_dim = (int)c->head_dim, page_size = (int)c->page_size, n_tokens = (int)c->n_tokens;
+    if (c->n_tokens > 0x7fffffff || c->num_heads > 65535 || c->num_kv_heads > 65535 || c->page_size > 0x7fffffff)
+        RV_FAIL("qk_norm_rope_write_8bit: bad sizes");
     if (n_tokens == 0) return 0;
     if (n_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 || pages < 0)
         RV_FAIL("qk_norm_rope_write_8bit: bad sizes");
@@ -411,8 +429,21 @@ __global__ void __launch_bounds__(256) read_8bit_kernel(const signed char* __res
     }
 }
 
-extern "C" int rv_read_8bit(const void* cache, const float* scales, const int* ids, void* out, int dtype, int n, int heads,
-                            int page_size, int head_dim, long long pages, void* stream) {
+struct C8ReadCall {
+    const void* cache;
+    const float* scales;
+    const int* ids;
+    void *out, *stream;
+    long long dtype, n, heads, page_size, head_dim, pages;
+};
+extern "C" int rv_read_8bit(const C8ReadCall* c) {
+    const void* cache = c->cache;
+    void *out = c->out, *stream = c->stream;
+    const float* scales = c->scales;
+    const int* ids = c->ids;
+    const long long pages = c->pages;
+    const int dtype = (int)c->dtype, n = (int)c->n, heads = (int)c->heads, page_size = (int)c->page_size, head_dim = (int)c->head_dim;
+    if (c->n > 0x7fffffff || c->heads > 65535 || c->page_size > 0x7fffffff) RV_FAIL("read_8bit: bad sizes");
     if (n == 0) return 0;
     if (n < 0 || heads <= 0 || page_size <= 0 || head_dim <= 0 || head_dim % 16) RV_FAIL("read_8bit: bad sizes");
     if (((uintptr_t)cache | (uintptr_t)out) % 16) RV_FAIL("read_8bit: pages must be 16-byte aligned");

@@ -414,9 +414,26 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
     }
 }
 
-extern "C" int rv_token_logprobs(const void* logits, int dtype, long long row_stride, int rows, int vocab, const int* tokens,
-                                 int top, float* logprob, int* rank, float* entropy, float* top_logprob, int* top_id,
-                                 void* stream) {
+// Arguments packed, 8 bytes each, as the calls of cache_8bit.cu.
+struct LpCall {
+    const void* logits;
+    const int* tokens;
+    float* logprob;
+    int* rank;
+    float *entropy, *top_logprob;
+    int* top_id;
+    void* stream;
+    long long dtype, row_stride, rows, vocab, top;
+};
+extern "C" int rv_token_logprobs(const LpCall* c) {
+    const void* logits = c->logits;
+    const int* tokens = c->tokens;
+    float *logprob = c->logprob, *entropy = c->entropy, *top_logprob = c->top_logprob;
+    int *rank = c->rank, *top_id = c->top_id;
+    void* stream = c->stream;
+    const long long row_stride = c->row_stride;
+    const int dtype = (int)c->dtype, rows = (int)c->rows, vocab = (int)c->vocab, top = (int)c->top;
+    if (c->rows > 0x7fffffff || c->vocab > 0x7fffffff) RV_FAIL("token_logprobs: bad sizes");
     if (rows == 0) return 0;
     if (rows < 0 || vocab <= 0) RV_FAIL("token_logprobs: bad sizes");
     if (top < 0 || top > 32 || top > vocab) RV_FAIL("token_logprobs: %d alternatives (0 to 32, at most the vocabulary)", top);

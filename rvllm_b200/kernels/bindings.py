@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
@@ -22,6 +23,10 @@ from ..errors import KernelError
 from .build import build, build_variant
 
 _F32, _BF16 = 0, 1
+
+# Records of 8-byte whole numbers and a real one or none behind them, as the 8-bit calls and the log probabilities take them
+_WRITE_8BIT, _READ_8BIT = struct.Struct("=22qd"), struct.Struct("=11q")
+_ATTEND_8BIT, _LOGPROBS = struct.Struct("=27qd"), struct.Struct("=13q")
 
 
 def _code(dtype: torch.dtype) -> int:
@@ -124,13 +129,12 @@ class CudaOps:
         self.gated_delta_above = 288
         P, I, L = c_void_p, c_int, c_longlong
         self._write_8bit = self.lib.rv_qk_norm_rope_write_8bit
-        self._write_8bit.argtypes = [P, I, L, I, I, I, I, P, P, c_float, P, P, L, P, P, P, P, P, P, P, L, I, P]
         self._read_8bit = self.lib.rv_read_8bit
-        self._read_8bit.argtypes = [P, P, P, P, I, I, I, I, I, L, P]
+        self._token_logprobs = self.lib.rv_token_logprobs
+        for fn in (self._write_8bit, self._read_8bit, self._token_logprobs):
+            fn.argtypes = [ctypes.c_char_p]                  # one record (`_record`)
         self._widen_8bit = self.lib.rv_widen_8bit
         self._widen_8bit.argtypes = [P, P, P, P, L, P, I, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P]
-        self._token_logprobs = self.lib.rv_token_logprobs
-        self._token_logprobs.argtypes = [P, I, L, I, I, P, I, P, P, P, P, P, P]
         # the library's float32 products must be float32: no TF32, no reduced-precision accumulation
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
@@ -926,7 +930,7 @@ class CudaOps:
             self._not_held(what, slot_mapping, "slots", i32, here)
         if slot_mapping.dim() != 1 or slot_mapping.numel() < n:
             self._fault(what, "a slot for every token")
-        qw = kw = cos_at = sin_at = at = None
+        qw = kw = cos_at = sin_at = at = 0
         if q_weight is not None:
             if q_weight.dtype is not f32 or not q_weight.is_contiguous() or q_weight.get_device() != here:
                 self._not_held(what, q_weight, "norm weight", f32, here)
@@ -953,10 +957,10 @@ class CudaOps:
             if positions.dim() != 1 or positions.numel() < n:
                 self._fault(what, "a position for every token")
             angles, cos_at, sin_at, at = cos.size(0), cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
-        self._check(self._write_8bit(
-            qkv.data_ptr(), code, stride, n, num_heads, num_kv_heads, head_dim, qw, kw, eps, cos_at, sin_at, angles, at,
-            slot_mapping.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), pages, page_size, self._raw_stream(here)), what)
+        self._check(self._write_8bit(_WRITE_8BIT.pack(
+            qkv.data_ptr(), qw, kw, cos_at, sin_at, at, slot_mapping.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self._raw_stream(here), code, stride, n, num_heads,
+            num_kv_heads, head_dim, angles, pages, page_size, eps)), what)
 
     def read_8bit(self, cache, scale, pages, dtype):
         """The pages `pages` (int32 [n]) of an 8-bit cache as values, `dtype` [n, kv heads, page size,
@@ -969,9 +973,11 @@ class CudaOps:
         if pages.dim() != 1:
             self._fault(what, "page numbers are one row")
         n = pages.numel()
-        out = torch.empty((n, heads, page_size, dim), dtype=dtype, device=cache.device)
-        self._check(self._read_8bit(cache.data_ptr(), scale.data_ptr(), pages.data_ptr(), out.data_ptr(), code, n, heads,
-                                    page_size, dim, have, self._raw_stream(here)), what)
+        size = page_size * dim
+        out = torch.empty_strided((n, heads, page_size, dim), (heads * size, size, dim, 1), dtype=dtype, device=cache.device)
+        self._check(self._read_8bit(_READ_8BIT.pack(
+            cache.data_ptr(), scale.data_ptr(), pages.data_ptr(), out.data_ptr(), self._raw_stream(here), code, n, heads,
+            page_size, dim, have)), what)
         return out
 
     def _attn8_lib(self, head_dim: int):
@@ -989,11 +995,10 @@ class CudaOps:
             error = getattr(lib, f"rv_attention_8bit_last_error_hd{head_dim}")
             error.restype = ctypes.c_char_p
             call = getattr(lib, f"rv_paged_attention_8bit_hd{head_dim}")
-            P, I, L = c_void_p, c_int, c_longlong
-            call.argtypes = [P, I, L, P, P, P, P, L, P, I, P, P, P, P, L, I, I, I, I, I, I, I, I, c_float, I, P, I, P]
+            call.argtypes = [ctypes.c_char_p]
             scratch = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")
             scratch.restype = c_longlong
-            scratch.argtypes = [I] * 6
+            scratch.argtypes = [c_int] * 6
             hit = self._attn_libs[key] = (call, scratch, error)
         return hit
 
@@ -1054,11 +1059,11 @@ class CudaOps:
         if n_decode or not tcgen05:
             need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms)
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-            rc = call(q.data_ptr(), code, stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                      v_scale.data_ptr(), pages, table.data_ptr(), table.size(1), q_start.data_ptr(), ctx_lens.data_ptr(),
-                      out.data_ptr(), None if scratch is None else scratch.data_ptr(), need, n_decode, n_reqs,
-                      portions and not tcgen05, longest, deepest, num_heads, num_kv_heads, page_size, scale, window, sinks_at,
-                      sms, stream)
+            rc = call(_ATTEND_8BIT.pack(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
+                q_start.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                sinks_at or 0, stream, code, stride, pages, table.size(1), need, n_decode, n_reqs, portions and not tcgen05,
+                longest, deepest, num_heads, num_kv_heads, page_size, window, sms, scale))
             self.launches += (n_decode > 0) + (need > 0) + (portions and not tcgen05)
             if rc != 0:
                 raise KernelError(error().decode())
@@ -2045,11 +2050,11 @@ class CudaOps:
             self._fault(what, f"{top} alternatives of {vocab} (0 to 32)")
         f32, i32, device = torch.float32, torch.int32, logits.device
         logprob = torch.empty(rows, dtype=f32, device=device)
-        entropy = torch.empty(rows, dtype=f32, device=device)
-        rank = torch.empty(rows, dtype=i32, device=device)
+        entropy = torch.empty_like(logprob)
+        rank = torch.empty_like(tokens)
         best = torch.empty((rows, top), dtype=f32, device=device)
-        ids = torch.empty((rows, top), dtype=i32, device=device)
-        self._check(self._token_logprobs(
-            logits.data_ptr(), code, stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(), rank.data_ptr(),
-            entropy.data_ptr(), best.data_ptr(), ids.data_ptr(), self._raw_stream(here)), what)
+        ids = torch.empty_like(best, dtype=i32)
+        self._check(self._token_logprobs(_LOGPROBS.pack(
+            logits.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), rank.data_ptr(), entropy.data_ptr(), best.data_ptr(),
+            ids.data_ptr(), self._raw_stream(here), code, stride, rows, vocab, top)), what)
         return logprob, rank, entropy, best, ids
