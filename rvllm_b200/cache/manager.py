@@ -46,6 +46,8 @@ class CacheView:
     group: int = -1                    # paged: index into StepContext.groups
     k: Optional[torch.Tensor] = None   # paged: [pages, page_size, kv_heads, head_dim]
     v: Optional[torch.Tensor] = None
+    k_scale: Optional[torch.Tensor] = None  # 8-bit pages: float32 [pages, kv_heads]; k and v are int8
+    v_scale: Optional[torch.Tensor] = None  # [pages, kv_heads, page_size, head_dim]
     state: Optional[torch.Tensor] = None   # state: float32 [slots, *shape]
     parts: Optional[list] = None       # several: one view (or None) per branch of the mixer
 
@@ -57,6 +59,8 @@ class Group:
     pool: PagePool
     k: Optional[torch.Tensor] = None
     v: Optional[torch.Tensor] = None
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
 
 
 class PageTable:
@@ -113,12 +117,18 @@ class RequestCache:
 class CacheManager:
     def __init__(self, needs: Sequence[Optional[object]], cache_of: Sequence[Optional[int]],
                  page_size: int, num_pages: int, max_requests: int,
-                 dtype: torch.dtype = torch.float32, device="cpu", allocate: bool = True):
+                 dtype: torch.dtype = torch.float32, device="cpu", allocate: bool = True,
+                 kv_dtype: Optional[torch.dtype] = None):
         """needs[i]: PagedNeed, StateNeed, SeveralNeeds (a mixer of several mixers: each part is
         handled as a call of its own, named (i, part)) or None for call i of the run order;
         cache_of[i]: the call whose cache call i reads, or None.  `num_pages` pages per
         group; `max_requests` state slots.  `allocate=False` keeps only the
-        bookkeeping (for tests and planning)."""
+        bookkeeping (for tests and planning).  `kv_dtype` torch.int8: keys and values in 8 bits,
+        [calls, pages, kv_heads, page_size, head_dim], with a float32 scale per page and head (for
+        one row a token whose values are as long as its keys); None: in `dtype`."""
+        if kv_dtype not in (None, dtype, torch.int8):
+            raise CacheError(f"keys and values are held in {dtype} or int8, not {kv_dtype}")
+        self.eight_bit = kv_dtype == torch.int8
         if page_size < 1:
             raise CacheError(f"page size must be at least 1, got {page_size}")
         self.page_size = page_size
@@ -171,6 +181,9 @@ class CacheManager:
                     self.states[i] = block[ci]
         for grp in self.groups:
             if allocate:
+                if self.eight_bit:
+                    self._allocate_8bit(grp)
+                    continue
                 shape = (len(grp.calls), grp.pool.num_pages, page_size, grp.need.num_kv_heads)
                 grp.k = torch.zeros(shape + (grp.need.head_dim,), dtype=dtype, device=device)
                 grp.v = torch.zeros(shape + (grp.need.value_dim,), dtype=dtype, device=device)
@@ -178,8 +191,8 @@ class CacheManager:
             if src in call_group:
                 grp = self.groups[call_group[src]]
                 ci = grp.calls.index(src)
-                return CacheView("paged", owns, call_group[src], grp.k[ci] if allocate else None,
-                                 grp.v[ci] if allocate else None)
+                return CacheView("paged", owns, call_group[src], *(
+                    t[ci] if t is not None else None for t in (grp.k, grp.v, grp.k_scale, grp.v_scale)))
             if src in self.states:
                 return CacheView("state", owns, state=self.states[src])
             return None
@@ -197,6 +210,15 @@ class CacheManager:
             self._views[i] = view(cache_of[i] if cache_of[i] is not None else i,
                                   cache_of[i] is None)
 
+    def _allocate_8bit(self, grp: Group) -> None:
+        need = grp.need
+        if not need.values or need.value_dim != need.head_dim or need.every != 1:
+            raise CacheError("8-bit pages hold one row a token with values as long as the keys")
+        pages = (len(grp.calls), grp.pool.num_pages, need.num_kv_heads)
+        grp.k, grp.v = (torch.zeros(pages + (self.page_size, need.head_dim), dtype=torch.int8, device=self.device)
+                        for _ in "kv")
+        grp.k_scale, grp.v_scale = (torch.zeros(pages, dtype=torch.float32, device=self.device) for _ in "kv")
+
     # ---- what the model sees ---------------------------------------------------------
 
     def views(self) -> List[Optional[CacheView]]:
@@ -204,6 +226,9 @@ class CacheManager:
 
     def bytes_per_token(self) -> int:
         """Bytes of keys and values one cached token takes over all groups."""
+        if self.eight_bit:                              # and two scales a page and head
+            return sum(len(g.calls) * g.need.num_kv_heads * (2 * g.need.head_dim + -(-8 // self.page_size))
+                       for g in self.groups)
         size = torch.empty((), dtype=self.dtype).element_size()
         return sum(len(g.calls) * g.need.num_kv_heads * (g.need.head_dim + g.need.value_dim) * size
                    // g.need.every for g in self.groups)

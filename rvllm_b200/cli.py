@@ -8,7 +8,7 @@ Option names, meanings and defaults are the reference's: each `--prompt` is one
 concurrent request; `--arrival-step`, one per prompt in order, is the engine step at
 which that request becomes eligible; `--max-tokens` defaults to 20; temperature 0 is
 greedy; one completion is printed per line in prompt order.  Added here: `--token-ids`
-(prompts are lists of token ids, printed back as ids), `--dtype`, `--prefill-chunk`,
+(prompts are lists of token ids, printed back as ids), `--dtype`, `--kv-cache`, `--prefill-chunk`,
 `--max-batched-tokens`, and the `random-model` command, which writes a model folder
 with random weights from a config.json and a seed.  The reference's interactive loop,
 chat formatting, terminal UI and server are outside this engine.
@@ -34,6 +34,8 @@ def build_parser() -> argparse.ArgumentParser:
                      help="tokenizer.json (default: the one beside the model)")
     cli.add_argument("--device", default="cuda", help="cuda or cuda:N (there is no CPU path)")
     cli.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    cli.add_argument("--kv-cache", default="auto", choices=["auto", "int8"],
+                     help="int8: keys and values in 8 bits with a scale per page and head")
     cli.add_argument("--block-size", type=int, default=16, help="tokens per KV page")
     cli.add_argument("--num-blocks", type=int, default=None,
                      help="KV pages in the pool (default: room for every request)")
@@ -71,7 +73,8 @@ def run_cli(args) -> int:
               f"CUDA only", file=sys.stderr)
         return 2
     from .engine import GenerateOptions, Generator
-    gen = Generator.load(args.model, args.tokenizer, args.device, args.dtype)
+    gen = Generator.load(args.model, args.tokenizer, args.device, args.dtype,
+                         **({} if args.kv_cache == "auto" else {"kv_cache": args.kv_cache}))
     prompts = [_ids(p) for p in args.prompt] if args.token_ids else list(args.prompt)
     opts = GenerateOptions(max_tokens=args.max_tokens, temperature=args.temperature,
                            top_p=args.top_p, seed=args.seed, block_size=args.block_size,

@@ -16,6 +16,9 @@ import time
 from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence
 
+import torch
+
+from ..sampling.logprobs import LogprobReader, TokenLogprob
 from ..sampling.sampler import BatchSampler
 from .batch import StepEntry
 from .scheduler import FinishReason, Request, Scheduler, SchedulerConfig, TokenEvent
@@ -39,6 +42,7 @@ class RunResult:
     outputs: Dict[Hashable, List[int]]
     finish: Dict[Hashable, FinishReason]
     stats: RunStats
+    logprobs: Optional[Dict[Hashable, List[TokenLogprob]]] = None    # one per output token, where asked for
 
 
 @dataclass
@@ -50,6 +54,14 @@ class _InFlight:
     ready: object                   # event recorded after the copy (or None)
 
     check: object = None            # called with the kernels' status word read beside the ids
+    logprobs: Optional[LogprobReader] = None
+
+    def token_logprobs(self) -> dict:
+        """By request, of the tokens that this step sampled (after `tokens`)."""
+        if self.logprobs is None:
+            return {}
+        who = [e.seq.request.id for e in self.plan if e.samples]
+        return dict(zip(who, self.logprobs.read()))
 
     def tokens(self) -> List[int]:
         if self.ids is None:
@@ -70,10 +82,16 @@ class Engine:
     step's sampled ids, so the GPU never waits for the host.  A sequence that turns out to have
     finished (a stop token) has then run one step too many; that step's result for it is
     dropped and its pages were freed only after the launch, in stream order.  The tokens a
-    request gets are the same with and without lookahead."""
+    request gets are the same with and without lookahead.
+
+    `logprobs`: the number of alternatives (0 to 32) with which every sampled token's log probability
+    comes in its event, or None."""
 
     def __init__(self, runner, config: SchedulerConfig, context_length: int, sampler=None,
-                 lookahead: bool = False):
+                 lookahead: bool = False, logprobs: Optional[int] = None):
+        if logprobs is not None and not 0 <= logprobs <= 32:
+            raise ValueError(f"logprobs asks for 0 to 32 alternatives, got {logprobs}")
+        self.logprobs = logprobs
         self.runner = runner
         self.scheduler = Scheduler(config, runner.cache, context_length)
         self.sampler = sampler or BatchSampler(runner.ops, runner.device)
@@ -111,11 +129,14 @@ class Engine:
         status = getattr(self.runner.ops, "status_word", None)
         if not self.lookahead:
             ids = self.sampler.sample(logits, params, counters)
+            reader = self._read_logprobs(logits, ids)
             if status is not None:
                 self.runner.ops.check_status()
-            return _InFlight(plan, _HostIds(ids), None, None)
-        import torch
+            if reader is not None and logits.is_cuda:
+                torch.cuda.current_stream().synchronize()
+            return _InFlight(plan, _HostIds(ids), None, None, None, reader)
         ids = self.sampler.sample_device(logits, params, counters)
+        reader = self._read_logprobs(logits, ids)
         n = ids.shape[0]
         host = torch.empty(n + (status is not None), dtype=ids.dtype, pin_memory=True)
         host[:n].copy_(ids, non_blocking=True)
@@ -128,7 +149,14 @@ class Engine:
             check = lambda code: ops.raise_for_status(code, ids.device)
         ready = torch.cuda.Event()
         ready.record()
-        return _InFlight(plan, ids, host, ready, check)
+        return _InFlight(plan, ids, host, ready, check, reader)
+
+    def _read_logprobs(self, logits, ids) -> Optional[LogprobReader]:
+        if self.logprobs is None:
+            return None
+        if not torch.is_tensor(ids):
+            ids = torch.tensor(ids, dtype=torch.int32, device=logits.device)
+        return LogprobReader(self.runner.ops, logits[:ids.shape[0]], ids, self.logprobs)
 
     def _can_look_ahead(self, plan) -> bool:
         sch = self.scheduler
@@ -172,6 +200,10 @@ class Engine:
             nxt = self._launch(ahead, device_tokens=flying.ids, extra_drawn=1)
             self.lookahead_steps += 1
         events = self.scheduler.update(flying.plan, flying.tokens())
+        if self.logprobs is not None:
+            of = flying.token_logprobs()
+            for ev in events:
+                ev.logprob = of[ev.id]
         if nxt is not None:
             # keep only the sequences that are still running; the others ran one step for nothing
             alive = [i for i, e in enumerate(nxt.plan) if e.seq.request.id in self.scheduler.seqs]
@@ -201,6 +233,9 @@ class _Subset(_InFlight):
         super().__init__([base.plan[i] for i in keep], base.ids.index_select(0, rows), base.host,
                          base.ready, None)
         self._base, self._keep = base, keep
+
+    def token_logprobs(self) -> dict:
+        return self._base.token_logprobs()
 
     def tokens(self) -> List[int]:
         all_tokens = self._base.tokens()
@@ -238,15 +273,16 @@ def settled_heap():
 
 
 def run(runner, requests: Sequence[Request], config: SchedulerConfig, context_length: int,
-        sampler=None, lookahead: bool = False) -> RunResult:
+        sampler=None, lookahead: bool = False, logprobs: Optional[int] = None) -> RunResult:
     """Run `requests` to completion; outputs hold the generated tokens, a stop token
     included when one ended the request."""
     with settled_heap():
-        return _run(runner, requests, config, context_length, sampler, lookahead)
+        return _run(runner, requests, config, context_length, sampler, lookahead, logprobs)
 
 
-def _run(runner, requests, config, context_length, sampler, lookahead) -> RunResult:
-    engine = Engine(runner, config, context_length, sampler, lookahead)
+def _run(runner, requests, config, context_length, sampler, lookahead, logprobs) -> RunResult:
+    engine = Engine(runner, config, context_length, sampler, lookahead, logprobs)
+    of: Dict[Hashable, List[TokenLogprob]] = {r.id: [] for r in requests}
     for r in requests:
         engine.add_request(r)
     outputs: Dict[Hashable, List[int]] = {r.id: [] for r in requests}
@@ -256,6 +292,8 @@ def _run(runner, requests, config, context_length, sampler, lookahead) -> RunRes
     while engine.has_work():
         for ev in engine.step():
             outputs[ev.id].append(ev.token)
+            if ev.logprob is not None:
+                of[ev.id].append(ev.logprob)
             if ev.ttft is not None:
                 stats.ttft[ev.id] = ev.ttft
             if ev.finish is not None:
@@ -268,4 +306,4 @@ def _run(runner, requests, config, context_length, sampler, lookahead) -> RunRes
     if runner.cache.groups:
         stats.page_allocs = sum(g.pool.total_allocs for g in runner.cache.groups)
         stats.pages_high_water = max(g.pool.high_water for g in runner.cache.groups)
-    return RunResult(outputs, finish, stats)
+    return RunResult(outputs, finish, stats, of if logprobs is not None else None)

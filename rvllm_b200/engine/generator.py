@@ -4,6 +4,10 @@
     gen = Generator.load(model_dir)                     # device "cuda", dtype "bfloat16"
     text = gen.complete("prompt", GenerateOptions(max_tokens=64))
     ids  = gen.complete([5, 17, 3], GenerateOptions(max_tokens=8))   # token ids in and out
+    lps  = gen.score([5, 17, 3])                        # log probabilities of a prompt's own tokens
+
+`Generator.load(..., kv_cache="int8")` holds keys and values in 8 bits with a scale per page and head;
+`score` under both caches says what that costs a model.
 
 `GenerateOptions` keeps the reference's fields and defaults (max_tokens 64, greedy,
 block_size 16, src/generator.rs:24-36) and adds the pool and scheduling knobs of the
@@ -21,9 +25,11 @@ from typing import List, Optional, Sequence, Union
 
 import torch
 
+from ..sampling.logprobs import LogprobReader, TokenLogprob
 from ..sampling.params import SamplingParams
+from .batch import StepEntry
 from .engine import RunResult, run
-from .loading import load_model, make_cache
+from .loading import load_model, make_cache, parse_kv_cache
 from .runner import ModelRunner
 from .scheduler import Request, SchedulerConfig
 
@@ -45,6 +51,8 @@ class GenerateOptions:
     max_batched_tokens: int = 8192            # token budget of a step
     max_running: Optional[int] = None
     stop_tokens: Optional[Sequence[int]] = None   # default: the model's eos token
+    logprobs: Optional[int] = None            # log probabilities of the generated tokens, with so many alternatives
+                                              # (0 to 32), in `last_result.logprobs`
 
     @property
     def sampling(self) -> SamplingParams:
@@ -55,8 +63,9 @@ Prompt = Union[str, Sequence[int]]
 
 
 class Generator:
-    def __init__(self, model, config, tokenizer=None):
+    def __init__(self, model, config, tokenizer=None, kv_cache: str = "auto"):
         self.model = model
+        self.kv_cache = kv_cache
         self.config = config
         self.ops = model.ops
         self.tokenizer = tokenizer
@@ -68,7 +77,9 @@ class Generator:
 
     @classmethod
     def load(cls, model_dir: str, tokenizer: Optional[str] = None, device: str = "cuda",
-             dtype: str = "bfloat16") -> "Generator":
+             dtype: str = "bfloat16", kv_cache: str = "auto") -> "Generator":
+        """`kv_cache`: "auto" (keys and values in `dtype`) or "int8"."""
+        parse_kv_cache(kv_cache)
         model, config = load_model(model_dir, dtype, device)
         tok_path = tokenizer or os.path.join(model_dir, "tokenizer.json")
         tok = None
@@ -78,7 +89,7 @@ class Generator:
                 tok = Tokenizer.from_file(tok_path)
             except ImportError:
                 tok = None
-        return cls(model, config, tok)
+        return cls(model, config, tok, kv_cache)
 
     # ---- helpers ---------------------------------------------------------------------
 
@@ -110,7 +121,7 @@ class Generator:
                 slots = max(slots, have.cache.max_requests)
                 key = (block_size, num_blocks, slots)
             self._runner = have = None
-            cache = make_cache(self.model, block_size, num_blocks, slots)
+            cache = make_cache(self.model, block_size, num_blocks, slots, self.kv_cache)
             self._runner = ModelRunner(self.model, cache, self.ops, use_graphs=graphs_default())
             self._runner_key = key
         return self._runner
@@ -169,5 +180,42 @@ class Generator:
             requests.append(Request(i, list(p), opts.max_tokens, stops,
                                     SamplingParams(opts.temperature, opts.top_p, opts.seed + i),
                                     arrival))
-        self.last_result = run(runner, requests, cfg, context, lookahead=self.lookahead)
+        self.last_result = run(runner, requests, cfg, context, lookahead=self.lookahead,
+                               logprobs=opts.logprobs)
         return self.last_result
+
+    def score(self, prompt: Prompt, top: int = 0, portion: int = 512,
+              block_size: int = 16) -> List[TokenLogprob]:
+        """The log probability of every token of `prompt` after the first, given those before it, with rank,
+        entropy and the `top` most probable tokens at its place.  The prompt is run `portion` tokens at a
+        time, so that no more rows of logits exist at once."""
+        ids = self._encode(prompt)
+        vocab, context = self.model.spec.vocab_size, self.model.spec.max_position
+        if any(t < 0 or t >= vocab for t in ids):
+            raise ValueError(f"the prompt has a token id outside the vocabulary of {vocab}")
+        if len(ids) > context:
+            raise ValueError(f"{len(ids)} tokens exceed the model's {context} positions")
+        if portion < 1 or not 0 <= top <= min(32, vocab):
+            raise ValueError("score takes portions of a token at least and 0 to 32 alternatives")
+        if len(ids) < 2:
+            return []
+        runner = self._runner_for(block_size, -(-len(ids) // block_size), 1, exact=False)
+        for rid in list(runner.cache.requests):       # left behind by a call that raised
+            runner.end_request(rid)
+        runner.add_request("score")
+        found: List[TokenLogprob] = []
+        try:
+            for a in range(0, len(ids) - 1, portion):
+                b = min(a + portion, len(ids) - 1)
+                logits = runner.step([StepEntry("score", ids[a:b], range(b - a))])
+                tokens = torch.tensor(ids[a + 1:b + 1], dtype=torch.int32, device=logits.device)
+                reader = LogprobReader(self.ops, logits, tokens, top)
+                if logits.is_cuda:
+                    torch.cuda.current_stream().synchronize()
+                found += reader.read()
+                status = getattr(self.ops, "check_status", None)
+                if status is not None:
+                    status()
+        finally:
+            runner.end_request("score")
+        return found

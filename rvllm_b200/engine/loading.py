@@ -9,6 +9,7 @@ import torch
 
 from ..cache import CacheManager
 from ..config.registry import architecture, load_config
+from ..parts.base import StateNeed, arrangement_class, mixer_class
 from ..parts.model import Model
 from ..weights.loader import load_tensors, tensor_shapes
 
@@ -45,7 +46,31 @@ def load_model(folder: str, dtype="bfloat16", device="cuda", ops=None):
     return model, config
 
 
-def make_cache(model: Model, page_size: int, num_pages: int, max_requests: int) -> CacheManager:
-    return CacheManager(model.cache_needs(), [c.cache_of for c in model.spec.order],
+KV_CACHES = {"auto": None, "int8": torch.int8}
+
+
+def parse_kv_cache(name):
+    """None (keys and values in the model's type) or torch.int8."""
+    if name is None or name == torch.int8:
+        return name
+    if name not in KV_CACHES:
+        raise ValueError(f"unknown key/value cache {name!r} (known: auto, int8)")
+    return KV_CACHES[name]
+
+
+def make_cache(model: Model, page_size: int, num_pages: int, max_requests: int,
+               kv_cache="auto") -> CacheManager:
+    """`kv_cache` "int8": keys and values in 8 bits with a scale per page and head, for models whose
+    attention layers all read such pages."""
+    kv_dtype, needs = parse_kv_cache(kv_cache), model.cache_needs()
+    if kv_dtype is not None:
+        for call in model.spec.order:
+            block = model.spec.layers[call.layer]
+            need = arrangement_class(block.arrangement).cache_need(block)
+            if need is not None and not isinstance(need, StateNeed) and \
+                    not mixer_class(block.mixer.kind).eight_bit_cache(block.mixer):
+                raise ValueError(f"a layer of kind {block.mixer.kind!r} as this model has it does not read "
+                                 f"keys and values in 8 bits")
+    return CacheManager(needs, [c.cache_of for c in model.spec.order],
                         page_size, num_pages, max_requests, dtype=model.dtype,
-                        device=model.device)
+                        device=model.device, kv_dtype=kv_dtype)

@@ -56,6 +56,7 @@ class TokenEvent:
     token: int
     finish: Optional[FinishReason] = None
     ttft: Optional[float] = None       # seconds from admission to the first token
+    logprob: Optional[object] = None   # `sampling.TokenLogprob`, where the engine was asked for them
 
 
 @dataclass

@@ -28,6 +28,10 @@ temperature and the cache write are `ops.qk_unit_write` after the one q|k|v prod
 per head (`head_gate`): head j's result is multiplied by sigmoid(W_g x)_j before the output
 product; W_g's rows ride at the end of the q|k|v product and `ops.head_gate` applies them.
 
+Where the cache holds keys and values in 8 bits (`CacheView.k_scale`), the plain form -- a weighted
+norm per head or none, a rotation by halves or none, a window, sinks -- writes and reads those
+(`_forward_8bit`); no other form does.
+
 A third form (`_prepared`), chosen by any of: biases on the q, k and v projections (`bias`); a
 norm over the whole query projection and one over the whole key projection, before the split
 into heads (`qk_norm` of kind "rms_full"); a rotation of neighbouring dimensions (position
@@ -129,6 +133,11 @@ class Attention(Mixer):
                          keep_first=spec.keep_first)
 
     @staticmethod
+    def eight_bit_cache(spec: AttentionSpec) -> bool:
+        return Attention._plain(spec) and not Attention._prepared(spec) and not spec.keep_first and \
+            spec.head_dim % 16 == 0 and spec.head_dim <= 256
+
+    @staticmethod
     def workspace_bytes(spec: AttentionSpec, ops, max_requests: int, max_context: int) -> int:
         if spec.keep_first:
             sizer = getattr(ops, "attention_pooled_scratch_bytes", None)
@@ -217,6 +226,8 @@ class Attention(Mixer):
             return self._forward_prepared(normed, ctx, cache, group)
         if not self._plain(s):
             return self._forward_options(normed, ctx, cache, group)
+        if cache.k_scale is not None:
+            return self._forward_8bit(normed, ctx, cache, group)
         qkv = self.ops.linear_qk_norm_rope_write(
             normed, self.w_qkv if owns else self.w_q, s.num_heads,
             s.num_kv_heads if owns else 0, s.head_dim,
@@ -225,6 +236,26 @@ class Attention(Mixer):
             cache.k if owns else None, cache.v if owns else None, out_dtype=self.dtype)
         out = self.ops.new_rows(normed.shape[0], s.num_heads * s.head_dim, self.dtype, normed.device)
         self._attend(qkv, cache, ctx, group, out)
+        return self.ops.linear(out, self.w_out, bias=self.b_out, out_dtype=self.dtype)
+
+    def _forward_8bit(self, normed, ctx, cache, group):
+        """The plain form over pages of 8 bits: q to rows of its own, k and v to the pages, which both
+        single tokens and portions read."""
+        s, n = self.spec, normed.shape[0]
+        table, eps = self.position.rotation_table(), s.qk_norm.eps if s.qk_norm else 0.0
+        rows = self.ops.linear(normed, self.w_qkv if cache.owns else self.w_q, out_dtype=self.dtype)
+        if cache.owns:
+            q = self.ops.new_rows(n, s.num_heads * s.head_dim, self.dtype, normed.device)
+            self.ops.qk_norm_rope_write_8bit(rows, s.num_heads, s.num_kv_heads, s.head_dim, self.q_norm, self.k_norm, eps,
+                                             table, ctx.positions, group.slot_mapping, q, cache.k, cache.v,
+                                             cache.k_scale, cache.v_scale)
+        else:
+            q = rows
+            self.ops.qk_norm_rope_write(rows, s.num_heads, 0, s.head_dim, self.q_norm, None, eps, table, ctx.positions,
+                                        group.slot_mapping, None, None)
+        out = self.ops.new_rows(n, s.num_heads * s.head_dim, self.dtype, normed.device)
+        self.ops.paged_attention_8bit(q, s.num_heads, s.num_kv_heads, s.head_dim, cache.k, cache.v, cache.k_scale,
+                                      cache.v_scale, ctx, group, self.scale, s.window, out, sinks=self.sinks)
         return self.ops.linear(out, self.w_out, bias=self.b_out, out_dtype=self.dtype)
 
     def _attend(self, rows, cache, ctx, group, out):

@@ -101,6 +101,11 @@ class Mixer:
         return 0
 
     @staticmethod
+    def eight_bit_cache(spec) -> bool:
+        """Whether the mixer works from pages of 8 bits as well (`CacheView.k_scale` is there then)."""
+        return False
+
+    @staticmethod
     def launch_rules(spec, ops):
         """(limits, shallow): None, or the lengths of a step's longest prompt portion above which
         the mixer launches another form (none of them: only its launches' sizes follow that
