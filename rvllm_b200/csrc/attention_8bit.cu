@@ -177,13 +177,14 @@ __device__ __forceinline__ void a8_load_n(const __nv_bfloat16* p, bool vec, floa
 }
 
 // ---- how single tokens' tiles are shared out --------------------------------------------------------
-// The tiles of (request, unit), one after the other, cut evenly into as many runs as there are warps (`used` of them
-// where there are fewer tiles).  A unit: a key/value head and 8 * NT of its query heads.  From one segment to the next
-// the run or the unit grows, so run + request * units + unit is a place of its own.
+// The tiles of all requests, one after the other, are cut evenly into as many runs as there are teams of warps (`used`
+// of them where there are fewer tiles).  A team has a warp for every unit: a key/value head and 8 * NT of its query heads.  Its warps walk
+// the same tiles, so the heads of a page, which lie side by side, are read at about the same time.  From one segment (a run's part of a request) to the next the run or the request grows, so run + request is
+// a place of its own, times the units.
 struct A8Shares {
     const int* ctx_lens;
-    int n_reqs, units, window, most;
-    long long total, before;           // tiles of all units; of a unit over the requests before the one asked for
+    int n_reqs, window, most;
+    long long total, before;           // tiles of all requests; of those before the one asked for
     int used;
     bool narrow;
     static constexpr int KEPT = 4;
@@ -195,8 +196,8 @@ struct A8Shares {
     }
     __device__ __forceinline__ int length(int r) const { return r < n_reqs ? ctx_lens[r] : 0; }
     // (a whole warp at once)
-    __device__ __forceinline__ A8Shares(const int* lens, int reqs, int u, int win, long long slots, int runs, int r)
-        : ctx_lens(lens), n_reqs(reqs), units(u), window(win), most((int)min(slots, 0x7fffffffll)), total(0), before(0) {
+    __device__ __forceinline__ A8Shares(const int* lens, int reqs, int win, long long slots, int runs, int r)
+        : ctx_lens(lens), n_reqs(reqs), window(win), most((int)min(slots, 0x7fffffffll)), total(0), before(0) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int k = 0; k < KEPT; ++k) kept[k] = 32 * k < n_reqs ? length(32 * k + lane) : 0;
@@ -213,7 +214,6 @@ struct A8Shares {
             total += __reduce_add_sync(0xffffffffu, (unsigned)mine);
             before += __reduce_add_sync(0xffffffffu, (unsigned)(at + lane < r ? mine : 0));
         }
-        total *= units;
         used = (int)min((long long)runs, max(1ll, total));
         narrow = total * (used + 1) < 0xffffffffll;
     }
@@ -227,9 +227,9 @@ struct A8Shares {
 };
 
 // ---- one warp's work ----------------------------------------------------------------------------------
-// A place in the walk over tiles: the tile `tile` of (request r, unit u).
+// A place in the walk over tiles: the tile `tile` of request r.
 struct A8Cursor {
-    int r, u, tile, last, clen;
+    int r, tile, last, clen;
 };
 
 template <typename T, int NT, int PARTS>
@@ -581,88 +581,84 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
     extern __shared__ __align__(128) unsigned char smem[];
     A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
     const int per_head = (w.G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
-    // neighbours in the order of tiles on different multiprocessors
-    const int run = (int)(threadIdx.x >> 5) * gridDim.x + blockIdx.x;
-    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size,
-                      gridDim.x * A8_BLOCK_WARPS, 0);
-    if (run >= sh.used || sh.total == 0) return;
-    const long long from = sh.start(run);
-    int n = (int)(sh.start(run + 1) - from);
-    // where the run begins
-    A8Cursor c = {0, 0, 0, 0, 0};
-    {
-        const int lane = threadIdx.x & 31;
-        long long sum = 0;
-        bool found = false;
-        auto look = [&](int at, int mine) {
-            int upto = mine;
+    const int warps = gridDim.x * A8_BLOCK_WARPS, teams = max(1, warps / units);
+    const A8Shares sh(a.ctx_lens, a.n_reqs, a.window, (long long)a.max_blocks * a.page_size, teams, 0);
+    if (sh.total == 0) return;
+    // (more units than warps: a warp has several of the one team's)
+    for (int slot = blockIdx.x * A8_BLOCK_WARPS + (threadIdx.x >> 5); slot < teams * units; slot += warps) {
+        const int run = slot / units, u = slot - run * units, head = u / per_head;
+        if (run >= sh.used) return;
+        const long long from = sh.start(run);
+        const int n = (int)(sh.start(run + 1) - from);
+        // where the run begins
+        A8Cursor c = {0, 0, 0, 0};
+        {
+            const int lane = threadIdx.x & 31;
+            long long sum = 0;
+            bool found = false;
+            auto look = [&](int at, int mine) {
+                int upto = mine;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += v;
-            }
-            const unsigned who = __ballot_sync(0xffffffffu, (sum + upto) * units > from);
-            if (who) {
-                const int l = __ffs(who) - 1;
-                const int tiles = __shfl_sync(0xffffffffu, mine, l);
-                const unsigned in = (unsigned)(from - (sum + __shfl_sync(0xffffffffu, upto, l) - tiles) * units);
-                c.r = at + l;
-                c.clen = sh.length(c.r);
-                c.u = (int)(in / (unsigned)tiles);
-                c.tile = sh.first(c.clen) + (int)(in - (unsigned)c.u * (unsigned)tiles);
-                c.last = (c.clen - 1) / A8_KEYS;
-                found = true;
-            }
-            sum += __shfl_sync(0xffffffffu, upto, 31);
-        };
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += v;
+                }
+                const unsigned who = __ballot_sync(0xffffffffu, sum + upto > from);
+                if (who) {
+                    const int l = __ffs(who) - 1;
+                    c.r = at + l;
+                    c.clen = sh.length(c.r);
+                    c.tile = sh.first(c.clen) + (int)(from - sum) - __shfl_sync(0xffffffffu, upto - mine, l);
+                    c.last = (c.clen - 1) / A8_KEYS;
+                    found = true;
+                }
+                sum += __shfl_sync(0xffffffffu, upto, 31);
+            };
 #pragma unroll
-        for (int k = 0; k < A8Shares::KEPT; ++k)
-            if (!found && 32 * k < a.n_reqs) look(32 * k, sh.kept[k]);
-        for (int at = 32 * A8Shares::KEPT; !found && at < a.n_reqs; at += 32) look(at, sh.tiles(sh.length(at + lane)));
-    }
-    auto advance = [&](A8Cursor& x) {
-        if (++x.tile <= x.last) return;
-        if (++x.u == units) {
-            x.u = 0;
+            for (int k = 0; k < A8Shares::KEPT; ++k)
+                if (!found && 32 * k < a.n_reqs) look(32 * k, sh.kept[k]);
+            for (int at = 32 * A8Shares::KEPT; !found && at < a.n_reqs; at += 32) look(at, sh.tiles(sh.length(at + lane)));
+        }
+        auto advance = [&](A8Cursor& x) {
+            if (++x.tile <= x.last) return;
             do ++x.r;
             while (x.r < a.n_reqs && sh.tiles(sh.length(x.r)) == 0);
             x.clen = sh.length(x.r);
             x.last = (x.clen - 1) / A8_KEYS;
-        }
-        x.tile = sh.first(x.clen);
-    };
-    A8Cursor ahead = c;
-    int page = w.page_of(ahead), requested = 0;
-    auto request_next = [&](int stage) {
-        if (requested < n) {
-            w.request(ahead, ahead.u / per_head, page, stage);
-            if (++requested < n) {
-                advance(ahead);
-                page = w.page_of(ahead);
+            x.tile = sh.first(x.clen);
+        };
+        A8Cursor ahead = c;
+        int page = w.page_of(ahead), requested = 0;
+        auto request_next = [&](int stage) {
+            if (requested < n) {
+                w.request(ahead, head, page, stage);
+                if (++requested < n) {
+                    advance(ahead);
+                    page = w.page_of(ahead);
+                }
             }
+            A8_COMMIT();
+        };
+        for (int i = 0; i < A8_STAGES - 1; ++i) request_next(i);
+        bool fresh = true;
+        int stage = 0;
+        for (int i = 0; i < n; ++i) {
+            if (fresh) {
+                w.begin(c.r, head, (u - head * per_head) * 8 * NT, 1, c.r, c.clen);
+                fresh = false;
+            }
+            A8_WAIT_STAGE();
+            __syncwarp();
+            request_next(stage == 0 ? A8_STAGES - 1 : stage - 1);
+            w.tile(c.tile, stage);
+            __syncwarp();
+            stage = stage + 1 == A8_STAGES ? 0 : stage + 1;
+            if (c.tile == c.last || i + 1 == n) {
+                w.leave(((size_t)run + c.r) * units + u);
+                fresh = true;
+            }
+            if (i + 1 < n) advance(c);
         }
-        A8_COMMIT();
-    };
-    for (int i = 0; i < A8_STAGES - 1; ++i) request_next(i);
-    bool fresh = true;
-    int stage = 0;
-    for (int i = 0; i < n; ++i) {
-        if (fresh) {
-            const int head = c.u / per_head;
-            w.begin(c.r, head, (c.u - head * per_head) * 8 * NT, 1, c.r, c.clen);
-            fresh = false;
-        }
-        A8_WAIT_STAGE();
-        __syncwarp();
-        request_next(stage == 0 ? A8_STAGES - 1 : stage - 1);
-        w.tile(c.tile, stage);
-        __syncwarp();
-        stage = stage + 1 == A8_STAGES ? 0 : stage + 1;
-        if (c.tile == c.last || i + 1 == n) {
-            w.leave((size_t)run + (size_t)c.r * units + c.u);
-            fresh = true;
-        }
-        if (i + 1 < n) advance(c);
     }
 }
 
@@ -734,7 +730,7 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
     const int t_all = (a.window > 0 ? max(0, p_first - a.window + 1) : 0) / A8_KEYS;
     const int count = p_last >= 0 && fits ? p_last / A8_KEYS - t_all + 1 : 0;
     const int t_lo = t_all + (int)((long long)count * part / parts), n = t_all + (int)((long long)count * (part + 1) / parts) - t_lo;
-    A8Cursor ahead = {r, 0, t_lo, t_lo + n - 1, clen};
+    A8Cursor ahead = {r, t_lo, t_lo + n - 1, clen};
     int page = n > 0 ? w.page_of(ahead) : -1, requested = 0;
     auto request_next = [&](int stage) {
         if (requested < n) {
@@ -833,7 +829,8 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
 // `W` warps a row, which share its segments (eight where there may be many; a lane has two of every 64 dimensions and
 // requests eight segments' before it uses any: one memory latency for eight).
 template <typename T, int W>
-__device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, int stride_rows, int row, int head, T* dst, bool bad) {
+__device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, int units, int rows, int row, int head, T* dst, bool bad) {
+    const size_t step = (size_t)units * rows, at0 = place * rows + row;           // of a place's row to the next run's
     const int lane = threadIdx.x & 31, part = W == 1 ? 0 : threadIdx.x >> 5;
     constexpr int PER = (A8_HD + 63) / 64, AHEAD = 8;
     float2 o[PER];
@@ -841,14 +838,14 @@ __device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, i
     for (int k = 0; k < PER; ++k) o[k] = make_float2(0.f, 0.f);
     float M = -INFINITY, L = 0.f;
     for (int at = part * AHEAD; at < n; at += W * AHEAD) {
-        const float2 ml = lane < AHEAD && at + lane < n ? a.part_ml[(place + at + lane) * stride_rows + row] : make_float2(-INFINITY, 0.f);
+        const float2 ml = lane < AHEAD && at + lane < n ? a.part_ml[at0 + (at + lane) * step] : make_float2(-INFINITY, 0.f);
         float2 v[AHEAD][PER];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
             for (int k = 0; k < PER; ++k)
                 v[i][k] = at + i < n && (A8_HD % 64 == 0 || 64 * k + 2 * lane < A8_HD)
-                              ? *(const float2*)(a.part_o + ((place + at + i) * stride_rows + row) * A8_HD + 64 * k + 2 * lane)
+                              ? *(const float2*)(a.part_o + (at0 + (at + i) * step) * A8_HD + 64 * k + 2 * lane)
                               : make_float2(0.f, 0.f);
         const float most = fmaxf(M, rv_warp_max(ml.x));
         const float off = most == -INFINITY ? 0.f : most;
@@ -904,10 +901,10 @@ __device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, i
         }
 }
 
-// A warp (W = 1: four rows a block) or a block a row; blockIdx.y: request, x: head.
+// A warp (W = 1: four rows a block) or a block a row; blockIdx.y: request, x: head.  It lets no launch behind it begin
+// before it is done: blocks of the next stream that wait where this one's have yet to run cost 17 us of 60 a call.
 template <typename T, int NT, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_merge_kernel(const __grid_constant__ A8Args a, int runs) {
-    rv_pdl_launch_dependents();
     const int G = a.num_heads / a.num_kv_heads, per_head = (G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
     const int r = blockIdx.y, head = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (head >= a.num_heads) {
@@ -915,16 +912,15 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_m
         return;
     }
     const int kvh = head / G, in = head - kvh * G, u = kvh * per_head + in / (8 * NT);
-    const A8Shares sh(a.ctx_lens, a.n_reqs, units, a.window, (long long)a.max_blocks * a.page_size, runs, r);
+    const A8Shares sh(a.ctx_lens, a.n_reqs, a.window, (long long)a.max_blocks * a.page_size, runs, r);
     const int clen = sh.length(r), tiles = sh.tiles(clen);
     int run0 = 0, n = 0;
     if (tiles) {
-        const long long start = sh.before * units + (long long)u * tiles;
-        run0 = sh.run_of(start);
-        n = sh.run_of(start + tiles - 1) - run0 + 1;
+        run0 = sh.run_of(sh.before);
+        n = sh.run_of(sh.before + tiles - 1) - run0 + 1;
     }
     rv_pdl_wait();
-    a8_merge<T, W>(a, (size_t)run0 + (size_t)r * units + u, n, 8 * NT, in % (8 * NT), head,
+    a8_merge<T, W>(a, ((size_t)run0 + r) * units + u, n, units, 8 * NT, in % (8 * NT), head,
                    (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
 }
 
@@ -972,7 +968,8 @@ extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode,
     const int G = num_heads / num_kv_heads, nt = a8_nt(G);
     const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
     if (n_decode <= 0 || a8_few(units * n_decode, a8_tiles(max_ctx_len, window, 1), n_sms)) return 0;
-    return ((long long)n_sms * A8_MOST_WARPS + n_decode * units) * a8_place_bytes(nt);
+    const long long all = (long long)n_sms * A8_MOST_WARPS;
+    return ((all > units ? all : units) + n_decode * units) * a8_place_bytes(nt);
 }
 
 // The limit of shared memory is a kernel's on a device: raised once on each.
@@ -995,18 +992,17 @@ static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
     auto kernel = attention_8bit_stream_kernel<T, NT, PARTS>;
     A8_CONFIGURE(kernel, smem);
     const int G = a.num_heads / a.num_kv_heads;
-    const long long places = (long long)blocks * A8_BLOCK_WARPS +
-                             (long long)a.n_reqs * a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT));
+    const long long per = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT)), all = (long long)blocks * A8_BLOCK_WARPS;
+    const long long places = (all > per ? all : per) + a.n_reqs * per;
     a.part_ml = (float2*)(a.part_o + places * 8 * NT * A8_HD);
     rv_launch(kernel, dim3(blocks), dim3(A8_BLOCK_WARPS * 32), smem, stream, a);
-    // segments of a request's heads, about
-    const int units = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT));
-    if (blocks * A8_BLOCK_WARPS > 8ll * a.n_reqs * units)
-        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 8>, dim3(a.num_heads, a.n_reqs), dim3(256), 0, stream, a,
-                  blocks * A8_BLOCK_WARPS);
+    // segments of a request, about: runs a request
+    const int units = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT)), warps = blocks * A8_BLOCK_WARPS;
+    const int teams = warps / units > 1 ? warps / units : 1;
+    if (teams > 8 * a.n_reqs)
+        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 8>, dim3(a.num_heads, a.n_reqs), dim3(256), 0, stream, a, teams);
     else
-        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 1>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a,
-                  blocks * A8_BLOCK_WARPS);
+        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 1>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a, teams);
     return 0;
 }
 template <typename T, int NT, int PARTS>

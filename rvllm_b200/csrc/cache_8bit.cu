@@ -14,14 +14,15 @@
 //
 // One kernel.  A lane has 8 dimensions of a head's first half and the 8 that they turn with, so a warp has
 // 32 / (head size / 16) heads at a time: of one token for the queries; for keys and values of as many tokens, one
-// head.  A warp of the latter takes a range of so many tokens and of it the pages that begin there, to their last token in the
-// call.  The rows are read once (three rounds of them stay in registers: the largest of a page has to be known before any is
+// head.  A block of the latter takes a range of tokens, up to 32, and of it the pages that begin there, to their last token in the
+// call.  The rows are read once (two rounds of them stay in registers: the largest of a page has to be known before any is
 // written), the pages' scales settled a lane each, then the rows written.  Bound by a chain of four reads that
 // wait for one another (slots, positions, angles and rows, scales) where tokens are few.
 #include "common.cuh"
 
 #define C8_MAX_HEAD 256
 #define C8_WARPS 4
+#define C8_BLOCKS 4                    // of a multiprocessor
 
 struct C8Write {
     const void* rows;                  // [tokens][heads q | kv heads k | kv heads v], `row_stride` elements apart
@@ -32,8 +33,8 @@ struct C8Write {
     float *k_scale, *v_scale;
     long long row_stride, total_slots, table_rows;
     float eps;
-    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, aligned;
-    long long kv_warps;
+    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, aligned, range;
+    long long kv_blocks;
 };
 
 __device__ __forceinline__ void c8_load8(const float* p, bool vec, float (&v)[8]) {
@@ -90,56 +91,67 @@ __device__ __forceinline__ int c8_exponent(float most) {
 }
 __device__ __forceinline__ float c8_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// One head of one token: norm and rotation in float32.  `lane0`: the first of the `lph` lanes that have the head.
-template <typename T>
+// One head of one token: norm and rotation, in float32 for queries; keys in float64, rounded once to float32: what a page
+// holds is then the formula's value but for one value in a million that lies on a border between two steps, whatever the
+// order of the sums (float32 throughout left ten times as many).  `lane0`: the first of the `lph` lanes that have
+// the head.
+__device__ __forceinline__ float c8_sqrt(float v) { return sqrtf(v); }
+__device__ __forceinline__ double c8_sqrt(double v) { return sqrt(v); }
+template <typename Acc, typename T>
 __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const float* w, bool turn, int t, bool live, int d0,
                                         int lane0, int lph, float (&x)[8], float (&y)[8]) {
     const int half = a.head_dim >> 1;
-    float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
     if (live) {
         c8_load8(src + d0, a.aligned, x);
         c8_load8(src + half + d0, a.aligned, y);
     }
+    if (!w && !turn) return;
+    Acc inv = 1;
     if (w) {
+        Acc ss = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+        for (int i = 0; i < 8; ++i) ss += (Acc)x[i] * (Acc)x[i] + (Acc)y[i] * (Acc)y[i];
         if ((lph & (lph - 1)) == 0) {
             for (int o = lph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         } else {
-            float sum = 0.f;
+            Acc sum = 0;
             for (int k = 0; k < lph; ++k) sum += __shfl_sync(0xffffffffu, ss, (lane0 + k) & 31);
             ss = sum;
         }
-        const float rms = sqrtf(ss / (float)a.head_dim + a.eps);
-        if (live) {
-            float wx[8], wy[8];
-            c8_load8(w + d0, a.aligned, wx);
-            c8_load8(w + half + d0, a.aligned, wy);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = x[i] / rms * wx[i];
-                y[i] = y[i] / rms * wy[i];
-            }
-        }
+        inv = (Acc)1 / c8_sqrt(ss / (Acc)a.head_dim + (Acc)a.eps);          // one division for sixteen
     }
-    if (turn && live) {
+    if (!live) return;
+    float wx[8], wy[8], c[8], s[8];
+    if (w) {
+        c8_load8(w + d0, a.aligned, wx);
+        c8_load8(w + half + d0, a.aligned, wy);
+    }
+    bool angle = turn;
+    if (turn) {
         const long long p = a.positions[t];
-        float c[8], s[8];
-        if (p >= 0 && p < a.table_rows) {
+        angle = p >= 0 && p < a.table_rows;
+        if (angle) {
             c8_load8(a.cos_table + p * half + d0, a.aligned, c);
             c8_load8(a.sin_table + p * half + d0, a.aligned, s);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float xr = x[i] * c[i] - y[i] * s[i];
-                y[i] = x[i] * s[i] + y[i] * c[i];
-                x[i] = xr;
-            }
-        } else {                                               // no angle: shows in what is read later
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = y[i] = NAN;
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        Acc u = (Acc)x[i], v = (Acc)y[i];
+        if (w) {
+            u = u * inv * (Acc)wx[i];
+            v = v * inv * (Acc)wy[i];
+        }
+        if (angle) {
+            const Acc turned = u * (Acc)c[i] - v * (Acc)s[i];
+            v = u * (Acc)s[i] + v * (Acc)c[i];
+            u = turned;
+        }
+        // (a position outside the table has no angle: that shows in what is read later)
+        x[i] = turn && !angle ? NAN : (float)u;
+        y[i] = turn && !angle ? NAN : (float)v;
     }
 }
 
@@ -161,32 +173,34 @@ __device__ __forceinline__ uint2 c8_pack(const float (&x)[8], float inv) {
     return make_uint2(u[0], u[1]);
 }
 
-// What a warp knows of the pages that begin in its range.
+// What a block knows of the pages that begin in its range.
 struct C8Runs {
     unsigned most[32];                 // bits of the largest finite |x| of each
     float inv[32];                     // 1 / scale
     int lowest[32];                    // first slot written
     int page[32];
+    unsigned slots[32][2];             // those written, modulo 64
+    int twice;                         // one of them twice, it may be
 };
 
 template <typename T>
-__global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
+__global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
     rv_pdl_prologue();
-    __shared__ C8Runs runs_of[C8_WARPS];
-    const long long id = (long long)blockIdx.x * C8_WARPS + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    __shared__ C8Runs run;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lph = a.head_dim >> 4, per = 32 / lph;           // lanes a head, heads a warp
     const int sub = lane / lph, d0 = (lane - sub * lph) * 8, lane0 = sub * lph;
     const int half = a.head_dim >> 1;
     float x[8], y[8];
-    if (id >= a.kv_warps) {
+    if ((long long)blockIdx.x >= a.kv_blocks) {
         // ---- query heads --------------------------------------------------------------------
+        const long long id = ((long long)blockIdx.x - a.kv_blocks) * C8_WARPS + warp;
         const int groups = (a.num_heads + per - 1) / per;
-        const long long t = (id - a.kv_warps) / groups;
-        const int h = (int)(id - a.kv_warps - t * groups) * per + sub;
+        const long long t = id / groups;
+        const int h = (int)(id - t * groups) * per + sub;
         if (t >= a.n_tokens) return;
         const bool live = sub < per && h < a.num_heads;
-        c8_head(a, (const T*)a.rows + (size_t)t * a.row_stride + (size_t)(live ? h : 0) * a.head_dim, a.q_weight,
+        c8_head<float>(a, (const T*)a.rows + (size_t)t * a.row_stride + (size_t)(live ? h : 0) * a.head_dim, a.q_weight,
                 a.cos_table != nullptr, (int)t, live, d0, lane0, lph, x, y);
         if (!live) return;
         T* dst = (T*)a.q_out + ((size_t)t * a.num_heads + h) * a.head_dim;
@@ -196,7 +210,7 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     }
     // ---- one key or value head of the pages that begin within a range of tokens ---------------
     const int pairs = 2 * a.num_kv_heads;
-    const int first = (int)(id / pairs) * per, pair = (int)(id % pairs);
+    const int first = (int)((long long)blockIdx.x / pairs) * a.range, pair = (int)((long long)blockIdx.x % pairs);
     const bool is_k = pair < a.num_kv_heads;
     const int g = is_k ? pair : pair - a.num_kv_heads;
     const T* src = (const T*)a.rows + (size_t)(a.num_heads + pair) * a.head_dim;
@@ -204,11 +218,11 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     const bool turn = is_k && a.cos_table != nullptr;
     signed char* cache = is_k ? a.k_cache : a.v_cache;
     float* scales = is_k ? a.k_scale : a.v_scale;
-    C8Runs& run = runs_of[threadIdx.x >> 5];
     auto slot_of = [&](int t) {
         const int s = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
         return s >= 0 && s < a.total_slots ? s : -1;
     };
+    // (every warp finds the same pages)
     const unsigned full = 0xffffffffu, below = (1u << lane) - 1u;
     // this window's tokens, and the page of the last token with a slot before it
     const int mine = slot_of(first + lane);
@@ -231,8 +245,8 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
     if (!earlier) prev = before;
     const bool changes = mine >= 0 && my_page != prev;
     const unsigned begins = __ballot_sync(full, changes);
-    const unsigned owned = begins & (per < 32 ? (1u << per) - 1u : full);
-    if (!owned) return;
+    const unsigned owned = begins & (a.range < 32 ? (1u << a.range) - 1u : full);
+    if (!owned) return;                                        // (the whole block)
     const int n_runs = __popc(owned), l0 = __ffs(owned) - 1, last = 31 - __clz(owned);
     // tokens [t0, t1): up to the first token behind the range that has a slot of another page
     const int t0 = first + l0;
@@ -252,15 +266,18 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
             t1 = min(t1, a.n_tokens);
         }
     }
-    run.most[lane] = 0u;
-    run.lowest[lane] = a.page_size;
-    if ((owned >> lane) & 1u) run.page[__popc(owned & below)] = my_page;
-    __syncwarp();
+    if (warp == 0) {
+        run.most[lane] = 0u;
+        run.lowest[lane] = a.page_size;
+        run.slots[lane][0] = run.slots[lane][1] = 0u;
+        run.twice = 0;
+        if ((owned >> lane) & 1u) run.page[__popc(owned & below)] = my_page;
+    }
+    __syncthreads();
     // lane i looks after run i: its page and what its scale was
     const int page_i = lane < n_runs ? run.page[lane] : 0;
     const size_t block_i = (size_t)page_i * a.num_kv_heads + g;
     const float old = lane < n_runs ? scales[block_i] : 0.f;
-    __syncwarp();
     // A group of lanes a token: `slot` (-1: none) and the number of its run.
     auto whose = [&](int t, int& slot, int& number) {
         const int in = t - first;
@@ -269,28 +286,33 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
         if (sub >= per || t >= t1) slot = -1;
         number = in < 32 ? __popc(owned & ((2u << in) - 1u)) - 1 : n_runs - 1;
     };
-    constexpr int HOLD = 3;             // rounds whose rows stay in registers: a range and the page that it ends in
+    constexpr int HOLD = 2;             // rounds whose rows stay in registers: a range and the page that it ends in
+    const int step = C8_WARPS * per, begin = t0 + warp * per;
     float hx[HOLD][8], hy[HOLD][8];
     auto measure = [&](int t, int slot, int number, float (&u)[8], float (&v)[8]) {
-        c8_head(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
+        c8_head<double>(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
         if (slot >= 0) {
             atomicMax(&run.most[number], __float_as_uint(c8_most(v, c8_most(u, 0.f))));
-            atomicMin(&run.lowest[number], slot % a.page_size);
+            if (d0 == 0) {
+                const unsigned in = slot % a.page_size, bit = 1u << (in & 31u);
+                atomicMin(&run.lowest[number], (int)in);
+                if (atomicOr(&run.slots[number][(in >> 5) & 1u], bit) & bit) run.twice = 1;
+            }
         }
     };
 #pragma unroll
     for (int i = 0; i < HOLD; ++i)
-        if (t0 + i * per < t1) {
+        if (begin + i * step < t1) {
             int slot, number;
-            whose(t0 + i * per + sub, slot, number);
-            measure(t0 + i * per + sub, slot, number, hx[i], hy[i]);
+            whose(begin + i * step + sub, slot, number);
+            measure(begin + i * step + sub, slot, number, hx[i], hy[i]);
         }
-    for (int t = t0 + HOLD * per; t < t1; t += per) {
+    for (int t = begin + HOLD * step; t < t1; t += step) {
         int slot, number;
         whose(t + sub, slot, number);
         measure(t + sub, slot, number, x, y);
     }
-    __syncwarp();
+    __syncthreads();
     bool grows = false;
     float ratio = 0.f;
     if (lane < n_runs) {
@@ -300,15 +322,17 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
             grows = s != old;
             ratio = old / s;
         }
-        scales[block_i] = s;
-        run.inv[lane] = 1.f / s;
+        if (warp == 0) {
+            scales[block_i] = s;
+            run.inv[lane] = 1.f / s;
+        }
     }
     // pages whose scale grew: what they hold follows (the slots written below too, which does no harm)
     for (unsigned todo = __ballot_sync(full, grows); todo; todo &= todo - 1) {
         const int i = __ffs(todo) - 1;
         const float by = __shfl_sync(full, ratio, i);
         signed char* held = cache + ((size_t)__shfl_sync(full, page_i, i) * a.num_kv_heads + g) * a.page_size * a.head_dim;
-        for (int at = lane * 16; at < a.page_size * a.head_dim; at += 512) {
+        for (int at = threadIdx.x * 16; at < a.page_size * a.head_dim; at += C8_WARPS * 512) {
             int4 v = *(const int4*)(held + at);
             signed char* b = (signed char*)&v;
 #pragma unroll
@@ -316,35 +340,36 @@ __global__ void __launch_bounds__(C8_WARPS * 32) qk_norm_rope_write_8bit_kernel(
             *(int4*)(held + at) = v;
         }
     }
-    __syncwarp();
-    auto store = [&](int slot, int number, const float (&u)[8], const float (&v)[8]) {
+    __syncthreads();
+    auto store = [&](int t, int slot, int number, const float (&u)[8], const float (&v)[8]) {
         // (of two tokens with one slot the later one is written)
+        const int page = slot / a.page_size;
         bool later = false;
-        for (int k = 1; k < per; ++k) {
-            const int other = __shfl_sync(full, slot, ((sub + k) * lph) & 31);
-            later |= sub + k < per && other == slot;
-        }
+        if (slot >= 0 && run.twice)
+            for (int k = t + 1; k < t1 && !later; ++k) {
+                const int s = slot_of(k);
+                if (s >= 0 && s / a.page_size != page) break;
+                later = s == slot;
+            }
         if (slot >= 0 && !later) {
             const float inv = run.inv[number];
-            const int page = slot / a.page_size;
             signed char* dst = cache + (((size_t)page * a.num_kv_heads + g) * a.page_size + (slot - page * a.page_size)) * a.head_dim;
             *(uint2*)(dst + d0) = c8_pack(u, inv);
             *(uint2*)(dst + half + d0) = c8_pack(v, inv);
         }
-        __syncwarp();
     };
 #pragma unroll
     for (int i = 0; i < HOLD; ++i)
-        if (t0 + i * per < t1) {
+        if (begin + i * step < t1) {
             int slot, number;
-            whose(t0 + i * per + sub, slot, number);
-            store(slot, number, hx[i], hy[i]);
+            whose(begin + i * step + sub, slot, number);
+            store(begin + i * step + sub, slot, number, hx[i], hy[i]);
         }
-    for (int t = t0 + HOLD * per; t < t1; t += per) {
+    for (int t = begin + HOLD * step; t < t1; t += step) {
         int slot, number;
         whose(t + sub, slot, number);
-        c8_head(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
-        store(slot, number, x, y);
+        c8_head<double>(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
+        store(t + sub, slot, number, x, y);
     }
 }
 
@@ -382,13 +407,14 @@ extern "C" int rv_qk_norm_rope_write_8bit(const C8WriteCall* c) {
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) RV_FAIL("qk_norm_rope_write_8bit: pages must be 16-byte aligned");
     C8Write a = {rows, q_out, q_weight, k_weight, cos_table, sin_table, positions, slots, (signed char*)k_cache,
                  (signed char*)v_cache, k_scale, v_scale, row_stride, pages * page_size, table_rows, eps, n_tokens,
-                 num_heads, num_kv_heads, head_dim, page_size, 0, 0};
+                 num_heads, num_kv_heads, head_dim, page_size, 0, 0, 0};
     const int size = dtype == RV_DTYPE_F32 ? 4 : 2, per = 32 / (head_dim >> 4);
     a.aligned = ((uintptr_t)rows | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
                  (uintptr_t)sin_table) % 16 == 0 && row_stride * size % 16 == 0;
+    a.range = C8_WARPS * per < 32 ? C8_WARPS * per : 32;
+    a.kv_blocks = (long long)((n_tokens + a.range - 1) / a.range) * 2 * num_kv_heads;
     const long long q_warps = (long long)n_tokens * ((num_heads + per - 1) / per);
-    a.kv_warps = (long long)((n_tokens + per - 1) / per) * 2 * num_kv_heads;
-    const long long blocks = (a.kv_warps + q_warps + C8_WARPS - 1) / C8_WARPS;
+    const long long blocks = a.kv_blocks + (q_warps + C8_WARPS - 1) / C8_WARPS;
     if (blocks > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: too many rows");
     RV_DISPATCH_DTYPE(dtype, "qk_norm_rope_write_8bit",
                       (rv_launch(qk_norm_rope_write_8bit_kernel<T>, dim3((int)blocks), dim3(C8_WARPS * 32), 0,
