@@ -956,7 +956,8 @@ static int a8_nsplit(long long units, long long tiles, int block_places) {
 // 700 keys 6.3 / 8.3, 64 of 100 8.3 / 12.4, 64 of 700 14 / 18.5, 128 of 700 25 / 27, 16 of 4,000 18.5 / 20.7; 8 / 8 heads of 128,
 // 32 of 1,000 14 / 19, 128 of 300 (1,024 blocks for 296 places) 27 / 23.  64 of 2,000 alike would take 29 / 33 too, but of
 // 2,340 to 3,900 52 / 44.)
-static bool a8_few(long long units, long long tiles, int n_sms) {
+static bool a8_few(long long units, long long tiles, int n_sms, int form) {
+    if (form != 0) return form == 2;               // 1: the stream, 2: blocks and clusters
     const int places = (A8_HD <= 64 ? 4 : 2) * n_sms;
     const int n = a8_nsplit(units, tiles, places);
     return units <= 2ll * places && tiles <= 8ll * A8_BLOCK_WARPS * (n ? n : 1);
@@ -964,10 +965,10 @@ static bool a8_few(long long units, long long tiles, int n_sms) {
 
 // Scratch for single tokens: requests [0, n_decode).
 extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode, int max_ctx_len, int num_heads, int num_kv_heads,
-                                                                   int window, int n_sms) {
+                                                                   int window, int n_sms, int form) {
     const int G = num_heads / num_kv_heads, nt = a8_nt(G);
     const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
-    if (n_decode <= 0 || a8_few(units * n_decode, a8_tiles(max_ctx_len, window, 1), n_sms)) return 0;
+    if (n_decode <= 0 || a8_few(units * n_decode, a8_tiles(max_ctx_len, window, 1), n_sms, form)) return 0;
     const long long all = (long long)n_sms * A8_MOST_WARPS;
     return ((all > units ? all : units) + n_decode * units) * a8_place_bytes(nt);
 }
@@ -1047,9 +1048,9 @@ static int a8_portions(const A8Args& a, int max_q_len, int max_ctx_len, int n_sm
                : a8_rows<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, max_q_len, max_ctx_len, n_sms, stream);
 }
 template <typename T, int PARTS>
-static int a8_singles(const A8Args& a, int max_ctx_len, int n_sms, cudaStream_t stream) {
+static int a8_singles(const A8Args& a, int max_ctx_len, int n_sms, int form, cudaStream_t stream) {
     const int G = a.num_heads / a.num_kv_heads, nt = a8_nt(G);
-    if (a8_few((long long)a.n_reqs * a.num_kv_heads * ((G + 8 * nt - 1) / (8 * nt)), a8_tiles(max_ctx_len, a.window, 1), n_sms))
+    if (a8_few((long long)a.n_reqs * a.num_kv_heads * ((G + 8 * nt - 1) / (8 * nt)), a8_tiles(max_ctx_len, a.window, 1), n_sms, form))
         return a8_portions<T, PARTS>(a, 1, max_ctx_len, n_sms, stream);
     return nt == 1 ? a8_stream<T, 1, PARTS>(a, n_sms, stream) : a8_stream<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, n_sms, stream);
 }
@@ -1064,7 +1065,7 @@ struct A8Call {
     const float* sinks;
     void* stream;
     long long dtype, q_stride, pages, max_blocks, scratch_bytes, n_decode, n_reqs, portions, max_q_len, max_ctx_len, num_heads,
-        num_kv_heads, page_size, window, n_sms;
+        num_kv_heads, page_size, window, n_sms, form;
     double scale;
 };
 extern "C" int A8_SYM(rv_paged_attention_8bit)(const A8Call* c) {
@@ -1078,7 +1079,7 @@ extern "C" int A8_SYM(rv_paged_attention_8bit)(const A8Call* c) {
     const int dtype = (int)c->dtype, max_blocks = (int)c->max_blocks, n_decode = (int)c->n_decode, n_reqs = (int)c->n_reqs;
     const int portions = (int)c->portions, max_q_len = (int)c->max_q_len, max_ctx_len = (int)c->max_ctx_len;
     const int num_heads = (int)c->num_heads, num_kv_heads = (int)c->num_kv_heads, page_size = (int)c->page_size;
-    const int window = (int)c->window, n_sms = (int)c->n_sms;
+    const int window = (int)c->window, n_sms = (int)c->n_sms, form = (int)c->form;
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
         A8_FAIL("paged_attention_8bit: invalid head counts: %d query, %d KV", num_heads, num_kv_heads);
     if (n_decode < 0 || n_reqs < n_decode || max_q_len < 0 || max_ctx_len < 0 || max_blocks < 0 || page_size <= 0 || window < 0 ||
@@ -1087,7 +1088,7 @@ extern "C" int A8_SYM(rv_paged_attention_8bit)(const A8Call* c) {
     if (n_reqs > 65535 || num_kv_heads > 65535) A8_FAIL("paged_attention_8bit: too many requests or heads");
     if (pages * num_kv_heads * page_size >= 0xffffffffll) A8_FAIL("paged_attention_8bit: more rows than 32 bits count");
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) A8_FAIL("paged_attention_8bit: pages must be 16-byte aligned");
-    if (A8_SYM(rv_paged_attention_8bit_scratch_bytes)(n_decode, max_ctx_len, num_heads, num_kv_heads, window, n_sms) > scratch_bytes)
+    if (A8_SYM(rv_paged_attention_8bit_scratch_bytes)(n_decode, max_ctx_len, num_heads, num_kv_heads, window, n_sms, form) > scratch_bytes)
         A8_FAIL("paged_attention_8bit: scratch too small");
     A8Args a = {q, (const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens, sinks,
                 out, (float*)scratch, nullptr, q_stride, pages, max_blocks, 0, n_decode, num_heads, num_kv_heads, page_size,
@@ -1096,8 +1097,8 @@ extern "C" int A8_SYM(rv_paged_attention_8bit)(const A8Call* c) {
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype != RV_DTYPE_F32 && dtype != RV_DTYPE_BF16) A8_FAIL("paged_attention_8bit: unknown dtype code %d", dtype);
     if (n_decode > 0) {
-        const int rc = dtype == RV_DTYPE_BF16 ? a8_singles<__nv_bfloat16, 1>(a, max_ctx_len, n_sms, s)
-                                              : a8_singles<float, 2>(a, max_ctx_len, n_sms, s);
+        const int rc = dtype == RV_DTYPE_BF16 ? a8_singles<__nv_bfloat16, 1>(a, max_ctx_len, n_sms, form, s)
+                                              : a8_singles<float, 2>(a, max_ctx_len, n_sms, form, s);
         if (rc) return rc;
     }
     if (portions && n_reqs > n_decode && max_q_len > 0) {

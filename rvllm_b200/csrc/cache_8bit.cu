@@ -22,6 +22,7 @@
 
 #define C8_MAX_HEAD 256
 #define C8_WARPS 4
+#define C8_ROUNDS 4                    // of a token's query heads, one warp
 #define C8_BLOCKS 4                    // of a multiprocessor
 
 struct C8Write {
@@ -33,7 +34,7 @@ struct C8Write {
     float *k_scale, *v_scale;
     long long row_stride, total_slots, table_rows;
     float eps;
-    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, aligned, range;
+    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, page_shift, aligned, range, q_rounds;
     long long kv_blocks;
 };
 
@@ -91,13 +92,22 @@ __device__ __forceinline__ int c8_exponent(float most) {
 }
 __device__ __forceinline__ float c8_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// One head of one token: norm and rotation, in float32 for queries; keys in float64, rounded once to float32: what a page
-// holds is then the formula's value but for one value in a million that lies on a border between two steps, whatever the
-// order of the sums (float32 throughout left ten times as many).  `lane0`: the first of the `lph` lanes that have
-// the head.
-__device__ __forceinline__ float c8_sqrt(float v) { return sqrtf(v); }
-__device__ __forceinline__ double c8_sqrt(double v) { return sqrt(v); }
-template <typename Acc, typename T>
+// Sum over the `lph` lanes from `lane0` on that have a head.
+template <typename A>
+__device__ __forceinline__ A c8_sum(A v, int lane0, int lph) {
+    if ((lph & (lph - 1)) == 0) {
+        for (int o = lph >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    A sum = 0;
+    for (int k = 0; k < lph; ++k) sum += __shfl_sync(0xffffffffu, v, (lane0 + k) & 31);
+    return sum;
+}
+
+// One key or value head of one token: norm and rotation in float64, rounded once to float32, so that what a page holds is
+// the formula's value but for one value in a million that lies on a border between two steps, whatever the order of
+// the sums (float32 throughout left ten times as many).
+template <typename T>
 __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const float* w, bool turn, int t, bool live, int d0,
                                         int lane0, int lph, float (&x)[8], float (&y)[8]) {
     const int half = a.head_dim >> 1;
@@ -108,19 +118,12 @@ __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const fl
         c8_load8(src + half + d0, a.aligned, y);
     }
     if (!w && !turn) return;
-    Acc inv = 1;
+    double inv = 1.0;
     if (w) {
-        Acc ss = 0;
+        double ss = 0.0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += (Acc)x[i] * (Acc)x[i] + (Acc)y[i] * (Acc)y[i];
-        if ((lph & (lph - 1)) == 0) {
-            for (int o = lph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        } else {
-            Acc sum = 0;
-            for (int k = 0; k < lph; ++k) sum += __shfl_sync(0xffffffffu, ss, (lane0 + k) & 31);
-            ss = sum;
-        }
-        inv = (Acc)1 / c8_sqrt(ss / (Acc)a.head_dim + (Acc)a.eps);          // one division for sixteen
+        for (int i = 0; i < 8; ++i) ss += (double)x[i] * x[i] + (double)y[i] * y[i];
+        inv = 1.0 / sqrt(c8_sum(ss, lane0, lph) / a.head_dim + (double)a.eps);
     }
     if (!live) return;
     float wx[8], wy[8], c[8], s[8];
@@ -139,19 +142,78 @@ __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const fl
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        Acc u = (Acc)x[i], v = (Acc)y[i];
+        double u = x[i], v = y[i];
         if (w) {
-            u = u * inv * (Acc)wx[i];
-            v = v * inv * (Acc)wy[i];
+            u = u * inv * wx[i];
+            v = v * inv * wy[i];
         }
         if (angle) {
-            const Acc turned = u * (Acc)c[i] - v * (Acc)s[i];
-            v = u * (Acc)s[i] + v * (Acc)c[i];
+            const double turned = u * c[i] - v * s[i];
+            v = u * s[i] + v * c[i];
             u = turned;
         }
-        // (a position outside the table has no angle: that shows in what is read later)
-        x[i] = turn && !angle ? NAN : (float)u;
+        x[i] = turn && !angle ? NAN : (float)u;                  // (held as 0)
         y[i] = turn && !angle ? NAN : (float)v;
+    }
+}
+
+// Query heads h0, h0 + per, ... of token t: the token's angles and the weights are read once, all rows requested before any is
+// used.
+template <typename T, int ROUNDS>
+__device__ __forceinline__ void c8_queries(const C8Write& a, int t, int h0, int per, bool mine, int d0, int lane0, int lph) {
+    const int half = a.head_dim >> 1;
+    const T* src = (const T*)a.rows + (size_t)t * a.row_stride;
+    T* dst = (T*)a.q_out + (size_t)t * a.num_heads * a.head_dim;
+    float x[ROUNDS][8], y[ROUNDS][8], wx[8], wy[8], c[8], s[8];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        const int h = h0 + k * per;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[k][i] = y[k][i] = 0.f;
+        if (mine && h < a.num_heads) {
+            c8_load8(src + (size_t)h * a.head_dim + d0, a.aligned, x[k]);
+            c8_load8(src + (size_t)h * a.head_dim + half + d0, a.aligned, y[k]);
+        }
+    }
+    if (a.q_weight) {
+        c8_load8(a.q_weight + d0, a.aligned, wx);
+        c8_load8(a.q_weight + half + d0, a.aligned, wy);
+    }
+    const bool turn = a.cos_table != nullptr;
+    bool angle = false;
+    if (turn) {
+        const long long p = a.positions[t];
+        angle = p >= 0 && p < a.table_rows;
+        if (angle) {
+            c8_load8(a.cos_table + p * half + d0, a.aligned, c);
+            c8_load8(a.sin_table + p * half + d0, a.aligned, s);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        const int h = h0 + k * per;
+        if (a.q_weight) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += x[k][i] * x[k][i] + y[k][i] * y[k][i];
+            const float inv = 1.f / sqrtf(c8_sum(ss, lane0, lph) / (float)a.head_dim + a.eps);       // one division for sixteen
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[k][i] = x[k][i] * inv * wx[i];
+                y[k][i] = y[k][i] * inv * wy[i];
+            }
+        }
+        if (turn)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float u = x[k][i], v = y[k][i];
+                x[k][i] = angle ? u * c[i] - v * s[i] : NAN;       // (a position outside the table has no angle)
+                y[k][i] = angle ? u * s[i] + v * c[i] : NAN;
+            }
+        if (mine && h < a.num_heads) {
+            c8_store8(dst + (size_t)h * a.head_dim + d0, a.aligned, x[k]);
+            c8_store8(dst + (size_t)h * a.head_dim + half + d0, a.aligned, y[k]);
+        }
     }
 }
 
@@ -195,17 +257,14 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
     if ((long long)blockIdx.x >= a.kv_blocks) {
         // ---- query heads --------------------------------------------------------------------
         const long long id = ((long long)blockIdx.x - a.kv_blocks) * C8_WARPS + warp;
-        const int groups = (a.num_heads + per - 1) / per;
-        const long long t = id / groups;
-        const int h = (int)(id - t * groups) * per + sub;
+        const int shares = (a.num_heads + per * a.q_rounds - 1) / (per * a.q_rounds);
+        const long long t = id / shares;
         if (t >= a.n_tokens) return;
-        const bool live = sub < per && h < a.num_heads;
-        c8_head<float>(a, (const T*)a.rows + (size_t)t * a.row_stride + (size_t)(live ? h : 0) * a.head_dim, a.q_weight,
-                a.cos_table != nullptr, (int)t, live, d0, lane0, lph, x, y);
-        if (!live) return;
-        T* dst = (T*)a.q_out + ((size_t)t * a.num_heads + h) * a.head_dim;
-        c8_store8(dst + d0, a.aligned, x);
-        c8_store8(dst + half + d0, a.aligned, y);
+        const int h0 = (int)(id - t * shares) * per * a.q_rounds + sub;
+        if (a.q_rounds == 1)
+            c8_queries<T, 1>(a, (int)t, h0, per, sub < per, d0, lane0, lph);
+        else
+            c8_queries<T, C8_ROUNDS>(a, (int)t, h0, per, sub < per, d0, lane0, lph);
         return;
     }
     // ---- one key or value head of the pages that begin within a range of tokens ---------------
@@ -222,18 +281,19 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         const int s = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
         return s >= 0 && s < a.total_slots ? s : -1;
     };
+    auto page_of = [&](int s) { return a.page_shift >= 0 ? s >> a.page_shift : s / a.page_size; };
     // (every warp finds the same pages)
     const unsigned full = 0xffffffffu, below = (1u << lane) - 1u;
     // this window's tokens, and the page of the last token with a slot before it
     const int mine = slot_of(first + lane);
     int back = slot_of(first - 1 - lane);
-    const int my_page = mine >= 0 ? mine / a.page_size : -1;
+    const int my_page = mine >= 0 ? page_of(mine) : -1;
     const unsigned real = __ballot_sync(full, mine >= 0);
     int before = -1;
     for (int at = first - 1;;) {
         const unsigned have = __ballot_sync(full, back >= 0);
         if (have) {
-            before = __shfl_sync(full, back, __ffs(have) - 1) / a.page_size;
+            before = page_of(__shfl_sync(full, back, __ffs(have) - 1));
             break;
         }
         at -= 32;
@@ -259,7 +319,7 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         } else {
             for (bool more = t1 < a.n_tokens; more;) {
                 const int s = slot_of(t1 + lane);
-                const unsigned stop = __ballot_sync(full, (s >= 0 && s / a.page_size != last_page) || t1 + lane >= a.n_tokens);
+                const unsigned stop = __ballot_sync(full, (s >= 0 && page_of(s) != last_page) || t1 + lane >= a.n_tokens);
                 t1 += stop ? __ffs(stop) - 1 : 32;
                 more = !stop;
             }
@@ -290,11 +350,11 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
     const int step = C8_WARPS * per, begin = t0 + warp * per;
     float hx[HOLD][8], hy[HOLD][8];
     auto measure = [&](int t, int slot, int number, float (&u)[8], float (&v)[8]) {
-        c8_head<double>(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
+        c8_head(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
         if (slot >= 0) {
             atomicMax(&run.most[number], __float_as_uint(c8_most(v, c8_most(u, 0.f))));
             if (d0 == 0) {
-                const unsigned in = slot % a.page_size, bit = 1u << (in & 31u);
+                const unsigned in = slot - page_of(slot) * a.page_size, bit = 1u << (in & 31u);
                 atomicMin(&run.lowest[number], (int)in);
                 if (atomicOr(&run.slots[number][(in >> 5) & 1u], bit) & bit) run.twice = 1;
             }
@@ -343,12 +403,12 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
     __syncthreads();
     auto store = [&](int t, int slot, int number, const float (&u)[8], const float (&v)[8]) {
         // (of two tokens with one slot the later one is written)
-        const int page = slot / a.page_size;
+        const int page = page_of(slot);
         bool later = false;
         if (slot >= 0 && run.twice)
             for (int k = t + 1; k < t1 && !later; ++k) {
                 const int s = slot_of(k);
-                if (s >= 0 && s / a.page_size != page) break;
+                if (s >= 0 && page_of(s) != page) break;
                 later = s == slot;
             }
         if (slot >= 0 && !later) {
@@ -368,7 +428,7 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
     for (int t = begin + HOLD * step; t < t1; t += step) {
         int slot, number;
         whose(t + sub, slot, number);
-        c8_head<double>(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
+        c8_head(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
         store(t + sub, slot, number, x, y);
     }
 }
@@ -407,13 +467,16 @@ extern "C" int rv_qk_norm_rope_write_8bit(const C8WriteCall* c) {
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) RV_FAIL("qk_norm_rope_write_8bit: pages must be 16-byte aligned");
     C8Write a = {rows, q_out, q_weight, k_weight, cos_table, sin_table, positions, slots, (signed char*)k_cache,
                  (signed char*)v_cache, k_scale, v_scale, row_stride, pages * page_size, table_rows, eps, n_tokens,
-                 num_heads, num_kv_heads, head_dim, page_size, 0, 0, 0};
+                 num_heads, num_kv_heads, head_dim, page_size, (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, 0, 0, 1, 0};
     const int size = dtype == RV_DTYPE_F32 ? 4 : 2, per = 32 / (head_dim >> 4);
     a.aligned = ((uintptr_t)rows | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
                  (uintptr_t)sin_table) % 16 == 0 && row_stride * size % 16 == 0;
     a.range = C8_WARPS * per < 32 ? C8_WARPS * per : 32;
     a.kv_blocks = (long long)((n_tokens + a.range - 1) / a.range) * 2 * num_kv_heads;
-    const long long q_warps = (long long)n_tokens * ((num_heads + per - 1) / per);
+    // a warp has more of a token's heads where there are more tokens than warps' places (2,048 tokens, 32 / 8 heads
+    // of 64: 16.5 -> 14.5 us)
+    a.q_rounds = n_tokens >= 8 * rv_sm_count() && num_heads > per ? C8_ROUNDS : 1;
+    const long long q_warps = (long long)n_tokens * ((num_heads + per * a.q_rounds - 1) / (per * a.q_rounds));
     const long long blocks = a.kv_blocks + (q_warps + C8_WARPS - 1) / C8_WARPS;
     if (blocks > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: too many rows");
     RV_DISPATCH_DTYPE(dtype, "qk_norm_rope_write_8bit",

@@ -26,7 +26,7 @@ _F32, _BF16 = 0, 1
 
 # Records of 8-byte whole numbers and a real one or none behind them, as the 8-bit calls and the log probabilities take them
 _WRITE_8BIT, _READ_8BIT = struct.Struct("=22qd"), struct.Struct("=11q")
-_ATTEND_8BIT, _LOGPROBS = struct.Struct("=27qd"), struct.Struct("=13q")
+_ATTEND_8BIT, _LOGPROBS = struct.Struct("=28qd"), struct.Struct("=13q")
 
 
 def _code(dtype: torch.dtype) -> int:
@@ -77,6 +77,9 @@ class CudaOps:
         # tcgen05 where it applies, else mma
         self.prefill_attention = os.environ.get("RVLLM_PREFILL_ATTENTION", "auto")
         self.decode_attention = os.environ.get("RVLLM_DECODE_ATTENTION", "mma")
+        # single tokens over 8-bit pages: "stream" = persistent warps and a merge, "blocks" = blocks and clusters
+        # that have a request's heads each, "auto" = the faster one
+        self.decode_8bit = os.environ.get("RVLLM_DECODE_8BIT", "auto")
         # portions over 8-bit pages: "rows" = mma.sync from the pages, any head size and type; "tcgen05" = bfloat16
         # pages for the step, then the tcgen05 kernel (bfloat16, head sizes 64 and 128); "auto" = the faster one,
         # while those pages take no more than `widen_8bit_bytes`
@@ -980,6 +983,8 @@ class CudaOps:
             page_size, dim, have)), what)
         return out
 
+    _FORMS_8BIT = {"auto": 0, "stream": 1, "blocks": 2}
+
     def _attn8_lib(self, head_dim: int):
         """The functions for attention over 8-bit pages with heads of this size (call, scratch, last error), built
         at first use."""
@@ -998,7 +1003,7 @@ class CudaOps:
             call.argtypes = [ctypes.c_char_p]
             scratch = getattr(lib, f"rv_paged_attention_8bit_scratch_bytes_hd{head_dim}")
             scratch.restype = c_longlong
-            scratch.argtypes = [c_int] * 6
+            scratch.argtypes = [c_int] * 7
             hit = self._attn_libs[key] = (call, scratch, error)
         return hit
 
@@ -1057,13 +1062,14 @@ class CudaOps:
         stream = self._raw_stream(here)
         tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window)
         if n_decode or not tcgen05:
-            need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms)
+            form = self._FORMS_8BIT[self.decode_8bit]
+            need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms, form)
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
             rc = call(_ATTEND_8BIT.pack(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
                 q_start.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
                 sinks_at or 0, stream, code, stride, pages, table.size(1), need, n_decode, n_reqs, portions and not tcgen05,
-                longest, deepest, num_heads, num_kv_heads, page_size, window, sms, scale))
+                longest, deepest, num_heads, num_kv_heads, page_size, window, sms, form, scale))
             self.launches += (n_decode > 0) + (need > 0) + (portions and not tcgen05)
             if rc != 0:
                 raise KernelError(error().decode())

@@ -31,6 +31,7 @@ def ops(monkeypatch):
     o.calls, o.launches, o._sm_count = [], 0, 148
     o._here = lambda: 0
     o._raw_stream = lambda device: 0
+    o.decode_8bit = "auto"
     o.prefill_8bit, o.prefill_attention, o.widen_8bit_bytes, o._attn_libs = "auto", "auto", 1 << 30, {}
     o.lib = SimpleNamespace(rv_last_error=lambda: b"refused by the library")
     note = lambda *a: o.calls.append(a) or 0  # noqa: E731
@@ -176,4 +177,4 @@ def test_a_code_from_the_library_is_an_error(ops):
 
 def test_records_hold_what_the_library_reads():
     """8 bytes an argument: addresses, whole numbers, a real number last."""
-    assert [r.size for r in (bindings._WRITE_8BIT, bindings._READ_8BIT, bindings._ATTEND_8BIT, bindings._LOGPROBS)] == [184, 88, 224, 104]
+    assert [r.size for r in (bindings._WRITE_8BIT, bindings._READ_8BIT, bindings._ATTEND_8BIT, bindings._LOGPROBS)] == [184, 88, 232, 104]

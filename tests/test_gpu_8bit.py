@@ -15,14 +15,15 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16]
 
 
-@pytest.fixture(params=["rows", "tcgen05"])
+@pytest.fixture(params=["blocks-rows", "stream-tcgen05"])
 def ops(request):
-    """With either kernel for the portions that both can take."""
+    """With either kernel for single tokens, and either for the portions that both can take."""
     from rvllm_b200.kernels import cuda_ops
     ops = cuda_ops()
-    was, ops.prefill_8bit = ops.prefill_8bit, request.param
+    was = ops.decode_8bit, ops.prefill_8bit
+    ops.decode_8bit, ops.prefill_8bit = request.param.split("-")
     yield ops
-    ops.prefill_8bit = was
+    ops.decode_8bit, ops.prefill_8bit = was
 
 
 def rnd(g, *shape, scale=1.0, dtype=torch.float32):
@@ -163,6 +164,26 @@ def test_write_of_what_is_not_finite(ops):
     assert not cache[0].any()
 
 
+@pytest.mark.parametrize("gap", [1, 31, 32, 33, 100])
+def test_write_with_gaps(ops, gap):
+    """Tokens without a slot between those of one page, before the first one and behind the last, more of them than a warp
+    looks at; a page larger than that too."""
+    g = torch.Generator().manual_seed(18)
+    for ps, dim in ((16, 64), (128, 128)):
+        slots = [-1] * gap
+        for i in range(ps + 5):
+            slots += [3 * ps + i if i < ps else 5 * ps + i - ps] + ([-1] * gap if i in (2, ps - 2, ps + 1) else [])
+        slots = torch.tensor(slots + [-1] * gap, dtype=torch.int32)
+        n = slots.shape[0]
+        k8, ks = pages_of(g, 7, 1, ps, dim)
+        v8, vs = pages_of(g, 7, 1, ps, dim)
+        caches, before = [k8, v8, ks, vs], [k8.clone(), v8.clone()]
+        ctx, group = plain.batch([1], [0], ps, 7, 0)
+        ctx.positions, group.slot_mapping = torch.arange(n, dtype=torch.int32) % 90, slots
+        got = write_both(ops, rnd(g, n, 4 * dim), 2, 1, dim, None, 1 + rnd(g, dim, scale=0.1), 1e-6, angles(90, dim), ctx, group, caches)
+        check_written(torch.float32, *got, caches, before)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("K,ps,D", [(2, 16, 64), (1, 5, 48), (3, 64, 256)])
 def test_read(ops, dtype, K, ps, D):
@@ -279,6 +300,37 @@ def test_value_scales_far_apart(ops, dtype):
     check_attention(ops, dtype, 4, 1, 64, 16, [1, 1, 20], [300, 80, 100], 2, spread=20)
     check_attention(ops, dtype, 4, 1, 64, 16, [1, 1, 20], [300, 80, 100], 2, q_scale=30.0)
     check_attention(ops, dtype, 4, 1, 64, 16, [1, 1, 20], [300, 80, 100], 2, q_scale=1e-20, sinks=True)
+
+
+def test_rows_behind_the_last_request_stay(ops):
+    """Rows of the buffers behind the step's last token are not touched, and no step at all touches none."""
+    g = torch.Generator().manual_seed(19)
+    for dtype in DTYPES:
+        ctx, group = plain.batch([1, 1, 30], [40, 70, 10], 16, 20, 2)
+        k8, ks = pages_of(g, 20, 2, 16, 64)
+        v8, vs = pages_of(g, 20, 2, 16, 64)
+        q = rnd(g, 50, 256, dtype=dtype).cuda()
+        out = torch.full((50, 256), 7.0, dtype=dtype, device="cuda")
+        pages = [t.cuda() for t in (k8, v8, ks, vs)]
+        ops.paged_attention_8bit(q, 4, 2, 64, *pages, plain.cuda(ctx), plain.cuda(group), 0.125, None, out)
+        assert bool((out[32:] == 7).all()) and not bool((out[:32] == 7).all(1).any())
+        ctx.n_reqs = ctx.n_tokens = ctx.n_decode = 0
+        out.fill_(7)
+        ops.paged_attention_8bit(q, 4, 2, 64, *pages, plain.cuda(ctx), plain.cuda(group), 0.125, None, out)
+        assert bool((out == 7).all())
+
+
+def test_forms_are_chosen_by_size():
+    """Few single tokens take blocks and clusters (one launch), many keys of many requests the stream and its merge."""
+    from rvllm_b200.kernels import cuda_ops
+    ops = cuda_ops()
+    for old, launches in (([700], 1), ([100] * 40, 1), ([3900] * 40, 2), ([60000], 2)):
+        ctx, group = plain.batch([1] * len(old), old, 16, 9800, len(old))
+        pages = [torch.zeros(9800, 8, 16, 64, dtype=torch.int8, device="cuda") for _ in "kv"] + [torch.ones(9800, 8, device="cuda") for _ in "kv"]
+        q = torch.randn(len(old), 2048, device="cuda").bfloat16()
+        before = ops.launches
+        ops.paged_attention_8bit(q, 32, 8, 64, *pages, plain.cuda(ctx), plain.cuda(group), 0.125, None, torch.empty_like(q))
+        assert ops.launches - before == launches, old
 
 
 def test_more_tokens_than_context(ops):
