@@ -123,7 +123,7 @@ __device__ __forceinline__ void lp_place(const u64* from, int n, int top, u64* t
 template <typename T, bool TOP>
 struct LpThread {
     static constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U;
-    float m = -INFINITY, s = 0.f, w = 0.f;
+    float m = -INFINITY, s = 0.f, w = 0.f, limit = -INFINITY;
     int above = 0;
     bool first = true;
     float given;
@@ -188,18 +188,21 @@ struct LpThread {
         const float was = m, bm = sums(x);
         if constexpr (TOP) {
             const int lane = threadIdx.x & 31;
-            if (__any_sync(0xffffffffu, m > was)) {
-                const unsigned b = rth(m == -INFINITY ? 0u : lp_key(m), (top + LP_WARPS - 1) / LP_WARPS);
-                if (lane == 0) sh.bound[threadIdx.x >> 5] = b;
+            // (below the limit nothing is wanted, nor does it change the warp's bound, which is not below the limit)
+            if (first || __any_sync(0xffffffffu, bm >= limit)) {
+                if (__any_sync(0xffffffffu, m > was)) {
+                    const unsigned b = rth(m == -INFINITY ? 0u : lp_key(m), (top + LP_WARPS - 1) / LP_WARPS);
+                    if (lane == 0) sh.bound[threadIdx.x >> 5] = b;
+                    __syncwarp();
+                }
+                if (first) __syncthreads();                          // every warp has a bound
+                first = false;
+                // the warps' bounds as they are: they only grow, so older ones hold too
+                const unsigned b = __reduce_min_sync(0xffffffffu, *(volatile unsigned*)&sh.bound[lane & (LP_WARPS - 1)]);
+                limit = b ? lp_value(b) : -INFINITY;
+                if (bm >= limit) collect(x, limit, col, real);
                 __syncwarp();
             }
-            if (first) __syncthreads();                              // every warp has a bound
-            first = false;
-            // the warps' bounds as they are: they only grow, so older ones hold too
-            const unsigned b = __reduce_min_sync(0xffffffffu, *(volatile unsigned*)&sh.bound[lane & (LP_WARPS - 1)]);
-            const float limit = b ? lp_value(b) : -INFINITY;
-            if (bm >= limit) collect(x, limit, col, real);
-            __syncwarp();
         }
     }
     // The same for the largest alone, a block together and never too many: what would overflow the memory is
