@@ -14,6 +14,10 @@ A group may hold one row per `every` tokens instead of one per token (pooled blo
 stands for that many positions).  Its tables and its pool count rows, so both are shorter by that
 factor; every live request may begin a page of its own, so the pool has one page per request more.
 
+Keys and values may be held in 8 bits: int8 [calls, pages, kv_heads, page_size, head_dim], so that what a (page, head)
+holds lies together, with float32 scales [calls, pages, kv_heads].  A page's scale begins anew when its
+first slot is written, so nothing is cleared when a page changes hands.
+
 A request's pages are given back when it ends (`free`) and, in a group whose reach
 is bounded (a window, or chunks that do not see one another), as soon as every slot of
 the page lies behind what any future query can see (`advance`).  Released block-table entries read -1; no kernel touches them because

@@ -2,31 +2,46 @@
 // [head size], one power-of-two scale per page and head), single tokens and portions of prompts.  Compiled for one head
 // size at a time (RV_HD: a multiple of 16, at most 256).
 //
-// A warp works alone.  It owns 8 (or 16) rows -- a row is a query token and one of the query heads that share the key/value head --
-// and walks tiles of keys, which it copies itself (cp.async) into a ring of its own in shared memory: nothing
-// but the warp's own copies is waited for.  Scores are computed transposed, S^T = K Q^T, by m16n8k16 products of float16
-// operands with float32 sums: 16 keys are the rows of the left operand, 8 query rows the columns of the right one.
-// With few query heads per key/value head the other order would leave most of a product's 16 rows empty.
+// A warp works alone.  It owns 8 or 16 rows -- a row is a query token and one of the query heads that share the key/value
+// head -- and walks tiles of 32 keys, which it copies itself (cp.async) into a ring of its own in shared memory: nothing
+// but the warp's own copies is waited for.  Scores are computed transposed, S^T = K Q^T: 16 keys are the rows of a product's
+// left operand, 8 query rows the columns of the right one.  With few query heads per key/value head the other order
+// would leave most of a product's 16 rows empty.
 //
-//   int8 -> float16   the byte q + 128 behind the exponent byte 0x64 is the float16 1024 + 128 + q; minus
-//                     1152 leaves q exactly: a byte permutation and a subtraction for two values.
-//   keys              a lane's four k-steps of 64 dimensions are 16 bytes that lie side by side: the order of a sum's
-//                     terms is free, so the queries are put in that order and the keys need no transposition.
-//   queries           times 2^e per row so that the largest is in [256, 512): float16 holds the bfloat16 values then to 2^-33
-//                     of the largest; float32 ones as a sum of two float16 values, 22 bits.
+//   bfloat16 rows     times 2^e, so that a row's largest value is in [2^14, 2^15), and rounded to whole numbers: upper bytes
+//                     (signed) and lower ones (unsigned) meet the keys' bytes in two products of 8-bit integers, whose
+//                     sums are exact (at most 32767 * 128 * 256 < 2^31).  A value loses at most 2^-15 of the row's largest,
+//                     as much as bfloat16 itself gives up on values of that size 2^-7 over; the keys are used as they lie,
+//                     without a conversion (64 requests of 2,000 keys, 32 / 8 heads of 64: 31.7 M warp instructions by
+//                     float16 products, 21.9 M so; 52 -> 43 us).
+//   float32 rows      times 2^e, the largest in [2^8, 2^9), as a sum of two float16 values (22 bits); keys become float16.
+//   int8 -> float16   the byte q + 128 behind the exponent byte 0x64 is the float16 1024 + 128 + q; minus 1152 leaves q
+//                     exactly: a byte permutation and a subtraction for two values.
 //   values            pairs of dimensions transposed by ldmatrix (two bytes travel as one 16-bit element), so even and odd
 //                     dimensions come out as the two halves of a product's 16 rows.
 //   scales            u_j = s_kj (k_j . q) scale log2(e) + log2(s_vj) in float32; p'_j = 2^(u_j - M) with M some 2^6 below
 //                     the largest u.  O = sum p'_j v8_j, l = sum p'_j / s_vj, and O / l is the result: the value's scale
 //                     rides in the exponent, so p' is as large as the term that it stands for.  p' is rounded to
 //                     float16 for the product (2^-12 of itself; 2^-23 in two parts for float32 rows); l adds the unrounded.
+//                     (Whole-number p' would spare the values' conversion too, but a fixed point takes away the weights of
+//                     many faint keys beside a strong one.)
 //
-// M moves lazily: only when a u has passed it by more than 2^14 is O rescaled, so most tiles need no
-// reduction over lanes at all.
+// M moves lazily: only when a u has passed it by more than 14 is O rescaled, so most tiles need no reduction over lanes
+// at all.
 //
-// Single tokens (attention_8bit_stream): as many warps as the GPU holds, the tiles of all requests and heads cut evenly
-// among them; a warp's part of one request's heads is a segment, left in scratch for the merge kernel.  Portions
-// (attention_8bit_rows): a warp, or `nsplit` warps that share its tiles, for every 8 or 16 rows.
+// Three forms:
+//   attention_8bit_stream   single tokens, long contexts: as many warps as the GPU holds, in teams of a warp for every
+//                           key/value head; the tiles of all requests are cut evenly among the teams.  A team's part of a
+//                           request is a segment, left in scratch for the merge kernel.
+//   attention_8bit_rows     portions, and few or short single tokens: a warp for every 8 or 16 rows, or a block or a
+//                           cluster of blocks whose warps share the rows' tiles and meet in shared memory.
+//   (bindings)              long bfloat16 portions: pages are widened to bfloat16 once (cache_8bit.cu) and read by the
+//                           tensor-memory kernel, whose 128-row tiles these 16-row ones cannot match.
+//
+// What bounds them.  The stream: 64 requests of 2,000 keys on average (205 MB) 43 us, 73 % of a copy's bandwidth, with
+// 0.56 instructions issued a cycle and scheduler: not the instructions but how evenly 2,368 warps end, plus some 5 us of
+// launch, first tiles and merge.  (16 / 2 heads of 128, 4 requests of 31,000 keys 26 us of 16.)  Rows: the matrix
+// instructions and conversions of 8 or 16 rows a tile; 2,048 new tokens take 135 us at 32 / 8 heads of 64, widened 45.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -178,9 +193,10 @@ __device__ __forceinline__ void a8_load_n(const __nv_bfloat16* p, bool vec, floa
 
 // ---- how single tokens' tiles are shared out --------------------------------------------------------
 // The tiles of all requests, one after the other, are cut evenly into as many runs as there are teams of warps (`used`
-// of them where there are fewer tiles).  A team has a warp for every unit: a key/value head and 8 * NT of its query heads.  Its warps walk
-// the same tiles, so the heads of a page, which lie side by side, are read at about the same time.  From one segment (a run's part of a request) to the next the run or the request grows, so run + request is
-// a place of its own, times the units.
+// of them where there are fewer tiles).  A team has a warp for every unit: a key/value head and 8 * NT of its query
+// heads.  Its warps walk the same tiles, so the heads of a page, which lie side by side, are read at about the same time.
+// From one segment (a run's part of a request) to the next the run or the request grows, so run + request is a place of
+// its own, times the units.
 struct A8Shares {
     const int* ctx_lens;
     int n_reqs, window, most;

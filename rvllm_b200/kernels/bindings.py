@@ -1014,7 +1014,8 @@ class CudaOps:
         Requests [0, ctx.n_decode) bring one token each, the others any number; the key at position j is seen from
         position p iff j <= p and, with a window, j > p - window.  A row that sees nothing is zeros; one that may see a key
         whose block-table entry is no page, or a request whose context is longer than its row of the table, has no valid
-        result (nothing outside the pages is read).  Scratch is allocated per call (in a captured graph: from the graph's
+        result (nothing outside the pages is read).  `ctx.max_q_len` and `ctx.max_ctx_len` are bounds over all requests: the
+        forms and the launches' sizes follow them.  Scratch is allocated per call (in a captured graph: from the graph's
         pool); long bfloat16 portions (heads of 64 or 128) take bfloat16 copies of what they may see for the call's duration."""
         what = "paged_attention_8bit"
         dtype, here = q.dtype, self._here()
