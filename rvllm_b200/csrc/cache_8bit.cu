@@ -15,18 +15,17 @@
 // One kernel.  A lane has 8 dimensions of a head's first half and the 8 that they turn with, so a warp has
 // 32 / (head size / 16) heads at a time: of one token for the queries; for keys and values of as many tokens, one
 // head.  A block of the latter takes a range of tokens, up to 32, and of it the pages that begin there, to their last
-// token in the call.  The rows are read once (two rounds of them stay in registers: the largest of a page has to be known
-// before any is written), the pages' scales settled a lane each, then the rows written.
+// token in the call.  The rows are read once (two rounds of them stay in shared memory, a thread its own: the largest of a page
+// has to be known before any is written), the pages' scales settled a lane each, then the rows written.
 //
-// What bounds it: four reads that wait for one another (slots, positions, angles and rows, scales), for as many waves of
-// blocks as there are; four blocks of 128 threads a multiprocessor are what the registers leave.  32 / 8 heads of 64:
-// 64 tokens 6 us, 2,048 tokens 14.5 us, 8,192 tokens 49 us; their bytes at a copy's bandwidth 0.1, 3.5 and 14 us.
+// What bounds it: what a block does beside its rows (whose tokens and pages they are, the pages' largest values, two
+// meetings of its warps) and four reads that wait for one another (slots, positions, angles and rows, scales), for as many
+// waves of blocks as there are; registers leave a multiprocessor four or five.  32 / 8 heads of 64: 64 tokens 4.1 us,
+// 2,048 tokens 11.3 us, 8,192 tokens 43 us; their bytes at a copy's bandwidth 0.1, 3.5 and 14 us.
 #include "common.cuh"
 
 #define C8_MAX_HEAD 256
 #define C8_WARPS 4
-#define C8_ROUNDS 4                    // of a token's query heads, one warp
-#define C8_BLOCKS 4                    // of a multiprocessor
 
 struct C8Write {
     const void* rows;                  // [tokens][heads q | kv heads k | kv heads v], `row_stride` elements apart
@@ -37,7 +36,7 @@ struct C8Write {
     float *k_scale, *v_scale;
     long long row_stride, total_slots, table_rows;
     float eps;
-    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, page_shift, aligned, range, q_rounds;
+    int n_tokens, num_heads, num_kv_heads, head_dim, page_size, page_shift, aligned, range;
     long long kv_blocks;
 };
 
@@ -220,20 +219,37 @@ __device__ __forceinline__ void c8_queries(const C8Write& a, int t, int h0, int 
     }
 }
 
+// The largest |x|, `most` among them; NaN if any is.
 __device__ __forceinline__ float c8_most(const float (&x)[8], float most) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(x[i])));
+    return most;
+}
+__device__ __forceinline__ float c8_most_finite(const float (&x)[8], float most) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float v = fabsf(x[i]);
-        if (v <= 3.402823466e38f) most = fmaxf(most, v);       // finite ones
+        if (v <= 3.402823466e38f) most = fmaxf(most, v);
     }
     return most;
 }
-__device__ __forceinline__ uint2 c8_pack(const float (&x)[8], float inv) {
+// rint(x / scale).  `plain`: all are within 127 scales, and the sum with 1.5 * 2^23 has the whole number in its last byte
+// (x * inv is exact, so that this rounds once, half to even).
+__device__ __forceinline__ uint2 c8_pack(const float (&x)[8], float inv, bool plain) {
     unsigned u[2] = {0u, 0u};
+    if (plain) {
+        unsigned b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int q = max(-127, min(127, __float2int_rn(x[i] * inv)));     // NaN: 0
-        u[i >> 2] |= (unsigned)(q & 0xff) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(x[i], inv, 12582912.f));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            u[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int q = max(-127, min(127, __float2int_rn(x[i] * inv)));     // NaN: 0
+            u[i >> 2] |= (unsigned)(q & 0xff) << (8 * (i & 3));
+        }
     }
     return make_uint2(u[0], u[1]);
 }
@@ -248,26 +264,26 @@ struct C8Runs {
     int twice;                         // one of them twice, it may be
 };
 
-template <typename T>
-__global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
+// `MANY`: for as many tokens as fill the GPU several times over.  Then blocks of a multiprocessor count (five: 96 registers a
+// thread), and a warp has two rounds of a token's query heads; else what a thread can request at once (us so / the other way:
+// 32 / 8 heads of 64, 64 tokens 4.1 / 4.4, 512 5.1 / 5.2, 2,048 12.5 / 11.4, 8,192 48.0 / 43.6).
+template <typename T, bool MANY>
+__global__ void __launch_bounds__(C8_WARPS * 32, MANY ? 5 : 4) qk_norm_rope_write_8bit_kernel(const __grid_constant__ C8Write a) {
     rv_pdl_prologue();
     __shared__ C8Runs run;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lph = a.head_dim >> 4, per = 32 / lph;           // lanes a head, heads a warp
     const int sub = lane / lph, d0 = (lane - sub * lph) * 8, lane0 = sub * lph;
     const int half = a.head_dim >> 1;
-    float x[8], y[8];
+    __align__(16) float x[8], y[8];
     if ((long long)blockIdx.x >= a.kv_blocks) {
         // ---- query heads --------------------------------------------------------------------
         const long long id = ((long long)blockIdx.x - a.kv_blocks) * C8_WARPS + warp;
-        const int shares = (a.num_heads + per * a.q_rounds - 1) / (per * a.q_rounds);
+        constexpr int ROUNDS = MANY ? 2 : 1;
+        const int shares = (a.num_heads + per * ROUNDS - 1) / (per * ROUNDS);
         const long long t = id / shares;
         if (t >= a.n_tokens) return;
-        const int h0 = (int)(id - t * shares) * per * a.q_rounds + sub;
-        if (a.q_rounds == 1)
-            c8_queries<T, 1>(a, (int)t, h0, per, sub < per, d0, lane0, lph);
-        else
-            c8_queries<T, C8_ROUNDS>(a, (int)t, h0, per, sub < per, d0, lane0, lph);
+        c8_queries<T, ROUNDS>(a, (int)t, (int)(id - t * shares) * per * ROUNDS + sub, per, sub < per, d0, lane0, lph);
         return;
     }
     // ---- one key or value head of the pages that begin within a range of tokens ---------------
@@ -349,13 +365,16 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         if (sub >= per || t >= t1) slot = -1;
         number = in < 32 ? __popc(owned & ((2u << in) - 1u)) - 1 : n_runs - 1;
     };
-    constexpr int HOLD = 2;             // rounds whose rows stay in registers: a range and the page that it ends in
+    constexpr int HOLD = 2;             // rounds whose rows are kept: a range and the page that it ends in
     const int step = C8_WARPS * per, begin = t0 + warp * per;
-    float hx[HOLD][8], hy[HOLD][8];
-    auto measure = [&](int t, int slot, int number, float (&u)[8], float (&v)[8]) {
+    __shared__ float4 held_rows[HOLD * 4][C8_WARPS * 32];
+    float hm[HOLD], m;                  // the largest |x| of each, or NaN
+    auto measure = [&](int t, int slot, int number, float (&u)[8], float (&v)[8], float& whole) {
         c8_head(a, src + (size_t)(slot >= 0 ? t : t0) * a.row_stride, w, turn, t, slot >= 0, d0, lane0, lph, u, v);
+        float most = whole = c8_most(v, c8_most(u, 0.f));
+        if (!(most <= 3.402823466e38f)) most = c8_most_finite(v, c8_most_finite(u, 0.f));
         if (slot >= 0) {
-            atomicMax(&run.most[number], __float_as_uint(c8_most(v, c8_most(u, 0.f))));
+            atomicMax(&run.most[number], __float_as_uint(most));
             if (d0 == 0) {
                 const unsigned in = slot - page_of(slot) * a.page_size, bit = 1u << (in & 31u);
                 atomicMin(&run.lowest[number], (int)in);
@@ -368,12 +387,16 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         if (begin + i * step < t1) {
             int slot, number;
             whose(begin + i * step + sub, slot, number);
-            measure(begin + i * step + sub, slot, number, hx[i], hy[i]);
+            measure(begin + i * step + sub, slot, number, x, y, hm[i]);
+            held_rows[4 * i][threadIdx.x] = *(const float4*)x;
+            held_rows[4 * i + 1][threadIdx.x] = *(const float4*)(x + 4);
+            held_rows[4 * i + 2][threadIdx.x] = *(const float4*)y;
+            held_rows[4 * i + 3][threadIdx.x] = *(const float4*)(y + 4);
         }
     for (int t = begin + HOLD * step; t < t1; t += step) {
         int slot, number;
         whose(t + sub, slot, number);
-        measure(t + sub, slot, number, x, y);
+        measure(t + sub, slot, number, x, y, m);
     }
     __syncthreads();
     bool grows = false;
@@ -404,7 +427,7 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         }
     }
     __syncthreads();
-    auto store = [&](int t, int slot, int number, const float (&u)[8], const float (&v)[8]) {
+    auto store = [&](int t, int slot, int number, const float (&u)[8], const float (&v)[8], float whole) {
         // (of two tokens with one slot the later one is written)
         const int page = page_of(slot);
         bool later = false;
@@ -416,9 +439,10 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
             }
         if (slot >= 0 && !later) {
             const float inv = run.inv[number];
+            const bool plain = whole * inv <= 127.f;
             signed char* dst = cache + (((size_t)page * a.num_kv_heads + g) * a.page_size + (slot - page * a.page_size)) * a.head_dim;
-            *(uint2*)(dst + d0) = c8_pack(u, inv);
-            *(uint2*)(dst + half + d0) = c8_pack(v, inv);
+            *(uint2*)(dst + d0) = c8_pack(u, inv, plain);
+            *(uint2*)(dst + half + d0) = c8_pack(v, inv, plain);
         }
     };
 #pragma unroll
@@ -426,13 +450,17 @@ __global__ void __launch_bounds__(C8_WARPS * 32, C8_BLOCKS) qk_norm_rope_write_8
         if (begin + i * step < t1) {
             int slot, number;
             whose(begin + i * step + sub, slot, number);
-            store(begin + i * step + sub, slot, number, hx[i], hy[i]);
+            *(float4*)x = held_rows[4 * i][threadIdx.x];
+            *(float4*)(x + 4) = held_rows[4 * i + 1][threadIdx.x];
+            *(float4*)y = held_rows[4 * i + 2][threadIdx.x];
+            *(float4*)(y + 4) = held_rows[4 * i + 3][threadIdx.x];
+            store(begin + i * step + sub, slot, number, x, y, hm[i]);
         }
     for (int t = begin + HOLD * step; t < t1; t += step) {
         int slot, number;
         whose(t + sub, slot, number);
         c8_head(a, src + (size_t)(slot >= 0 ? t + sub : t0) * a.row_stride, w, turn, t + sub, slot >= 0, d0, lane0, lph, x, y);
-        store(t + sub, slot, number, x, y);
+        store(t + sub, slot, number, x, y, c8_most(y, c8_most(x, 0.f)));
     }
 }
 
@@ -470,20 +498,19 @@ extern "C" int rv_qk_norm_rope_write_8bit(const C8WriteCall* c) {
     if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) RV_FAIL("qk_norm_rope_write_8bit: pages must be 16-byte aligned");
     C8Write a = {rows, q_out, q_weight, k_weight, cos_table, sin_table, positions, slots, (signed char*)k_cache,
                  (signed char*)v_cache, k_scale, v_scale, row_stride, pages * page_size, table_rows, eps, n_tokens,
-                 num_heads, num_kv_heads, head_dim, page_size, (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, 0, 0, 1, 0};
+                 num_heads, num_kv_heads, head_dim, page_size, (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1, 0, 0, 0};
     const int size = dtype == RV_DTYPE_F32 ? 4 : 2, per = 32 / (head_dim >> 4);
     a.aligned = ((uintptr_t)rows | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight | (uintptr_t)cos_table |
                  (uintptr_t)sin_table) % 16 == 0 && row_stride * size % 16 == 0;
     a.range = C8_WARPS * per < 32 ? C8_WARPS * per : 32;
     a.kv_blocks = (long long)((n_tokens + a.range - 1) / a.range) * 2 * num_kv_heads;
-    // a warp has more of a token's heads where there are more tokens than warps' places (2,048 tokens, 32 / 8 heads
-    // of 64: 16.5 -> 14.5 us)
-    a.q_rounds = n_tokens >= 8 * rv_sm_count() && num_heads > per ? C8_ROUNDS : 1;
-    const long long q_warps = (long long)n_tokens * ((num_heads + per * a.q_rounds - 1) / (per * a.q_rounds));
+    const bool many = n_tokens >= 8 * rv_sm_count();
+    const int share = per * (many ? 2 : 1);                // of a token's query heads, a warp's
+    const long long q_warps = (long long)n_tokens * ((num_heads + share - 1) / share);
     const long long blocks = a.kv_blocks + (q_warps + C8_WARPS - 1) / C8_WARPS;
     if (blocks > 0x7fffffffLL) RV_FAIL("qk_norm_rope_write_8bit: too many rows");
     RV_DISPATCH_DTYPE(dtype, "qk_norm_rope_write_8bit",
-                      (rv_launch(qk_norm_rope_write_8bit_kernel<T>, dim3((int)blocks), dim3(C8_WARPS * 32), 0,
+                      (rv_launch(many ? qk_norm_rope_write_8bit_kernel<T, true> : qk_norm_rope_write_8bit_kernel<T, false>, dim3((int)blocks), dim3(C8_WARPS * 32), 0,
                                  (cudaStream_t)stream, a)));
     RV_CHECK_LAUNCH("qk_norm_rope_write_8bit");
     return 0;

@@ -98,6 +98,33 @@ def test_write_without_norm_or_rotation(ops, norm, turn):
     check_written(torch.float32, *got, caches, before)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_write_of_many_tokens(ops, dtype):
+    """As many tokens as take the form for long prompts, pages that begin anywhere in a block's range of tokens, heads that leave
+    a warp's lanes without one; values that are not finite, and ones beyond the largest scale, among ordinary ones."""
+    g = torch.Generator().manual_seed(19)
+    for H, K, D, ps, new, old in ((3, 2, 64, 16, [1, 1, 700, 490, 60], [15, 40, 5, 0, 3]), (1, 1, 48, 64, [1200], [70])):
+        pages = 3 + sum(-(-(a + b) // ps) for a, b in zip(new, old))
+        ctx, group = plain.batch(new, old, ps, pages, 0, seed=3)
+        n = sum(new)
+        assert n >= 8 * torch.cuda.get_device_properties(0).multi_processor_count
+        rows = rnd(g, n, (H + 2 * K) * D, dtype=dtype)
+        finite = rows.clone()
+        values = rows[:, (H + K) * D:]
+        for t, x in ((3, math.nan), (40, math.inf), (41, -math.inf), (700, math.nan), (900, 3e38), (901, -3e38), (1100, 2.0 ** -70)):
+            values[t, (7 * t) % (K * D)] = x
+        k8, ks = pages_of(g, pages, K, ps, D)
+        v8, vs = pages_of(g, pages, K, ps, D, 4.0)
+        caches, before = [k8, v8, ks, vs], [k8.clone(), v8.clone()]
+        again = [c.clone() for c in caches]
+        w = 1 + rnd(g, D, scale=0.1)
+        got = write_both(ops, finite, H, K, D, w, w, 1e-6, angles(1300, D), ctx, group, caches)
+        check_written(dtype, *got, caches, before)
+        dev = write_both(ops, rows, H, K, D, w, w, 1e-6, angles(1300, D), ctx, group, again)[3]
+        assert torch.equal(dev[3], again[3]) and torch.equal(dev[1], again[1])
+        assert torch.equal(dev[0], got[3][0]) and torch.equal(dev[2], got[3][2])
+
+
 def test_write_token_by_token_is_the_portion(ops):
     """A page filled by 16 calls holds what one call leaves, but for the bits that its growing scale dropped: a
     step of the last scale at most in all (halves of steps that double)."""
