@@ -155,7 +155,8 @@ class Engine:
         if self.logprobs is None:
             return None
         if not torch.is_tensor(ids):
-            ids = torch.tensor(ids, dtype=torch.int32, device=logits.device)
+            ids = torch.tensor(ids)
+        ids = ids.to(device=logits.device, dtype=torch.int32)
         return LogprobReader(self.runner.ops, logits[:ids.shape[0]], ids, self.logprobs)
 
     def _can_look_ahead(self, plan) -> bool:

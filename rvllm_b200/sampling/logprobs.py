@@ -21,7 +21,7 @@ class TokenLogprob:
 
 class LogprobReader:
     """Launches `ops.token_logprobs` and copies its results to the host without waiting; `read` is called when the copies
-    are known to be done (or None of them was asynchronous)."""
+    are known to be done."""
 
     def __init__(self, ops, logits: torch.Tensor, tokens: torch.Tensor, top: int):
         results = (tokens,) + ops.token_logprobs(logits, tokens, top)
