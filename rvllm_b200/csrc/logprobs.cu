@@ -16,11 +16,11 @@
 // would not hold them (rising rows, values all alike) the row is walked a second time, the block together.
 //
 // A row is a cluster's of 1 to 8 blocks (as many as the GPU has room for when rows are few); parts meet in the
-// first block in a fixed order, so a row's results do not depend on what else is in the launch.
+// first block in a fixed order, so a row's results do not depend on the other rows' values nor on who came first.
 // Bound by reading the logits, then by what a value costs beside its load: float32 rows of 65,536, 2,047 of them (537 MB,
-// 82 us at a copy's bandwidth), take 93 us without alternatives, 105 with five, 121 with twenty (a bound of more lanes
-// needs more maxima over a warp, and more values pass it).  64 rows with twenty take 17 us of 3, one row 7: starts, the
-// row's walk by a cluster of eight and its meeting.
+// 82 us at a copy's bandwidth), take 90 us without alternatives, 98 with five, 114 with twenty (a bound of more lanes
+// needs more maxima over a warp, and more values pass it).  64 rows with twenty take 13 us of 3, one row 4 without
+// alternatives and 7 with twenty: a chain of the first loads, the warps' first bound, the cluster's meeting and the places.
 #include "common.cuh"
 
 #define LP_THREADS 256
@@ -79,21 +79,20 @@ struct __align__(16) LpPart { float m, s, w; int above; };
 __device__ __forceinline__ float lp_ref(float m) { return m == -INFINITY ? 0.f : m; }
 // From one reference to a larger one, in units of log2; far ones stay finite (2^-300 is 0).
 __device__ __forceinline__ float lp_move(float from, float to) { return fmaxf((from - to) * LP_LOG2E, -300.f); }
-__device__ __forceinline__ void lp_add(LpPart& a, const LpPart& b) {
-    // both to the larger reference
-    const float top = fmaxf(a.m, b.m), c = lp_ref(top);
+// A warp's lanes put together, always in the same order: to the largest reference, then sums.
+__device__ __forceinline__ LpPart lp_meet(const LpPart& a) {
+    LpPart p;
+    p.m = rv_warp_max(a.m);
+    p.s = p.w = 0.f;
     if (a.s != 0.f) {
-        const float d = lp_move(lp_ref(a.m), c), f = lp_exp2(d);
-        a.w = (a.w + a.s * d) * f;
-        a.s *= f;
+        const float d = lp_move(lp_ref(a.m), lp_ref(p.m)), f = lp_exp2(d);
+        p.s = a.s * f;
+        p.w = (a.w + a.s * d) * f;
     }
-    if (b.s != 0.f) {
-        const float d = lp_move(lp_ref(b.m), c), f = lp_exp2(d);
-        a.w += (b.w + b.s * d) * f;
-        a.s += b.s * f;
-    }
-    a.m = top;
-    a.above += b.above;
+    p.s = rv_warp_sum(p.s);
+    p.w = rv_warp_sum(p.w);
+    p.above = __reduce_add_sync(0xffffffffu, a.above);
+    return p;
 }
 
 template <bool TOP> struct LpShared {
@@ -134,7 +133,7 @@ struct LpThread {
     u64 least = 0ull;                  // only larger keys are wanted
     LpShared<TOP>& sh;
 
-    __device__ __forceinline__ LpThread(LpShared<TOP>& shared, int k, float x) : given(x), top(k), sh(shared) {}
+    __device__ __forceinline__ LpThread(LpShared<TOP>& shared, int k) : top(k), sh(shared) {}
 
     // Of E values: the sums; the largest.
     __device__ __forceinline__ float sums(const float (&x)[E]) {
@@ -175,15 +174,27 @@ struct LpThread {
     }
     template <typename Col, typename Real>
     __device__ __forceinline__ void collect(const float (&x)[E], float limit, Col col, Real real) {
+        // (few lanes have any, and one at most: a loop over them is shorter than their code written out, which costs more to fetch
+        // than to run)
+        unsigned which = 0u;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (x[i] >= limit) {                                     // few
-                const u64 key = ((u64)lp_key(x[i]) << 32) | (0xffffffffu - (unsigned)col(i));
-                if (key > least && real(i)) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < LP_ROOM) sh.room[at] = key;
-                }
+        for (int i = 0; i < E; ++i) which |= x[i] >= limit ? 1u << i : 0u;
+        while (which) {
+            const int i = __ffs(which) - 1;
+            which &= which - 1;
+            float v[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = x[k];
+#pragma unroll
+            for (int h = E / 2; h > 0; h >>= 1)
+#pragma unroll
+                for (int k = 0; k < h; ++k) v[k] = (i & h) ? v[k + h] : v[k];
+            const u64 key = ((u64)lp_key(v[0]) << 32) | (0xffffffffu - (unsigned)col(i));
+            if (key > least && real(i)) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < LP_ROOM) sh.room[at] = key;
             }
+        }
     }
     // Adds E values of this thread (the whole block comes here): x[i] is column col(i), if real(i).
     template <typename Col, typename Real>
@@ -236,8 +247,9 @@ struct LpThread {
 
 // Walks a row's part: `body(values, column of value i, whether there is one)` of every thread, round by round; the next round's
 // values are requested before a round is taken.
-template <typename T, typename Body>
-__device__ __forceinline__ void lp_walk(const T* x, int vocab, int part, int parts, Body body) {
+// `ready()` comes behind the first requests.
+template <typename T, typename Ready, typename Body>
+__device__ __forceinline__ void lp_walk(const T* x, int vocab, int part, int parts, Ready ready, Body body) {
     constexpr int N = LpVec<T>::N, U = LpVec<T>::UNROLL, E = N * U, ROUND = U * LP_THREADS;
     const int tid = threadIdx.x;
     // whole 16-byte vectors from the first aligned one on, shared out over the parts; what lies
@@ -260,6 +272,7 @@ __device__ __forceinline__ void lp_walk(const T* x, int vocab, int part, int par
         }
     };
     if (v0 < v1) load(v0);
+    ready();
     for (int at = v0; at < v1; at += ROUND) {
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = next[i];
@@ -289,35 +302,25 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
     const long long row = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - row * parts);
     const T* x = logits + row * row_stride;
-    const int token = tokens[row];
-    const bool known = token >= 0 && token < vocab;
-    const float given = known ? rv_load(x + token) : INFINITY;
     if constexpr (TOP) {
         if (tid == 0) sh.count = sh.kept = 0;
         if (tid < LP_WARPS) sh.bound[tid] = 0u;
         __syncthreads();
     }
-    LpThread<T, TOP> th(sh, top, given);
-    lp_walk(x, vocab, part, parts, [&](auto& v, auto col, auto real) { th.take(v, col, real); });
+    const int token = tokens[row];
+    const bool known = token >= 0 && token < vocab;
+    LpThread<T, TOP> th(sh, top);
+    lp_walk(x, vocab, part, parts, [&] { th.given = known ? rv_load(x + token) : INFINITY; },
+            [&](auto& v, auto col, auto real) { th.take(v, col, real); });
     // ---- the warp's, the block's, the cluster's ------------------------------------------------
     {
-        const float most = rv_warp_max(th.m), c = lp_ref(most);
-        float s = 0.f, w = 0.f;
-        if (th.s != 0.f) {
-            const float d = lp_move(lp_ref(th.m), c), f = lp_exp2(d);
-            s = th.s * f;
-            w = (th.w + th.s * d) * f;
-        }
-        s = rv_warp_sum(s);
-        w = rv_warp_sum(w);
-        const int above = __reduce_add_sync(0xffffffffu, th.above);
-        if (lane == 0) sh.part[warp] = {most, s, w, above};
+        const LpPart p = lp_meet({th.m, th.s, th.w, th.above});
+        if (lane == 0) sh.part[warp] = p;
     }
     __syncthreads();
-    if (tid == 0) {
-        LpPart p = sh.part[0];
-        for (int i = 1; i < LP_WARPS; ++i) lp_add(p, sh.part[i]);
-        sh.whole = p;
+    if (warp == LP_WARPS - 1) {
+        const LpPart none = {-INFINITY, 0.f, 0.f, 0}, p = lp_meet(lane < LP_WARPS ? sh.part[lane] : none);
+        if (lane == 0) sh.whole = p;
     }
     if constexpr (TOP) {
         const int n = sh.count;
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
             if (tid == 0) sh.count = 0;
             __syncthreads();
             th.least = b ? ((u64)b << 32) - 1ull : 0ull;
-            lp_walk(x, vocab, part, parts, [&](auto& v, auto col, auto real) { th.take_again(v, col, real); });
+            lp_walk(x, vocab, part, parts, [] {}, [&](auto& v, auto col, auto real) { th.take_again(v, col, real); });
             lp_place(sh.room, sh.count, top, sh.best[0]);
         } else {
             // those that the last bound leaves
@@ -360,21 +363,13 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
             }
             if (warp == 0) {
                 // lane k brings part k's sums
-                LpPart q = sh.whole;
-                if (lane > 0 && lane < parts)
+                LpPart q = {-INFINITY, 0.f, 0.f, 0};
+                if (lane < parts)
                     asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
                                  : "=f"(q.m), "=f"(q.s), "=f"(q.w), "=r"(q.above) : "r"(remote(&sh.whole, lane)) : "memory");
-                LpPart p = sh.whole;
-                for (int k = 1; k < parts; ++k) {
-                    LpPart o;
-                    o.m = __shfl_sync(0xffffffffu, q.m, k);
-                    o.s = __shfl_sync(0xffffffffu, q.s, k);
-                    o.w = __shfl_sync(0xffffffffu, q.w, k);
-                    o.above = __shfl_sync(0xffffffffu, q.above, k);
-                    lp_add(p, o);
-                }
+                q = lp_meet(q);
                 __syncwarp();
-                if (lane == 0) sh.whole = p;
+                if (lane == 0) sh.whole = q;
             }
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // nobody leaves while it is read
@@ -385,37 +380,35 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT) token_logprobs_kernel
     const float c = lp_ref(p.m), logs = logf(p.s);
     if (tid == 0) {
         const float h = logs - LP_LN2 * (p.w / p.s);
-        logprob[row] = known ? (given - c) - logs : NAN;
+        logprob[row] = known ? (th.given - c) - logs : NAN;
         rank[row] = known ? p.above + 1 : 0;
         entropy[row] = h < 0.f ? 0.f : h;
     }
     if constexpr (TOP) {
-        // a key of part `warp`: how many are larger in each part, by bisection
-        if (warp < parts && lane < top) {
-            const u64 key = sh.best[warp][lane];
-            int larger[LP_MAX_CLUSTER];                              // how many of part k are
+        // a key of part `warp`: its place is how many of all the parts' are larger
+        const u64 key = warp < parts && lane < top ? sh.best[warp][lane] : 0ull;
+        // (lists are in order: bisection in all of them at once)
+        int place = lane;
+        if (parts > 1) {
+            int larger[LP_MAX_CLUSTER];
 #pragma unroll
             for (int k = 0; k < LP_MAX_CLUSTER; ++k) larger[k] = 0;
-#pragma unroll
-            for (int step = 32; step > 0; step >>= 1)
+            for (int step = top == 32 ? 16 : 1 << (31 - __clz(top)); step > 0; step >>= 1)
 #pragma unroll
                 for (int k = 0; k < LP_MAX_CLUSTER; ++k)
-                    if (k < parts && larger[k] + step <= 32 && sh.best[k][larger[k] + step - 1] > key) larger[k] += step;
-            int place = 0;
+                    larger[k] += (sh.best[k][larger[k] + step - 1] > key) ? step : 0;
+            place = 0;
 #pragma unroll
-            for (int k = 0; k < LP_MAX_CLUSTER; ++k) place += larger[k];
-            if (key != 0ull && place < top) {
-                top_logprob[row * top + place] = (lp_value((unsigned)(key >> 32)) - c) - logs;
-                top_id[row * top + place] = (int)(0xffffffffu - (unsigned)key);
-            }
+            for (int k = 0; k < LP_MAX_CLUSTER; ++k) place += k < parts ? larger[k] + (sh.best[k][larger[k]] > key) : 0;   // (31 + 1)
         }
-        if (warp == 0) {                                             // places that nothing takes
-            int have = 0;
-            for (int k = 0; k < parts; ++k) have += __popc(__ballot_sync(0xffffffffu, sh.best[k][lane] != 0ull));
-            if (lane < top && lane >= have) {
-                top_logprob[row * top + lane] = NAN;
-                top_id[row * top + lane] = -1;
-            }
+        if (key != 0ull && place < top) {
+            top_logprob[row * top + place] = (lp_value((unsigned)(key >> 32)) - c) - logs;
+            top_id[row * top + place] = (int)(0xffffffffu - (unsigned)key);
+        }
+        const int have = __syncthreads_count(key != 0ull);
+        if (tid < top && tid >= have) {                               // places that nothing takes
+            top_logprob[row * top + tid] = NAN;
+            top_id[row * top + tid] = -1;
         }
     }
 }
