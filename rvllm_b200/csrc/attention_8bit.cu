@@ -139,6 +139,7 @@ __device__ __forceinline__ float a8_exp2(float x) {              // -inf: 0
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float a8_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 // Bytes `sel` of x, each behind 0x64, minus 1152 (x: bytes of q + 128).
 __device__ __forceinline__ unsigned a8_pair(unsigned x, unsigned sel) {
     const unsigned h = __byte_perm(x, 0x64646464u, sel);
@@ -324,19 +325,20 @@ struct A8Warp {
                 }
             most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            // the largest in [2^14, 2^15), or in [2^8, 2^9)
-            int e = (WHOLE ? 14 : 8) - ((int)(__float_as_uint(most) >> 23) - 127);
-            e = most > 0.f ? max(-100, min(100, e)) : 0;                // (NaN: 0)
-            const float up = __uint_as_float((unsigned)(e + 127) << 23);
-            float down = __uint_as_float((unsigned)(127 - e) << 23);
-            if (WHOLE && !(most <= 3.402823466e38f)) down = NAN;       // whole numbers hold no infinity
+            // the largest in [2^14, 2^15), or in [2^8, 2^9): times 2^e, e between -120 and 141, as two factors that float32
+            // holds (a row's values may be of any size)
+            const int e = most > 0.f ? (WHOLE ? 14 : 8) - ((int)(__float_as_uint(most) >> 23) - 127) : 0;     // (NaN: 0)
+            const int e1 = e / 2, e2 = e - e1;
+            const float up1 = a8_pow2(e1), up2 = a8_pow2(e2);
+            float mine = a.scale_log2 * a8_pow2(-e1) * a8_pow2(-e2);
+            if (WHOLE && !(most <= 3.402823466e38f)) mine = NAN;       // whole numbers hold no infinity
 #pragma unroll
             for (int c = 0; c < A8_CHUNKS; ++c) {
                 if constexpr (WHOLE) {
                     unsigned upper = 0u, lower = 0u;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int v = min(32767, __float2int_rn(x[c][k] * up));
+                        const int v = __float2int_rn(x[c][k] * up1 * up2);        // (bfloat16: at most 255 * 2^7)
                         upper |= ((unsigned)(v >> 8) & 0xffu) << (8 * k);
                         lower |= ((unsigned)v & 0xffu) << (8 * k);
                     }
@@ -345,13 +347,12 @@ struct A8Warp {
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float x0 = x[c][2 * h] * up, x1 = x[c][2 * h + 1] * up;
+                        const float x0 = x[c][2 * h] * up1 * up2, x1 = x[c][2 * h + 1] * up1 * up2;
                         q[c][n][h] = a8_pack(x0, x1);
                         q2[c][n][h] = a8_rest(x0, x1, q[c][n][h]);
                     }
                 }
             }
-            const float mine = down * a.scale_log2;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 // the rows of this lane's scores: columns 2 t, 2 t + 1
@@ -467,7 +468,7 @@ struct A8Warp {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) s[m][n][2 * h + j] = fmaf(s[m][n][2 * h + j] * f[n][j], sk, ev);
+                    for (int j = 0; j < 2; ++j) s[m][n][2 * h + j] = fmaf(s[m][n][2 * h + j], f[n][j] * sk, ev);
             }
         if (key0 + A8_KEYS - 1 > p_min || key0 < lo_max) {
 #pragma unroll
