@@ -8,12 +8,10 @@
 // left operand, 8 query rows the columns of the right one.  With few query heads per key/value head the other order
 // would leave most of a product's 16 rows empty.
 //
-//   bfloat16 rows     times 2^e, so that a row's largest value is in [2^14, 2^15), and rounded to whole numbers: upper bytes
-//                     (signed) and lower ones (unsigned) meet the keys' bytes in two products of 8-bit integers, whose
-//                     sums are exact (at most 32767 * 128 * 256 < 2^31).  A value loses at most 2^-15 of the row's largest,
-//                     as much as bfloat16 itself gives up on values of that size 2^-7 over; the keys are used as they lie,
-//                     without a conversion (64 requests of 2,000 keys, 32 / 8 heads of 64: 31.7 M warp instructions by
-//                     float16 products, 21.9 M so; 52 -> 43 us).
+//   bfloat16 rows     times 2^e, so that a row's largest value is in [2^22, 2^23), and rounded to whole numbers: their three
+//                     bytes (the upper one signed) meet the keys' bytes in products of 8-bit integers, whose sums are exact
+//                     (at most 255 * 128 * 256 < 2^23 each).  Values down to 2^-15 of the row's largest lose nothing, smaller ones
+//                     2^-23 of the largest at most; the keys are used as they lie, without a conversion.
 //   float32 rows      times 2^e, the largest in [2^8, 2^9), as a sum of two float16 values (22 bits); keys become float16.
 //   int8 -> float16   the byte q + 128 behind the exponent byte 0x64 is the float16 1024 + 128 + q; minus 1152 leaves q
 //                     exactly: a byte permutation and a subtraction for two values.
@@ -21,10 +19,10 @@
 //                     dimensions come out as the two halves of a product's 16 rows.
 //   scales            u_j = s_kj (k_j . q) scale log2(e) + log2(s_vj) in float32; p'_j = 2^(u_j - M) with M some 2^6 below
 //                     the largest u.  O = sum p'_j v8_j, l = sum p'_j / s_vj, and O / l is the result: the value's scale
-//                     rides in the exponent, so p' is as large as the term that it stands for.  p' is rounded to
-//                     float16 for the product (2^-12 of itself; 2^-23 in two parts for float32 rows); l adds the unrounded.
-//                     (Whole-number p' would spare the values' conversion too, but a fixed point takes away the weights of
-//                     many faint keys beside a strong one.)
+//                     rides in the exponent, so p' is as large as the term that it stands for.  p' is multiplied as
+//                     two float16 parts (what they leave is 2^-22 of itself, or 2^-25 beside a largest of 2^6 and more); l adds
+//                     the unrounded.  (Whole-number p' would spare the values' conversion too, but a fixed point takes away the
+//                     weights of many faint keys beside a strong one.)
 //
 // M moves lazily: only when a u has passed it by more than 14 is O rescaled, so most tiles need no reduction over lanes
 // at all.
@@ -255,10 +253,11 @@ struct A8Warp {
     const unsigned ring;               // in shared memory
     const int lane, g, t;
     int rows_first, rows_count, kvh, G, qs;        // of the segment: its first row, rows, head, query heads a head, first token
-    static constexpr bool WHOLE = PARTS == 1;      // queries as whole numbers of 16 bits
+    static constexpr bool WHOLE = PARTS == 1;      // queries as whole numbers of 24 bits
+    static constexpr int PIECES = WHOLE ? 3 : 2;
     // O^T of 16 dimensions and 8 rows: dimension 2 g (even ones) of rows 2 t, 2 t + 1, then 2 g + 1 of the same
     float o[A8_CHUNKS][NT][4];
-    unsigned q[A8_CHUNKS][NT][2];                  // WHOLE: upper and lower bytes of 4 values; else of 2 and 2, float16
+    unsigned q[A8_CHUNKS][NT][PIECES];             // WHOLE: upper, middle and lower bytes of 4 values; else 2 and 2, float16
     unsigned q2[WHOLE ? 1 : A8_CHUNKS][NT][2];     // what float16 left of them
     float f[NT][2], M[NT][2], l[NT][2];
     int hi[NT][2], lo[NT][2], p_min, lo_max;
@@ -325,9 +324,9 @@ struct A8Warp {
                 }
             most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = a8_max_nan(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            // the largest in [2^14, 2^15), or in [2^8, 2^9): times 2^e, e between -120 and 141, as two factors that float32
+            // the largest in [2^22, 2^23), or in [2^8, 2^9): times 2^e, e between -120 and 149, as two factors that float32
             // holds (a row's values may be of any size)
-            const int e = most > 0.f ? (WHOLE ? 14 : 8) - ((int)(__float_as_uint(most) >> 23) - 127) : 0;     // (NaN: 0)
+            const int e = most > 0.f ? (WHOLE ? 22 : 8) - ((int)(__float_as_uint(most) >> 23) - 127) : 0;     // (NaN: 0)
             const int e1 = e / 2, e2 = e - e1;
             const float up1 = a8_pow2(e1), up2 = a8_pow2(e2);
             float mine = a.scale_log2 * a8_pow2(-e1) * a8_pow2(-e2);
@@ -335,15 +334,14 @@ struct A8Warp {
 #pragma unroll
             for (int c = 0; c < A8_CHUNKS; ++c) {
                 if constexpr (WHOLE) {
-                    unsigned upper = 0u, lower = 0u;
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p) q[c][n][p] = 0u;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int v = __float2int_rn(x[c][k] * up1 * up2);        // (bfloat16: at most 255 * 2^7)
-                        upper |= ((unsigned)(v >> 8) & 0xffu) << (8 * k);
-                        lower |= ((unsigned)v & 0xffu) << (8 * k);
+                        const int v = __float2int_rn(x[c][k] * up1 * up2);        // (bfloat16: at most 255 * 2^15)
+#pragma unroll
+                        for (int p = 0; p < PIECES; ++p) q[c][n][p] |= ((unsigned)(v >> (16 - 8 * p)) & 0xffu) << (8 * k);
                     }
-                    q[c][n][0] = upper;
-                    q[c][n][1] = lower;
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -380,7 +378,7 @@ struct A8Warp {
     __device__ __forceinline__ void scores(unsigned base, int m, float (&s)[NT][4]) {
         // pieces c and c + 1 of the 16 keys' rows: lanes 0-7, 8-15 name keys 0-7, 8-15 of piece c, the others of c + 1
         const int key = 16 * m + (lane & 15);
-        int up[NT][4], low[NT][4];
+        int up[NT][4], mid[NT][4], low[NT][4];
         auto half = [&](int c, unsigned w0, unsigned w1) {            // 16 dimensions, float16
             w0 ^= 0x80808080u;
             w1 ^= 0x80808080u;
@@ -404,7 +402,8 @@ struct A8Warp {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         a8_imma<false>(up[n], w[0], w[1], w[2], w[3], q[c][n][0], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][0], c == 0);
-                        a8_imma<true>(low[n], w[0], w[1], w[2], w[3], q[c][n][1], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][1], c == 0);
+                        a8_imma<true>(mid[n], w[0], w[1], w[2], w[3], q[c][n][1], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][1], c == 0);
+                        a8_imma<true>(low[n], w[0], w[1], w[2], w[3], q[c][n][PIECES - 1], q[c + 1 < A8_CHUNKS ? c + 1 : c][n][PIECES - 1], c == 0);
                     }
                 } else {
                     half(c, w[0], w[1]);
@@ -417,7 +416,8 @@ struct A8Warp {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         a8_imma<false>(up[n], w[0], w[1], q[c][n][0], c == 0);
-                        a8_imma<true>(low[n], w[0], w[1], q[c][n][1], c == 0);
+                        a8_imma<true>(mid[n], w[0], w[1], q[c][n][1], c == 0);
+                        a8_imma<true>(low[n], w[0], w[1], q[c][n][PIECES - 1], c == 0);
                     }
                 } else {
                     half(c, w[0], w[1]);
@@ -428,7 +428,7 @@ struct A8Warp {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[n][k] = (float)(up[n][k] * 256 + low[n][k]);
+                for (int k = 0; k < 4; ++k) s[n][k] = fmaf((float)(up[n][k] * 256 + mid[n][k]), 256.f, (float)low[n][k]);
         }
     }
 
@@ -526,7 +526,7 @@ struct A8Warp {
                     l[n][1] = fmaf(p1, inv[m][h], l[n][1]);
                     const unsigned w = a8_pack(p0, p1);
                     p[n][m][h] = a8_transpose(w);
-                    if (!WHOLE) p2[n][m][h] = a8_transpose(a8_rest(p0, p1, w));
+                    p2[n][m][h] = a8_transpose(a8_rest(p0, p1, w));
                 }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -553,7 +553,7 @@ struct A8Warp {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         a8_mma(o[c + k][n], a0, a1, a2, a3, p[n][m][0], p[n][m][1]);
-                        if (!WHOLE) a8_mma(o[c + k][n], a0, a1, a2, a3, p2[n][m][0], p2[n][m][1]);
+                        a8_mma(o[c + k][n], a0, a1, a2, a3, p2[n][m][0], p2[n][m][1]);
                     }
                 }
             }

@@ -6,8 +6,8 @@ Tolerances.  The result's own rounding, `half` of itself (bfloat16 2^-8, float32
 operands of 22 bits and more, weights from exponentials of 2^-22, and both enter the products with 22 bits: 2^-20 of the largest
 value seen for each unit of the largest sum |q| |k| scale, and 8 units of them (as in `plain_8bit.attention_room`).  A weight
 below 2^-8 of the row's reference has no more than the smallest step of its second part, 2^-25, beside a largest of 2^6: 2^-31 of
-the largest term for each of `keys`, some sqrt(keys) of them together.  Portions that are widened multiply weights of float16,
-half a step of which is 2^-11 of itself: as much of the largest value seen more."""
+the largest term for each of `keys`, some sqrt(keys) of them together.  Portions that are widened multiply weights of bfloat16,
+half a step of which is 2^-8 of itself: as much of the largest value seen more."""
 import math
 
 import pytest
@@ -27,8 +27,26 @@ def room(dtype, want, most, portions_from=None):
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
     off = most[..., 0] * 2.0 ** -20 * (most[..., 1] + 8) + 2.0 ** -31 * most[..., 4] * most[..., 3]
     if portions_from is not None:
-        off[portions_from:] += most[portions_from:, :, 0] * 2.0 ** -11
+        off[portions_from:] += most[portions_from:, :, 0] * 2.0 ** -8
     return half * want.abs() + off.repeat_interleave(want.shape[1] // most.shape[1], 1) + 1e-30
+
+
+def left_out(q, H, K, D, pages, ctx, group, scale):
+    """What a score can be off by because bfloat16 rows are whole numbers of 24 bits, the row's largest value in [2^22, 2^23): the
+    rounding of each value, which this repeats, times the keys' size.  A weight is off by as much of itself, the result by twice that
+    of the largest value."""
+    k8, _, ks, _ = pages
+    x = q.double().reshape(q.shape[0], H, D)
+    unit = torch.exp2(torch.floor(torch.log2(x.abs().amax(2, keepdim=True))) - 22)
+    lost = (torch.round(x / unit) * unit - x).abs()
+    off = torch.zeros(q.shape[0], H, dtype=torch.float64)
+    for r in range(ctx.n_reqs):
+        clen, a, b = int(ctx.ctx_lens[r]), int(ctx.q_start[r]), int(ctx.q_start[r + 1])
+        j = torch.arange(clen)
+        page = group.block_table[r][j // group.page_size].long()
+        k = (k8[page, :, j % group.page_size].double() * ks[page].double()[..., None]).abs().amax(0)        # [kv, dim]
+        off[a:b] = (lost[a:b] * k.repeat_interleave(H // K, 0)).sum(2) * scale
+    return off
 
 
 def attend(ops, q, H, K, D, pages, ctx, group, scale, window=None, sinks=None):
@@ -42,6 +60,9 @@ def check(ops, q, H, K, D, pages, ctx, group, scale, window=None):
     got = attend(ops, q, H, K, D, pages, ctx, group, scale, window)
     want, most = plain.attention(q, H, K, D, *pages, ctx, group, scale, window)
     limit = room(q.dtype, want, most, ctx.n_decode if widened(ops, q.dtype, D) else None)
+    if q.dtype == torch.bfloat16:
+        n = ctx.n_decode if widened(ops, q.dtype, D) else q.shape[0]
+        limit[:n] += (2 * most[:n, :, 0] * left_out(q, H, K, D, pages, ctx, group, scale)[:n]).repeat_interleave(D, 1)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert bool(((got - want).abs() <= limit).all()), float(((got - want).abs() / limit).max())
 
@@ -89,3 +110,97 @@ def test_large_queries_over_small_keys(ops, dtype, power):
                 clear += 1
     assert clear >= 70
     assert bool(((got - want).abs() <= limit).all())
+
+
+# ---- bits that must not go ------------------------------------------------------------------------------
+
+def opposite_pairs(g, pages, kv, ps, D):
+    """Keys 2 i and 2 i + 1 differ by a step in one dimension, their values by their sign: what is left of them shows every bit
+    that the weights have."""
+    k8, ks = pages_of(g, pages, kv, ps, D)
+    v8, vs = pages_of(g, pages, kv, ps, D)
+    k8 = k8.clamp(-126, 126)
+    k8[:, :, 1::2] = k8[:, :, ::2]
+    k8[:, :, 1::2, 5] += 1
+    v8[:, :, 1::2] = -v8[:, :, ::2]
+    return k8, v8, ks, vs
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,K,D", [(8, 2, 64), (16, 1, 64), (4, 2, 128), (4, 2, 48), (2, 1, 256)])
+def test_weights_that_nearly_cancel(ops, dtype, H, K, D):
+    g = torch.Generator().manual_seed(42)
+    new, old = [1] * 12 + [9, 30], [1, 3, 3, 5, 7, 7, 9, 15, 31, 63, 127, 801, 2, 20]
+    pages = sum(-(-(a + b) // 16) for a, b in zip(new, old))
+    ctx, group = plain.batch(new, old, 16, pages, 12, seed=4)
+    check(ops, rnd(g, sum(new), H * D, dtype=dtype), H, K, D, opposite_pairs(g, pages, K, 16, D), ctx, group, D ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("large", [30.0, 1000.0, 20000.0])
+def test_one_large_value_beside_small_ones(ops, dtype, large):
+    """A query value that meets zeros takes no bits from the others, on which the scores hang."""
+    g = torch.Generator().manual_seed(43)
+    for H, K, D in ((8, 2, 64), (4, 1, 128), (6, 2, 48)):
+        new, old = [1] * 6 + [25], [1, 7, 15, 100, 333, 900, 40]
+        pages = sum(-(-(a + b) // 16) for a, b in zip(new, old))
+        ctx, group = plain.batch(new, old, 16, pages, 6, seed=5)
+        k8, v8, ks, vs = opposite_pairs(g, pages, K, 16, D)
+        k8[..., 3] = 0
+        q = rnd(g, sum(new), H * D, dtype=dtype)
+        q[:, 3::D] = large
+        # (the room counts what is multiplied: the large value meets zeros)
+        check(ops, q, H, K, D, (k8, v8, ks, vs), ctx, group, D ** -0.5)
+
+
+# ---- values of neighbouring pages far apart ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", [3, 10, 20, 30])
+def test_pages_side_by_side_far_apart(ops, dtype, D, step):
+    """Values that grow by 2^step from a page of eight tokens to the next, and that fall so: rows see the first pages alone, or all
+    of them, and what a row sees is right by its own largest value."""
+    g = torch.Generator().manual_seed(44)
+    for sign in (1, -1):
+        ctx, group = plain.batch([1, 32, 70], [31, 0, 40], 8, 24, 1, seed=6)
+        k8, ks = pages_of(g, 24, 2, 8, D)
+        v8, vs = pages_of(g, 24, 2, 8, D)
+        for r in range(3):
+            for b, page in enumerate(group.block_table[r].tolist()):
+                if page >= 0:
+                    vs[page] = 2.0 ** max(-60, min(60, sign * (step * (b % 4) - 45)))
+        check(ops, rnd(g, 103, 4 * D, dtype=dtype), 4, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5)
+        sinks = rnd(g, 4)
+        got = attend(ops, (q := rnd(g, 103, 4 * D, dtype=dtype)), 4, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5, 20, sinks.cuda())
+        want, most = plain.attention(q, 4, 2, D, k8, v8, ks, vs, ctx, group, D ** -0.5, 20, sinks)
+        assert bool(((got - want).abs() <= room(dtype, want, most, 1 if widened(ops, dtype, D) else None)).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_portions_of_long_contexts_far_apart(ops, D):
+    """The same where the tiles of a portion are shared out over blocks and put together."""
+    g = torch.Generator().manual_seed(45)
+    new, old = [40, 5], [2000, 700]
+    pages = sum(-(-(a + b) // 16) for a, b in zip(new, old))
+    ctx, group = plain.batch(new, old, 16, pages, 0, seed=7)
+    k8, ks = pages_of(g, pages, 1, 16, D)
+    v8, vs = pages_of(g, pages, 1, 16, D)
+    vs = vs * 2.0 ** torch.randint(-9, 9, vs.shape, generator=g).float()
+    vs[::7] *= 2.0 ** -30
+    check(ops, rnd(g, 45, 4 * D, dtype=torch.bfloat16), 4, 1, D, (k8, v8, ks, vs), ctx, group, D ** -0.5)
+
+
+def test_the_same_call_gives_the_same_bits(ops):
+    g = torch.Generator().manual_seed(46)
+    for dtype in DTYPES:
+        for D in (64, 128):
+            new, old = [1] * 20 + [60, 300], [97 * i + 5 for i in range(20)] + [900, 0]
+            pages = sum(-(-(a + b) // 16) for a, b in zip(new, old))
+            ctx, group = plain.batch(new, old, 16, pages, 20, seed=8)
+            k8, ks = pages_of(g, pages, 2, 16, D)
+            v8, vs = pages_of(g, pages, 2, 16, D)
+            q = rnd(g, sum(new), 8 * D, dtype=dtype)
+            first = attend(ops, q, 8, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5)
+            for _ in range(3):
+                assert torch.equal(first, attend(ops, q, 8, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5))
