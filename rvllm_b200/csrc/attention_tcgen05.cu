@@ -19,6 +19,15 @@
 // values are the keys (a latent row): a tile is copied once and its stage is free when P V is
 // done, and the ring has three stages.
 //
+// RV_SCALED: keys and values widened from 8 bits (cache_8bit.cu), a page of 64 a tile.  Values are float16, V = q 2^(e - t + 8) with
+// the value's own exponent e (of its 8-bit page) and the tile's t, the largest of them: exact while a tile's exponents lie within 32 of
+// one another.  P = 2^(u - M) with u = s + t - 8, s a score in units of log2: the tile's power of two rides in the exponent, P is rounded
+// to float16 (2^-11 of itself, where bfloat16 would lose 2^-8) and O += P V is as large as the terms that it stands for; l adds
+// 2^(8 - t) P.  M is set 2^6 below a row's largest u and moves when that has passed it by 2^14, at both head sizes.  A tile whose
+// exponents lie further apart is marked: it holds V = 2^8 q, and its P carries each key's own exponent.  Scores past 2^24 are
+// rounded before M is taken away (by a multiply-add alone what the product's rounding left would be an exponent of its own).
+// Widened and attended, 2,048 tokens: 32 / 8 heads of 64 46.9 us (44.4 with bfloat16 values and weights), 16 / 2 heads of 128 44.0 (45.8).
+//
 // Several blocks may share the key tiles of one block of query tokens (`nsplit`): a cluster of up to four,
 // whose unnormalised rows meet in distributed shared memory, or up to 16 through memory and a merge kernel.
 //
@@ -59,10 +68,20 @@
 #ifndef RV_SAME
 #define RV_SAME 0           // 1: the values are the keys
 #endif
+#ifndef RV_SCALED
+#define RV_SCALED 0         // 1: float16 values with a power of two a tile
+#endif
+#if RV_SCALED
+#include <cuda_fp16.h>
+#define AT_SCALED(...) __VA_ARGS__
+#else
+#define AT_SCALED(...)
+#endif
 #define AT_ROWS 128
 #define AT_KEYS 64
 #define AT_STAGES (RV_SAME ? 3 : 2)
 #define AT_TILES (RV_SAME ? 1 : 2)       // tiles a stage holds: keys, values
+#define AT_EXPS 4                        // tiles whose exponents are kept
 #define AT_WAIT_CYCLES 400000000ll       // about 0.2 s: far beyond any real wait
 
 typedef __nv_bfloat16 bf16;
@@ -178,6 +197,7 @@ __device__ __forceinline__ unsigned long long at_desc(const void* tile) {
     return addr | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+template <bool B> struct AtMarked { static constexpr bool value = B; };
 #define AT_THREADS 192
 #define AT_MAX_CLUSTER 4            // blocks that share a block's key tiles and meet in distributed shared memory
 __device__ __forceinline__ void at_cluster_sync() {
@@ -229,6 +249,11 @@ struct AtShared {
     unsigned long long k_full[AT_STAGES], k_empty[AT_STAGES], v_full[AT_STAGES], v_empty[AT_STAGES];
     unsigned tmem_base;
     volatile int failed;
+#if RV_SCALED
+    // of tiles n to n + 3: the one of tile n + 4 comes behind S of tile n + 2, which comes behind the rows' reading of tile n + 1
+    volatile float exp[AT_EXPS], inv[AT_EXPS];           // t - 8 and 2^(8 - t)
+    volatile int apart[AT_EXPS];                         // marked
+#endif
 };
 static_assert(sizeof(AtShared) <= 512, "fits the larger part of the alignment's bytes");
 template <int HD>
@@ -246,7 +271,8 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
     const int* __restrict__ q_start, const int* __restrict__ ctx_lens, bf16* __restrict__ out,
     int first_req, int num_heads, int num_kv_heads, int q_block, int page_size, float scale_log2,
     int window, int* __restrict__ status, int nsplit, float* __restrict__ part_o,
-    float2* __restrict__ part_ml, const float* __restrict__ sinks) {
+    float2* __restrict__ part_ml, const float* __restrict__ sinks
+    AT_SCALED(, const int* __restrict__ tile_exps, const signed char* __restrict__ key_exps)) {
     const bool clustered = nsplit > 1 && part_o == nullptr;
     static_assert(HD == 64 || HD == 128, "128-byte swizzle rows: 64 dimensions each");
     constexpr bool SAME = RV_SAME != 0;
@@ -356,6 +382,15 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
             int page = -1;
             if (lane < ppt && blk < max_blocks && (blk << page_shift) < clen)
                 page = block_table[(size_t)r * max_blocks + blk];
+#if RV_SCALED
+            // (seen by who waits for S of this tile: written before the keys' barrier is armed)
+            if (!values && lane == 0) {
+                const int exps = blk < max_blocks ? tile_exps[((size_t)r * max_blocks + blk) * num_kv_heads + g] : 0;
+                sh.exp[n & (AT_EXPS - 1)] = (float)(short)exps;
+                sh.inv[n & (AT_EXPS - 1)] = __uint_as_float((unsigned)(127 - (int)(short)exps) << 23);
+                sh.apart[n & (AT_EXPS - 1)] = (exps >> 16) & 1;
+            }
+#endif
             const unsigned have = __ballot_sync(0xffffffffu, lane < ppt && page >= 0);
             const unsigned miss = __ballot_sync(0xffffffffu, lane < ppt && page < 0);
             if (miss) {                     // pages past the context or given back: zeros
@@ -428,11 +463,11 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
         // ---- MMA issuer: the sixth warp walks the tiles together, one lane issues ------------
         // S = Q K^T of tile n + 1 is issued as soon as every row has read S of tile n out of
         // TMEM, so it runs while the rows do their softmax; O += P V of tile n when its P is
-        // written.  instruction descriptors: D float32, A and B bfloat16; N >> 3 at bit 17,
+        // written.  instruction descriptors: D float32, A and B bfloat16 (RV_SCALED: P and V float16); N >> 3 at bit 17,
         // M >> 4 at bit 24; bit 16: B is MN-major (V lies [key][dim]).
         const unsigned idesc_qk = (1u << 4) | (1u << 7) | (1u << 10) |
                                   ((unsigned)(AT_KEYS >> 3) << 17) | ((unsigned)(AT_ROWS >> 4) << 24);
-        const unsigned idesc_pv = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+        const unsigned idesc_pv = (1u << 4) | (RV_SCALED ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) |
                                   ((unsigned)(64 >> 3) << 17) | ((unsigned)(AT_ROWS >> 4) << 24);
         bool live = true;                                   // the same in every lane
         auto wait = [&](unsigned long long* bar, unsigned parity) {
@@ -502,6 +537,20 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
         const int lo_row = window > 0 ? max(0, p_row - window + 1) : 0;
         const unsigned lane_base = ((unsigned)(warp * 32)) << 16;
         float m_run = -INFINITY, l_run = 0.f;                   // exponent offset (scaled) and sum
+#if RV_SCALED
+        // the keys' own exponents in a marked tile
+        auto own_exps = [&](int n) {
+            return key_exps + ((size_t)max(0, block_table[(size_t)r * max_blocks + t_lo + n]) * num_kv_heads + g) * AT_KEYS;
+        };
+#endif
+#if RV_SCALED
+        // (a walk of its own where a tile is marked: as a branch within the one walk it would cost every tile, 2,048 tokens 49 us)
+        bool marked = false;
+        for (int n = lane; n < n_tiles; n += 32)
+            if (t_lo + n < max_blocks) marked |= (tile_exps[((size_t)r * max_blocks + t_lo + n) * num_kv_heads + g] >> 16) & 1;
+        marked = __any_sync(0xffffffffu, marked);
+        auto walk = [&](auto marked_walk) {
+#endif
         for (int n = 0; n < n_tiles; ++n) {
             if (!at_mbar_wait(&s_bar, (unsigned)n & 1u, &failed) && !failed) {
                 failed = 1;
@@ -513,6 +562,18 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
             at_tmem_ld64(tmem_s + lane_base, sv);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             at_mbar_arrive(&s_read);                                // S may be overwritten
+#if RV_SCALED
+            const bool apart = decltype(marked_walk)::value && sh.apart[n & (AT_EXPS - 1)];
+            float mul = scale_log2;
+            if (apart) {
+                const signed char* own = own_exps(n);
+#pragma unroll
+                for (int j = 0; j < AT_KEYS; ++j) sv[j] = fmaf(sv[j], scale_log2, (float)own[j]);
+                mul = 1.f;
+            }
+#else
+            const float mul = scale_log2;
+#endif
             // masked where this tile can hold keys the row may not see (a tile wholly inside
             // every row's range needs no compare)
             const int key0 = (t_lo + n) * AT_KEYS;
@@ -531,7 +592,40 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
                 mx4[2] = fmaxf(mx4[2], sv[j + 2]);
                 mx4[3] = fmaxf(mx4[3], sv[j + 3]);
             }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
+#if RV_SCALED
+            const float most = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul, et = sh.exp[n & (AT_EXPS - 1)], mx = most + et;
+            if (__builtin_expect(__any_sync(0xffffffffu, fabsf(most) > 16777216.f && most > -INFINITY), 0)) {
+#pragma unroll
+                for (int j = 0; j < AT_KEYS; ++j) sv[j] *= mul;
+                mul = 1.f;
+            }
+            const bool moved = mx > m_run + 14.f;                       // also from -inf
+            const float m_new = moved ? mx - 6.f : m_run;
+            const float off = m_new == -INFINITY ? 0.f : m_new;
+            const float corr = moved ? at_exp2(m_run - off) : 1.f;  // m_run = -inf -> 0
+            m_run = m_new;
+            const float away = off - et;
+            float sum_apart = 0.f;
+            if (apart) {
+                const signed char* own = own_exps(n);
+#pragma unroll
+                for (int j = 0; j < AT_KEYS; ++j)
+                    sum_apart = fmaf(at_exp2(fmaf(sv[j], mul, -away)), __uint_as_float((unsigned)(127 - own[j]) << 23), sum_apart);
+            }
+            unsigned pk[AT_KEYS / 2];
+            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < AT_KEYS; j += 2) {
+                const float e0 = at_exp2(fmaf(sv[j], mul, -away));
+                const float e1 = at_exp2(fmaf(sv[j + 1], mul, -away));
+                const __half2 pr = __floats2half2_rn(e0, e1);
+                pk[j >> 1] = *(const unsigned*)&pr;
+                sum4[(j >> 1) & 3] += e0 + e1;
+            }
+            const float sum = apart ? sum_apart : (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            l_run = l_run * corr + sum * sh.inv[n & (AT_EXPS - 1)];
+#else
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mul;
             // Head size 64: the exponent's offset follows the row maximum lazily: it moves only when
             // the maximum has grown by more than 2^8 since it was set (P then stays below 256,
             // harmless in the float32 sums), so O is rescaled on few tiles.  128: it moves with the
@@ -548,8 +642,8 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < AT_KEYS; j += 2) {
-                const float e0 = at_exp2(fmaf(sv[j], scale_log2, -off));
-                const float e1 = at_exp2(fmaf(sv[j + 1], scale_log2, -off));
+                const float e0 = at_exp2(fmaf(sv[j], mul, -off));
+                const float e1 = at_exp2(fmaf(sv[j + 1], mul, -off));
                 const __nv_bfloat162 pr = __floats2bfloat162_rn(e0, e1);
                 pk[j >> 1] = *(const unsigned*)&pr;
                 if constexpr (HD == 128) {
@@ -560,6 +654,7 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
                 }
             }
             l_run = l_run * corr + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+#endif
             // the previous tile's P V must be done before O is touched and P overwritten
             if (n > 0 && !at_mbar_wait(&pv_bar, (unsigned)(n - 1) & 1u, &failed) && !failed) {
                 failed = 1;
@@ -603,6 +698,11 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             at_mbar_arrive(&p_ready);
         }
+#if RV_SCALED
+        };
+        if (marked) walk(AtMarked<true>());
+        else walk(AtMarked<false>());
+#endif
         const bool done = at_mbar_wait(&pv_bar, (unsigned)(n_tiles - 1) & 1u, &failed);
         if (__all_sync(0xffffffffu, done && !failed)) {         // one answer per warp: the reads
                                                                 // below are warp-wide
@@ -888,14 +988,19 @@ extern "C" long long AT_SYM(rv_paged_attention_prefill_tcgen05_shared_bytes)() {
 
 // Requests [first_req, first_req + n_reqs), the longest bringing max_q_len tokens and holding
 // max_ctx_len; `q` is the q|k|v buffer [n_tokens, q_stride] (the query heads first), `out` is
-// [n_tokens, heads * head size]; `scratch` (may be null: no sharing out) holds the parts.
+// [n_tokens, heads * head size]; `scratch` (may be null: no sharing out) holds the parts.  RV_SCALED: `tile_exps`
+// [requests][max_blocks][kv heads], `key_exps` [pages][kv heads][64] of marked tiles.
 extern "C" int AT_SYM(rv_paged_attention_prefill_tcgen05)(
     const void* q, int q_stride, int n_tokens, const void* k_cache, const void* v_cache,
     long long total_slots, const int* block_table, int max_blocks, const int* q_start,
     const int* ctx_lens, void* out, int first_req, int n_reqs, int max_q_len, int max_ctx_len,
     int num_heads, int num_kv_heads, int page_size, float scale, int window, int* status,
-    void* scratch, long long scratch_bytes, int n_sms, const float* sinks, void* stream) {
+    void* scratch, long long scratch_bytes, int n_sms, const float* sinks, void* stream
+    AT_SCALED(, const int* tile_exps, const signed char* key_exps)) {
     if (n_reqs == 0 || max_q_len == 0) return 0;
+#if RV_SCALED
+    if (page_size != AT_KEYS || first_req != 0) return at_fail("paged_attention_prefill_tcgen05: widened pages hold a tile each");
+#endif
     if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || n_reqs < 0)
         return at_fail("paged_attention_prefill_tcgen05: bad head counts");
     const int G = num_heads / num_kv_heads;
@@ -942,7 +1047,7 @@ extern "C" int AT_SYM(rv_paged_attention_prefill_tcgen05)(
     cudaError_t e = cudaLaunchKernelEx(&cfg, paged_attention_prefill_tcgen05_kernel<RV_HD>, map_q, map_k, map_v, block_table,
                                        max_blocks, q_start, ctx_lens, (bf16*)out, first_req, num_heads, num_kv_heads,
                                        q_block, page_size, scale * 1.4426950408889634f, window, status, parts * cluster,
-                                       cluster > 1 ? (float*)nullptr : part_o, part_ml, sinks);
+                                       cluster > 1 ? (float*)nullptr : part_o, part_ml, sinks AT_SCALED(, tile_exps, key_exps));
     if (e != cudaSuccess) return at_fail(cudaGetErrorString(e));
     if (parts > 1) {
         rv_launch(paged_attention_prefill_merge_kernel<RV_HD>,

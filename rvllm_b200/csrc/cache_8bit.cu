@@ -22,6 +22,8 @@
 // meetings of its warps) and four reads that wait for one another (slots, positions, angles and rows, scales), for as many
 // waves of blocks as there are; registers leave a multiprocessor four or five.  32 / 8 heads of 64: 64 tokens 4.1 us,
 // 2,048 tokens 11.3 us, 8,192 tokens 43 us; their bytes at a copy's bandwidth 0.1, 3.5 and 14 us.
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 
 #define C8_MAX_HEAD 256
@@ -577,19 +579,25 @@ extern "C" int rv_read_8bit(const C8ReadCall* c) {
 }
 
 // ---- contexts widened for long portions ------------------------------------------------------------
-// The keys and values that requests' portions may see, as bfloat16 pages of 64 tokens [page][64][kv heads][head size]
-// and a block table for them, as the tcgen05 attention reads them.  Its blocks of 128 rows each read a request's whole context, so that
+// The keys and values that requests' portions may see, as pages of 64 tokens [page][64][kv heads][head size] and a block
+// table for them, as the tcgen05 attention reads them: keys in bfloat16, values in float16 times a power of two of their page's
+// own (attention_tcgen05.cu, RV_SCALED, says which).  Its blocks of 128 rows each read a request's whole context, so that
 // one pass here costs less than widening the tiles in each of them (a prompt of 2,048 tokens, 32 / 8 heads of 64: 64
 // blocks a head; 68 us with the tiles widened in place by three warps a block, which they keep waiting).  Exact,
 // as scales are powers of two.
+// `tile_exps`: the powers of the pages of 64, by request and place, marked in bit 16 where the exponents of the 8-bit pages within lie more
+// than 32 apart; then `key_exps` has each key's.
 // blockIdx.x: a page of 64, y: request, z: key/value head.  Slots behind the context are zeros, keys without a page NaN.
 // Rows of a portion before position 0 are not the attention's: they are set to zero here.
 struct C8Widen {
     const signed char *k, *v;
     const float *k_scale, *v_scale;
     const int *block_table, *q_start, *ctx_lens;
-    __nv_bfloat16 *wide_k, *wide_v, *out;
-    int* wide_table;
+    __nv_bfloat16* wide_k;
+    __half* wide_v;
+    __nv_bfloat16* out;
+    int *wide_table, *tile_exps;
+    signed char* key_exps;
     long long pages;
     int max_blocks, first_req, num_heads, num_kv_heads, head_dim, page_size, window, width, room;
 };
@@ -598,10 +606,12 @@ __global__ void __launch_bounds__(256) widen_8bit_kernel(const __grid_constant__
     const int i = blockIdx.y, r = a.first_req + i, g = blockIdx.z;
     const int clen = a.ctx_lens[r], qs = a.q_start[r], qlen = a.q_start[r + 1] - qs;
     const int lo = a.window > 0 ? max(0, clen - qlen - a.window + 1) : 0, b0 = lo / 64, b = b0 + blockIdx.x;
-    if (blockIdx.x == 0 && g == 0)
-        for (int k = threadIdx.x; k < a.width; k += 256)
-            a.wide_table[(size_t)i * a.width + k] =
-                k >= b0 && k < b0 + a.room && (long long)k * 64 < clen && qlen > 0 ? i * a.room + k - b0 : -1;
+    if (blockIdx.x == 0)
+        for (int k = threadIdx.x; k < a.width; k += 256) {
+            const bool here = k >= b0 && k < b0 + a.room && (long long)k * 64 < clen && qlen > 0;
+            if (g == 0) a.wide_table[(size_t)i * a.width + k] = here ? i * a.room + k - b0 : -1;
+            if (!here) a.tile_exps[((size_t)i * a.width + k) * a.num_kv_heads + g] = 0;
+        }
     if (blockIdx.x == 0 && clen < qlen) {
         const int per = a.num_heads / a.num_kv_heads * a.head_dim, pairs = per / 2;
         for (long long k = threadIdx.x; k < (long long)(qlen - clen) * pairs; k += 256) {
@@ -610,36 +620,59 @@ __global__ void __launch_bounds__(256) widen_8bit_kernel(const __grid_constant__
         }
     }
     if ((long long)b * 64 >= clen || qlen <= 0) return;
+    __shared__ int key_page[64], key_exp[64], most[2], least[2];
+    if (threadIdx.x < 64) {
+        const int key = b * 64 + threadIdx.x, blk = key / a.page_size;
+        int page = key < clen && blk < a.max_blocks ? a.block_table[(size_t)r * a.max_blocks + blk] : -1;
+        if (page >= a.pages) page = -1;
+        const int e = page < 0 ? 0 : max(-60, min(60, (int)((__float_as_uint(a.v_scale[(size_t)page * a.num_kv_heads + g]) >> 23) & 0xff) - 127));
+        key_page[threadIdx.x] = page;
+        key_exp[threadIdx.x] = e;
+        const int hi = __reduce_max_sync(0xffffffffu, page < 0 ? -999 : e), lo = __reduce_min_sync(0xffffffffu, page < 0 ? 999 : e);
+        if ((threadIdx.x & 31) == 0) {
+            most[threadIdx.x >> 5] = hi;
+            least[threadIdx.x >> 5] = lo;
+        }
+    }
+    __syncthreads();
+    const int high = max(most[0], most[1]), spread = high - min(least[0], least[1]);
+    const bool apart = spread > 32;
+    const int tile_e = high == -999 ? 0 : high;
+    if (threadIdx.x == 0 && b < a.width)
+        a.tile_exps[((size_t)i * a.width + b) * a.num_kv_heads + g] = apart ? 0x10000 | (-8 & 0xffff) : (tile_e - 8) & 0xffff;
+    if (apart && threadIdx.x < 64)
+        a.key_exps[(((size_t)i * a.room + blockIdx.x) * a.num_kv_heads + g) * 64 + threadIdx.x] = (signed char)key_exp[threadIdx.x];
     const int pieces = a.head_dim / 16;
     for (int k = threadIdx.x; k < 64 * pieces; k += 256) {
-        const int in = k / pieces, c = k - in * pieces, key = b * 64 + in, blk = key / a.page_size;
-        const int page = key < clen && blk < a.max_blocks ? a.block_table[(size_t)r * a.max_blocks + blk] : -1;
-        const bool ok = page >= 0 && page < a.pages;
+        const int in = k / pieces, c = k - in * pieces, key = b * 64 + in, page = key_page[in];
+        const bool ok = page >= 0;
         const size_t block = ok ? (size_t)page * a.num_kv_heads + g : 0;
-        const size_t from = (block * a.page_size + (ok ? key - blk * a.page_size : 0)) * a.head_dim + 16 * c;
+        const size_t from = (block * a.page_size + (ok ? key % a.page_size : 0)) * a.head_dim + 16 * c;
         const size_t to = (((size_t)i * a.room + blockIdx.x) * 64 + in) * a.num_kv_heads * a.head_dim + (size_t)g * a.head_dim + 16 * c;
         const int4 zero = make_int4(0, 0, 0, 0);
         const int4 kr = ok ? *(const int4*)(a.k + from) : zero, vr = ok ? *(const int4*)(a.v + from) : zero;
-        const float sk = ok ? a.k_scale[block] : key < clen ? NAN : 0.f, sv = ok ? a.v_scale[block] : 0.f;
+        const float sk = ok ? a.k_scale[block] : key < clen ? NAN : 0.f, sv = c8_pow2(apart ? 8 : key_exp[in] - tile_e + 8);
         const signed char *kb = (const signed char*)&kr, *vb = (const signed char*)&vr;
 #pragma unroll
         for (int h = 0; h < 16; h += 8) {
-            float x[8], y[8];
+            float x[8];
+            __align__(16) __half2 y[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = (float)kb[h + j] * sk;
-                y[j] = (float)vb[h + j] * sv;
-            }
+            for (int j = 0; j < 8; ++j) x[j] = (float)kb[h + j] * sk;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = __floats2half2_rn((float)vb[h + 2 * j] * sv, (float)vb[h + 2 * j + 1] * sv);
             c8_store8(a.wide_k + to + h, true, x);
-            c8_store8(a.wide_v + to + h, true, y);
+            *(uint4*)(a.wide_v + to + h) = *(const uint4*)y;
         }
     }
 }
 
-// Requests [first_req, first_req + n_reqs): `room` pages of 64 for each in `wide_k` and `wide_v`, `width` entries in `wide_table`.
+// Requests [first_req, first_req + n_reqs): `room` pages of 64 for each in `wide_k`, `wide_v` and `key_exps` [page][kv heads][64], `width`
+// entries in `wide_table` and, a kv head each, in `tile_exps`.
 extern "C" int rv_widen_8bit(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, long long pages,
                              const int* block_table, int max_blocks, const int* q_start, const int* ctx_lens, void* wide_k,
-                             void* wide_v, int* wide_table, int width, int room, void* out, int first_req, int n_reqs, int num_heads,
+                             void* wide_v, int* wide_table, int* tile_exps, signed char* key_exps, int width, int room, void* out,
+                             int first_req, int n_reqs, int num_heads,
                              int num_kv_heads, int head_dim, int page_size, int window, void* stream) {
     if (n_reqs == 0) return 0;
     if (n_reqs < 0 || n_reqs > 65535 || num_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_heads % num_kv_heads ||
@@ -648,7 +681,7 @@ extern "C" int rv_widen_8bit(const void* k_cache, const void* v_cache, const flo
     if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)wide_k | (uintptr_t)wide_v) % 16)
         RV_FAIL("widen_8bit: pages must be 16-byte aligned");
     const C8Widen a = {(const signed char*)k_cache, (const signed char*)v_cache, k_scale, v_scale, block_table, q_start, ctx_lens,
-                       (__nv_bfloat16*)wide_k, (__nv_bfloat16*)wide_v, (__nv_bfloat16*)out, wide_table, pages, max_blocks, first_req,
+                       (__nv_bfloat16*)wide_k, (__half*)wide_v, (__nv_bfloat16*)out, wide_table, tile_exps, key_exps, pages, max_blocks, first_req,
                        num_heads, num_kv_heads, head_dim, page_size, window, width, room};
     rv_launch(widen_8bit_kernel, dim3(room, n_reqs, num_kv_heads), dim3(256), 0, (cudaStream_t)stream, a);
     RV_CHECK_LAUNCH("widen_8bit");

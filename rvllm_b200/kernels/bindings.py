@@ -137,7 +137,7 @@ class CudaOps:
         for fn in (self._write_8bit, self._read_8bit, self._token_logprobs):
             fn.argtypes = [ctypes.c_char_p]                  # one record (`_record`)
         self._widen_8bit = self.lib.rv_widen_8bit
-        self._widen_8bit.argtypes = [P, P, P, P, L, P, I, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P]
+        self._widen_8bit.argtypes = [P, P, P, P, L, P, I, P, P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, P]
         # the library's float32 products must be float32: no TF32, no reduced-precision accumulation
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
@@ -579,16 +579,19 @@ class CudaOps:
         """The tensor-core attention library for keys and values of this size."""
         return self._mma_lib(head_dim, head_dim, False, False)[0]
 
-    def _attn5_lib(self, head_dim: int, same: bool = False):
+    def _attn5_lib(self, head_dim: int, same: bool = False, scaled: bool = False):
         """The tcgen05 prefill attention library for this head size (`same`: the values are the
-        keys), built at first use."""
-        key = ("tcgen05", head_dim, same)
+        keys; `scaled`: pages widened from 8 bits), built at first use."""
+        key = ("tcgen05", head_dim, same, scaled)
         lib = self._attn_libs.get(key)
         if lib is None:
             defines, tag = {"RV_HD": head_dim}, f"attn5_hd{head_dim}"
             if same:
                 defines["RV_SAME"] = 1
                 tag += "s"
+            if scaled:
+                defines["RV_SCALED"] = 1
+                tag += "w"
             path = build_variant("attention_tcgen05.cu", defines, tag, verbose=self._verbose_build)
             try:
                 lib = ctypes.CDLL(path)
@@ -1101,13 +1104,17 @@ class CudaOps:
         reqs, longest, deepest = ctx.n_reqs - nd, ctx.max_q_len, ctx.max_ctx_len
         width = -(-deepest // 64)
         room = min(width, (window + longest) // 64 + 2) if window else width
+        # (keys in bfloat16, values in float16)
         wide = torch.empty((2, reqs * room * 64, num_kv_heads, head_dim), dtype=torch.bfloat16, device=device)
         wide_table = torch.empty((reqs, width), dtype=torch.int32, device=device)
+        tile_exps = torch.empty((reqs, width, num_kv_heads), dtype=torch.int32, device=device)
+        key_exps = torch.empty((reqs * room, num_kv_heads, 64), dtype=torch.int8, device=device)
         wide_at = wide.data_ptr()
         wide_v = wide_at + wide.numel()                               # half of its bytes
         self._check(self._widen_8bit(
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0), table.data_ptr(),
-            table.size(1), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), wide_at, wide_v, wide_table.data_ptr(), width, room,
+            table.size(1), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), wide_at, wide_v, wide_table.data_ptr(),
+            tile_exps.data_ptr(), key_exps.data_ptr(), width, room,
             out.data_ptr(), nd, reqs, num_heads, num_kv_heads, head_dim, page_size, window, stream), "widen_8bit")
         fn, error = self._attn5_wide(head_dim)
         # room for the parts of a short portion's blocks at the end of a long context
@@ -1117,20 +1124,21 @@ class CudaOps:
         rc = fn(q.data_ptr(), stride, q.size(0), wide_at, wide_v, reqs * room * 64, wide_table.data_ptr(), width,
                 ctx.q_start.data_ptr() + 4 * nd, ctx.ctx_lens.data_ptr() + 4 * nd, out.data_ptr(), 0, reqs, longest, deepest,
                 num_heads, num_kv_heads, 64, scale, window, self._gemm_status(device).data_ptr(),
-                None if scratch is None else scratch.data_ptr(), need, self._sm_count, sinks_at, stream)
+                None if scratch is None else scratch.data_ptr(), need, self._sm_count, sinks_at, stream, tile_exps.data_ptr(),
+                key_exps.data_ptr())
         self.launches += 1
         if rc != 0:
             raise KernelError(f"paged_attention_8bit: {error().decode()}")
 
     def _attn5_wide(self, head_dim: int):
-        """The tcgen05 attention (call, last error) with its argument types declared."""
-        key = ("tcgen05 declared", head_dim)
+        """The tcgen05 attention over widened pages (call, last error) with its argument types declared."""
+        key = ("tcgen05 widened", head_dim)
         hit = self._attn_libs.get(key)
         if hit is None:
-            lib = self._attn5_lib(head_dim)
+            lib = self._attn5_lib(head_dim, scaled=True)
             fn = lib[f"rv_paged_attention_prefill_tcgen05_hd{head_dim}"]
             P, I, L = c_void_p, c_int, c_longlong
-            fn.argtypes = [P, I, I, P, P, L, P, I, P, P, P, I, I, I, I, I, I, I, c_float, I, P, P, L, I, P, P]
+            fn.argtypes = [P, I, I, P, P, L, P, I, P, P, P, I, I, I, I, I, I, I, c_float, I, P, P, L, I, P, P, P, P]
             hit = self._attn_libs[key] = (fn, getattr(lib, f"rv_attention_tcgen05_last_error_hd{head_dim}"))
         return hit
 

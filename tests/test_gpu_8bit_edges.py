@@ -6,8 +6,8 @@ Tolerances.  The result's own rounding, `half` of itself (bfloat16 2^-8, float32
 operands of 22 bits and more, weights from exponentials of 2^-22, and both enter the products with 22 bits: 2^-20 of the largest
 value seen for each unit of the largest sum |q| |k| scale, and 8 units of them (as in `plain_8bit.attention_room`).  A weight
 below 2^-8 of the row's reference has no more than the smallest step of its second part, 2^-25, beside a largest of 2^6: 2^-31 of
-the largest term for each of `keys`, some sqrt(keys) of them together.  Portions that are widened multiply weights of bfloat16,
-half a step of which is 2^-8 of itself: as much of the largest value seen more."""
+the largest term for each of `keys`, some sqrt(keys) of them together.  Portions that are widened multiply weights of float16,
+half a step of which is 2^-11 of itself: as much of the largest value seen more."""
 import math
 
 import pytest
@@ -27,7 +27,7 @@ def room(dtype, want, most, portions_from=None):
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
     off = most[..., 0] * 2.0 ** -20 * (most[..., 1] + 8) + 2.0 ** -31 * most[..., 4] * most[..., 3]
     if portions_from is not None:
-        off[portions_from:] += most[portions_from:, :, 0] * 2.0 ** -8
+        off[portions_from:] += most[portions_from:, :, 0] * 2.0 ** -11
     return half * want.abs() + off.repeat_interleave(want.shape[1] // most.shape[1], 1) + 1e-30
 
 
@@ -85,8 +85,6 @@ def test_large_queries_over_small_keys(ops, dtype, power):
     2^13 and more, of which one is the largest by far.  A score is off by 2^-20 of S, the largest sum |q| |k| scale, at most: where
     the next one is 2^-18 S + 40 behind, each other key weighs e^-39 of the largest at most (which may be lost, being below 2^-31), and the
     result is the largest one's value but for its rounding; where it is nearer, `room` holds."""
-    if widened(ops, dtype, 64):
-        ops.prefill_8bit = "rows"
     g = torch.Generator().manual_seed(41)
     ctx, group = plain.batch([1, 1, 20], [70, 3, 0], 16, 12, 2)
     k8, _ = pages_of(g, 12, 2, 16, 64)
