@@ -582,7 +582,7 @@ class CudaOps:
     def _attn5_lib(self, head_dim: int, same: bool = False, scaled: bool = False):
         """The tcgen05 prefill attention library for this head size (`same`: the values are the
         keys; `scaled`: pages widened from 8 bits), built at first use."""
-        key = ("tcgen05", head_dim, same, scaled)
+        key = ("tcgen05", head_dim, same) + (("widened",) if scaled else ())
         lib = self._attn_libs.get(key)
         if lib is None:
             defines, tag = {"RV_HD": head_dim}, f"attn5_hd{head_dim}"
