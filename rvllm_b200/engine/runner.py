@@ -244,7 +244,7 @@ class ModelRunner:
             g.graph = None
             self.capture_failures += 1
             import warnings
-            warnings.warn(f"capturing a graph for steps padded to {T} tokens failed ({e}); "
+            warnings.warn(f"capturing a graph for steps padded to {key[2]} tokens failed ({e}); "
                           f"running such steps without it")
             return None
         self.graph_steps += 1

@@ -1,0 +1,59 @@
+"""What the step function does when a launch sequence cannot be captured, on the host: the graphs are stand-ins."""
+import pytest
+import torch
+
+from plain_ops import PlainOps
+from rvllm_b200.engine import ModelRunner, StepEntry, load_model, make_cache
+from rvllm_b200.engine import runner as runner_module
+from tiny import write_tiny
+
+
+@pytest.fixture(scope="module")
+def model(tmp_path_factory):
+    return load_model(write_tiny(str(tmp_path_factory.mktemp("models")), "A"), "float32", "cpu", PlainOps())[0]
+
+
+def portions(runner, lengths, start=0):
+    """Logits of the last token of a request of each length, one step."""
+    ids = [f"{start}-{i}" for i in range(len(lengths))]
+    for r in ids:
+        runner.add_request(r)
+    out = runner.step([StepEntry(r, [(7 * j + 3 * i) % 500 for j in range(n)], (n - 1,)) for i, (r, n) in enumerate(zip(ids, lengths))])
+    for r in ids:
+        runner.end_request(r)
+    return out
+
+
+@pytest.mark.parametrize("kind", ["_MixedGraph", "_ShapeGraph"])
+def test_a_capture_that_fails_leaves_the_step_to_its_launches(model, monkeypatch, kind):
+    """A capture that ends in an error (no memory, a call that cannot be captured) costs a warning; this step and later ones of its
+    sizes run without it."""
+    tried = []
+
+    class Fails:
+        graph, broken, capturing, last_used = None, False, False, 0
+
+        def __init__(self, runner, *key):
+            pass
+
+        def run(self, entries, row_order=None):
+            tried.append(len(entries))
+            self.capturing = True
+            raise torch.cuda.OutOfMemoryError("no memory left")
+
+    monkeypatch.setattr(runner_module, kind, Fails)
+    cache = lambda: make_cache(model, 8, 32, 3)  # noqa: E731
+    runner, plain = ModelRunner(model, cache(), model.ops), ModelRunner(model, cache(), model.ops)
+    runner.use_graphs = True
+    if kind == "_ShapeGraph":
+        runner.max_mixed_graphs = -1
+    for k in range(4):
+        lengths = (9, 14)
+        if k == 1:                                     # the second step of these sizes
+            with pytest.warns(UserWarning, match="capturing a graph"):
+                got = portions(runner, lengths, k)
+        else:
+            got = portions(runner, lengths, k)
+        assert torch.allclose(got, portions(plain, lengths, k), atol=1e-5)
+    assert tried == [2] and runner.capture_failures == 1 and runner.graph_steps == 0
+    runner.cache.check()
