@@ -105,10 +105,12 @@ class ModelRunner:
 
     # ---- the step ----------------------------------------------------------------
 
-    def step(self, entries: Sequence[StepEntry], device_tokens=None) -> torch.Tensor:
+    def step(self, entries: Sequence[StepEntry], device_tokens=None, replayed: bool = True) -> torch.Tensor:
         """float32 logits [wanted, vocab], in the order of the entries and of `want`.
         With `device_tokens` (int32 device tensor, one id per entry) every entry brings one
-        token whose id is taken from that tensor instead of `entry.tokens`."""
+        token whose id is taken from that tensor instead of `entry.tokens`.  `replayed` False: the step is
+        launched kernel by kernel and counts towards no capture, whose logits stay allocated (for steps that
+        want the logits of every token)."""
         if not entries:
             return torch.empty((0, self.model.spec.vocab_size), dtype=torch.float32,
                                device=self.device)
@@ -139,18 +141,19 @@ class ModelRunner:
         elif order != list(range(len(entries))):
             # the wanted rows come out in the callers' order: the row list is written that way
             where = {oi: k for k, oi in enumerate(order)}
-            logits = self._run(ordered, row_order=[where[i] for i in range(len(entries))])
+            logits = self._run(ordered, row_order=[where[i] for i in range(len(entries))], replayed=replayed)
         else:
-            logits = self._run(ordered)
+            logits = self._run(ordered, replayed=replayed)
         for e, total in zip(entries, totals):
             self.cache.advance(e.req, total)
         self.steps += 1
         return logits
 
-    def _run(self, ordered: List[StepEntry], device_tokens=None, row_order=None) -> torch.Tensor:
-        if self.use_graphs and all(len(e.tokens) == 1 for e in ordered):
+    def _run(self, ordered: List[StepEntry], device_tokens=None, row_order=None, replayed: bool = True) -> torch.Tensor:
+        replayed = replayed and self.use_graphs
+        if replayed and all(len(e.tokens) == 1 for e in ordered):
             return self._run_graph(ordered, device_tokens)
-        if self.use_graphs and device_tokens is None:
+        if replayed and device_tokens is None:
             logits = self._run_padded_mixture(ordered, row_order)
             if logits is None:
                 logits = self._run_repeated_shape(ordered, row_order)

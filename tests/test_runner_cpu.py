@@ -3,14 +3,21 @@ import pytest
 import torch
 
 from plain_ops import PlainOps
+from rvllm_b200 import GenerateOptions
 from rvllm_b200.engine import ModelRunner, StepEntry, load_model, make_cache
 from rvllm_b200.engine import runner as runner_module
+from test_8bit_engine_cpu import generator
 from tiny import write_tiny
 
 
 @pytest.fixture(scope="module")
-def model(tmp_path_factory):
-    return load_model(write_tiny(str(tmp_path_factory.mktemp("models")), "A"), "float32", "cpu", PlainOps())[0]
+def folder(tmp_path_factory):
+    return write_tiny(str(tmp_path_factory.mktemp("models")), "A")
+
+
+@pytest.fixture
+def model(folder):
+    return load_model(folder, "float32", "cpu", PlainOps())[0]
 
 
 def portions(runner, lengths, start=0):
@@ -57,3 +64,20 @@ def test_a_capture_that_fails_leaves_the_step_to_its_launches(model, monkeypatch
         assert torch.allclose(got, portions(plain, lengths, k), atol=1e-5)
     assert tried == [2] and runner.capture_failures == 1 and runner.graph_steps == 0
     runner.cache.check()
+
+
+def test_scoring_captures_nothing(folder, monkeypatch):
+    """Scoring wants a row of logits for every token: a launch sequence that kept them would hold them for good, one for every
+    length of a text's last portion."""
+    gen = generator(folder)
+    ids = [(29 * i + 3) % 500 for i in range(40)]
+    first = gen.score(ids, portion=13)
+    for kind in ("_DecodeGraph", "_MixedGraph", "_ShapeGraph"):
+        monkeypatch.setattr(runner_module, kind, lambda *a: pytest.fail("a capture"))
+    gen._runner.use_graphs = True
+    for _ in range(3):
+        assert gen.score(ids, portion=13) == first
+    assert not gen._runner._seen_shapes and not gen._runner._shape_graphs
+    gen._runner.use_graphs = False
+    assert gen.generate_ids([ids], GenerateOptions(max_tokens=2, stop_tokens=[])).outputs[0]
+
