@@ -9,7 +9,7 @@ import torch
 
 from ..cache import CacheManager
 from ..config.registry import architecture, load_config
-from ..parts.base import StateNeed, arrangement_class, mixer_class
+from ..parts.base import PagedNeed, SeveralNeeds, arrangement_class, mixer_class
 from ..parts.model import Model
 from ..weights.loader import load_tensors, tensor_shapes
 
@@ -58,6 +58,12 @@ def parse_kv_cache(name):
     return KV_CACHES[name]
 
 
+def _holds_pages(need) -> bool:
+    if isinstance(need, SeveralNeeds):
+        return any(_holds_pages(part) for part in need.parts)
+    return isinstance(need, PagedNeed)
+
+
 def make_cache(model: Model, page_size: int, num_pages: int, max_requests: int,
                kv_cache="auto") -> CacheManager:
     """`kv_cache` "int8": keys and values in 8 bits with a scale per page and head, for models whose
@@ -67,8 +73,7 @@ def make_cache(model: Model, page_size: int, num_pages: int, max_requests: int,
         for call in model.spec.order:
             block = model.spec.layers[call.layer]
             need = arrangement_class(block.arrangement).cache_need(block)
-            if need is not None and not isinstance(need, StateNeed) and \
-                    not mixer_class(block.mixer.kind).eight_bit_cache(block.mixer):
+            if _holds_pages(need) and not mixer_class(block.mixer.kind).eight_bit_cache(block.mixer):
                 raise ValueError(f"a layer of kind {block.mixer.kind!r} as this model has it does not read "
                                  f"keys and values in 8 bits")
     return CacheManager(needs, [c.cache_of for c in model.spec.order],
