@@ -82,7 +82,7 @@ class CudaOps:
         self.decode_8bit = os.environ.get("RVLLM_DECODE_8BIT", "auto")
         # portions over 8-bit pages: "rows" = mma.sync from the pages, any head size and type; "tcgen05" = bfloat16
         # pages for the step, then the tcgen05 kernel (bfloat16, head sizes 64 and 128); "auto" = the faster one,
-        # while those pages take no more than `widen_8bit_bytes`
+        # while those pages take no more than `widen_8bit_bytes` and `prefill_attention` keeps no prompt off that kernel
         self.widen_8bit_bytes = 1 << 30
         self.prefill_8bit = os.environ.get("RVLLM_PREFILL_8BIT", "auto")
         # keys per block of the tensor-core decode kernel: 256 (four warps) or 128 (two)
@@ -1060,13 +1060,13 @@ class CudaOps:
             if sinks.shape != (num_heads,):
                 self._fault(what, "one sink per query head")
             sinks_at = sinks.data_ptr()
+        form = self._FORMS_8BIT[self.decode_8bit]
         call, scratch_bytes, error = self._attn8_lib(head_dim)
         portions = n_tokens > n_decode
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
         stream = self._raw_stream(here)
         tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window)
         if n_decode or not tcgen05:
-            form = self._FORMS_8BIT[self.decode_8bit]
             need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms, form)
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
             rc = call(_ATTEND_8BIT.pack(
@@ -1084,7 +1084,8 @@ class CudaOps:
     def _tcgen05_8bit(self, q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window) -> bool:
         """Whether portions are widened to bfloat16 and go to the tcgen05 kernel."""
         group, reqs, longest = num_heads // num_kv_heads, ctx.n_reqs - ctx.n_decode, ctx.max_q_len
-        if (self.prefill_8bit == "rows" or code != _BF16 or head_dim not in (64, 128) or group > 128 or stride % head_dim
+        if (self.prefill_8bit == "rows" or (self.prefill_8bit == "auto" and self.prefill_attention not in ("auto", "tcgen05"))
+                or code != _BF16 or head_dim not in (64, 128) or group > 128 or stride % head_dim
                 or (q.data_ptr() | out.data_ptr()) % 16 or reqs > 4095 or longest > 65535 * (128 // group)):
             return False
         keys = min(ctx.max_ctx_len, window + longest) if window else ctx.max_ctx_len
