@@ -1060,7 +1060,10 @@ class CudaOps:
             if sinks.shape != (num_heads,):
                 self._fault(what, "one sink per query head")
             sinks_at = sinks.data_ptr()
-        form = self._FORMS_8BIT[self.decode_8bit]
+        form = self._FORMS_8BIT.get(self.decode_8bit)
+        if form is None or self.prefill_8bit not in ("auto", "rows", "tcgen05"):
+            self._fault(what, f"unknown forms: {self.decode_8bit!r} for single tokens (auto, stream, blocks), "
+                              f"{self.prefill_8bit!r} for portions (auto, rows, tcgen05)")
         call, scratch_bytes, error = self._attn8_lib(head_dim)
         portions = n_tokens > n_decode
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count

@@ -27,3 +27,11 @@ def test_the_switch_of_prompt_attention_holds_here_too(ops, switch):  # noqa: F8
     assert portions(ops) == 3
     ops.prefill_attention, ops.prefill_8bit = "tcgen05", "rows"
     assert portions(ops) == 1
+
+
+@pytest.mark.parametrize("name", ["decode_8bit", "prefill_8bit"])
+def test_unknown_forms_are_refused(ops, name):  # noqa: F811
+    setattr(ops, name, "fast")
+    with pytest.raises(KernelError, match="paged_attention_8bit: .*fast"):
+        portions(ops)
+    assert not ops.calls
