@@ -63,6 +63,9 @@ class StepContext:
     ctx_lens_host: List[int] = field(default_factory=list)
     max_q_len: int = 0
     max_ctx_len: int = 0
+    # of a step padded to sizes that come again: tokens of the portions, portions and deepest context that such steps have, about.
+    # What follows `max_q_len` and `max_ctx_len` covers every step of these sizes; a choice between kernels may follow this
+    likely: Optional[tuple] = None
     n_wanted: int = 0               # logit rows that were asked for (the first ones)
     # what one call of the run order leaves for later calls of the same step (by name)
     carry: dict = field(default_factory=dict)

@@ -262,7 +262,16 @@ class ModelRunner:
                                  pad_mixed=(D, P, T, D + P))
         ctx.max_ctx_len = deepest
         ctx.max_q_len = longest
+        ctx.likely = self._likely(key)
         return self.model.forward(ctx, self.cache.views())[:ctx.n_wanted]
+
+    def _likely(self, key) -> tuple:
+        """`StepContext.likely` of the steps that `_mixture_sizes` pads to `key` (sizes alone say it, so that a step takes the
+        same kernels whether it is replayed or not): all tokens, of which few are padding, and the middle of the portions and of the
+        depths that it may have."""
+        D, P, T, block_bucket, _, deepest = key
+        depth = block_bucket * self.cache.page_size * 3 // 4
+        return max(1, T - D), (P + P // 2 - 1) // 2, max(1, min(depth, deepest))
 
     def _run_repeated_shape(self, ordered: List[StepEntry], row_order=None) -> Optional[torch.Tensor]:
         """Steps with prompt portions: the second time the same shape comes (the same token
@@ -492,6 +501,7 @@ class _MixedGraph:
     def __init__(self, runner: ModelRunner, key):
         self.runner = weakref.proxy(runner)     # no cycle: graphs die with their runner
         self.D, self.P, self.T, self.block_bucket, self.longest, self.deepest = key
+        self.likely = runner._likely(key)
         self.last_used = 0
         R, W = self.D + self.P, self.D + self.P
         n_groups = len(runner.cache.groups)
@@ -511,6 +521,7 @@ class _MixedGraph:
                                    pad_mixed=(self.D, self.P, self.T, self.D + self.P))
         ctx.max_ctx_len = self.deepest
         ctx.max_q_len = self.longest
+        ctx.likely = self.likely
         return ctx
 
     def run(self, entries, row_order=None) -> torch.Tensor:

@@ -1065,17 +1065,20 @@ class CudaOps:
             self._fault(what, f"unknown forms: {self.decode_8bit!r} for single tokens (auto, stream, blocks), "
                               f"{self.prefill_8bit!r} for portions (auto, rows, tcgen05)")
         call, scratch_bytes, error = self._attn8_lib(head_dim)
+        # about how many tokens the portions bring, how many portions, how deep: as a padded step has them
+        likely = getattr(ctx, "likely", None) or (n_tokens - n_decode, n_reqs - n_decode, ctx.max_ctx_len)
         portions = n_tokens > n_decode
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
         stream = self._raw_stream(here)
-        tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window)
+        tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window, likely)
         if n_decode or not tcgen05:
             need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms, form)
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
             rc = call(_ATTEND_8BIT.pack(
                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr(),
                 q_start.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
-                sinks_at or 0, stream, code, stride, pages, table.size(1), need, n_decode, n_reqs, portions and not tcgen05,
+                sinks_at or 0, stream, code, stride, pages, table.size(1), need, n_decode, n_reqs,
+                likely[0] | likely[2] << 32 if portions and not tcgen05 else 0,
                 longest, deepest, num_heads, num_kv_heads, page_size, window, sms, form, scale))
             self.launches += (n_decode > 0) + (need > 0) + (portions and not tcgen05)
             if rc != 0:
@@ -1084,8 +1087,8 @@ class CudaOps:
             self._attend_widened(q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
                                  page_size, scale, window, out, sinks_at, stream)
 
-    def _tcgen05_8bit(self, q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window) -> bool:
-        """Whether portions are widened to bfloat16 and go to the tcgen05 kernel."""
+    def _tcgen05_8bit(self, q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window, likely) -> bool:
+        """Whether portions are widened and go to the tcgen05 kernel."""
         group, reqs, longest = num_heads // num_kv_heads, ctx.n_reqs - ctx.n_decode, ctx.max_q_len
         if (self.prefill_8bit == "rows" or (self.prefill_8bit == "auto" and self.prefill_attention not in ("auto", "tcgen05"))
                 or code != _BF16 or head_dim not in (64, 128) or group > 128 or stride % head_dim
@@ -1094,11 +1097,14 @@ class CudaOps:
         keys = min(ctx.max_ctx_len, window + longest) if window else ctx.max_ctx_len
         if 4 * reqs * keys * num_kv_heads * head_dim > self.widen_8bit_bytes:
             return False
-        # tiles of 16 rows and 32 keys, of 64 dimensions.  us by mma.sync from the pages / widened: 32 / 8 heads of 64, 64 tokens
-        # after 1,000 (4,352 tiles) 12 / 18, 16 x 20 after 500 (10,880) 22.5 / 23, 512 (16,384) 23 / 16.5, 2,048 135 / 45; 16 / 8
-        # heads 16 x 20 after 500 (6,528) 14.5 / 23, 64 after 16,000 (32,128) 39 / 37; 16 / 2 heads of 128 16 x 20 after 500
-        # (10,880) 26 / 23, 2,048 91 / 50; 8 / 8 heads of 128 512 (8,192) 14.5 / 16.5
-        tiles = -(-longest * group // 16) * -(-keys // 32) * reqs * num_kv_heads * (head_dim // 64)
+        # tiles of 16 rows and 32 keys, of 64 dimensions, that are there (a padded step's longest portion, requests and context are
+        # up to twice what it has each).  us by mma.sync from the pages / widened: 32 / 8 heads of 64, 64 tokens after 1,000 (4,352
+        # tiles) 14.5 / 17, 16 x 20 after 500 (10,880) 23 / 22, 512 (16,384) 24 / 16, 64 after 4,000 (16,256) 33 / 22; 16 / 8 heads
+        # 16 x 20 after 500 (6,528) 14 / 22, 64 after 16,000 (32,128) 57 / 36; 16 / 2 heads of 128 16 x 20 after 500 (10,880) 26 / 21,
+        # 64 after 1,000 (4,352) 13 / 20; 8 / 8 heads of 128 512 (8,192) 14.5 / 16.5
+        tokens, few, depth = likely
+        seen = min(depth, window + longest) if window else depth
+        tiles = (-(-tokens * group // 16) + few // 2) * -(-seen // 32) * num_kv_heads * (head_dim // 64)
         return self.prefill_8bit == "tcgen05" or tiles > 10000
 
     def _attend_widened(self, q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,

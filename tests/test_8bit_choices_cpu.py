@@ -35,3 +35,49 @@ def test_unknown_forms_are_refused(ops, name):  # noqa: F811
     with pytest.raises(KernelError, match="paged_attention_8bit: .*fast"):
         portions(ops)
     assert not ops.calls
+
+
+class Pool:
+    """A cache manager's live requests, as far as padding asks."""
+
+    def __init__(self, page_size, computed):
+        self.page_size = page_size
+        self.requests = {r: SimpleNamespace(computed=n) for r, n in enumerate(computed)}
+
+
+def engine_step(ops, new, old, page_size=16, H=32, K=8, D=64, dtype=BF16):  # noqa: F811
+    """The attention call of a step of portions `new` after `old` tokens, padded as `ModelRunner` pads it: whether it is widened."""
+    from rvllm_b200.engine import ModelRunner, StepEntry
+    runner = object.__new__(ModelRunner)
+    runner.cache, runner._portion_limits, runner._shallow = Pool(page_size, old), None, 0
+    entries = sorted((StepEntry(r, range(n), (n - 1,)) for r, n in enumerate(new)), key=lambda e: len(e.tokens) != 1)
+    key = runner._mixture_sizes(entries)
+    singles, reqs, tokens, width, longest, deepest = key
+    ops.calls.clear()
+    ops.paged_attention_8bit(**attend_args(
+        dict(q=there(tokens, H * D, dtype=dtype), out=there(tokens, H * D, dtype=dtype), num_heads=H, num_kv_heads=K, head_dim=D,
+             k_cache=there(7, K, page_size, D, dtype=I8), v_cache=there(7, K, page_size, D, dtype=I8), k_scale=there(7, K), v_scale=there(7, K)),
+        dict(n_reqs=singles + reqs, n_tokens=tokens, n_decode=singles, q_start=there(singles + reqs + 1, dtype=I32),
+             ctx_lens=there(singles + reqs, dtype=I32), max_q_len=longest, max_ctx_len=deepest, likely=runner._likely(key)),
+        dict(block_table=there(singles + reqs, width, dtype=I32), page_size=page_size)))
+    return any(len(c) > 20 for c in ops.calls)         # (the record of the other kernel is one argument)
+
+
+@pytest.mark.parametrize("new,old,H,K,D,widened", [
+    ([64], [1000], 32, 8, 64, False), ([60], [900], 32, 8, 64, False), ([16], [500], 32, 8, 64, False), ([64], [0], 32, 8, 64, False),
+    ([20] * 3, [900] * 3, 16, 8, 64, False), ([10] * 16, [100] * 16, 32, 8, 64, False), ([64] + [1] * 31, [1000] * 32, 32, 8, 64, False),
+    ([100], [400], 16, 2, 128, False), ([512], [0], 32, 8, 64, True), ([2048], [0], 32, 8, 64, True), ([64], [4000], 32, 8, 64, True),
+    ([512] * 4, [1000] * 4, 32, 8, 64, True), ([500] + [1] * 31, [2000] * 32, 32, 8, 64, True), ([256], [1000], 16, 2, 128, True)])
+def test_padded_steps_choose_by_what_is_there(ops, new, old, H, K, D, widened):  # noqa: F811
+    """An engine's step counts an empty portion more, all tokens as one portion and the next power of two of pages; the choice
+    follows what a step of these sizes has, not what its launches have to cover."""
+    assert engine_step(ops, new, old, H=H, K=K, D=D) == widened
+
+
+def test_sizes_alone_say_what_is_likely():
+    from rvllm_b200.engine import ModelRunner
+    runner = object.__new__(ModelRunner)
+    runner.cache = Pool(16, [])
+    assert runner._likely((0, 2, 64, 128, 64, 2048)) == (64, 1, 1536)
+    assert runner._likely((32, 4, 2048, 16, 2016, 64)) == (2016, 2, 64)
+    assert runner._likely((64, 2, 64, 16, 1, 256)) == (1, 1, 192)
