@@ -81,8 +81,8 @@ class CudaOps:
         # that have a request's heads each, "auto" = the faster one
         self.decode_8bit = os.environ.get("RVLLM_DECODE_8BIT", "auto")
         # portions over 8-bit pages: "rows" = mma.sync from the pages, any head size and type; "tcgen05" = bfloat16
-        # pages for the step, then the tcgen05 kernel (bfloat16, head sizes 64 and 128); "auto" = the faster one,
-        # while those pages take no more than `widen_8bit_bytes` and `prefill_attention` keeps no prompt off that kernel
+        # pages for the call, then the tcgen05 kernel (bfloat16, head sizes 64 and 128), as many portions at a time as
+        # `widen_8bit_bytes` hold; "auto" = the faster one, while one portion's pages take no more and `prefill_attention` keeps no prompt off that kernel
         self.widen_8bit_bytes = 1 << 30
         self.prefill_8bit = os.environ.get("RVLLM_PREFILL_8BIT", "auto")
         # keys per block of the tensor-core decode kernel: 256 (four warps) or 128 (two)
@@ -1019,7 +1019,8 @@ class CudaOps:
         whose block-table entry is no page, or a request whose context is longer than its row of the table, has no valid
         result (nothing outside the pages is read).  `ctx.max_q_len` and `ctx.max_ctx_len` are bounds over all requests: the
         forms and the launches' sizes follow them.  Scratch is allocated per call (in a captured graph: from the graph's
-        pool); long bfloat16 portions (heads of 64 or 128) take bfloat16 copies of what they may see for the call's duration."""
+        pool); long bfloat16 portions (heads of 64 or 128) take 16-bit copies of what they may see for the call's duration, up to
+        `widen_8bit_bytes` and, where there is no memory for these, none."""
         what = "paged_attention_8bit"
         dtype, here = q.dtype, self._here()
         code = _code(dtype)
@@ -1071,6 +1072,8 @@ class CudaOps:
         longest, deepest, sms = ctx.max_q_len, ctx.max_ctx_len, self._sm_count
         stream = self._raw_stream(here)
         tcgen05 = portions and self._tcgen05_8bit(q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window, likely)
+        wide_pages = self._wide_pages(ctx, window, num_kv_heads, head_dim, q.device) if tcgen05 else None
+        tcgen05 = wide_pages is not None               # (without memory for them the other kernel reads the pages as they are)
         if n_decode or not tcgen05:
             need = scratch_bytes(n_decode, deepest, num_heads, num_kv_heads, window, sms, form)
             scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
@@ -1085,17 +1088,16 @@ class CudaOps:
                 raise KernelError(error().decode())
         if tcgen05:
             self._attend_widened(q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
-                                 page_size, scale, window, out, sinks_at, stream)
+                                 page_size, scale, window, out, sinks_at, stream, wide_pages)
 
     def _tcgen05_8bit(self, q, stride, out, code, num_heads, num_kv_heads, head_dim, ctx, window, likely) -> bool:
         """Whether portions are widened and go to the tcgen05 kernel."""
         group, reqs, longest = num_heads // num_kv_heads, ctx.n_reqs - ctx.n_decode, ctx.max_q_len
         if (self.prefill_8bit == "rows" or (self.prefill_8bit == "auto" and self.prefill_attention not in ("auto", "tcgen05"))
                 or code != _BF16 or head_dim not in (64, 128) or group > 128 or stride % head_dim
-                or (q.data_ptr() | out.data_ptr()) % 16 or reqs > 4095 or longest > 65535 * (128 // group)):
+                or (q.data_ptr() | out.data_ptr()) % 16 or not 0 < reqs <= 4095 or longest > 65535 * (128 // group)):
             return False
-        keys = min(ctx.max_ctx_len, window + longest) if window else ctx.max_ctx_len
-        if 4 * reqs * keys * num_kv_heads * head_dim > self.widen_8bit_bytes:
+        if not 0 < self._wide_bytes(ctx, window, num_kv_heads, head_dim) <= self.widen_8bit_bytes:
             return False
         # tiles of 16 rows and 32 keys, of 64 dimensions, that are there (a padded step's longest portion, requests and context are
         # up to twice what it has each).  us by mma.sync from the pages / widened: 32 / 8 heads of 64, 64 tokens after 1,000 (4,352
@@ -1107,38 +1109,55 @@ class CudaOps:
         tiles = (-(-tokens * group // 16) + few // 2) * -(-seen // 32) * num_kv_heads * (head_dim // 64)
         return self.prefill_8bit == "tcgen05" or tiles > 10000
 
-    def _attend_widened(self, q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
-                        page_size, scale, window, out, sinks_at, stream):
-        """Portions: what they may see of their contexts as bfloat16 pages, then the tcgen05 attention over those."""
-        nd, device = ctx.n_decode, q.device
-        reqs, longest, deepest = ctx.n_reqs - nd, ctx.max_q_len, ctx.max_ctx_len
+    def _wide_bytes(self, ctx, window, num_kv_heads, head_dim) -> int:
+        """What one portion's keys and values take in 16 bits."""
+        longest, deepest = ctx.max_q_len, ctx.max_ctx_len
+        return 4 * (min(deepest, window + longest) if window else deepest) * num_kv_heads * head_dim
+
+    def _wide_pages(self, ctx, window, num_kv_heads, head_dim, device):
+        """Room for what portions may see: for as many at a time as `widen_8bit_bytes` allow.  (portions, pages of 64 a portion, width of
+        their table, keys in bfloat16 and values in float16, the table, the exponents of the tiles, of the keys), or None where there
+        is no memory for it."""
+        reqs, longest, deepest = ctx.n_reqs - ctx.n_decode, ctx.max_q_len, ctx.max_ctx_len
+        reqs = min(reqs, max(1, self.widen_8bit_bytes // self._wide_bytes(ctx, window, num_kv_heads, head_dim)))
         width = -(-deepest // 64)
         room = min(width, (window + longest) // 64 + 2) if window else width
-        # (keys in bfloat16, values in float16)
-        wide = torch.empty((2, reqs * room * 64, num_kv_heads, head_dim), dtype=torch.bfloat16, device=device)
-        wide_table = torch.empty((reqs, width), dtype=torch.int32, device=device)
-        tile_exps = torch.empty((reqs, width, num_kv_heads), dtype=torch.int32, device=device)
-        key_exps = torch.empty((reqs * room, num_kv_heads, 64), dtype=torch.int8, device=device)
+        try:
+            wide = torch.empty((2, reqs * room * 64, num_kv_heads, head_dim), dtype=torch.bfloat16, device=device)
+            return (reqs, room, width, wide, torch.empty((reqs, width), dtype=torch.int32, device=device),
+                    torch.empty((reqs, width, num_kv_heads), dtype=torch.int32, device=device),
+                    torch.empty((reqs * room, num_kv_heads, 64), dtype=torch.int8, device=device))
+        except torch.cuda.OutOfMemoryError:
+            return None
+
+    def _attend_widened(self, q, stride, num_heads, num_kv_heads, head_dim, k_cache, v_cache, k_scale, v_scale, ctx, table,
+                        page_size, scale, window, out, sinks_at, stream, wide_pages):
+        """Portions: what they may see of their contexts as pages of 16 bits, then the tcgen05 attention over those."""
+        device = q.device
+        longest, deepest = ctx.max_q_len, ctx.max_ctx_len
+        at_once, room, width, wide, wide_table, tile_exps, key_exps = wide_pages
         wide_at = wide.data_ptr()
         wide_v = wide_at + wide.numel()                               # half of its bytes
-        self._check(self._widen_8bit(
-            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0), table.data_ptr(),
-            table.size(1), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), wide_at, wide_v, wide_table.data_ptr(),
-            tile_exps.data_ptr(), key_exps.data_ptr(), width, room,
-            out.data_ptr(), nd, reqs, num_heads, num_kv_heads, head_dim, page_size, window, stream), "widen_8bit")
         fn, error = self._attn5_wide(head_dim)
         # room for the parts of a short portion's blocks at the end of a long context
         need = self._prefill_scratch_bytes(head_dim) if deepest - longest >= 512 else 0
         scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        # (the attention's requests are counted from the first portion: its arrays begin there)
-        rc = fn(q.data_ptr(), stride, q.size(0), wide_at, wide_v, reqs * room * 64, wide_table.data_ptr(), width,
-                ctx.q_start.data_ptr() + 4 * nd, ctx.ctx_lens.data_ptr() + 4 * nd, out.data_ptr(), 0, reqs, longest, deepest,
-                num_heads, num_kv_heads, 64, scale, window, self._gemm_status(device).data_ptr(),
-                None if scratch is None else scratch.data_ptr(), need, self._sm_count, sinks_at, stream, tile_exps.data_ptr(),
-                key_exps.data_ptr())
-        self.launches += 1
-        if rc != 0:
-            raise KernelError(f"paged_attention_8bit: {error().decode()}")
+        for first in range(ctx.n_decode, ctx.n_reqs, at_once):
+            reqs = min(at_once, ctx.n_reqs - first)
+            self._check(self._widen_8bit(
+                k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.size(0), table.data_ptr(),
+                table.size(1), ctx.q_start.data_ptr(), ctx.ctx_lens.data_ptr(), wide_at, wide_v, wide_table.data_ptr(),
+                tile_exps.data_ptr(), key_exps.data_ptr(), width, room,
+                out.data_ptr(), first, reqs, num_heads, num_kv_heads, head_dim, page_size, window, stream), "widen_8bit")
+            # (the attention's requests are counted from the first one widened: its arrays begin there)
+            rc = fn(q.data_ptr(), stride, q.size(0), wide_at, wide_v, reqs * room * 64, wide_table.data_ptr(), width,
+                    ctx.q_start.data_ptr() + 4 * first, ctx.ctx_lens.data_ptr() + 4 * first, out.data_ptr(), 0, reqs, longest, deepest,
+                    num_heads, num_kv_heads, 64, scale, window, self._gemm_status(device).data_ptr(),
+                    None if scratch is None else scratch.data_ptr(), need, self._sm_count, sinks_at, stream, tile_exps.data_ptr(),
+                    key_exps.data_ptr())
+            self.launches += 1
+            if rc != 0:
+                raise KernelError(f"paged_attention_8bit: {error().decode()}")
 
     def _attn5_wide(self, head_dim: int):
         """The tcgen05 attention over widened pages (call, last error) with its argument types declared."""

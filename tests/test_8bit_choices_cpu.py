@@ -81,3 +81,45 @@ def test_sizes_alone_say_what_is_likely():
     assert runner._likely((0, 2, 64, 128, 64, 2048)) == (64, 1, 1536)
     assert runner._likely((32, 4, 2048, 16, 2016, 64)) == (2016, 2, 64)
     assert runner._likely((64, 2, 64, 16, 1, 256)) == (1, 1, 192)
+
+
+def test_portions_are_widened_as_many_at_a_time_as_may_be(ops):  # noqa: F811
+    """Many portions of long contexts need not all be widened at once: each pass has those that the limit holds, and names the requests,
+    lengths and first tokens that are its own."""
+    q_start, lens = there(8, dtype=I32), there(7, dtype=I32)
+    q_start[:], lens[:] = torch.tensor([0, 1, 2, 514, 1026, 1538, 2050, 2050]), torch.tensor([9, 9, 4096, 4000, 3000, 2000, 0])
+    args = lambda: attend_args(dict(q=there(2050, 256, dtype=BF16), out=there(2050, 256, dtype=BF16)),  # noqa: E731
+                               dict(n_reqs=7, n_tokens=2050, max_q_len=512, max_ctx_len=4096, n_decode=2, q_start=q_start, ctx_lens=lens),
+                               dict(block_table=there(7, 256, dtype=I32)))
+    a_portion = 4 * 4096 * 2 * 64
+    for limit, passes in ((5 * a_portion, [5]), (5 * a_portion - 1, [4, 1]), (2 * a_portion, [2, 2, 1]), (a_portion, [1] * 5), (a_portion - 1, None)):
+        ops.calls.clear()
+        ops.widen_8bit_bytes = limit
+        ops.paged_attention_8bit(**args())
+        if passes is None:
+            assert len(ops.calls) == 1
+            continue
+        assert len(ops.calls) == 1 + 2 * len(passes)
+        first = 2
+        for widen, attend, n in zip(ops.calls[1::2], ops.calls[2::2], passes):
+            assert widen[17:19] == (first, n) and attend[11:13] == (0, n)
+            assert attend[8] == q_start.data_ptr() + 4 * first and attend[9] == lens.data_ptr() + 4 * first
+            first += n
+
+
+def test_without_memory_the_pages_are_read_as_they_are(ops, monkeypatch):  # noqa: F811
+    """Copies that find no memory are no error: the kernel that needs none takes the portions."""
+    assert portions(ops) == 3
+    real = torch.empty
+
+    def empty(*a, **k):
+        if k.get("dtype") == BF16:
+            raise torch.cuda.OutOfMemoryError("no memory left")
+        return real(*a, **k)
+
+    monkeypatch.setattr(torch, "empty", empty)
+    args = attend_args(dict(q=there(2050, 256, dtype=BF16), out=there(2050, 256, dtype=BF16)),
+                       dict(n_tokens=2050, max_q_len=2048, max_ctx_len=2048, n_decode=2))
+    ops.calls.clear()
+    ops.paged_attention_8bit(**args)
+    assert len(ops.calls) == 1

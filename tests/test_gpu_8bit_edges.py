@@ -42,6 +42,8 @@ def left_out(q, H, K, D, pages, ctx, group, scale):
     off = torch.zeros(q.shape[0], H, dtype=torch.float64)
     for r in range(ctx.n_reqs):
         clen, a, b = int(ctx.ctx_lens[r]), int(ctx.q_start[r]), int(ctx.q_start[r + 1])
+        if clen == 0:
+            continue
         j = torch.arange(clen)
         page = group.block_table[r][j // group.page_size].long()
         k = (k8[page, :, j % group.page_size].double() * ks[page].double()[..., None]).abs().amax(0)        # [kv, dim]
@@ -202,3 +204,35 @@ def test_the_same_call_gives_the_same_bits(ops):
             first = attend(ops, q, 8, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5)
             for _ in range(3):
                 assert torch.equal(first, attend(ops, q, 8, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_portions_widened_in_passes(ops, D, monkeypatch):
+    """Portions of which memory holds one or two at a time, beside single tokens and an empty one, and the same call captured."""
+    g = torch.Generator().manual_seed(47)
+    new, old = [1, 1, 40, 70, 3, 0, 130], [30, 200, 500, 0, 90, -1, 300]
+    pages = sum(-(-max(0, a + b) // 16) for a, b in zip(new, old))
+    ctx, group = plain.batch(new, old, 16, pages, 2, seed=9)
+    k8, ks = pages_of(g, pages, 2, 16, D)
+    v8, vs = pages_of(g, pages, 2, 16, D)
+    q = rnd(g, sum(new), 4 * D, dtype=torch.bfloat16)
+    for window in (None, 60):
+        a_portion = 4 * 2 * D * (min(ctx.max_ctx_len, window + ctx.max_q_len) if window else ctx.max_ctx_len)
+        for n in (1, 2, 5):
+            monkeypatch.setattr(ops, "widen_8bit_bytes", n * a_portion)
+            check(ops, q, 4, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5, window)
+    monkeypatch.setattr(ops, "widen_8bit_bytes", 2 * a_portion)
+    dev, on, out = [plain.cuda(ctx), plain.cuda(group)], [t.cuda() for t in (k8, v8, ks, vs)], torch.empty_like(q).cuda()
+    call = lambda: ops.paged_attention_8bit(q_dev, 4, 2, D, *on, *dev, D ** -0.5, 60, out)  # noqa: E731
+    q_dev = q.cuda()
+    call()
+    torch.cuda.synchronize()
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
