@@ -229,8 +229,9 @@ class CacheManager:
         return self._views
 
     def bytes_per_token(self) -> int:
-        """Bytes of keys and values one cached token takes over all groups."""
-        if self.eight_bit:                              # and two scales a page and head
+        """Bytes of keys and values one cached token takes over all groups (in 8 bits with its share of each head's two scales a
+        page, rounded up to a byte a head: pages of 16 take half of that)."""
+        if self.eight_bit:
             return sum(len(g.calls) * g.need.num_kv_heads * (2 * g.need.head_dim + -(-8 // self.page_size))
                        for g in self.groups)
         size = torch.empty((), dtype=self.dtype).element_size()

@@ -10,7 +10,9 @@
 // A page is filled from its first slot on.  A call that writes slot 0 begins the page anew: its scale comes from
 // the call's rows alone, whatever an earlier holder of the page left.  Otherwise the scale is the larger
 // of the old one and what the rows need, and where it grew the other slots become rint(q * old / new).
-// A page's tokens stand together in the call (nothing but tokens without a slot between them).
+// A page's tokens stand together in the call (nothing but tokens without a slot between them): the block of a run settles its page's
+// scale alone, and two of them would both change one page.  Nothing looks for that: blocks that hold every run's page against
+// all later ones took 3 of a short call's 4 us, 24 us at 2,048 tokens.
 //
 // One kernel.  A lane has 8 dimensions of a head's first half and the 8 that they turn with, so a warp has
 // 32 / (head size / 16) heads at a time: of one token for the queries; for keys and values of as many tokens, one

@@ -914,7 +914,8 @@ class CudaOps:
         largest value is 127 or less.  NaN is held as 0, infinities and what 127 * 2^60 does not reach as
         the largest value.  Writing slot 0 begins a page anew; otherwise the scale only grows, and the page's other
         slots follow it.  The tokens of one page stand together in the call (tokens without a slot may
-        stand between them), and each slot comes once (of several tokens for one slot the last is kept)."""
+        stand between them; the caller sees to it: what a page that comes in two runs holds afterwards is not said, nothing else
+        is touched), and each slot comes once (of several tokens for one slot the last is kept)."""
         what = "qk_norm_rope_write_8bit"
         dtype, here = qkv.dtype, self._here()
         code = _code(dtype)
@@ -2079,9 +2080,9 @@ class CudaOps:
         token (int32 [rows]): (log probability, rank, entropy in nats, log probabilities of the `top` largest logits, their
         ids), float32 [rows], int32 [rows], float32 [rows], float32 [rows, top], int32 [rows, top].  The rank is 1
         plus the number of larger logits; equal logits come in the order of their ids; `top` is at most 32.
-        A token outside the vocabulary has log probability NaN and rank 0.  A NaN or an infinity among a row's logits
-        makes its probabilities NaN, as do logits that are all -inf; NaN is never among the largest (id -1 where
-        there are not enough others)."""
+        A token outside the vocabulary has log probability NaN and rank 0.  A logit of -inf is one that is masked; a NaN or a
+        +inf among a row's logits makes its probabilities NaN, as do logits that are all -inf; NaN is never among the largest
+        (id -1 where there are not enough others)."""
         what, here = "token_logprobs", self._here()
         code = _code(logits.dtype)
         rows, stride = self._row_shape(what, logits, 1, here)
