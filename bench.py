@@ -615,6 +615,105 @@ def run_kernels(args):
     return 0
 
 
+KV8_POINTS = [(1, 3900), (8, 3900), (16, 3900), (64, 3900), (8, 30000), (32, 15000)]     # requests, context
+
+
+def run_kv8(args):
+    """Whole steps over keys and values in bfloat16 and in 8 bits, and with log probabilities (`--only kv8`): ms a replayed
+    step of single tokens (device time, tokens fed back on the device), of a prompt of 2,048 tokens and of 64 tokens after 1,000 (the
+    third step of each and later ones, device time), of a step through `Engine` with and without log probabilities, and of
+    scoring 2,048 tokens (wall time, the device waited for)."""
+    import torch
+    from rvllm_b200.config import config_from_dict
+    from rvllm_b200.engine import (Engine, Generator, ModelRunner, Request, SchedulerConfig, StepEntry, graphs_default,
+                                   load_model, make_cache)
+    from rvllm_b200.sampling import SamplingParams
+    from rvllm_b200.weights import write_random_model
+    cfg = config_from_dict({**LFM2_1_2B, **SIZES[args.size], "max_position_embeddings": 32768})
+    tmp = tempfile.mkdtemp(prefix="rvllm_bench_")
+    try:
+        model, cfg = load_model(write_random_model(os.path.join(tmp, "lfm2"), cfg, seed=0), "bfloat16", "cuda")
+    finally:
+        shutil.rmtree(tmp, ignore_errors=True)
+    gen = torch.Generator().manual_seed(0)
+    ids = lambda n: torch.randint(0, cfg.vocab_size, (n,), generator=gen).tolist()  # noqa: E731
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+
+    def timed(fn):
+        torch.cuda.synchronize()
+        e0.record()
+        fn()
+        e1.record()
+        torch.cuda.synchronize()
+        return e0.elapsed_time(e1)
+
+    def fresh(kv, batch, context):
+        cache = make_cache(model, PAGE, batch * ((context + 256) // PAGE + 1), batch, kv)
+        return ModelRunner(model, cache, model.ops, use_graphs=graphs_default())
+
+    def decode(kv, batch, context):
+        runner = fresh(kv, batch, context)
+        for i in range(batch):
+            runner.add_request(i)
+            text = ids(context)
+            for a in range(0, context, 2048):
+                runner.step([StepEntry(i, text[a:a + 2048], ())])
+        first = runner.decode_greedy(range(batch), [1] * batch, 8)[-1].tolist()
+        return round(timed(lambda: runner.decode_greedy(range(batch), first, 96)) / 96, 4)
+
+    def portion(kv, tokens, before):
+        runner, took = fresh(kv, 2, tokens + before), []
+        for _ in range(8):
+            runner.add_request("r")
+            if before:
+                runner.step([StepEntry("r", ids(before), ())])
+            text = ids(tokens)
+            took.append(timed(lambda: runner.step([StepEntry("r", text, (tokens - 1,))])))
+            runner.end_request("r")
+        return round(sorted(took[2:])[2], 4)
+
+    def engine_step(kv, batch, context, logprobs):
+        runner = fresh(kv, batch, context)
+        engine = Engine(runner, SchedulerConfig(block_size=PAGE, num_blocks=runner.cache.num_pages, max_num_batched_tokens=8192,
+                                                prefill_chunk=2048), 32768, lookahead=True, logprobs=logprobs)
+        for i in range(batch):
+            engine.add_request(Request(i, ids(context), 240, (), SamplingParams()))
+        seqs = list(engine.scheduler.seqs.values())
+        while min(len(q.generated) for q in seqs) < 8:
+            engine.step()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(160):
+            engine.step()
+        torch.cuda.synchronize()
+        return round((time.perf_counter() - t0) / 160 * 1e3, 4)
+
+    def score(kv, top):
+        g, text, took = Generator(model, cfg, None, kv), ids(2048), []
+        for _ in range(5):
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+            g.score(text, top=top)
+            took.append((time.perf_counter() - t0) * 1e3)
+        return round(sorted(took[1:])[1], 3)
+
+    sampler = ClockSampler()
+    sampler.start()
+    out = {"only": "kv8", "size": args.size}
+    for kv in ("auto", "int8"):
+        t = out["bfloat16" if kv == "auto" else "int8"] = {"bytes_a_token": fresh(kv, 1, PAGE).cache.bytes_per_token()}
+        t["decode_ms"] = {f"{b} x {c}": decode(kv, b, c) for b, c in KV8_POINTS}
+        t["portion_ms"] = {"2048": portion(kv, 2048, 0), "512": portion(kv, 512, 0), "64 after 1000": portion(kv, 64, 1000),
+                           "512 after 8000": portion(kv, 512, 8000)}
+        t["engine_step_ms"] = {f"{b} x 1000, logprobs {k}": engine_step(kv, b, 1000, k)
+                               for b in (1, 8, 64) for k in (None, 0, 5, 20)}
+        t["score_2048_ms"] = {f"top {k}": score(kv, k) for k in (0, 5)}
+    out["clocks"] = sampler.stop()
+    model.ops.check_status()
+    print(json.dumps(out))
+    return 0
+
+
 def run_workload(name, verbose=False):
     """One scheduler workload through `Engine.step`, after two untimed runs of the same
     requests (the reference's bench discards a warm-up run too, src/bin/bench.rs:215-232;
@@ -1679,7 +1778,7 @@ def main():
     ap.add_argument("--impl", default="ours", choices=["ours", "reference"])
     ap.add_argument("--size", default="1.2b", choices=sorted(SIZES),
                     help="layer sizes: LFM2-1.2B (the default and the headline), 700M or 350M")
-    ap.add_argument("--only", default="all", choices=["all", "decode", "prefill", "kernels", "breakdown", "workload", "further", "retorax", "bizenex", "vifanex", "mevuvik", "fekizen", "dopuvik"],
+    ap.add_argument("--only", default="all", choices=["all", "decode", "prefill", "kernels", "breakdown", "workload", "further", "kv8", "retorax", "bizenex", "vifanex", "mevuvik", "fekizen", "dopuvik"],
                     help="run one part only (for profiling); the JSON line then lacks the rest")
     ap.add_argument("--workloads", default="both", choices=["both", "none"] + sorted(WORKLOADS),
                     help="scheduler workloads to add to the line (default: both)")
@@ -1709,6 +1808,8 @@ def main():
         return run_kernels(args)
     if args.only == "further":
         return run_further(args)
+    if args.only == "kv8":
+        return run_kv8(args)
     if args.only == "retorax":
         return run_designs(args)
     if args.only == "bizenex":
