@@ -2,7 +2,7 @@
 // [head size], one power-of-two scale per page and head), single tokens and portions of prompts.  Compiled for one head
 // size at a time (RV_HD: a multiple of 16, at most 256).
 //
-// A warp works alone.  It owns 8 or 16 rows -- a row is a query token and one of the query heads that share the key/value
+// A warp works alone.  It owns 4, 8 or 16 rows -- a row is a query token and one of the query heads that share the key/value
 // head -- and walks tiles of 32 keys, which it copies itself (cp.async) into a ring of its own in shared memory: nothing
 // but the warp's own copies is waited for.  Scores are computed transposed, S^T = K Q^T: 16 keys are the rows of a product's
 // left operand, 8 query rows the columns of the right one.  With few query heads per key/value head the other order
@@ -52,7 +52,8 @@ static_assert(A8_HD % 16 == 0 && A8_HD >= 16 && A8_HD <= 256, "head sizes");
 #define A8_KEYS 32                                                // a tile, a lane's key each
 #define A8_CHUNKS (A8_HD / 16)                                    // 16-byte pieces of a row
 // Warps of a multiprocessor: what the registers (16: 128 a thread, 12: 168, 8: 255) and the rings leave room for.
-template <int NT, int PARTS> constexpr int a8_warps() {
+template <int ROWS, int PARTS> constexpr int a8_warps() {
+    constexpr int NT = ROWS > 8 ? 2 : 1;
     return A8_HD <= 64 ? (NT * PARTS == 1 ? 16 : NT * PARTS == 2 ? 12 : 8) : A8_HD <= 192 ? 8 : 6;
 }
 #define A8_MOST_WARPS 16
@@ -192,7 +193,7 @@ __device__ __forceinline__ void a8_load_n(const __nv_bfloat16* p, bool vec, floa
 
 // ---- how single tokens' tiles are shared out --------------------------------------------------------
 // The tiles of all requests, one after the other, are cut evenly into as many runs as there are teams of warps (`used`
-// of them where there are fewer tiles).  A team has a warp for every unit: a key/value head and 8 * NT of its query
+// of them where there are fewer tiles).  A team has a warp for every unit: a key/value head and ROWS of its query
 // heads.  Its warps walk the same tiles, so the heads of a page, which lie side by side, are read at about the same time.
 // From one segment (a run's part of a request) to the next the run or the request grows, so run + request is a place of
 // its own, times the units.
@@ -247,8 +248,12 @@ struct A8Cursor {
     int r, tile, last, clen;
 };
 
-template <typename T, int NT, int PARTS>
+template <typename T, int ROWS, int PARTS>
 struct A8Warp {
+    static constexpr int NT = ROWS > 8 ? 2 : 1;        // products of 8 columns
+    // Four rows take a product's columns twice: what float16 leaves of a weight has the second four, so it costs no product of its own
+    // (64 requests of some 3,100 keys, 32 / 8 heads of 64: 44.3 us; as eight rows 46.9).
+    static constexpr bool TWICE = ROWS == 4;
     const A8Args& a;
     const unsigned ring;               // in shared memory
     const int lane, g, t;
@@ -296,10 +301,10 @@ struct A8Warp {
         }
     }
 
-    // Rows [first, first + 8 NT) of the `qlen` tokens times G heads of request r.
+    // Rows [first, first + ROWS) of the `qlen` tokens times G heads of request r.
     __device__ __forceinline__ void begin(int r, int head, int first, int qlen, int q_first, int clen) {
         rows_first = first;
-        rows_count = min(8 * NT, qlen * G - first);
+        rows_count = min(ROWS, qlen * G - first);
         kvh = head;
         qs = q_first;
         p_min = clen;
@@ -307,7 +312,7 @@ struct A8Warp {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             // the row whose values this lane holds: column g
-            const int i = first + 8 * n + g, tok = i / G;
+            const int i = first + 8 * n + (g & (TWICE ? 3 : 7)), tok = i / G;
             const bool real = i < qlen * G;
             const T* src = (const T*)a.q + (size_t)(qs + (real ? tok : 0)) * a.q_stride +
                            (size_t)(kvh * G + (real ? i - tok * G : 0)) * A8_HD;
@@ -355,7 +360,7 @@ struct A8Warp {
             for (int h = 0; h < 2; ++h) {
                 // the rows of this lane's scores: columns 2 t, 2 t + 1
                 f[n][h] = __shfl_sync(0xffffffffu, mine, (2 * t + h) * 4);
-                const int j = first + 8 * n + 2 * t + h;
+                const int j = first + 8 * n + ((2 * t + h) & (TWICE ? 3 : 7));
                 hi[n][h] = j < qlen * G ? clen - qlen + j / G : -1;
                 lo[n][h] = a.window > 0 ? max(0, hi[n][h] - a.window + 1) : 0;
                 M[n][h] = -INFINITY;
@@ -525,8 +530,9 @@ struct A8Warp {
                     l[n][0] = fmaf(p0, inv[m][h], l[n][0]);
                     l[n][1] = fmaf(p1, inv[m][h], l[n][1]);
                     const unsigned w = a8_pack(p0, p1);
-                    p[n][m][h] = a8_transpose(w);
-                    p2[n][m][h] = a8_transpose(a8_rest(p0, p1, w));
+                    const unsigned rest = a8_rest(p0, p1, w);
+                    p[n][m][h] = a8_transpose(TWICE && t >= 2 ? rest : w);
+                    if (!TWICE) p2[n][m][h] = a8_transpose(rest);
                 }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -553,7 +559,7 @@ struct A8Warp {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         a8_mma(o[c + k][n], a0, a1, a2, a3, p[n][m][0], p[n][m][1]);
-                        a8_mma(o[c + k][n], a0, a1, a2, a3, p2[n][m][0], p2[n][m][1]);
+                        if (!TWICE) a8_mma(o[c + k][n], a0, a1, a2, a3, p2[n][m][0], p2[n][m][1]);
                     }
                 }
             }
@@ -569,6 +575,11 @@ struct A8Warp {
                 l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
                 l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
             }
+        if (TWICE)
+#pragma unroll
+            for (int c = 0; c < A8_CHUNKS; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[c][0][k] += __shfl_xor_sync(0xffffffffu, o[c][0][k], 2);
     }
     __device__ __forceinline__ void leave(size_t place) {
         finish();
@@ -578,7 +589,7 @@ struct A8Warp {
             for (int j = 0; j < 2; ++j) {
                 const int row = 8 * n + 2 * t + j;
                 if (row >= rows_count) continue;
-                const size_t at = place * (8 * NT) + row;
+                const size_t at = place * ROWS + row;
                 if (g == 0) a.part_ml[at] = make_float2(M[n][j], l[n][j]);
 #pragma unroll
                 for (int c = 0; c < A8_CHUNKS; ++c)
@@ -591,13 +602,13 @@ struct A8Warp {
 #define A8_COMMIT() asm volatile("cp.async.commit_group;" ::: "memory")
 
 // Requests [0, n_reqs) with one token each.
-template <typename T, int NT, int PARTS>
-__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_stream_kernel(const __grid_constant__ A8Args a) {
+template <typename T, int ROWS, int PARTS>
+__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<ROWS, PARTS>() / A8_BLOCK_WARPS) attention_8bit_stream_kernel(const __grid_constant__ A8Args a) {
     rv_pdl_wait();
     rv_pdl_launch_dependents();        // the merge may read what was there before this launch as soon as it begins
     extern __shared__ __align__(128) unsigned char smem[];
-    A8Warp<T, NT, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
-    const int per_head = (w.G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
+    A8Warp<T, ROWS, PARTS> w(a, smem + (threadIdx.x >> 5) * A8_WARP_BYTES);
+    const int per_head = (w.G + ROWS - 1) / ROWS, units = a.num_kv_heads * per_head;
     const int warps = gridDim.x * A8_BLOCK_WARPS, teams = max(1, warps / units);
     const A8Shares sh(a.ctx_lens, a.n_reqs, a.window, (long long)a.max_blocks * a.page_size, teams, 0);
     if (sh.total == 0) return;
@@ -661,7 +672,7 @@ __global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A
         int stage = 0;
         for (int i = 0; i < n; ++i) {
             if (fresh) {
-                w.begin(c.r, head, (u - head * per_head) * 8 * NT, 1, c.r, c.clen);
+                w.begin(c.r, head, (u - head * per_head) * ROWS, 1, c.r, c.clen);
                 fresh = false;
             }
             A8_WAIT_STAGE();
@@ -723,25 +734,26 @@ __device__ __forceinline__ void a8_put(const A8Args& a, int row_token, int head,
     rv_store(dst + 1, o.y * by);
 }
 
-// Requests [first_req, first_req + n_reqs) with any number of tokens.  blockIdx.z: request, y: key/value head, x: 8 NT rows
+// Requests [first_req, first_req + n_reqs) with any number of tokens.  blockIdx.z: request, y: key/value head, x: ROWS rows
 // a warp (nsplit 0), or a cluster of nsplit blocks: their warps share the rows' tiles and meet in the blocks'
 // shared memory, then in the cluster's.
-template <typename T, int NT, int PARTS, bool SHARED>
-__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<NT, PARTS>() / A8_BLOCK_WARPS) attention_8bit_rows_kernel(
+template <typename T, int ROWS, int PARTS, bool SHARED>
+__global__ void __launch_bounds__(A8_BLOCK_WARPS * 32, a8_warps<ROWS, PARTS>() / A8_BLOCK_WARPS) attention_8bit_rows_kernel(
     const __grid_constant__ A8Args a) {
     rv_pdl_prologue();
+    constexpr int NT = ROWS > 8 ? 2 : 1;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, rank = SHARED && a.nsplit > 1 ? (int)a8_rank() : 0;
     const int rt = SHARED ? blockIdx.x / a.nsplit : blockIdx.x * A8_BLOCK_WARPS + warp;
     const int parts = SHARED ? a.nsplit * A8_BLOCK_WARPS : 1, part = SHARED ? rank * A8_BLOCK_WARPS + warp : 0;
     const int r = a.first_req + blockIdx.z, head = blockIdx.y;
     const int qs = a.q_start[r], qlen = a.q_start[r + 1] - qs, clen = a.ctx_lens[r];
-    A8Warp<T, NT, PARTS> w(a, smem + warp * A8_WARP_BYTES);
+    A8Warp<T, ROWS, PARTS> w(a, smem + warp * A8_WARP_BYTES);
     // the rows with the longest contexts first
-    const int tiles = (qlen * w.G + 8 * NT - 1) / (8 * NT);
+    const int tiles = (qlen * w.G + ROWS - 1) / ROWS;
     if (rt >= tiles) return;                                           // (a whole cluster)
-    const int first = (tiles - 1 - rt) * 8 * NT;
-    const int end = min(qlen * w.G, first + 8 * NT);
+    const int first = (tiles - 1 - rt) * ROWS;
+    const int end = min(qlen * w.G, first + ROWS);
     const int p_first = clen - qlen + first / w.G, p_last = clen - qlen + (end - 1) / w.G;
     const bool fits = clen <= (long long)a.max_blocks * a.page_size;
     const int t_all = (a.window > 0 ? max(0, p_first - a.window + 1) : 0) / A8_KEYS;
@@ -920,15 +932,15 @@ __device__ __forceinline__ void a8_merge(const A8Args& a, size_t place, int n, i
 
 // A warp (W = 1: four rows a block) or a block a row; blockIdx.y: request, x: head.  It lets no launch behind it begin
 // before it is done: blocks of the next stream that wait where this one's have yet to run cost 17 us of 60 a call.
-template <typename T, int NT, int W>
+template <typename T, int ROWS, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_merge_kernel(const __grid_constant__ A8Args a, int runs) {
-    const int G = a.num_heads / a.num_kv_heads, per_head = (G + 8 * NT - 1) / (8 * NT), units = a.num_kv_heads * per_head;
+    const int G = a.num_heads / a.num_kv_heads, per_head = (G + ROWS - 1) / ROWS, units = a.num_kv_heads * per_head;
     const int r = blockIdx.y, head = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (head >= a.num_heads) {
         rv_pdl_wait();
         return;
     }
-    const int kvh = head / G, in = head - kvh * G, u = kvh * per_head + in / (8 * NT);
+    const int kvh = head / G, in = head - kvh * G, u = kvh * per_head + in / ROWS;
     const A8Shares sh(a.ctx_lens, a.n_reqs, a.window, (long long)a.max_blocks * a.page_size, runs, r);
     const int clen = sh.length(r), tiles = sh.tiles(clen);
     int run0 = 0, n = 0;
@@ -937,7 +949,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) attention_8bit_stream_m
         n = sh.run_of(sh.before + tiles - 1) - run0 + 1;
     }
     rv_pdl_wait();
-    a8_merge<T, W>(a, ((size_t)run0 + r) * units + u, n, units, 8 * NT, in % (8 * NT), head,
+    a8_merge<T, W>(a, ((size_t)run0 + r) * units + u, n, units, ROWS, in % ROWS, head,
                    (T*)a.out + ((size_t)r * a.num_heads + head) * A8_HD, clen > 0 && tiles == 0);
 }
 
@@ -950,16 +962,16 @@ static thread_local char g_a8_error[512] = "";
 
 extern "C" const char* A8_SYM(rv_attention_8bit_last_error)() { return g_a8_error; }
 
-// Rows of a warp: 16 where a key/value head has more than 8 of them and the accumulators fit the registers.
-static int a8_nt(long long rows) { return rows > 8 && A8_HD <= 128 ? 2 : 1; }
-static long long a8_place_bytes(int nt) { return 8ll * nt * (A8_HD * 4 + 8); }
+// Rows of a warp: 16 where a key/value head has more than 8 of them and the accumulators fit the registers, 4 where it has no more.
+static int a8_row_count(long long rows) { return rows <= 4 ? 4 : rows > 8 && A8_HD <= 128 ? 16 : 8; }
+static long long a8_place_bytes(int rows) { return (long long)rows * (A8_HD * 4 + 8); }
 
 static long long a8_tiles(int max_ctx_len, int window, int max_q_len) {
     long long keys = max_ctx_len;
     if (window > 0 && (long long)window + max_q_len < keys) keys = (long long)window + max_q_len;
     return (keys + A8_KEYS - 1) / A8_KEYS;
 }
-// Blocks whose warps share the tiles of 8 NT rows: 0 (a warp has them alone) where there are warps enough, else as many as the
+// Blocks whose warps share the tiles of ROWS rows: 0 (a warp has them alone) where there are warps enough, else as many as the
 // GPU holds at once, up to a cluster, while every warp has a tile.  (us by warps alone / a block / two / four / eight: 32 / 8
 // heads of 64, 128 requests of 700 keys 35 / 25 / 35 / 54 / 85, 32 of 1,000 23 / 12.4 / 12.5 / 18 / 26, 16 of 4,000 72 / 27 / 22 / 18.5 / 23.)
 static int a8_nsplit(long long units, long long tiles, int block_places) {
@@ -983,11 +995,11 @@ static bool a8_few(long long units, long long tiles, int n_sms, int form) {
 // Scratch for single tokens: requests [0, n_decode).
 extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode, int max_ctx_len, int num_heads, int num_kv_heads,
                                                                    int window, int n_sms, int form) {
-    const int G = num_heads / num_kv_heads, nt = a8_nt(G);
-    const long long units = (long long)num_kv_heads * ((G + 8 * nt - 1) / (8 * nt));
+    const int G = num_heads / num_kv_heads, rows = a8_row_count(G);
+    const long long units = (long long)num_kv_heads * ((G + rows - 1) / rows);
     if (n_decode <= 0 || a8_few(units * n_decode, a8_tiles(max_ctx_len, window, 1), n_sms, form)) return 0;
     const long long all = (long long)n_sms * A8_MOST_WARPS;
-    return ((all > units ? all : units) + n_decode * units) * a8_place_bytes(nt);
+    return ((all > units ? all : units) + n_decode * units) * a8_place_bytes(rows);
 }
 
 // The limit of shared memory is a kernel's on a device: raised once on each.
@@ -1003,47 +1015,47 @@ extern "C" long long A8_SYM(rv_paged_attention_8bit_scratch_bytes)(int n_decode,
         }                                                                                                       \
     } while (0)
 
-template <typename T, int NT, int PARTS>
+template <typename T, int ROWS, int PARTS>
 static int a8_stream(A8Args a, int n_sms, cudaStream_t stream) {
     const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
-    const int blocks = n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS);
-    auto kernel = attention_8bit_stream_kernel<T, NT, PARTS>;
+    const int blocks = n_sms * (a8_warps<ROWS, PARTS>() / A8_BLOCK_WARPS);
+    auto kernel = attention_8bit_stream_kernel<T, ROWS, PARTS>;
     A8_CONFIGURE(kernel, smem);
     const int G = a.num_heads / a.num_kv_heads;
-    const long long per = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT)), all = (long long)blocks * A8_BLOCK_WARPS;
+    const long long per = a.num_kv_heads * ((G + ROWS - 1) / ROWS), all = (long long)blocks * A8_BLOCK_WARPS;
     const long long places = (all > per ? all : per) + a.n_reqs * per;
-    a.part_ml = (float2*)(a.part_o + places * 8 * NT * A8_HD);
+    a.part_ml = (float2*)(a.part_o + places * ROWS * A8_HD);
     rv_launch(kernel, dim3(blocks), dim3(A8_BLOCK_WARPS * 32), smem, stream, a);
     // segments of a request, about: runs a request
-    const int units = a.num_kv_heads * ((G + 8 * NT - 1) / (8 * NT)), warps = blocks * A8_BLOCK_WARPS;
+    const int units = a.num_kv_heads * ((G + ROWS - 1) / ROWS), warps = blocks * A8_BLOCK_WARPS;
     const int teams = warps / units > 1 ? warps / units : 1;
     if (teams > 8 * a.n_reqs)
-        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 8>, dim3(a.num_heads, a.n_reqs), dim3(256), 0, stream, a, teams);
+        rv_launch(attention_8bit_stream_merge_kernel<T, ROWS, 8>, dim3(a.num_heads, a.n_reqs), dim3(256), 0, stream, a, teams);
     else
-        rv_launch(attention_8bit_stream_merge_kernel<T, NT, 1>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a, teams);
+        rv_launch(attention_8bit_stream_merge_kernel<T, ROWS, 1>, dim3((a.num_heads + 3) / 4, a.n_reqs), dim3(128), 0, stream, a, teams);
     return 0;
 }
 // `tokens`, `depth`: about how many tokens the requests bring in all, and how deep they are.  Which form is chosen follows these; the
 // launch's size follows the longest.
-template <typename T, int NT, int PARTS>
+template <typename T, int ROWS, int PARTS>
 static int a8_rows(A8Args a, long long tokens, int max_q_len, int depth, int n_sms, cudaStream_t stream) {
     const size_t smem = (size_t)A8_BLOCK_WARPS * A8_WARP_BYTES;
     const long long rows = (long long)max_q_len * (a.num_heads / a.num_kv_heads);
     if (rows > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
-    const int row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
+    const int row_tiles = (int)((rows + ROWS - 1) / ROWS);
     // (a padded step launches blocks for every request as if it were the longest, most of which find no rows: of one portion of 64
     // tokens after 1,000 beside an empty one 17.8 us by what is launched, 14.6 by what is there)
-    const long long there = tokens * (a.num_heads / a.num_kv_heads) / (8 * NT) + a.n_reqs, launched = (long long)row_tiles * a.n_reqs;
+    const long long there = tokens * (a.num_heads / a.num_kv_heads) / ROWS + a.n_reqs, launched = (long long)row_tiles * a.n_reqs;
     a.nsplit = a8_nsplit((there < launched ? there : launched) * a.num_kv_heads, a8_tiles(depth, a.window, max_q_len),
-                         n_sms * (a8_warps<NT, PARTS>() / A8_BLOCK_WARPS));
+                         n_sms * (a8_warps<ROWS, PARTS>() / A8_BLOCK_WARPS));
     if (a.nsplit == 0) {
-        auto kernel = attention_8bit_rows_kernel<T, NT, PARTS, false>;
+        auto kernel = attention_8bit_rows_kernel<T, ROWS, PARTS, false>;
         A8_CONFIGURE(kernel, smem);
         rv_launch(kernel, dim3((unsigned)((row_tiles + A8_BLOCK_WARPS - 1) / A8_BLOCK_WARPS), a.num_kv_heads, a.n_reqs),
                   dim3(A8_BLOCK_WARPS * 32), smem, stream, a);
         return 0;
     }
-    auto kernel = attention_8bit_rows_kernel<T, NT, PARTS, true>;
+    auto kernel = attention_8bit_rows_kernel<T, ROWS, PARTS, true>;
     A8_CONFIGURE(kernel, smem);
     if ((long long)row_tiles * a.nsplit > 0x7fffffffll) A8_FAIL("paged_attention_8bit: too many rows");
     cudaLaunchConfig_t cfg = {};
@@ -1065,16 +1077,18 @@ static int a8_rows(A8Args a, long long tokens, int max_q_len, int depth, int n_s
 }
 template <typename T, int PARTS>
 static int a8_portions(const A8Args& a, long long tokens, int max_q_len, int depth, int n_sms, cudaStream_t stream) {
-    return a8_nt(max_q_len * (long long)(a.num_heads / a.num_kv_heads)) == 1
-               ? a8_rows<T, 1, PARTS>(a, tokens, max_q_len, depth, n_sms, stream)
-               : a8_rows<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, tokens, max_q_len, depth, n_sms, stream);
+    const int rows = a8_row_count(max_q_len * (long long)(a.num_heads / a.num_kv_heads));
+    return rows == 4   ? a8_rows<T, 4, PARTS>(a, tokens, max_q_len, depth, n_sms, stream)
+           : rows == 8 ? a8_rows<T, 8, PARTS>(a, tokens, max_q_len, depth, n_sms, stream)
+                       : a8_rows<T, A8_HD <= 128 ? 16 : 8, PARTS>(a, tokens, max_q_len, depth, n_sms, stream);
 }
 template <typename T, int PARTS>
 static int a8_singles(const A8Args& a, int max_ctx_len, int n_sms, int form, cudaStream_t stream) {
-    const int G = a.num_heads / a.num_kv_heads, nt = a8_nt(G);
-    if (a8_few((long long)a.n_reqs * a.num_kv_heads * ((G + 8 * nt - 1) / (8 * nt)), a8_tiles(max_ctx_len, a.window, 1), n_sms, form))
+    const int G = a.num_heads / a.num_kv_heads, rows = a8_row_count(G);
+    if (a8_few((long long)a.n_reqs * a.num_kv_heads * ((G + rows - 1) / rows), a8_tiles(max_ctx_len, a.window, 1), n_sms, form))
         return a8_portions<T, PARTS>(a, a.n_reqs, 1, max_ctx_len, n_sms, stream);
-    return nt == 1 ? a8_stream<T, 1, PARTS>(a, n_sms, stream) : a8_stream<T, A8_HD <= 128 ? 2 : 1, PARTS>(a, n_sms, stream);
+    return rows == 4 ? a8_stream<T, 4, PARTS>(a, n_sms, stream) : rows == 8 ? a8_stream<T, 8, PARTS>(a, n_sms, stream)
+                                                                            : a8_stream<T, A8_HD <= 128 ? 16 : 8, PARTS>(a, n_sms, stream);
 }
 
 // Requests [0, n_decode) bring one token each, [n_decode, n_reqs) up to max_q_len; `portions`: about how many tokens the latter bring
