@@ -188,8 +188,8 @@ class Generator:
               block_size: int = 16) -> List[TokenLogprob]:
         """The log probability of every token of `prompt` after the first, given those before it, with rank,
         entropy and the `top` most probable tokens at its place.  The prompt is run `portion` tokens at a
-        time, kernel by kernel, so that no more rows of logits exist at once (a captured launch sequence would keep
-        its own, one for every length of a last portion)."""
+        time, so that no more rows of logits exist at once; whole portions are captured when they come again, as far as the
+        logits that this keeps are few (`ModelRunner.max_shape_logits`), a text's last one is not."""
         ids = self._encode(prompt)
         vocab, context = self.model.spec.vocab_size, self.model.spec.max_position
         if any(t < 0 or t >= vocab for t in ids):
@@ -208,7 +208,7 @@ class Generator:
         try:
             for a in range(0, len(ids) - 1, portion):
                 b = min(a + portion, len(ids) - 1)
-                logits = runner.step([StepEntry("score", ids[a:b], range(b - a))], replayed=False)
+                logits = runner.step([StepEntry("score", ids[a:b], range(b - a))], replayed=b - a == portion)
                 tokens = torch.tensor(ids[a + 1:b + 1], dtype=torch.int32, device=logits.device)
                 reader = LogprobReader(self.ops, logits, tokens, top)
                 if logits.is_cuda:

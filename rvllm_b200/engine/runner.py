@@ -39,6 +39,7 @@ class ModelRunner:
         self._shape_graphs: Dict[tuple, "_ShapeGraph"] = {}
         self._seen_shapes = set()
         self.max_shape_graphs = 16
+        self.max_shape_logits = 512 << 20        # bytes of logits that the exact shapes' captures may keep
         self._mixed_graphs: Dict[tuple, "_MixedGraph"] = {}
         self.max_mixed_graphs = int(os.environ.get("RVLLM_MIXED_GRAPHS", "32"))
         self.mixed_graph_idle_steps = 1024
@@ -109,8 +110,7 @@ class ModelRunner:
         """float32 logits [wanted, vocab], in the order of the entries and of `want`.
         With `device_tokens` (int32 device tensor, one id per entry) every entry brings one
         token whose id is taken from that tensor instead of `entry.tokens`.  `replayed` False: the step is
-        launched kernel by kernel and counts towards no capture, whose logits stay allocated (for steps that
-        want the logits of every token)."""
+        launched kernel by kernel and counts towards no capture (for shapes that are not likely to come again)."""
         if not entries:
             return torch.empty((0, self.model.spec.vocab_size), dtype=torch.float32,
                                device=self.device)
@@ -294,12 +294,13 @@ class ModelRunner:
                     self._seen_shapes.clear()
                 self._seen_shapes.add(key)
                 return None
-            if len(self._shape_graphs) >= self.max_shape_graphs:
+            if not self._room_for_shape(key):
                 return None
             g = _ShapeGraph(self, key, block_bucket)
             self._shape_graphs[key] = g
         if g.broken:
             return None
+        g.last_used = self.steps
         try:
             logits = g.run(ordered, row_order)
         except RuntimeError as e:
@@ -314,6 +315,23 @@ class ModelRunner:
             return None
         self.graph_steps += 1
         return logits
+
+    def _room_for_shape(self, key) -> bool:
+        """Whether one exact shape more may be captured: there are so many at most, and what their logits, which a capture keeps,
+        take is bounded.  Room is made by those that have not been replayed for a long time."""
+        row = 4 * self.model.spec.vocab_size
+        held = lambda k: row * sum(len(w) for w in k[1])  # noqa: E731
+        while len(self._shape_graphs) >= self.max_shape_graphs or \
+                held(key) + sum(held(k) for k in self._shape_graphs) > self.max_shape_logits:
+            idle = [k for k, g in self._shape_graphs.items() if self.steps - g.last_used >= self.mixed_graph_idle_steps]
+            if not idle:
+                return False
+            oldest = min(idle, key=lambda k: self._shape_graphs[k].last_used)
+            if self.is_cuda:
+                torch.cuda.synchronize()          # nothing of it may still be running when its memory goes
+            del self._shape_graphs[oldest]
+            self._seen_shapes.discard(oldest)
+        return True
 
     def decode_greedy(self, reqs: Sequence[Hashable], first_tokens: Sequence[int],
                       steps: int) -> torch.Tensor:
@@ -557,6 +575,7 @@ class _ShapeGraph:
     def __init__(self, runner: ModelRunner, key, block_bucket: int):
         self.runner = weakref.proxy(runner)     # no cycle: graphs die with their runner
         self.block_bucket, self.deepest = block_bucket, key[-1]
+        self.last_used = 0
         n_tokens, n_reqs = sum(key[0]), len(key[0])
         n_want = sum(len(w) for w in key[1])
         n_groups = len(runner.cache.groups)

@@ -66,18 +66,65 @@ def test_a_capture_that_fails_leaves_the_step_to_its_launches(model, monkeypatch
     runner.cache.check()
 
 
-def test_scoring_captures_nothing(folder, monkeypatch):
-    """Scoring wants a row of logits for every token: a launch sequence that kept them would hold them for good, one for every
-    length of a text's last portion."""
+class Replays:
+    """A capture that launches its step kernel by kernel."""
+
+    def __init__(self, runner, key, block_bucket):
+        self.runner, self.key, self.width = runner, key, block_bucket
+        self.graph, self.broken, self.capturing, self.last_used = object(), False, False, 0
+
+    def run(self, entries, row_order=None):
+        ctx = self.runner.builder.build(entries, pad_blocks=self.width, row_order=row_order)
+        return self.runner.model.forward(ctx, self.runner.cache.views())
+
+
+def test_scoring_captures_whole_portions_alone(folder, monkeypatch):
+    """A text's last portion has a length of its own: a capture of each would hold the logits of all its tokens, and a place that other
+    steps' captures want."""
     gen = generator(folder)
     ids = [(29 * i + 3) % 500 for i in range(40)]
     first = gen.score(ids, portion=13)
-    for kind in ("_DecodeGraph", "_MixedGraph", "_ShapeGraph"):
+    for kind in ("_DecodeGraph", "_MixedGraph"):
         monkeypatch.setattr(runner_module, kind, lambda *a: pytest.fail("a capture"))
-    gen._runner.use_graphs = True
-    for _ in range(3):
-        assert gen.score(ids, portion=13) == first
-    assert not gen._runner._seen_shapes and not gen._runner._shape_graphs
-    gen._runner.use_graphs = False
+    monkeypatch.setattr(runner_module, "_ShapeGraph", Replays)
+    runner = gen._runner
+    runner.use_graphs = True
+    for n in (40, 40, 33, 33, 36, 36, 20, 20):
+        got = gen.score(ids[:n], portion=13)
+        assert all(abs(a.logprob - b.logprob) <= 1e-5 and a.rank == b.rank for a, b in zip(got, first)) and len(got) == n - 1
+    assert [k[0] for k in runner._shape_graphs] == [(13,)] and runner.graph_steps > 0
+    runner.use_graphs = False
     assert gen.generate_ids([ids], GenerateOptions(max_tokens=2, stop_tokens=[])).outputs[0]
 
+
+def test_captures_of_exact_shapes_are_bounded(model, monkeypatch):
+    """By their number and by the logits that they keep; room is made by those that have not been replayed for a long time."""
+    monkeypatch.setattr(runner_module, "_ShapeGraph", Replays)
+    runner = ModelRunner(model, make_cache(model, 8, 32, 3), model.ops)
+    runner.use_graphs, runner.max_mixed_graphs = True, -1
+    runner.max_shape_logits = 20 * 4 * model.spec.vocab_size          # of twenty tokens
+
+    def step(n, wanted):
+        runner.add_request("r")
+        runner.step([StepEntry("r", range(n), range(wanted))])
+        runner.end_request("r")
+
+    def twice(n, wanted):
+        step(n, wanted)
+        step(n, wanted)
+        return [(k[0][0], len(k[1][0])) for k in runner._shape_graphs]
+
+    assert twice(9, 9) == [(9, 9)] and twice(11, 11) == [(9, 9), (11, 11)]
+    assert twice(12, 1) == [(9, 9), (11, 11)]                          # twenty are held
+    assert twice(30, 30) == [(9, 9), (11, 11)]
+    runner.mixed_graph_idle_steps = 8
+    for _ in range(8):
+        step(11, 11)
+    assert twice(12, 1) == [(11, 11), (12, 1)]                         # the other one made room
+    assert twice(30, 30) == [(11, 11), (12, 1)]                        # more than all may hold
+    runner.max_shape_graphs, runner.max_shape_logits = 2, 1 << 40
+    assert twice(14, 2) == [(11, 11), (12, 1)]
+    runner.steps += 100
+    step(12, 1)
+    assert twice(15, 2) == [(12, 1), (15, 2)]
+    runner.cache.check()
