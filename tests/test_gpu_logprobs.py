@@ -122,3 +122,19 @@ def test_a_row_does_not_depend_on_the_others(ops):
 def test_no_rows(ops):
     got = ops.token_logprobs(torch.empty(0, 100, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), 3)
     assert [tuple(t.shape) for t in got] == [(0,), (0,), (0,), (0, 3), (0, 3)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [4, 900])
+def test_tokens_outside_the_vocabulary(ops, dtype, rows):
+    """They have rank 0 and no log probability, in rows of any kind; the row's entropy and its largest are what they are."""
+    v = 3000
+    x = torch.randn(rows, v, generator=torch.Generator().manual_seed(9)).to(dtype)
+    x[1, 5] = math.nan
+    x[2] = -math.inf
+    inside = torch.full((rows,), 7, dtype=torch.int32)
+    outside = torch.tensor([-1, v, 2 ** 31 - 1, -2 ** 31] * (rows // 4), dtype=torch.int32)
+    a, b = (ops.token_logprobs(x.cuda(), t.cuda(), 3) for t in (inside, outside))
+    assert not b[1].any() and torch.isnan(b[0]).all() and bool((a[1] >= 1).all())
+    for i in (2, 3, 4):
+        assert torch.equal(torch.nan_to_num(a[i], nan=-5.0), torch.nan_to_num(b[i], nan=-5.0))
