@@ -110,9 +110,15 @@ __device__ __forceinline__ A c8_sum(A v, int lane0, int lph) {
     return sum;
 }
 
-// One key or value head of one token: norm and rotation in float64, rounded once to float32, so that what a page holds is
-// the formula's value but for one value in a million that lies on a border between two steps, whatever the order of
-// the sums (float32 throughout left ten times as many).
+// To float32, to odd: cut off, the last bit set where something was.  What is rounded to eight bits and what is held against 127 steps
+// afterwards comes out as if float64 had been.
+__device__ __forceinline__ float c8_odd(double v) {
+    // (29 bits go; below 2^-126 more do, of what is zero in eight bits)
+    return __uint_as_float(__float_as_uint(__double2float_rz(v)) | ((__double2loint(v) & 0x1fffffff) != 0));
+}
+// One key or value head of one token: norm and rotation in float64, so that what a page holds is the formula's value, whatever
+// the order of the sums (float32 throughout left ten values in a million on the wrong side of a border between two steps,
+// rounding to the nearest float32 first one).
 template <typename T>
 __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const float* w, bool turn, int t, bool live, int d0,
                                         int lane0, int lph, float (&x)[8], float (&y)[8]) {
@@ -158,8 +164,8 @@ __device__ __forceinline__ void c8_head(const C8Write& a, const T* src, const fl
             v = u * s[i] + v * c[i];
             u = turned;
         }
-        x[i] = turn && !angle ? NAN : (float)u;                  // (held as 0)
-        y[i] = turn && !angle ? NAN : (float)v;
+        x[i] = turn && !angle ? NAN : c8_odd(u);                  // (held as 0)
+        y[i] = turn && !angle ? NAN : c8_odd(v);
     }
 }
 

@@ -236,3 +236,54 @@ def test_portions_widened_in_passes(ops, D, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+# ---- keys that lie beside a border -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [16, 1300])
+def test_keys_beside_a_border(ops, n):
+    """Keys half way between two steps but for 2^-30 of a turn, and largest values that pass 127 steps by as much: what a page holds
+    is the value's own rounding, not that of its rounding to float32, scales included."""
+    ps, D = 16, 64
+    g = torch.Generator().manual_seed(49)
+    ctx, group = plain.batch([n], [0], ps, -(-n // ps) + 1, 0)
+    rows = torch.zeros(n, 3 * D)
+    k = rows[:, D:2 * D]
+    k[:, :D // 2] = (torch.randint(-126, 126, (n, D // 2), generator=g) + 0.5) * 2.0 ** -5
+    k[:, D // 2:] = torch.where(torch.rand(n, D // 2, generator=g) < 0.5, -1.0, 1.0)
+    k[::3, 0] = torch.where(torch.rand(k[::3, 0].shape, generator=g) < 0.5, -127.0, 127.0) * 2.0 ** -5
+    k[5::ps, 1] = 127 * 2.0 ** -5
+    table = torch.ones(n, D // 2), torch.full((n, D // 2), 2.0 ** -30)
+    pages = group.block_table.shape[1] + 1
+    host = [torch.zeros(pages, 1, ps, D, dtype=torch.int8) for _ in "kv"] + [torch.ones(pages, 1) for _ in "kv"]
+    dev = [t.cuda() for t in host]
+    ops.qk_norm_rope_write_8bit(rows.cuda(), 1, 1, D, None, None, 0.0, tuple(t.cuda() for t in table), ctx.positions.cuda(),
+                                group.slot_mapping.cuda(), torch.empty(n, D, device="cuda"), *dev)
+    plain.write(rows, 1, 1, D, None, None, 0.0, table, ctx.positions, group.slot_mapping, *host)
+    assert torch.equal(dev[2].cpu(), host[2])
+    assert torch.equal(dev[0].cpu(), host[0]), int((dev[0].cpu() != host[0]).sum())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_keys_are_the_formulas(ops, dtype):
+    """Two million keys, normed and turned: every one the rounding of what 64 bits give."""
+    n, K, D, ps = 4000, 8, 64, 16
+    g = torch.Generator().manual_seed(50)
+    rows = rnd(g, n, 3 * K * D, dtype=dtype).cuda()
+    w = (1 + rnd(g, D, scale=0.1)).cuda()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    angle = torch.outer(torch.arange(n, dtype=torch.float64), 1e4 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D))
+    cos, sin = angle.cos().float().cuda(), angle.sin().float().cuda()
+    pages = [torch.zeros(n // ps, K, ps, D, dtype=torch.int8, device="cuda") for _ in "kv"] + [torch.ones(n // ps, K, device="cuda") for _ in "kv"]
+    ops.qk_norm_rope_write_8bit(rows, K, K, D, w, w, 1e-5, (cos, sin), pos, pos, torch.empty(n, K * D, dtype=dtype, device="cuda"), *pages)
+    x = rows[:, K * D:2 * K * D].double().view(n, K, D)
+    x = x / torch.sqrt((x * x).mean(2, keepdim=True) + 1e-5) * w.double()
+    a, b = x.chunk(2, 2)
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    x = torch.cat([a * c - b * s, a * s + b * c], 2).view(n // ps, ps, K, D).transpose(1, 2)
+    most = x.abs().amax((2, 3))
+    scale = torch.exp2(torch.ceil(torch.log2(most / 127)))
+    scale = torch.where(most > 127 * scale, 2 * scale, torch.where(most <= 63.5 * scale, scale / 2, scale))
+    assert torch.equal(pages[2].double(), scale)
+    want = torch.round(x / scale[:, :, None, None])
+    assert torch.equal(pages[0].double(), want), int((pages[0].double() != want).sum())
