@@ -540,7 +540,8 @@ __global__ void __launch_bounds__(HD == 64 ? 192 : 256, HD == 64 ? 3 : 2) paged_
 #if RV_SCALED
         // the keys' own exponents in a marked tile
         auto own_exps = [&](int n) {
-            return key_exps + ((size_t)max(0, block_table[(size_t)r * max_blocks + t_lo + n]) * num_kv_heads + g) * AT_KEYS;
+            const int page = t_lo + n < max_blocks ? block_table[(size_t)r * max_blocks + t_lo + n] : 0;
+            return key_exps + ((size_t)max(0, page) * num_kv_heads + g) * AT_KEYS;
         };
 #endif
 #if RV_SCALED

@@ -81,21 +81,22 @@ def test_queries_of_any_size(ops, dtype, power):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("power", [66, 115, 120, 124])
-def test_large_queries_over_small_keys(ops, dtype, power):
+def test_large_queries_over_small_keys(ops, dtype, power, D):
     """Sums of whole numbers that a query's power of two would take past float32 before the keys' scale takes them back: scores of
     2^13 and more, of which one is the largest by far.  A score is off by 2^-20 of S, the largest sum |q| |k| scale, at most: where
     the next one is 2^-18 S + 40 behind, each other key weighs e^-39 of the largest at most (which may be lost, being below 2^-31), and the
     result is the largest one's value but for its rounding; where it is nearer, `room` holds."""
     g = torch.Generator().manual_seed(41)
     ctx, group = plain.batch([1, 1, 20], [70, 3, 0], 16, 12, 2)
-    k8, _ = pages_of(g, 12, 2, 16, 64)
-    v8, vs = pages_of(g, 12, 2, 16, 64)
+    k8, _ = pages_of(g, 12, 2, 16, D)
+    v8, vs = pages_of(g, 12, 2, 16, D)
     ks = torch.full((12, 2), 2.0 ** -60)
-    q = rnd(g, 22, 256, scale=2.0 ** power, dtype=dtype)
-    got = attend(ops, q, 4, 2, 64, (k8, v8, ks, vs), ctx, group, 0.125)
-    want, most = plain.attention(q, 4, 2, 64, k8, v8, ks, vs, ctx, group, 0.125, None)
-    limit = room(dtype, want, most, 2 if widened(ops, dtype, 64) else None)
+    q = rnd(g, 22, 4 * D, scale=2.0 ** power, dtype=dtype)
+    got = attend(ops, q, 4, 2, D, (k8, v8, ks, vs), ctx, group, 0.125)
+    want, most = plain.attention(q, 4, 2, D, k8, v8, ks, vs, ctx, group, 0.125, None)
+    limit = room(dtype, want, most, 2 if widened(ops, dtype, D) else None)
     clear = 0
     for t in range(22):
         r = min(t, 2)
@@ -103,10 +104,10 @@ def test_large_queries_over_small_keys(ops, dtype, power):
         j = torch.arange(last + 1)
         page = group.block_table[r][j // 16].long()
         for h in range(4):
-            s = (k8[page, h // 2, j % 16].double() * 2.0 ** -60) @ q[t, 64 * h:64 * h + 64].double() * 0.125
+            s = (k8[page, h // 2, j % 16].double() * 2.0 ** -60) @ q[t, D * h:D * h + D].double() * 0.125
             two = torch.topk(s, min(2, last + 1)).values
             if last == 0 or float(two[0] - two[1]) >= 2.0 ** -18 * float(most[t, h, 1]) + 40:
-                limit[t, 64 * h:64 * h + 64] = 2.0 ** -8 * want[t, 64 * h:64 * h + 64].abs() + (last + 1) * math.exp(-39) * most[t, h, 0]
+                limit[t, D * h:D * h + D] = 2.0 ** -8 * want[t, D * h:D * h + D].abs() + (last + 1) * math.exp(-39) * most[t, h, 0]
                 clear += 1
     assert clear >= 70
     assert bool(((got - want).abs() <= limit).all())
