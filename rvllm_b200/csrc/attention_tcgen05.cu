@@ -968,12 +968,14 @@ extern "C" int AT_SYM(rv_paged_attention_prefill_tcgen05_cluster)(int n_tokens, 
 }
 
 static int at_configure(size_t smem) {
-    static bool configured = false;
-    if (configured) return 0;
+    static bool configured[64];                                  // on each device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return at_fail("paged_attention_prefill_tcgen05: no device");
+    if (configured[dev]) return 0;
     cudaError_t e = cudaFuncSetAttribute(paged_attention_prefill_tcgen05_kernel<RV_HD>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return at_fail(cudaGetErrorString(e));
-    configured = true;
+    configured[dev] = true;
     return 0;
 }
 // Shared memory of a block, all that counts against a multiprocessor's (-1: an error).
