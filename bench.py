@@ -620,9 +620,9 @@ KV8_POINTS = [(1, 3900), (8, 3900), (16, 3900), (64, 3900), (8, 30000), (32, 150
 
 def run_kv8(args):
     """Whole steps over keys and values in bfloat16 and in 8 bits, and with log probabilities (`--only kv8`): ms a replayed
-    step of single tokens (device time, tokens fed back on the device), of a prompt of 2,048 tokens and of 64 tokens after 1,000 (the
-    third step of each and later ones, device time), of a step through `Engine` with and without log probabilities, and of
-    scoring 2,048 tokens (wall time, the device waited for)."""
+    step of single tokens (device time, tokens fed back on the device), of steps with prompt portions (their captured launches
+    replayed back to back), of a step through `Engine` with and without log probabilities, and of scoring 2,048 tokens (wall
+    time, the device waited for)."""
     import torch
     from rvllm_b200.config import config_from_dict
     from rvllm_b200.engine import (Engine, Generator, ModelRunner, Request, SchedulerConfig, StepEntry, graphs_default,
@@ -661,16 +661,22 @@ def run_kv8(args):
         first = runner.decode_greedy(range(batch), [1] * batch, 8)[-1].tolist()
         return round(timed(lambda: runner.decode_greedy(range(batch), first, 96)) / 96, 4)
 
-    def portion(kv, tokens, before):
-        runner, took = fresh(kv, 2, tokens + before), []
-        for _ in range(8):
-            runner.add_request("r")
-            if before:
-                runner.step([StepEntry("r", ids(before), ())])
-            text = ids(tokens)
-            took.append(timed(lambda: runner.step([StepEntry("r", text, (tokens - 1,))])))
-            runner.end_request("r")
-        return round(sorted(took[2:])[2], 4)
+    def portion(kv, n, tokens, before):
+        runner = fresh(kv, n, tokens + before)
+        for _ in range(3):                              # the second step of its sizes is captured
+            for i in range(n):
+                runner.add_request(i)
+                if before:
+                    runner.step([StepEntry(i, ids(before), ())])
+            runner.step([StepEntry(i, ids(tokens), (tokens - 1,)) for i in range(n)])
+            graph = max(runner._mixed_graphs.values(), key=lambda g: g.last_used).graph if runner._mixed_graphs else None
+            for i in range(n):
+                runner.end_request(i)
+
+        def replays():
+            for _ in range(20):
+                graph.replay()
+        return round(min(timed(replays) for _ in range(4)) / 20, 4)
 
     def engine_step(kv, batch, context, logprobs):
         runner = fresh(kv, batch, context)
@@ -703,8 +709,8 @@ def run_kv8(args):
     for kv in ("auto", "int8"):
         t = out["bfloat16" if kv == "auto" else "int8"] = {"bytes_a_token": fresh(kv, 1, PAGE).cache.bytes_per_token()}
         t["decode_ms"] = {f"{b} x {c}": decode(kv, b, c) for b, c in KV8_POINTS}
-        t["portion_ms"] = {"2048": portion(kv, 2048, 0), "512": portion(kv, 512, 0), "64 after 1000": portion(kv, 64, 1000),
-                           "512 after 8000": portion(kv, 512, 8000)}
+        t["portion_ms"] = {f"{n} x {k} after {b}": portion(kv, n, k, b)
+                           for n, k, b in ((1, 2048, 0), (1, 512, 0), (1, 64, 0), (1, 64, 1000), (1, 512, 8000), (8, 20, 500))}
         t["engine_step_ms"] = {f"{b} x 1000, logprobs {k}": engine_step(kv, b, 1000, k)
                                for b in (1, 8, 64) for k in (None, 0, 5, 20)}
         t["score_2048_ms"] = {f"top {k}": score(kv, k) for k in (0, 5)}

@@ -33,13 +33,13 @@
 //                           request is a segment, left in scratch for the merge kernel.
 //   attention_8bit_rows     portions, and few or short single tokens: a warp for every 8 or 16 rows, or a block or a
 //                           cluster of blocks whose warps share the rows' tiles and meet in shared memory.
-//   (bindings)              long bfloat16 portions: pages are widened to bfloat16 once (cache_8bit.cu) and read by the
+//   (bindings)              long bfloat16 portions: pages are widened to 16 bits once (cache_8bit.cu) and read by the
 //                           tensor-memory kernel, whose 128-row tiles these 16-row ones cannot match.
 //
-// What bounds them.  The stream: 64 requests of 2,000 keys on average (205 MB) 43 us, 73 % of a copy's bandwidth, with
-// 0.56 instructions issued a cycle and scheduler: not the instructions but how evenly 2,368 warps end, plus some 5 us of
-// launch, first tiles and merge.  (16 / 2 heads of 128, 4 requests of 31,000 keys 26 us of 16.)  Rows: the matrix
-// instructions and conversions of 8 or 16 rows a tile; 2,048 new tokens take 135 us at 32 / 8 heads of 64, widened 45.
+// What bounds them.  The stream: 64 requests of 3,100 keys on average (205 MB, 31 us at a copy's bandwidth) 44 us: the
+// instructions of 16 warps a multiprocessor, how evenly 2,368 of them end, and some 5 us of launch, first tiles and merge.
+// (16 / 2 heads of 128, 8 requests of 25,000 keys on average 26.5 us of 16.)  Rows: the matrix instructions and conversions of
+// 8 or 16 rows a tile; 2,048 new tokens take 174 us at 32 / 8 heads of 64, widened 47.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -973,7 +973,7 @@ static long long a8_tiles(int max_ctx_len, int window, int max_q_len) {
 }
 // Blocks whose warps share the tiles of ROWS rows: 0 (a warp has them alone) where there are warps enough, else as many as the
 // GPU holds at once, up to a cluster, while every warp has a tile.  (us by warps alone / a block / two / four / eight: 32 / 8
-// heads of 64, 128 requests of 700 keys 35 / 25 / 35 / 54 / 85, 32 of 1,000 23 / 12.4 / 12.5 / 18 / 26, 16 of 4,000 72 / 27 / 22 / 18.5 / 23.)
+// heads of 64, 128 requests of 700 keys 35 / 23 / 34 / 53 / 84, 32 of 1,000 24 / 15 / 11.8 / 16 / 25, 16 of 4,000 78 / 30 / 26 / 17 / 22.)
 static int a8_nsplit(long long units, long long tiles, int block_places) {
     if (units > 4ll * block_places || tiles < 2) return 0;
     int n = 1;
@@ -982,9 +982,9 @@ static int a8_nsplit(long long units, long long tiles, int block_places) {
 }
 // Single tokens by blocks or clusters, which need no scratch and no second launch, but take as long as the longest context: while
 // a warp has no more than eight tiles of that, in two rounds at most.  (us so / by the stream: 32 / 8 heads of 64, 1 request of
-// 700 keys 6.3 / 8.3, 64 of 100 8.3 / 12.4, 64 of 700 14 / 18.5, 128 of 700 25 / 27, 16 of 4,000 18.5 / 20.7; 8 / 8 heads of 128,
-// 32 of 1,000 14 / 19, 128 of 300 (1,024 blocks for 296 places) 27 / 23.  64 of 2,000 alike would take 29 / 33 too, but of
-// 2,340 to 3,900 52 / 44.)
+// 700 keys 5.2 / 6.0, 64 of 100 7.4 / 10.6, 64 of 700 12.6 / 17.6, 128 of 700 23.6 / 26.3, 16 of 4,000 16.9 / 19.9; 8 / 8 heads of
+// 128, 32 of 1,000 13.8 / 17.6, 128 of 300 (1,024 blocks for 296 places) 25 / 22; 16 / 2 heads of 128, 8 of 31,000 43 / 30.  Near the
+// border, 64 of 2,000 alike 28 / 33, of 2,340 to 3,850 43 / 44.)
 static bool a8_few(long long units, long long tiles, int n_sms, int form) {
     if (form != 0) return form == 2;               // 1: the stream, 2: blocks and clusters
     const int places = (A8_HD <= 64 ? 4 : 2) * n_sms;

@@ -22,8 +22,8 @@
 //
 // What bounds it: what a block does beside its rows (whose tokens and pages they are, the pages' largest values, two
 // meetings of its warps) and four reads that wait for one another (slots, positions, angles and rows, scales), for as many
-// waves of blocks as there are; registers leave a multiprocessor four or five.  32 / 8 heads of 64: 64 tokens 4.1 us,
-// 2,048 tokens 11.3 us, 8,192 tokens 43 us; their bytes at a copy's bandwidth 0.1, 3.5 and 14 us.
+// waves of blocks as there are; registers leave a multiprocessor four or five.  32 / 8 heads of 64: 64 tokens 4.2 us,
+// 2,048 tokens 11.4 us, 8,192 tokens 44 us; their bytes at a copy's bandwidth 0.1, 3.5 and 14 us.
 #include <cuda_fp16.h>
 
 #include "common.cuh"

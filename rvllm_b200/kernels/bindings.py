@@ -1100,15 +1100,19 @@ class CudaOps:
             return False
         if not 0 < self._wide_bytes(ctx, window, num_kv_heads, head_dim) <= self.widen_8bit_bytes:
             return False
-        # tiles of 16 rows and 32 keys, of 64 dimensions, that are there (a padded step's longest portion, requests and context are
-        # up to twice what it has each).  us by mma.sync from the pages / widened: 32 / 8 heads of 64, 64 tokens after 1,000 (4,352
-        # tiles) 14.5 / 17, 16 x 20 after 500 (10,880) 23 / 22, 512 (16,384) 24 / 16, 64 after 4,000 (16,256) 33 / 22; 16 / 8 heads
-        # 16 x 20 after 500 (6,528) 14 / 22, 64 after 16,000 (32,128) 57 / 36; 16 / 2 heads of 128 16 x 20 after 500 (10,880) 26 / 21,
-        # 64 after 1,000 (4,352) 13 / 20; 8 / 8 heads of 128 512 (8,192) 14.5 / 16.5
+        # Tiles of 16 rows and 32 keys, of 64 dimensions, that are there (a padded step's longest portion, requests and context are
+        # up to twice what it has each), against what widening takes: whole contexts, however few rows they have, and beside single
+        # tokens a third launch.  Measured in replayed steps, where weights push the pages out of the caches (calls one after another
+        # on the same pages favour the other kernel by some 5 us); us a layer, mma.sync from the pages - widened, in 216 steps the
+        # rule costs 0.7 more than the better one on average, 14 at most: 32 / 8 heads of 64, 64 tokens alone -0, after 500 2, after
+        # 1,000 3.4, after 6,000 23; 256 alone 6; 8 x 20 after 500 -7, 16 x 10 after 1,500 -33, 16 x 40 after 500 22; 100 beside 8
+        # single tokens after 300 -5, after 3,000 17; 16 / 2 heads of 128, 64 after 1,000 3, 8 x 20 after 500 -12, 100 beside 31 after
+        # 1,000 -11; 16 / 8 heads of 64, 64 after 1,000 0, after 6,000 8, 32 x 10 after 1,500 -40
         tokens, few, depth = likely
         seen = min(depth, window + longest) if window else depth
         tiles = (-(-tokens * group // 16) + few // 2) * -(-seen // 32) * num_kv_heads * (head_dim // 64)
-        return self.prefill_8bit == "tcgen05" or tiles > 10000
+        widening = 2500 + few * seen * num_kv_heads * head_dim // 500 + (16000 if ctx.n_decode else 0)
+        return self.prefill_8bit == "tcgen05" or tiles > widening
 
     def _wide_bytes(self, ctx, window, num_kv_heads, head_dim) -> int:
         """What one portion's keys and values take in 16 bits."""
