@@ -91,6 +91,8 @@ class Engine:
                  lookahead: bool = False, logprobs: Optional[int] = None):
         if logprobs is not None and not 0 <= logprobs <= 32:
             raise ValueError(f"logprobs asks for 0 to 32 alternatives, got {logprobs}")
+        if logprobs and logprobs > runner.model.spec.vocab_size:
+            raise ValueError(f"logprobs asks for {logprobs} alternatives of a vocabulary of {runner.model.spec.vocab_size}")
         self.logprobs = logprobs
         self.runner = runner
         self.scheduler = Scheduler(config, runner.cache, context_length)

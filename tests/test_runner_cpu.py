@@ -128,3 +128,14 @@ def test_captures_of_exact_shapes_are_bounded(model, monkeypatch):
     step(12, 1)
     assert twice(15, 2) == [(12, 1), (15, 2)]
     runner.cache.check()
+
+
+def test_more_alternatives_than_the_vocabulary_are_refused_before_a_step(folder, tmp_path):
+    """As scoring refuses them: not by the kernel, when the first step has run and requests hold pages."""
+    gen = generator(write_tiny(str(tmp_path), "A", vocab_size=20, bos_token_id=1, eos_token_id=7))
+    for logprobs in (21, 32):
+        with pytest.raises(ValueError, match="20"):
+            gen.generate_ids([[1, 2, 3]], GenerateOptions(max_tokens=2, logprobs=logprobs))
+    assert not gen._runner.cache.requests and gen._runner.steps == 0
+    result = gen.generate_ids([[1, 2, 3]], GenerateOptions(max_tokens=2, logprobs=20, stop_tokens=[]))
+    assert all(len(t.top) == 20 for t in result.logprobs[0])
