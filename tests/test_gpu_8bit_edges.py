@@ -207,6 +207,20 @@ def test_the_same_call_gives_the_same_bits(ops):
                 assert torch.equal(first, attend(ops, q, 8, 2, D, (k8, v8, ks, vs), ctx, group, D ** -0.5))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,K,D", [(2, 2, 64), (4, 2, 64), (3, 1, 64), (4, 1, 128), (2, 2, 48), (5, 1, 64), (8, 8, 256)])
+def test_portions_of_a_few_rows(ops, dtype, H, K, D):
+    """Portions of two to four tokens alone: four rows and fewer a key/value head, and just more."""
+    g = torch.Generator().manual_seed(51)
+    for new, old in (([2, 2], [0, 30]), ([2, 3, 4], [100, 0, 700]), ([1, 2, 1], [40, 5, 9]), ([4] * 40, [13 * i for i in range(40)])):
+        pages = sum(-(-(a + b) // 16) for a, b in zip(new, old))
+        new, old = zip(*sorted(zip(new, old), key=lambda e: e[0] != 1))
+        ctx, group = plain.batch(list(new), list(old), 16, pages, sum(n == 1 for n in new), seed=10)
+        pages_ = opposite_pairs(g, pages, K, 16, D)
+        for window in (None, 3):
+            check(ops, rnd(g, sum(new), H * D, dtype=dtype), H, K, D, pages_, ctx, group, D ** -0.5, window)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_portions_widened_in_passes(ops, D, monkeypatch):
     """Portions of which memory holds one or two at a time, beside single tokens and an empty one, and the same call captured."""
